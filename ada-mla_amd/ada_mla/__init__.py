@@ -9,6 +9,14 @@ reference's ``ada_mla`` extension module (csrc/mla_api.cpp:115-120).
     q = ada_mla.mla_absorb_query(q_nope, q_rope, w_uk)     # the projections around
     y = ada_mla.mla_project_output(o_star, w_uv, w_o)      # the decode (MLA block)
 
+and what a serving loop runs around it on the paged cache:
+
+    cu, cu_new, slots, positions, free = ada_mla.mla_paged_tables(  # block table, slots, positions
+        context_lens, new_lens, block_table, free_pages, free_start, page_size, total_new)
+    q_rope = ada_mla.mla_append_kv(kv, norm_weight, cos_sin, positions, slots, kv_pages, q_rope=q_rope)
+    o = ada_mla.mla_prefill(q_nope, q_rope, w_uk, w_uv, kv_pages, cu_new, cu, block_table=block_table)
+    out = ada_mla.mla_decode_tree(q, kv_pages, block_table, cu, tree_mask)  # drafted tokens
+
 The functions live in the compiled extension ``ada_mla._C`` (built by
 ada-mla_amd/build.py), which calls the HIP library through its C ABI
 (include/mla_mi355x.h). They are resolved on first use; if the extension is
@@ -19,10 +27,12 @@ from __future__ import annotations
 import importlib
 
 __all__ = ["mla_decode_split", "mla_decode_fused", "mla_decode_split_batched", "mla_decode_paged",
-           "mla_absorb_query", "mla_project_output", "HEAD_DIM_C", "HEAD_DIM_ROPE", "HEAD_DIM_K", "extension"]
+           "mla_absorb_query", "mla_project_output", "mla_paged_tables", "mla_append_kv", "mla_decode_tree",
+           "mla_prefill", "HEAD_DIM_C", "HEAD_DIM_ROPE", "HEAD_DIM_K", "extension"]
 
 _EXPORTS = {"mla_decode_split", "mla_decode_fused", "mla_decode_split_batched", "mla_decode_paged",
-            "mla_absorb_query", "mla_project_output", "HEAD_DIM_C", "HEAD_DIM_ROPE", "HEAD_DIM_K"}
+            "mla_absorb_query", "mla_project_output", "mla_paged_tables", "mla_append_kv", "mla_decode_tree",
+           "mla_prefill", "HEAD_DIM_C", "HEAD_DIM_ROPE", "HEAD_DIM_K"}
 
 
 def extension():

@@ -27,8 +27,10 @@ FLAG_SCALAR_TRANSPOSE = 1
 FLAG_FP32_PARTIALS = 4
 FLAG_FP8_CACHE = 16  # plan queries: the fp8-cache entries' plan
 FLAG_TWO_LAUNCHES = 8
+FLAG_ROPE_HALVES = 32  # append_kv: pairs i, i + 32
 
 _vp, _i, _u, _sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_uint, ctypes.c_size_t
+_f, _ll = ctypes.c_float, ctypes.c_longlong
 _SIGNATURES = {
     "mla_abi_version": (_i, []),
     "mla_status_string": (ctypes.c_char_p, [_i]),
@@ -61,6 +63,15 @@ _SIGNATURES = {
     "mla_project_output_bf16": (_i, [_vp, _vp, _vp, _vp, _vp, _sz, _i, _i, _i, _vp]),
     "mla_decode_paged_fp16": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _sz, _i, _i, _i, _i, _i, _i, _i, _vp]),
     "mla_decode_paged_bf16": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _sz, _i, _i, _i, _i, _i, _i, _i, _vp]),
+    "mla_paged_tables": (_i, [_vp] * 10 + [_i] * 5 + [_vp]),
+    "mla_append_kv_fp16": (_i, [_vp] * 8 + [_f, _f, _i, _i, _i, _ll, _ll, _ll, _ll, _u, _vp]),
+    "mla_append_kv_bf16": (_i, [_vp] * 8 + [_f, _f, _i, _i, _i, _ll, _ll, _ll, _ll, _u, _vp]),
+    "mla_decode_tree_workspace_size": (_sz, [_i] * 5),
+    "mla_decode_tree_fp16": (_i, [_vp] * 8 + [_sz] + [_i] * 8 + [_vp]),
+    "mla_decode_tree_bf16": (_i, [_vp] * 8 + [_sz] + [_i] * 8 + [_vp]),
+    "mla_prefill_workspace_size": (_sz, [_i] * 3),
+    "mla_prefill_fp16": (_i, [_vp] * 10 + [_sz] + [_i] * 7 + [_vp]),
+    "mla_prefill_bf16": (_i, [_vp] * 10 + [_sz] + [_i] * 7 + [_vp]),
 }
 
 _lib = None
@@ -298,4 +309,102 @@ def decode_split_batched_fp8(q, c_fp8, c_scale: float, cu_seqlens, num_splits: i
            lib.mla_decode_split_batched_fp8(q.data_ptr(), c_fp8.data_ptr() if total else None, float(c_scale),
                                             cu_seqlens.data_ptr(), out.data_ptr(), ws.data_ptr(), ws_bytes, b, n_h,
                                             total, num_splits, _stream(q)))
+    return out
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def paged_tables(context_lens, new_lens, block_table, free_pages, free_start, page_size: int, total_new: int):
+    """mla_paged_tables: int32 device tensors context_lens, new_lens [B], block_table [B, max_pages] (new
+    pages written in place), free_pages [F], free_start [1] -> (cu_seqlens [B+1], cu_new [B+1], slots
+    [total_new] int64, positions [total_new], free_next [1])."""
+    import torch
+    lib = load()
+    for t in (context_lens, new_lens, block_table, free_pages, free_start):
+        assert t.dtype == torch.int32 and t.is_contiguous()
+    b = context_lens.shape[0]
+    i32 = dict(dtype=torch.int32, device=context_lens.device)
+    cu_seqlens, cu_new = torch.empty(b + 1, **i32), torch.empty(b + 1, **i32)
+    slots = torch.empty(total_new, dtype=torch.int64, device=context_lens.device)
+    positions, free_next = torch.empty(total_new, **i32), torch.empty(1, **i32)
+    _check("mla_paged_tables",
+           lib.mla_paged_tables(_ptr(context_lens), _ptr(new_lens), _ptr(free_pages), _ptr(free_start),
+                                _ptr(block_table), _ptr(cu_seqlens), _ptr(cu_new), _ptr(slots), _ptr(positions),
+                                _ptr(free_next), b, total_new, free_pages.shape[0], page_size, block_table.shape[1],
+                                _stream(context_lens)))
+    return cu_seqlens, cu_new, slots, positions, free_next
+
+
+def append_kv(kv, norm_weight, cos_sin, positions, slots, kv_cache, q_rope=None, eps: float = 1e-6,
+              cache_scale: float = 1.0, interleaved: bool = True, out=None):
+    """mla_append_kv_*: kv [T, 576] and q_rope [T, n_h, 64] (last dimension contiguous, other strides
+    multiples of 8), kv_cache [..., 576] contiguous, of kv's type or float8_e4m3fn -> rotated q_rope or None."""
+    import torch
+    lib = load()
+    tokens = kv.shape[0]
+    assert kv.shape == (tokens, HEAD_DIM_K) and kv.stride(1) == 1 and kv_cache.is_contiguous()
+    assert norm_weight.dtype == kv.dtype and cos_sin.dtype == torch.float32 and cos_sin.shape[1] == 64
+    assert positions.dtype == torch.int32 and slots.dtype == torch.int64
+    n_h = 0 if q_rope is None else q_rope.shape[1]
+    if q_rope is not None:
+        assert q_rope.dtype == kv.dtype and q_rope.stride(2) == 1 and q_rope.shape == (tokens, n_h, 64)
+        if out is None:
+            out = torch.empty((tokens, n_h, 64), dtype=kv.dtype, device=kv.device)
+    flags = (FLAG_FP8_CACHE if kv_cache.dtype == torch.float8_e4m3fn else 0) | (0 if interleaved else FLAG_ROPE_HALVES)
+    fn = "mla_append_kv_" + _suffix(kv)
+    _check(fn, getattr(lib, fn)(_ptr(kv), _ptr(norm_weight), _ptr(cos_sin), _ptr(positions), _ptr(slots), _ptr(q_rope),
+                                _ptr(kv_cache), _ptr(out), eps, cache_scale, tokens, n_h, cos_sin.shape[0],
+                                kv_cache.numel() // HEAD_DIM_K, kv.stride(0), q_rope.stride(0) if n_h else 0,
+                                q_rope.stride(1) if n_h else 0, flags, _stream(kv)))
+    return out
+
+
+def decode_tree(q, kv_cache, block_table, cu_seqlens, tree_mask, total_tokens: int, draft_lens=None,
+                num_splits: int = 0, out=None, workspace=None):
+    """mla_decode_tree_*: q [B, drafts, n_h, 576], kv_cache [num_pages, page_size, 576], block_table
+    [B, max_pages] int32, cu_seqlens [B+1] int32, tree_mask [B, drafts] int64, draft_lens [B] int32 or None."""
+    import torch
+    lib = load()
+    b, drafts, n_h, _ = q.shape
+    assert kv_cache.dtype == q.dtype and block_table.dtype == torch.int32 and cu_seqlens.dtype == torch.int32
+    assert tree_mask.dtype == torch.int64 and tree_mask.shape == (b, drafts)
+    assert q.is_contiguous() and kv_cache.is_contiguous() and block_table.is_contiguous() and tree_mask.is_contiguous()
+    if out is None:
+        out = torch.empty((b, drafts, n_h, HEAD_DIM_V), dtype=q.dtype, device=q.device)
+    ws_bytes = lib.mla_decode_tree_workspace_size(b, drafts, n_h, total_tokens, num_splits)
+    if ws_bytes == 0:
+        raise MlaError("mla_decode_tree_workspace_size", STATUS_INVALID_VALUE)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if workspace is None else workspace
+    fn = "mla_decode_tree_" + _suffix(q)
+    _check(fn, getattr(lib, fn)(_ptr(q), _ptr(kv_cache), _ptr(block_table), _ptr(cu_seqlens), _ptr(tree_mask),
+                                _ptr(draft_lens), _ptr(out), _ptr(ws), ws.numel(), b, drafts, n_h, total_tokens,
+                                kv_cache.shape[1], kv_cache.shape[0], block_table.shape[1], num_splits, _stream(q)))
+    return out
+
+
+def prefill(q_nope, q_rope, w_uk, w_uv, kv_cache, cu_q, cu_seqlens, total_tokens: int, block_table=None, out=None,
+            workspace=None):
+    """mla_prefill_*: q_nope [T, n_h, 128], q_rope [T, n_h, 64], w_uk / w_uv [n_h, 128, 512], kv_cache
+    [total_tokens, 576] or, with block_table [B, max_pages] int32, [num_pages, page_size, 576]."""
+    import torch
+    lib = load()
+    queries, n_h, _ = q_nope.shape
+    b = cu_q.shape[0] - 1
+    assert q_nope.dtype == q_rope.dtype == w_uk.dtype == w_uv.dtype == kv_cache.dtype
+    for t in (q_nope, q_rope, w_uk, w_uv, kv_cache, cu_q, cu_seqlens):
+        assert t.is_contiguous()
+    if out is None:
+        out = torch.empty((queries, n_h, 128), dtype=q_nope.dtype, device=q_nope.device)
+    ws_bytes = lib.mla_prefill_workspace_size(b, n_h, total_tokens)
+    if ws_bytes == 0:
+        raise MlaError("mla_prefill_workspace_size", STATUS_INVALID_VALUE)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q_nope.device) if workspace is None else workspace
+    paged = block_table is not None
+    fn = "mla_prefill_" + _suffix(q_nope)
+    _check(fn, getattr(lib, fn)(_ptr(q_nope), _ptr(q_rope), _ptr(w_uk), _ptr(w_uv), _ptr(kv_cache), _ptr(block_table),
+                                _ptr(cu_q), _ptr(cu_seqlens), _ptr(out), _ptr(ws), ws.numel(), b, n_h, queries,
+                                total_tokens, kv_cache.shape[1] if paged else 0, kv_cache.shape[0] if paged else 0,
+                                block_table.shape[1] if paged else 0, _stream(q_nope)))
     return out

@@ -1,0 +1,128 @@
+// Building blocks of the many-row attention kernels (drafted trees, prompts):
+// 32x32 MFMA tiles on which every lane owns one query row.
+//
+// Both products run transposed: S^T = K Q^T and O^T = V^T P^T. The D tile of
+// S^T then holds, in lane l, 16 keys of query row l mod 32 (lane l ^ 32 the
+// other 16), so the softmax is per lane with one exchange between two lanes;
+// and those 16 registers, rounded, are the B operand of O^T as they stand: the
+// order of the keys within a product is free, so V^T's rows are read in the
+// order that P's registers have. P never leaves the registers and the running
+// maximum's factor is one value a lane.
+#pragma once
+
+#include "mla_device.hpp"
+#include "mla_internal.hpp"
+#include "mla_ring.hpp"
+
+namespace mla {
+
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+
+// D[32x32] += A[32x16] * B[16x32], fp32 accumulate. Lane l supplies
+// A[l % 32][8 * (l / 32) + j] and B[8 * (l / 32) + j][l % 32] (j = 0..7) and
+// holds D[8 * (i / 4) + 4 * (l / 32) + i % 4][l % 32] (i = 0..15).
+__device__ __forceinline__ floatx16 mfma32x32x16(half8 a, half8 b, floatx16 c)
+{
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+
+__device__ __forceinline__ floatx16 mfma32x32x16(bf16x8 a, bf16x8 b, floatx16 c)
+{
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+// Keeps an accumulator tile in the accumulation registers across this point,
+// so that 16 of them and 144 registers of Q* fit one wave's 512: left to
+// itself the compiler moves them into the 256 others for a rescale and spills.
+__device__ __forceinline__ void in_accumulators(floatx16 &v)
+{
+    asm volatile("" : "+a"(v));
+}
+
+// f over lanes l and l ^ 32, on the VALU (see reduce_over_lane_groups).
+template <typename F>
+__device__ __forceinline__ float reduce_halves(float v, F f)
+{
+    const unsigned u = __float_as_uint(v);
+    const auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return f(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+
+// The key of a 32-key block that sits in row rho of the S^T tile:
+// rho = 16 a + 8 b + 4 c + j is key 16 a + 8 c + 2 j + b. Lane half c then
+// holds keys 16 a + 8 c + {0, 2, 4, 6} in registers 8 a .. 8 a + 3 and
+// {1, 3, 5, 7} in 8 a + 4 .. 8 a + 7, so that each of the two transpose reads
+// of V^T that match a P operand takes four keys of one parity, which the row
+// swizzle (chunk c of row r at c ^ (r mod 16)) serves without bank conflicts.
+__device__ __forceinline__ int key_of_row(int rho)
+{
+    return (rho & 16) + ((rho & 4) << 1) + 2 * (rho & 3) + ((rho >> 3) & 1);
+}
+
+// The key (within its 32-key block) in register i of a lane of half hl.
+__device__ __forceinline__ int key_of_reg(int i, int hl)
+{
+    return (i & 8) * 2 + 8 * hl + 2 * (i & 3) + ((i >> 2) & 1);
+}
+
+// P's registers 8 a .. 8 a + 7, rounded to the type of V: the B operand of keys 16 a ..
+// 16 a + 15 of its block. P is in [0, 2^8] and the rounding at most half a
+// step of each term; the sums of P that normalise the result stay in fp32.
+template <typename E>
+__device__ __forceinline__ typename Vec<E>::v8 p_operand(const float *p)
+{
+    typename Vec<E>::v8 v;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        v[i] = (E)p[i];
+    return v;
+}
+
+// Whether a 16-bit value is an infinity or a NaN.
+template <typename E>
+__device__ __forceinline__ bool not_finite(unsigned short bits)
+{
+    const unsigned e = __is_same(E, _Float16) ? 0x7c00u : 0x7f80u;
+    return (bits & e) == e;
+}
+
+// 16 bytes per lane from a per-lane address into LDS at lds + 16 * lane
+// (lds: a wave-uniform LDS byte address); see global_to_lds16.
+__device__ __forceinline__ void gather_to_lds16(const void *p, unsigned lds)
+{
+    unsigned saved_m0;
+    asm volatile("s_mov_b32 %0, m0\n\t"
+                 "s_mov_b32 m0, %2\n\t"
+                 "global_load_lds_dwordx4 %1, off\n\t"
+                 "s_mov_b32 m0, %0"
+                 : "=&s"(saved_m0) : "v"(p), "s"(lds) : "memory");
+}
+
+__device__ __forceinline__ unsigned lds_address(const void *p)
+{
+    return __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(const __attribute__((address_space(3))) void *)p);
+}
+
+// A load of what the kernel does not write, at a wave-uniform address, by the
+// scalar unit: a vector load would be waited for with vmcnt, behind every
+// global->LDS load in flight.
+template <typename T>
+__device__ __forceinline__ T scalar_load(const T *p)
+{
+    return *(const __attribute__((address_space(4))) T *)p;
+}
+
+// A read, and a transpose read (lds_read_tr16), at an LDS byte address.
+template <typename T>
+__device__ __forceinline__ T lds_load(unsigned addr)
+{
+    return *(const MLA_LDS T *)(uintptr_t)addr;
+}
+
+template <typename E>
+__device__ __forceinline__ typename Vec<E>::v4 lds_load_tr16(unsigned addr)
+{
+    return __builtin_bit_cast(typename Vec<E>::v4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((MLA_LDS shortx4 *)(uintptr_t)addr));
+}
+
+}  // namespace mla

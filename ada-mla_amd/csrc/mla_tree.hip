@@ -1,0 +1,513 @@
+// Attention of a tree of drafted tokens over the paged latent cache, absorbed
+// form (mla_decode_tree_*):
+//
+//   O*[b, i, h] = softmax_t( Q*[b, i, h] . C[t] / sqrt(192) ) C_N[t]
+//
+// over the tokens t that drafted token i of request b sees: all of its context
+// and the drafted tokens of the request whose bit is set in tree_mask[b][i]
+// (its ancestors and itself). The drafted tokens' latent rows are the last
+// ones of the request's cache.
+//
+// Against the single-token decode, drafts x heads rows share each latent row,
+// so from about 256 rows on the call is bound by the matrix units and, next,
+// by LDS: a workgroup is 4 waves of one per SIMD, each owning 32 query rows
+// whole (Q* 144 registers, O* 256 accumulators, P in registers, see
+// mla_flash.hpp), so the waves meet only to hand over cache blocks.
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+
+#include "mla_flash.hpp"
+#include "mla_mi355x.h"
+
+namespace mla {
+namespace {
+
+constexpr int kBlock = 32;                // tokens per cache block
+constexpr int kWaves = 4;                 // waves per workgroup
+constexpr int kRows = 32 * kWaves;        // query rows per workgroup
+constexpr int kRing = 4;                  // LDS ring slots
+constexpr int kSlotElems = kBlock * kDK;  // 36 KB
+constexpr int kRopeDim = kDK - kDV;
+constexpr int kRopeElems = kBlock * kDV;  // the rope part of a slot, after its C_N rows
+constexpr int kUnitsPerWave = 9;          // 1 KB load units of a block per wave: 8 rows, 1 rope unit
+constexpr int kMaxDrafts = 64;
+
+bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+struct TreeArgs {
+    const void *q;
+    const void *cache;
+    const int *block_table;
+    const int *cu_seqlens;
+    const unsigned long long *tree_mask;
+    const int *draft_lens;
+    void *out;
+    float *part_o;  // [slot][row tile][wave][16 column tiles][4][64 lanes][4]
+    float *part_m;  // [slot][row tile * 128]
+    float *part_l;
+    int batch, drafts, num_heads, total_tokens;
+    int chunk;      // tokens per split
+    int row_tiles;  // of 128 rows, per request
+    int n_slots;    // total_tokens / chunk + batch
+    int page_shift, num_pages, bt_stride;
+    float scale_log2;
+};
+
+// Request b's tokens [lo, hi) of the packed numbering and its splits. Request
+// b's splits take the slots lo / chunk + b, ..., which never meet those of
+// another request, whatever the lengths.
+struct Request {
+    int lo, len, n_splits, slot0, drafts;
+    __device__ __forceinline__ void read(const TreeArgs &a, int b)
+    {
+        lo = min(max(a.cu_seqlens[b], 0), a.total_tokens);
+        len = min(max(a.cu_seqlens[b + 1], lo), a.total_tokens) - lo;
+        n_splits = max(1, (len + a.chunk - 1) / a.chunk);
+        slot0 = lo / a.chunk + b;
+        drafts = a.draft_lens ? min(max(a.draft_lens[b], 0), a.drafts) : a.drafts;
+    }
+};
+
+template <typename E>
+__global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_per_eu(1, 1))) void tree_kernel(TreeArgs a)
+{
+    using E8 = typename Vec<E>::v8;
+    using E4 = typename Vec<E>::v4;
+    __shared__ __attribute__((aligned(1024))) E s_ring[kRing * kSlotElems];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r32 = lane & 31, hl = lane >> 5;
+    const unsigned ring = lds_address(s_ring);
+
+    // workgroup -> (slot, row tile): the row tiles of a slot, which read the
+    // same tokens, get ids equal mod 8, i.e. one XCD and its L2
+    const int slot = (blockIdx.x >> 3) / a.row_tiles * 8 + (blockIdx.x & 7);
+    const int rt = (blockIdx.x >> 3) % a.row_tiles;
+    if (slot >= a.n_slots)
+        return;
+    int b = 0;  // the last request whose first slot is at or before `slot`
+    for (int base = 0; base < a.batch; base += 64) {
+        const int i = base + lane;
+        const bool in = i < a.batch && min(max(a.cu_seqlens[i], 0), a.total_tokens) / a.chunk + i <= slot;
+        const unsigned long long m = __builtin_amdgcn_ballot_w64(in);
+        if (m != 0)
+            b = base + 63 - __builtin_clzll(m);
+        if (m != ~0ull)
+            break;
+    }
+    b = __builtin_amdgcn_readfirstlane(b);
+    Request rq;
+    rq.read(a, b);
+    const int split = slot - rq.slot0;
+    if (split < 0 || split >= rq.n_splits)
+        return;
+    const int rows = a.drafts * a.num_heads;      // of the request's output
+    const int live = rq.drafts * a.num_heads;     // of its drafted tokens
+    const int row = rt * kRows + 32 * wave + r32; // this lane's
+    E *out = (E *)a.out + (size_t)b * rows * kDV;
+    if (rt * kRows >= live) {  // only padding rows
+        if (rq.n_splits == 1)
+            for (int i = threadIdx.x; i < min(kRows, rows - rt * kRows) * (kDV / 8); i += 256)
+                *(uint4 *)(out + (size_t)rt * kRows * kDV + 8 * i) = uint4{0, 0, 0, 0};
+        return;
+    }
+    const int context = rq.len - rq.drafts;
+    const int t_lo = split * a.chunk, t_hi = min(t_lo + a.chunk, rq.len);
+    const int n_blocks = (t_hi - t_lo + kBlock - 1) / kBlock;
+
+    // block i of the split into its ring slot; every block lies in one page.
+    // Page ids and columns are clamped, so a bad table gives wrong results and
+    // no stray access; rows past the request's end re-read its last one.
+    auto load_block = [&](int i) {
+        const int t = t_lo + i * kBlock;
+        const int col = min(t >> a.page_shift, a.bt_stride - 1);
+        const int page = min(max(scalar_load(a.block_table + (size_t)b * a.bt_stride + col), 0), a.num_pages - 1);
+        const E *base = (const E *)a.cache + (((size_t)page << a.page_shift) + (t & ((1 << a.page_shift) - 1))) * kDK;
+        const int lim = min(kBlock - 1, rq.len - 1 - t);
+        const unsigned dst = ring + (i & (kRing - 1)) * (kSlotElems * 2);
+        int ln = lane;  // opaque: the offsets are formed at each load, not kept in registers
+        asm volatile("" : "+v"(ln));
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const int r = 8 * wave + u;
+            global_to_lds16_at(base + (size_t)min(r, lim) * kDK, 16 * (ln ^ row_swizzle(r)), dst + r * (kDV * 2));
+        }
+        const int r = 8 * wave + (ln >> 3);
+        global_to_lds16_at(base, min(r, lim) * (kDK * 2) + 2 * (kDV + 8 * ((ln & 7) ^ rope_swizzle(r))),
+                           dst + 2 * kRopeElems + 1024 * wave);
+    };
+
+    // Q*: the B operand of S^T, whole rows in registers. Rows past the
+    // drafted tokens re-read the last one; their results are never stored.
+    E8 q[kDK / 16];
+    {
+        const E *src = (const E *)a.q + ((size_t)b * rows + min(row, live - 1)) * kDK + 8 * hl;
+#pragma unroll
+        for (int k = 0; k < kDK / 16; ++k)
+            q[k] = *(const E8 *)(src + 16 * k);
+    }
+    const unsigned long long mask = a.tree_mask[(size_t)b * a.drafts + min(row, live - 1) / a.num_heads];
+    for (int i = 0; i < min(kRing - 1, n_blocks); ++i)
+        load_block(i);
+
+    floatx16 o[kDV / 32];
+#pragma unroll
+    for (int c = 0; c < kDV / 32; ++c) {
+        o[c] = floatx16{};
+        in_accumulators(o[c]);
+    }
+    float m = -INFINITY, l = 0.0f;
+
+    // LDS addresses, less the slot's, of the lane's operands. A chunk's place
+    // differs from chunk 0's in the same row only by an XOR of its low four
+    // bits and an offset of the others, so one address each serves all chunks.
+    const int key = key_of_row(r32);
+    const unsigned k_lane = key * (kDV * 2) + 16 * (hl ^ row_swizzle(key));
+    const unsigned rope_lane = 2 * kRopeElems + key * (kRopeDim * 2) + 16 * (hl ^ rope_swizzle(key));
+    unsigned v_lane[2];  // the two transpose reads: 4 keys of one parity
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int j = lane & 15, r = 8 * hl + 2 * (j >> 2) + h;
+        v_lane[h] = r * (kDV * 2) + 16 * ((2 * ((lane >> 4) & 1) + ((j & 3) >> 1)) ^ row_swizzle(r)) + 8 * (j & 1);
+    }
+    for (int i = 0; i < n_blocks; ++i) {
+        if (i + 2 < n_blocks)
+            MLA_WAIT_VMCNT(2 * kUnitsPerWave);
+        else if (i + 1 < n_blocks)
+            MLA_WAIT_VMCNT(kUnitsPerWave);
+        else
+            MLA_WAIT_VMCNT(0);
+        lds_barrier();  // block i is there, and block i - 1's slot is free
+        if (i + kRing - 1 < n_blocks)
+            load_block(i + kRing - 1);
+        const unsigned blk = ring + (i & (kRing - 1)) * (kSlotElems * 2);
+
+        const unsigned k_at = blk + k_lane, rope_at = blk + rope_lane;
+        auto k_operand = [&](int k) -> E8 {  // values 16 k + 8 hl .. +7 of the lane's key
+            return k < kDV / 16 ? lds_load<E8>((k_at ^ (32 * (k & 7))) + 256 * (k >> 3))
+                                : lds_load<E8>(rope_at ^ (32 * (k - kDV / 16)));
+        };
+        floatx16 s = {};
+        {
+            E8 kv[2][4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                kv[0][j] = k_operand(j);
+#pragma unroll
+            for (int k = 0; k < kDK / 16; k += 4) {
+                if (k + 4 < kDK / 16) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        kv[(k / 4 + 1) & 1][j] = k_operand(k + 4 + j);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    s = mfma32x32x16(kv[(k / 4) & 1][j], q[k + j], s);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        const int t0 = t_lo + i * kBlock;
+        const bool edge = t0 + kBlock > context;  // holds drafted tokens, or the end
+        if (edge) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int t = t0 + key_of_reg(r, hl);
+                const unsigned bit = (unsigned)(mask >> ((t - context) & 63)) & 1u;
+                const unsigned seen = (unsigned)(t < context) | ((unsigned)(t < rq.len) & bit);
+                s[r] = seen ? s[r] : -INFINITY;
+            }
+        }
+        float most = s[0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r)
+            most = fmaxf(most, s[r]);
+        most = reduce_halves(most, [](float x, float y) { return fmaxf(x, y); }) * a.scale_log2;
+        // the reference moves only past kLazyRescale, so P is at most 2^8
+        if (__builtin_amdgcn_ballot_w64(most > m + kLazyRescale) != 0) {
+            const float next = most > m + kLazyRescale ? most : m;  // each row by itself
+            const float f = next == -INFINITY ? 1.0f : fast_exp2(m - next);
+            m = next;
+            l *= f;
+#pragma unroll
+            for (int c = 0; c < kDV / 32; ++c) {
+                in_accumulators(o[c]);
+                o[c] *= f;
+                in_accumulators(o[c]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        const float ref = m == -INFINITY ? 0.0f : m;
+        float p[16];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            p[r] = fast_exp2(s[r] * a.scale_log2 - ref);
+            l += p[r];
+        }
+        const E8 pb[2] = {p_operand<E>(p), p_operand<E>(p + 8)};
+        if (edge) {
+            // A drafted token that a row does not see meets it with weight 0:
+            // 0 times an infinity or NaN in its row would still be NaN, so
+            // those become 0 for the second product. A row that does see such
+            // a token has its sum l a NaN from the first product already.
+            lds_barrier();  // every wave has its logits
+            for (int u = threadIdx.x; u < kBlock * kDV / 8; u += 256) {
+                uint4 *at = (uint4 *)(s_ring + (i & (kRing - 1)) * kSlotElems + 8 * u);
+                uint4 v = *at;
+                unsigned *w = (unsigned *)&v;
+                bool bad = false;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    if (not_finite<E>((unsigned short)w[k])) {
+                        w[k] &= 0xffff0000u;
+                        bad = true;
+                    }
+                    if (not_finite<E>((unsigned short)(w[k] >> 16))) {
+                        w[k] &= 0xffffu;
+                        bad = true;
+                    }
+                }
+                if (bad)
+                    *at = v;
+            }
+            lds_barrier();
+        }
+        const unsigned v_at[2] = {blk + v_lane[0], blk + v_lane[1]};
+        auto v_operand = [&](int u) -> E8 {  // 32 columns of tile c, keys 16 ks .. +15 in the order of P's registers
+            const int ks = u / (kDV / 32), c = u % (kDV / 32);
+            E4 part[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                part[h] = lds_load_tr16<E>((v_at[h] ^ (64 * (c & 3))) + 256 * (c >> 2) + 16 * ks * (kDV * 2));
+            return E8{part[0][0], part[0][1], part[0][2], part[0][3], part[1][0], part[1][1], part[1][2], part[1][3]};
+        };
+        {
+            constexpr int kOps = 2 * kDV / 32;
+            E8 v[2][4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                v[0][j] = v_operand(j);
+#pragma unroll
+            for (int u = 0; u < kOps; u += 4) {
+                if (u + 4 < kOps) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        v[(u / 4 + 1) & 1][j] = v_operand(u + 4 + j);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    floatx16 &acc = o[(u + j) % (kDV / 32)];
+                    acc = mfma32x32x16(v[(u / 4) & 1][j], pb[u / (kDV / 32)], acc);
+                    in_accumulators(acc);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+    }
+
+#pragma unroll
+    for (int c = 0; c < kDV / 32; ++c)
+        in_accumulators(o[c]);
+    l = reduce_halves(l, [](float x, float y) { return x + y; });
+    if (rq.n_splits == 1) {
+        // a row that sees nothing has l = 0 and gives zeros
+        const float inv = l == 0.0f || row >= live ? 0.0f : 1.0f / l;
+        if (row < rows) {
+#pragma unroll
+            for (int c = 0; c < kDV / 32; ++c) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    E4 v;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        v[j] = row < live ? (E)(o[c][4 * k + j] * inv) : (E)0.0f;
+                    *(E4 *)(out + (size_t)row * kDV + 32 * c + 8 * k + 4 * hl) = v;
+                }
+            }
+        }
+        return;
+    }
+    const size_t tile = (size_t)slot * a.row_tiles + rt;
+    float *po = a.part_o + (tile * kWaves + wave) * (32 * kDV);
+#pragma unroll
+    for (int c = 0; c < kDV / 32; ++c)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            *(floatx4 *)(po + ((c * 4 + k) * 64 + lane) * 4) =
+                floatx4{o[c][4 * k], o[c][4 * k + 1], o[c][4 * k + 2], o[c][4 * k + 3]};
+    if (hl == 0) {
+        a.part_m[tile * kRows + 32 * wave + r32] = m;
+        a.part_l[tile * kRows + 32 * wave + r32] = l;
+    }
+}
+
+// Merges the splits of a request (those of more than one): a wave takes 32 rows x 32
+// columns, and a lane the 16 values it would hold in the split kernel.
+template <typename E>
+__global__ __launch_bounds__(256) void tree_combine_kernel(TreeArgs a)
+{
+    using E4 = typename Vec<E>::v4;
+    const int lane = threadIdx.x & 63;
+    const int item = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c = item & 15, w = (item >> 4) & 3, rest = item >> 6;
+    const int rt = rest % a.row_tiles, b = rest / a.row_tiles;
+    if (b >= a.batch)
+        return;
+    Request rq;
+    rq.read(a, b);
+    if (rq.n_splits == 1)
+        return;
+    const int rows = a.drafts * a.num_heads, live = rq.drafts * a.num_heads;
+    const int r32 = lane & 31, hl = lane >> 5;
+    const int row = rt * kRows + 32 * w + r32;
+    E *out = (E *)a.out + ((size_t)b * rows + row) * kDV + 32 * c + 4 * hl;
+    floatx4 acc[4] = {};
+    float m = -INFINITY, l = 0.0f;
+    if (rt * kRows < live) {
+        for (int s = 0; s < rq.n_splits; ++s)
+            m = fmaxf(m, a.part_m[((size_t)(rq.slot0 + s) * a.row_tiles + rt) * kRows + 32 * w + r32]);
+        const float ref = m == -INFINITY ? 0.0f : m;
+        for (int s = 0; s < rq.n_splits; ++s) {
+            const size_t tile = (size_t)(rq.slot0 + s) * a.row_tiles + rt;
+            const float f = fast_exp2(a.part_m[tile * kRows + 32 * w + r32] - ref);
+            l += f * a.part_l[tile * kRows + 32 * w + r32];
+            const float *po = a.part_o + (tile * kWaves + w) * (32 * kDV);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                acc[k] += f * *(const floatx4 *)(po + ((c * 4 + k) * 64 + lane) * 4);
+        }
+    }
+    if (row >= rows)
+        return;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        E4 v;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            v[j] = row < live ? (E)(acc[k][j] * inv) : (E)0.0f;
+        *(E4 *)(out + 8 * k) = v;
+    }
+}
+
+size_t align256(size_t n) { return (n + 255) / 256 * 256; }
+
+struct TreePlan {
+    int row_tiles, chunk, n_slots;
+    size_t o_bytes, ml_bytes;
+};
+
+// Splits: as many workgroups as CUs, no shorter than 4 blocks.
+TreePlan tree_plan(int batch, int drafts, int num_heads, int total_tokens, int num_splits, int cu_count)
+{
+    TreePlan p;
+    p.row_tiles = (drafts * num_heads + kRows - 1) / kRows;
+    const int longest = (total_tokens + batch - 1) / batch;  // mean
+    int splits = num_splits;
+    if (splits <= 0)
+        splits = std::max(1, std::min(cu_count / std::max(1, p.row_tiles * batch), longest / (4 * kBlock)));
+    int64_t chunk = (longest + splits - 1) / splits;
+    chunk = std::max<int64_t>(kBlock, (chunk + kBlock - 1) / kBlock * kBlock);
+    p.chunk = (int)chunk;
+    p.n_slots = total_tokens / p.chunk + batch;
+    const size_t tiles = (size_t)p.n_slots * p.row_tiles;
+    p.o_bytes = align256(tiles * kRows * kDV * sizeof(float));
+    p.ml_bytes = align256(tiles * kRows * sizeof(float));
+    return p;
+}
+
+bool tree_sizes_ok(int batch, int drafts, int num_heads, int total_tokens)
+{
+    return batch >= 1 && drafts >= 1 && drafts <= kMaxDrafts && num_heads > 0 && num_heads % 16 == 0 &&
+           num_heads <= 4096 && total_tokens >= 0 && total_tokens <= INT32_MAX - 4096;
+}
+
+template <typename E>
+void launch_tree(const TreeArgs &a, hipStream_t s)
+{
+    hipLaunchKernelGGL(tree_kernel<E>, dim3((a.n_slots + 7) / 8 * 8 * a.row_tiles), dim3(256), 0, s, a);
+    if (a.total_tokens > a.chunk)
+        hipLaunchKernelGGL(tree_combine_kernel<E>, dim3(a.batch * a.row_tiles * 16), dim3(256), 0, s, a);
+}
+
+int decode_tree(bool bf16, const void *query, const void *kv_cache, const int *block_table, const int *cu_seqlens,
+                const long long *tree_mask, const int *draft_lens, void *out, void *workspace, size_t workspace_bytes,
+                int batch, int drafts, int num_heads, int total_tokens, int page_size, int num_pages,
+                int block_table_stride, int num_splits, void *stream)
+{
+    if (!tree_sizes_ok(batch, drafts, num_heads, total_tokens) || !query || !kv_cache || !block_table || !cu_seqlens ||
+        !tree_mask || !out || !workspace || page_size < 32 || page_size > (1 << 20) ||
+        (page_size & (page_size - 1)) != 0 || num_pages < 1 || block_table_stride < 1)
+        return MLA_STATUS_INVALID_VALUE;
+    if (!aligned16(query) || !aligned16(kv_cache) || !aligned16(out) || !aligned16(workspace))
+        return MLA_STATUS_MISALIGNED;
+    const TreePlan p = tree_plan(batch, drafts, num_heads, total_tokens, num_splits, current_cu_count());
+    if ((int64_t)(p.n_slots + 7) * p.row_tiles > INT32_MAX / 256 || (int64_t)batch * p.row_tiles > INT32_MAX / 4096)
+        return MLA_STATUS_INVALID_VALUE;
+    if (workspace_bytes < p.o_bytes + 2 * p.ml_bytes)
+        return MLA_STATUS_WORKSPACE_TOO_SMALL;
+    TreeArgs a;
+    a.q = query;
+    a.cache = kv_cache;
+    a.block_table = block_table;
+    a.cu_seqlens = cu_seqlens;
+    a.tree_mask = reinterpret_cast<const unsigned long long *>(tree_mask);
+    a.draft_lens = draft_lens;
+    a.out = out;
+    char *ws = static_cast<char *>(workspace);
+    a.part_o = reinterpret_cast<float *>(ws);
+    a.part_m = reinterpret_cast<float *>(ws + p.o_bytes);
+    a.part_l = reinterpret_cast<float *>(ws + p.o_bytes + p.ml_bytes);
+    a.batch = batch;
+    a.drafts = drafts;
+    a.num_heads = num_heads;
+    a.total_tokens = total_tokens;
+    a.chunk = p.chunk;
+    a.row_tiles = p.row_tiles;
+    a.n_slots = p.n_slots;
+    a.page_shift = __builtin_ctz((unsigned)page_size);
+    a.num_pages = num_pages;
+    a.bt_stride = block_table_stride;
+    a.scale_log2 = (float)(1.4426950408889634 / std::sqrt(192.0));
+    if (bf16)
+        launch_tree<__bf16>(a, static_cast<hipStream_t>(stream));
+    else
+        launch_tree<_Float16>(a, static_cast<hipStream_t>(stream));
+    const hipError_t e = hipPeekAtLastError();
+    return e == hipSuccess ? MLA_STATUS_SUCCESS : record_hip_error(e);
+}
+
+}  // namespace
+}  // namespace mla
+
+extern "C" {
+
+size_t mla_decode_tree_workspace_size(int batch, int drafts, int num_heads, int total_tokens, int num_splits)
+{
+    if (!mla::tree_sizes_ok(batch, drafts, num_heads, total_tokens))
+        return 0;
+    const mla::TreePlan p = mla::tree_plan(batch, drafts, num_heads, total_tokens, num_splits, mla::current_cu_count());
+    return p.o_bytes + 2 * p.ml_bytes;
+}
+
+int mla_decode_tree_fp16(const void *query, const void *kv_cache, const int *block_table, const int *cu_seqlens,
+                         const long long *tree_mask, const int *draft_lens, void *out, void *workspace,
+                         size_t workspace_bytes, int batch, int drafts, int num_heads, int total_tokens, int page_size,
+                         int num_pages, int block_table_stride, int num_splits, void *stream)
+{
+    return mla::decode_tree(false, query, kv_cache, block_table, cu_seqlens, tree_mask, draft_lens, out, workspace,
+                            workspace_bytes, batch, drafts, num_heads, total_tokens, page_size, num_pages,
+                            block_table_stride, num_splits, stream);
+}
+
+int mla_decode_tree_bf16(const void *query, const void *kv_cache, const int *block_table, const int *cu_seqlens,
+                         const long long *tree_mask, const int *draft_lens, void *out, void *workspace,
+                         size_t workspace_bytes, int batch, int drafts, int num_heads, int total_tokens, int page_size,
+                         int num_pages, int block_table_stride, int num_splits, void *stream)
+{
+    return mla::decode_tree(true, query, kv_cache, block_table, cu_seqlens, tree_mask, draft_lens, out, workspace,
+                            workspace_bytes, batch, drafts, num_heads, total_tokens, page_size, num_pages,
+                            block_table_stride, num_splits, stream);
+}
+
+}  // extern "C"

@@ -75,8 +75,13 @@ extern "C" {
  * report the plan of the fp8-cache entry mla_decode_split_fp8 for these
  * sizes. Its cache streams half the bytes of a 16-bit one, so with few heads
  * and long sequences its plan can take more splits, or another head tile,
- * than the 16-bit plan. The decode entry points ignore it. */
+ * than the 16-bit plan. The decode entry points ignore it; mla_append_kv_*
+ * takes it for a cache of E4M3FN bytes. */
 #define MLA_FLAG_FP8_CACHE 16u
+
+/* mla_append_kv_*: the rotation's pairs are values i and i + 32, not 2 i and
+ * 2 i + 1. */
+#define MLA_FLAG_ROPE_HALVES 32u
 
 int mla_abi_version(void);
 const char *mla_status_string(int status);
@@ -333,6 +338,131 @@ int mla_project_output_bf16(const void *o_star, const void *w_uv,
                             const void *w_o, void *out, void *workspace,
                             size_t workspace_bytes, int batch, int num_heads,
                             int d_model, void *stream);
+
+/* Block table, slots and positions of one step's tokens, from the requests'
+ * lengths (no reference counterpart). All pointers are on the device and
+ * aligned to their type.
+ *
+ * Request b holds context_lens[b] tokens and gets new_lens[b] more (negative
+ * values count as 0; new_lens beyond total_new tokens in all are clipped).
+ * Its tokens' pages are columns 0, 1, .. of row b of block_table
+ * [batch][block_table_stride]; those of its context are read from there. Each
+ * page that the new tokens start takes the next id of free_pages [num_free],
+ * request after request from index *free_start on, and is written to the table.
+ *   cu_seqlens, cu_new [batch + 1]  prefix sums of the lengths with the new
+ *                                   tokens, and of the new tokens alone
+ *                                   (both stop at INT_MAX)
+ *   slots, positions [total_new]    of the new tokens, in request order: the
+ *                                   cache row page * page_size + offset, and
+ *                                   the position in its request
+ *   free_next                       *free_start + pages taken
+ * Entries past the last new token are slot -1, position 0. Where the free list
+ * or the table's columns end, or a context's page is negative, the token's slot
+ * is -1 (and a page that the list no longer has is written as -1); free_next
+ * then exceeds num_free by the pages missing. free_next must not be
+ * free_start. page_size is a power of two from 32 to 2^20. One launch. */
+int mla_paged_tables(const int *context_lens, const int *new_lens,
+                     const int *free_pages, const int *free_start,
+                     int *block_table, int *cu_seqlens, int *cu_new,
+                     long long *slots, int *positions, int *free_next,
+                     int batch, int total_new, int num_free, int page_size,
+                     int block_table_stride, void *stream);
+
+/* A step's latent rows into the cache, and its queries' rotary parts (no
+ * reference counterpart; the reference's cache comes ready made). Token t:
+ *   kv_cache[slots[t]][:512] = kv[t][:512] norm_weight / sqrt(mean(kv[t][:512]^2) + eps)
+ *   kv_cache[slots[t]][512:] = rotated kv[t][512:]
+ *   q_rope_out[t][h]         = rotated q_rope[t][h]
+ * computed in fp32 and rounded once. The rotation turns pair i (values 2 i and
+ * 2 i + 1, or i and i + 32 with MLA_FLAG_ROPE_HALVES) by the angle whose
+ * cosine and sine are cos_sin[positions[t]][i] and [32 + i] (fp32
+ * [num_positions][64]; positions are clamped to it). kv [tokens] rows of 576
+ * values, kv_stride values apart; q_rope [tokens][num_heads] rows of 64,
+ * q_token_stride and q_head_stride values apart (strides: multiples of 8),
+ * q_rope_out contiguous; num_heads 0: no queries, both NULL. kv_cache holds
+ * cache_rows rows of 576 values of the input's type, or with
+ * MLA_FLAG_FP8_CACHE of E4M3FN bytes of value / cache_scale (to nearest even,
+ * saturated at 448, NaN kept). Slots outside [0, cache_rows) are not written;
+ * two tokens with one slot leave a mix of both rows in it. One launch. */
+int mla_append_kv_fp16(const void *kv, const void *norm_weight,
+                       const float *cos_sin, const int *positions,
+                       const long long *slots, const void *q_rope,
+                       void *kv_cache, void *q_rope_out, float eps,
+                       float cache_scale, int tokens, int num_heads,
+                       int num_positions, long long cache_rows,
+                       long long kv_stride, long long q_token_stride,
+                       long long q_head_stride, unsigned flags, void *stream);
+int mla_append_kv_bf16(const void *kv, const void *norm_weight,
+                       const float *cos_sin, const int *positions,
+                       const long long *slots, const void *q_rope,
+                       void *kv_cache, void *q_rope_out, float eps,
+                       float cache_scale, int tokens, int num_heads,
+                       int num_positions, long long cache_rows,
+                       long long kv_stride, long long q_token_stride,
+                       long long q_head_stride, unsigned flags, void *stream);
+
+/* Decode of a tree of drafted tokens a request, over the paged cache (no
+ * reference counterpart: the reference decodes one token). kv_cache,
+ * block_table, cu_seqlens, page_size, total_tokens as for mla_decode_paged_*;
+ * a request's drafted tokens are the last draft_lens[b] ones of its cache
+ * (draft_lens [batch], clamped to [0, drafts]; NULL: drafts for every request),
+ * already written. query [batch x drafts x num_heads x 576] -> out [batch x
+ * drafts x num_heads x 512]. Drafted token i sees the request's whole context
+ * and drafted token j where bit j of tree_mask[b][i] ([batch x drafts]) is set:
+ * its ancestors and itself, or, with masks 2^(i+1) - 1, a plain chain. A row
+ * that sees nothing, and the rows from draft_lens[b] on, are zeros. Infinities
+ * and NaN in a drafted token's row reach only the rows that see it (NaN there). drafts
+ * is at most 64. num_splits <= 0 picks the splits of each request's tokens. */
+size_t mla_decode_tree_workspace_size(int batch, int drafts, int num_heads,
+                                      int total_tokens, int num_splits);
+int mla_decode_tree_fp16(const void *query, const void *kv_cache,
+                         const int *block_table, const int *cu_seqlens,
+                         const long long *tree_mask, const int *draft_lens,
+                         void *out, void *workspace, size_t workspace_bytes,
+                         int batch, int drafts, int num_heads,
+                         int total_tokens, int page_size, int num_pages,
+                         int block_table_stride, int num_splits, void *stream);
+int mla_decode_tree_bf16(const void *query, const void *kv_cache,
+                         const int *block_table, const int *cu_seqlens,
+                         const long long *tree_mask, const int *draft_lens,
+                         void *out, void *workspace, size_t workspace_bytes,
+                         int batch, int drafts, int num_heads,
+                         int total_tokens, int page_size, int num_pages,
+                         int block_table_stride, int num_splits, void *stream);
+
+/* Causal attention of prompts, or chunks of prompts, in the expanded form (no
+ * reference code; the math is README.md:64-85): with c_t, r_t the 512 latent
+ * and 64 rotary values of cache row t,
+ *   k[t][h] = [w_uk[h] c_t, r_t], v[t][h] = w_uv[h] c_t,
+ *   out[i][h] = softmax_t( [q_nope, q_rope][i][h] . k[t][h] / sqrt(192) ) v[t][h].
+ * Request b has the queries cu_q[b] .. cu_q[b + 1] - 1 of q_nope [queries x
+ * num_heads x 128], q_rope [queries x num_heads x 64] and out [queries x
+ * num_heads x 128], and the keys of its cache, cu_seqlens as for
+ * mla_decode_split_batched_*; its queries are the last of its keys, and each
+ * sees the keys up to its own position (zeros where there is none). kv_cache
+ * is paged as for mla_decode_paged_*, or packed [total_tokens x 576] where
+ * block_table is NULL (the page arguments are then ignored). Both prefix sums
+ * start at 0 and are clamped to [0, queries] and [0, total_tokens]; rows of out
+ * behind the last request's are zeros. w_uk, w_uv as for
+ * mla_absorb_query_* / mla_project_output_*. K and V are rounded to the
+ * inputs' type; a query that sees a key whose V is not finite gives NaN, and
+ * what it does not see never reaches it. The workspace holds K and V: 512
+ * bytes a key and head. Two launches. */
+size_t mla_prefill_workspace_size(int batch, int num_heads, int total_tokens);
+int mla_prefill_fp16(const void *q_nope, const void *q_rope, const void *w_uk,
+                     const void *w_uv, const void *kv_cache,
+                     const int *block_table, const int *cu_q,
+                     const int *cu_seqlens, void *out, void *workspace,
+                     size_t workspace_bytes, int batch, int num_heads,
+                     int queries, int total_tokens, int page_size,
+                     int num_pages, int block_table_stride, void *stream);
+int mla_prefill_bf16(const void *q_nope, const void *q_rope, const void *w_uk,
+                     const void *w_uv, const void *kv_cache,
+                     const int *block_table, const int *cu_q,
+                     const int *cu_seqlens, void *out, void *workspace,
+                     size_t workspace_bytes, int batch, int num_heads,
+                     int queries, int total_tokens, int page_size,
+                     int num_pages, int block_table_stride, void *stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,203 @@
+"""Causal attention of prompts in the expanded form (mla_prefill) against
+float64. Tolerances: operators_reference."""
+import random
+
+import pytest
+import torch
+
+import ada_mla
+from ada_mla import capi
+from operators_reference import attention_check, gather_paged, half_step, paged_case
+
+pytestmark = pytest.mark.gpu
+
+
+def _inputs(gen, queries, heads, dtype):
+    qn = torch.randn(max(1, queries), heads, 128, generator=gen).to(dtype).cuda()
+    qr = torch.randn(max(1, queries), heads, 64, generator=gen).to(dtype).cuda()
+    uk, uv = ((torch.randn(heads, 128, 512, generator=gen) * 512 ** -0.5).to(dtype).cuda() for _ in range(2))
+    return qn, qr, uk, uv
+
+
+def _cu(lengths):
+    cu = [0]
+    for n in lengths:
+        cu.append(cu[-1] + n)
+    return torch.tensor(cu, dtype=torch.int32, device="cuda")
+
+
+def _check(got, qn, qr, uk, uv, rows, queries, lengths, dtype, what):
+    se = sn = 0.0
+    at = 0
+    uk, uv, got = uk.double().cpu(), uv.double().cpu(), got.cpu()
+    for b, (m, n) in enumerate(zip(queries, lengths)):
+        c = rows(b)
+        seen = torch.arange(n)[None] <= torch.arange(m)[:, None] + n - m
+        for h in range(uk.shape[0]):
+            k = torch.cat([c[:, :512] @ uk[h].T, c[:, 512:]], 1)
+            q = torch.cat([qn[at:at + m, h], qr[at:at + m, h]], 1).double().cpu()
+            e = attention_check(got[at:at + m, h], q, k, c[:, :512] @ uv[h].T, seen, dtype, rounded_kv=True,
+                                what=f"{what} request {b} head {h}")
+            se, sn = se + e[0], sn + e[1]
+        at += m
+    if sn:
+        assert (se / sn) ** 0.5 <= 2 * half_step(dtype), f"{what}: 2-norm {(se / sn) ** 0.5:.2e}"
+
+
+def _run(queries, context, heads, dtype, page, seed):
+    rng = random.Random(seed)
+    gen = torch.Generator()
+    gen.manual_seed(seed)
+    lengths = [q + c for q, c in zip(queries, context)]
+    qn, qr, uk, uv = _inputs(gen, sum(queries), heads, dtype)
+    cu_q, cu = _cu(queries), _cu(lengths)
+    if page:
+        cache, table, _ = paged_case(gen, rng, lengths, page, dtype)
+        rows = lambda b: gather_paged(cache, table[b], lengths[b])  # noqa: E731
+    else:
+        cache, table = torch.randn(max(1, sum(lengths)), 576, generator=gen).to(dtype).cuda(), None
+        rows = lambda b: cache[int(cu[b]):int(cu[b + 1])].double().cpu()  # noqa: E731
+    got = ada_mla.mla_prefill(qn, qr, uk, uv, cache, cu_q, cu, block_table=table, total_tokens=sum(lengths))
+    torch.cuda.synchronize()
+    _check(got, qn, qr, uk, uv, rows, queries, lengths, dtype, f"{queries} {context} heads {heads} page {page}")
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("page", [0, 32, 256])
+def test_lengths_at_edges(page, dtype):
+    _run([1, 2, 31, 32, 33, 63, 64, 65, 127, 128, 129, 200], [0] * 12, 16, dtype, page, seed=page)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("page", [0, 64])
+def test_chunks_behind_a_context(page, dtype):
+    _run([1, 40, 128, 7, 150], [300, 64, 1, 0, 129], 16, dtype, page, seed=page + 1)
+
+
+@pytest.mark.parametrize("heads", [16, 48, 128])
+def test_heads(heads):
+    _run([70, 3], [0, 66], heads, torch.float16, 32, seed=heads)
+
+
+def test_long_prompt():
+    _run([1500], [0], 16, torch.bfloat16, 64, seed=2)
+    _run([300], [2200], 16, torch.float16, 0, seed=3)
+
+
+def test_many_requests():
+    rng = random.Random(4)
+    queries = [rng.randint(0, 40) for _ in range(130)]
+    _run(queries, [rng.randint(0, 30) for _ in queries], 16, torch.float16, 32, seed=4)
+
+
+def test_requests_without_queries_or_keys():
+    _run([0, 5, 0, 9], [20, 0, 0, 3], 16, torch.float16, 0, seed=5)
+
+
+def test_more_queries_than_keys():
+    # the first queries stand before the first key and see nothing
+    gen = torch.Generator()
+    gen.manual_seed(6)
+    qn, qr, uk, uv = _inputs(gen, 150, 16, torch.float16)
+    cache = torch.randn(10, 576, generator=gen).half().cuda()
+    got = ada_mla.mla_prefill(qn, qr, uk, uv, cache, _cu([150]), _cu([10]))
+    _check(got, qn, qr, uk, uv, lambda b: cache.double().cpu(), [150], [10], torch.float16, "early queries")
+    got = ada_mla.mla_prefill(qn, qr, uk, uv, cache[:0], _cu([150]), _cu([0]))
+    assert not got.any()
+
+
+def test_rows_behind_the_last_request_are_zero():
+    gen = torch.Generator()
+    gen.manual_seed(7)
+    for total in (130, 300):
+        qn, qr, uk, uv = _inputs(gen, total, 16, torch.float16)
+        cache = torch.randn(100, 576, generator=gen).half().cuda()
+        cu = _cu([60, 40])
+        out = torch.full((total, 16, 128), float("nan"), dtype=torch.float16, device="cuda")
+        got = capi.prefill(qn, qr, uk, uv, cache, cu, cu, 100, out=out)
+        assert torch.isfinite(got).all() and not got[100:].any()
+        _check(got[:100], qn, qr, uk, uv, lambda b: cache[int(cu[b]):int(cu[b + 1])].double().cpu(), [60, 40], [60, 40],
+               torch.float16, "padded")
+
+
+@pytest.mark.parametrize("value", [float("inf"), float("nan")])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_a_key_that_is_not_finite_reaches_only_who_sees_it(value, dtype):
+    gen = torch.Generator()
+    gen.manual_seed(8)
+    qn, qr, uk, uv = _inputs(gen, 200, 16, dtype)
+    cache = torch.randn(200, 576, generator=gen).to(dtype).cuda()
+    cu = _cu([200])
+    want = ada_mla.mla_prefill(qn, qr, uk, uv, cache, cu, cu)
+    for t in (37, 64, 130):
+        bad = cache.clone()
+        bad[t, 9] = value
+        got = ada_mla.mla_prefill(qn, qr, uk, uv, bad, cu, cu)
+        assert torch.equal(got[:t], want[:t])
+        assert torch.isnan(got[t:]).all()
+
+
+def test_a_value_that_overflows_fp16():
+    # finite keys whose values pass 65504: NaN for who sees them, nothing for the others
+    gen = torch.Generator()
+    gen.manual_seed(9)
+    qn, qr, uk, uv = _inputs(gen, 100, 16, torch.float16)
+    uk = torch.zeros_like(uk)
+    cache = torch.randn(100, 576, generator=gen).half().cuda()
+    cache[50, :512] = 60000.0 * (uv[3, 17].sign() + (uv[3, 17] == 0))
+    cu = _cu([100])
+    got = ada_mla.mla_prefill(qn, qr, uk, uv, cache, cu, cu)
+    assert torch.isfinite(got[:50]).all() and torch.isnan(got[50:, 3]).all()
+
+
+def test_workspace_of_nans():
+    gen = torch.Generator()
+    gen.manual_seed(10)
+    lib = capi.load()
+    ws = torch.full((lib.mla_prefill_workspace_size(4, 16, 500),), 255, dtype=torch.uint8, device="cuda")
+    for lengths in ([100, 3, 64, 65], [1, 1, 1, 1], [0, 200, 0, 31]):
+        qn, qr, uk, uv = _inputs(gen, sum(lengths), 16, torch.float16)
+        cache = torch.randn(sum(lengths), 576, generator=gen).half().cuda()
+        cu = _cu(lengths)
+        got = capi.prefill(qn, qr, uk, uv, cache, cu, cu, sum(lengths), workspace=ws)
+        _check(got, qn, qr, uk, uv, lambda b: cache[int(cu[b]):int(cu[b + 1])].double().cpu(), lengths, lengths,
+               torch.float16, f"{lengths}")
+
+
+def test_captured_and_replayed():
+    gen = torch.Generator()
+    gen.manual_seed(11)
+    qn, qr, uk, uv = _inputs(gen, 200, 16, torch.float16)
+    cache = torch.randn(300, 576, generator=gen).half().cuda()
+    cu_q, cu = _cu([150, 50]), _cu([150, 150])
+    call = lambda: ada_mla.mla_prefill(qn, qr, uk, uv, cache, cu_q, cu, total_tokens=300)  # noqa: E731
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for r in range(4):
+        qn.normal_()
+        cache.normal_()
+        cu_q[1:].sub_(10)
+        want = call().clone()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.isfinite(want).all() and torch.equal(out, want), r
+
+
+def test_agrees_with_the_absorbed_form():
+    # a prompt's last query, expanded, against the decode with the absorbed query and W_UV behind it
+    gen = torch.Generator()
+    gen.manual_seed(12)
+    qn, qr, uk, uv = _inputs(gen, 90, 16, torch.float16)
+    cache = torch.randn(90, 576, generator=gen).half().cuda()
+    cu = _cu([90])
+    expanded = ada_mla.mla_prefill(qn, qr, uk, uv, cache, cu, cu)[-1].double().cpu()
+    q = ada_mla.mla_absorb_query(qn[-1:].contiguous(), qr[-1:].contiguous(), uk)
+    o = ada_mla.mla_decode_split(q[0], cache).double().cpu()
+    absorbed = (uv.double().cpu() @ o[:, :, None])[:, :, 0]
+    # norms: 2 u for the expanded form; the absorbed one rounds q*, p, its partials and o*: below 2 u again
+    err = (expanded - absorbed).norm() / absorbed.norm()
+    assert err <= 4 * half_step(torch.float16), err
