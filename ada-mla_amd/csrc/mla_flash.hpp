@@ -48,21 +48,21 @@ __device__ __forceinline__ float reduce_halves(float v, F f)
     return f(__uint_as_float(a[0]), __uint_as_float(a[1]));
 }
 
-// The key of a 32-key block that sits in row rho of the S^T tile:
-// rho = 16 a + 8 b + 4 c + j is key 16 a + 8 c + 2 j + b. Lane half c then
-// holds keys 16 a + 8 c + {0, 2, 4, 6} in registers 8 a .. 8 a + 3 and
-// {1, 3, 5, 7} in 8 a + 4 .. 8 a + 7, so that each of the two transpose reads
-// of V^T that match a P operand takes four keys of one parity, which the row
-// swizzle (chunk c of row r at c ^ (r mod 16)) serves without bank conflicts.
-__device__ __forceinline__ int key_of_row(int rho)
-{
-    return (rho & 16) + ((rho & 4) << 1) + 2 * (rho & 3) + ((rho >> 3) & 1);
-}
-
-// The key (within its 32-key block) in register i of a lane of half hl.
+// The key (within its 32-key block) in register i of a lane of half hl: that
+// register's row of the D tile.
 __device__ __forceinline__ int key_of_reg(int i, int hl)
 {
-    return (i & 8) * 2 + 8 * hl + 2 * (i & 3) + ((i >> 2) & 1);
+    return 8 * (i >> 2) + 4 * hl + (i & 3);
+}
+
+// Keys in LDS, rows of at least 256 bytes: 16-byte chunk c of row r sits at c
+// ^ key_swizzle(r). Both reads are then free of bank conflicts: a product's row
+// reads take 16 lanes, one chunk of 16 rows in a row, at a time, and all 16 places
+// differ; a transpose read takes 32 lanes, 4 chunks of 4 rows in a row, and those 4
+// rows differ in the upper two bits of their place.
+__device__ __forceinline__ int key_swizzle(int r)
+{
+    return 4 * (r & 3) + ((r >> 2) & 3);
 }
 
 // P's registers 8 a .. 8 a + 7, rounded to the type of V: the B operand of keys 16 a ..

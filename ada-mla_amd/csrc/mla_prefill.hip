@@ -25,6 +25,9 @@ namespace {
 
 constexpr int kNope = 128, kRopeDim = 64, kLatent = 512;
 constexpr int kTile = 64;      // keys per tile; sequences are padded to it in the workspace
+typedef unsigned long long ulong4x __attribute__((ext_vector_type(4)));
+typedef unsigned uint4x __attribute__((ext_vector_type(4)));
+typedef unsigned short ushort2x __attribute__((ext_vector_type(2)));
 constexpr int kQueries = 128;  // queries per workgroup: 32 a wave
 
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -36,10 +39,11 @@ struct PrefillArgs {
     void *out;
     void *k, *v;                // [head][padded key][128]
     void *rope;                 // [padded key][64]
-    unsigned long long *flags;  // [head][tile][2]: keys whose V holds an infinity or NaN, by half of its columns
+    unsigned long long *flags;  // [head][tile][4]: keys whose V holds an infinity or NaN, by 32 of its columns
     int batch, num_heads, queries, total_tokens;
     int padded;  // keys of the workspace: whole tiles
     int q_slots;
+    int group_blocks;  // weight blocks of an expanding workgroup
     int page_shift, num_pages, bt_stride;
     float scale_log2;
 };
@@ -65,149 +69,228 @@ __device__ __forceinline__ int owner_of_slot(const int *cu, int batch, int most,
 }
 
 // ---- expansion --------------------------------------------------------------
-// One workgroup (4 waves): 128 keys x the 128 columns of K or of V of one head,
-// k = 512 in steps of 64. Rows of 128 bytes in LDS, 16-byte chunk c of row r
-// at c ^ (r mod 8).
-constexpr int kStep = 64;
-constexpr int kStepElems = 128 * kStep;  // of one operand
+// A product of [keys x 512] latents with [512 x 256 heads] weights, whose depth
+// is short: with both operands streamed, a workgroup would spend as long on its
+// first loads and its stores as on the product. So the keys stay: a wave keeps
+// 64 of them (one tile of the workspace) whole in registers, 256 a workgroup,
+// and the weights stream past in blocks of 32 rows through an LDS ring, each
+// block read once for 256 keys (two products a LDS read). With the weights as
+// the A operand a lane owns a key and, with the rows of a block read in the
+// order of weight_row, 16 adjacent columns of it: two 16-byte stores.
+constexpr int kWeightRows = 32;                       // rows of W a block
+constexpr int kWeightElems = kWeightRows * kLatent;   // 32 KB
+constexpr int kWeightRing = 4;
+constexpr int kExpandTiles = 4;                       // key tiles a workgroup: one a wave
+constexpr int kBlocksPerSide = kNope / kWeightRows;   // blocks of one head's W_UK or W_UV
+
+// The row of a weight block in row rho = 8 q + 4 c + j of the product's tile:
+// lane half c then holds columns 16 c .. 16 c + 15 in register order.
+__device__ __forceinline__ int weight_row(int rho)
+{
+    return 16 * ((rho >> 2) & 1) + 4 * (rho >> 3) + (rho & 3);
+}
+
+// 16-byte chunk c of row r sits at c ^ weight_swizzle(r): rho mod 16, so that
+// 16 lanes that read one chunk of 16 successive rho meet 16 places.
+__device__ __forceinline__ int weight_swizzle(int r)
+{
+    return 8 * ((r >> 2) & 1) + 4 * (r >> 4) + (r & 3);
+}
 
 template <typename E>
-__global__ __launch_bounds__(256) void expand_kernel(PrefillArgs a)
+__global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_per_eu(1, 1))) void
+expand_kernel(PrefillArgs a)
 {
     using E8 = typename Vec<E>::v8;
-    using E4 = typename Vec<E>::v4;
-    __shared__ __attribute__((aligned(1024))) E s_buf[2][2][kStepElems];  // [stage][keys, weights]
+    __shared__ __attribute__((aligned(1024))) E s_ring[kWeightRing * kWeightElems];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r32 = lane & 31, hl = lane >> 5;
-    // workgroup -> (head and side, key tile pair): an XCD takes one head's side
-    // through all keys, so that its weights stay in that L2
-    const int pairs = (a.padded / kTile + 1) / 2;
-    const int hs = (blockIdx.x >> 3) / pairs * 8 + (blockIdx.x & 7);
-    const int pair = (blockIdx.x >> 3) % pairs;
-    const int h = hs >> 1, side = hs & 1;
-    if (h >= a.num_heads)
+    // workgroup -> (group of weight blocks, four key tiles): the key tiles of a
+    // group get ids that differ by 8, one XCD, whose L2 then holds the group's weights
+    const int tiles = a.padded / kTile, quads = (tiles + kExpandTiles - 1) / kExpandTiles;
+    const int group = (blockIdx.x >> 3) / quads * 8 + (blockIdx.x & 7);
+    const int tile = (blockIdx.x >> 3) % quads * kExpandTiles + wave;
+    const int n_blocks = 2 * kBlocksPerSide * a.num_heads;
+    const int blk0 = group * a.group_blocks, blk1 = min(blk0 + a.group_blocks, n_blocks);
+    if (blk0 >= n_blocks)
         return;
 
-    // the two tiles' sequences
-    int seq[2], seq_lo[2], len[2], t0[2];
-    bool any = false;
+    // block i: rows 32 (i mod 4) .. of side (i / 4) mod 2 of head i / 8
+    const unsigned ring = lds_address(s_ring);
+    auto load_block = [&](int i) {
+        const int h = i / (2 * kBlocksPerSide), rest = i % (2 * kBlocksPerSide);
+        const E *w = (const E *)(rest >= kBlocksPerSide ? a.w_uv : a.w_uk) +
+                     ((size_t)h * kNope + rest % kBlocksPerSide * kWeightRows) * kLatent;
+        const unsigned dst = ring + ((i - blk0) & (kWeightRing - 1)) * (kWeightElems * 2);
+        int ln = lane;
+        asm volatile("" : "+v"(ln));
 #pragma unroll
-    for (int g = 0; g < 2; ++g) {
-        const int tile = 2 * pair + g;
-        const int b = owner_of_slot(a.cu_seqlens, a.batch, a.total_tokens, kTile, tile, lane);
-        seq[g] = b;
-        seq_lo[g] = clamped(a.cu_seqlens, b, a.total_tokens);
-        len[g] = max(clamped(a.cu_seqlens, b + 1, a.total_tokens), seq_lo[g]) - seq_lo[g];
-        t0[g] = (tile - seq_lo[g] / kTile - b) * kTile;  // the tile's first key within its sequence
-        if (tile * kTile >= a.padded)
-            len[g] = 0;
-        any |= t0[g] < len[g];
-    }
-    if (!any)
+        for (int u = 0; u < kWeightRows / 4; ++u) {
+            const int r = kWeightRows / 4 * wave + u;
+            global_to_lds16_at(w + (size_t)r * kLatent, 16 * (ln ^ weight_swizzle(r)), dst + r * (kLatent * 2));
+        }
+    };
+    // The wave's keys: latent rows of 1 KB by direct loads into the wave's own
+    // ring slot, 32 at a time, then into registers (chunk c of row r at c ^ (r
+    // mod 16)). Loaded into registers at once, every load touched 32 rows: 18 us
+    // a workgroup with all CUs loading. Rows past the sequence are zeros.
+    const int b = owner_of_slot(a.cu_seqlens, a.batch, a.total_tokens, kTile, tile, lane);
+    const int seq_lo = clamped(a.cu_seqlens, b, a.total_tokens);
+    const int len = max(clamped(a.cu_seqlens, b + 1, a.total_tokens), seq_lo) - seq_lo;
+    const int t0 = (tile - seq_lo / kTile - b) * kTile;
+    const bool live = tile < tiles && t0 < len;  // else nobody reads this tile
+    if (!__syncthreads_or(live))
         return;
-    auto key_source = [&](int r) -> const E * {  // latent row of the pair's key r; keys past a sequence re-read a real one
-        const int g = r >> 6;
-        const int b = g ? seq[1] : seq[0], lo = g ? seq_lo[1] : seq_lo[0], n = g ? len[1] : len[0];
-        const int t = max(min((g ? t0[1] : t0[0]) + (r & 63), n - 1), 0);
+    auto block_source = [&](int t) -> const E * {  // latent row t of the sequence; the 32 rows of a block follow it
         size_t row;
         if (a.block_table) {
             const int col = min(t >> a.page_shift, a.bt_stride - 1);
-            const int page = min(max(a.block_table[(size_t)b * a.bt_stride + col], 0), a.num_pages - 1);
+            const int page = min(max(scalar_load(a.block_table + (size_t)b * a.bt_stride + col), 0), a.num_pages - 1);
             row = ((size_t)page << a.page_shift) + (t & ((1 << a.page_shift) - 1));
         } else {
-            row = min(lo + t, a.total_tokens - 1);
+            row = seq_lo + t;
         }
         return (const E *)a.cache + row * kDK;
     };
-    const E *w = (const E *)(side ? a.w_uv : a.w_uk) + (size_t)h * kNope * kLatent;
-    const E *src[8];  // the lane's place in the wave's 8 load units of 8 rows: 4 of keys, 4 of weights
+    E8 key[2][kLatent / 16];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-        const int r = 32 * wave + 8 * u + (lane >> 3);
-        const int c = (lane & 7) ^ (r & 7);
-        src[u] = key_source(r) + 8 * c;
-        src[4 + u] = w + (size_t)r * kLatent + 8 * c;
-    }
-    const unsigned lds = lds_address(s_buf);
-    auto load_step = [&](int s) {
-        const unsigned at = lds + (s & 1) * (4 * kStepElems) + 32 * wave * (kStep * 2);
+    for (int g = 0; g < 2; ++g) {
+        const int t = t0 + 32 * g;
+        if (live && t < len) {
+            const E *src = block_source(t);
+            const int lim = min(31, len - 1 - t);
+            const unsigned own = ring + wave * (kWeightElems * 2);
 #pragma unroll
-        for (int u = 0; u < 8; ++u)
-            gather_to_lds16(src[u] + s * kStep, at + (u >> 2) * (2 * kStepElems) + (u & 3) * 1024);
-    };
-    load_step(0);
-    if (hs == 0) {  // the rotary parts: 8 chunks a key
-        for (int i = threadIdx.x; i < 128 * 8; i += 256) {
-            const int r = i >> 3, p = 2 * pair * kTile + r;
-            if (p < a.padded)
-                *(uint4 *)((E *)a.rope + (size_t)p * kRopeDim + 8 * (i & 7)) =
-                    *(const uint4 *)(key_source(r) + kLatent + 8 * (i & 7));
-        }
-    }
-    // wave (i, j): columns 64 i .. +63 of the head's 128, keys 64 j .. +63
-    const int wi = wave >> 1, wj = wave & 1;
-    floatx16 acc[2][2] = {};
-    for (int s = 0; s < kLatent / kStep; ++s) {
-        MLA_WAIT_VMCNT(0);
-        lds_barrier();
-        if (s + 1 < kLatent / kStep)
-            load_step(s + 1);
-        const unsigned at = lds + (s & 1) * (4 * kStepElems);
-        auto operand = [&](unsigned base, int r, int k) -> E8 {
-            return lds_load<E8>(base + r * (kStep * 2) + 16 * ((2 * k + hl) ^ (r & 7)));
-        };
+            for (int r = 0; r < 32; ++r)
+                global_to_lds16_at(src + (size_t)min(r, lim) * kDK, 16 * (lane ^ row_swizzle(r)), own + r * (kLatent * 2));
+            if (group == 0) {  // the rotary parts: 8 chunks a key
 #pragma unroll
-        for (int k = 0; k < kStep / 16; ++k) {
-            E8 wv[2], cv[2];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                wv[i] = operand(at + 2 * kStepElems, 64 * wi + 32 * i + r32, k);
-                cv[i] = operand(at, 64 * wj + 32 * i + r32, k);
-            }
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-                    acc[i][j] = mfma32x32x16(wv[i], cv[j], acc[i][j]);
-        }
-    }
-    // lane: key 32 j + r32 of the wave's 64, columns 32 i + 8 k + 4 hl .. +3
-    const int tile = 2 * pair + wj;
-    const int t_first = wj ? t0[1] : t0[0], n = wj ? len[1] : len[0];
-    if (t_first >= n)
-        return;
-    E *dst = (E *)(side ? a.v : a.k) + ((size_t)h * a.padded + (size_t)tile * kTile) * kNope + 64 * wi + 4 * hl;
-    unsigned long long bad = 0;
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const bool real = t_first + 32 * j + r32 < n;  // keys past the sequence hold zeros
-        bool lane_bad = false;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                E4 v;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    // V: what is not finite becomes 0 and flags its key, so
-                    // that a query that must not see the key can meet it with
-                    // weight 0
-                    E x = real ? (E)acc[i][j][4 * k + e] : (E)0.0f;
-                    if (side && not_finite<E>(__builtin_bit_cast(unsigned short, x))) {
-                        x = (E)0.0f;
-                        lane_bad = true;
-                    }
-                    v[e] = x;
+                for (int u = 0; u < 4; ++u) {
+                    const int r = 8 * u + (lane >> 3);
+                    *(uint4 *)((E *)a.rope + ((size_t)tile * kTile + 32 * g + r) * kRopeDim + 8 * (lane & 7)) =
+                        *(const uint4 *)(src + (size_t)min(r, lim) * kDK + kLatent + 8 * (lane & 7));
                 }
-                *(E4 *)(dst + (size_t)(32 * j + r32) * kNope + 32 * i + 8 * k) = v;
             }
+            MLA_WAIT_VMCNT(0);
+            asm volatile("" ::: "memory");
+            const unsigned at = own + r32 * (kLatent * 2) + 16 * (hl ^ row_swizzle(r32));
+            const bool real = r32 <= lim;
+#pragma unroll
+            for (int k = 0; k < kLatent / 16; ++k) {
+                const uint4x v = lds_load<uint4x>((at ^ (32 * (k & 7))) + 256 * (k >> 3));
+                key[g][k] = __builtin_bit_cast(E8, real ? v : uint4x{0, 0, 0, 0});
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        } else {
+#pragma unroll
+            for (int k = 0; k < kLatent / 16; ++k)
+                key[g][k] = E8{};
         }
-        const unsigned long long m = __builtin_amdgcn_ballot_w64(lane_bad);
-        bad |= (unsigned long long)((unsigned)m | (unsigned)(m >> 32)) << (32 * j);
     }
-    if (side && lane == 0)
-        a.flags[((size_t)h * (a.padded / kTile) + tile) * 2 + wi] = bad;
+    lds_barrier();  // the ring is free
+    for (int i = blk0; i < min(blk0 + kWeightRing - 1, blk1); ++i)
+        load_block(i);
+
+    const int row = weight_row(r32);
+    const unsigned w_lane = row * (kLatent * 2) + 16 * (hl ^ weight_swizzle(row));
+    unsigned long long bad = 0;  // the tile's keys whose V is not finite, in the block of `store`
+    floatx16 prev[2];            // the block before: rounded and stored between this one's products
+    // Rounds and stores quarter `part` of key group g of block i.
+    auto store = [&](int i, int g, int part, unsigned &top, E8 (&v)[2]) {
+#pragma unroll
+        for (int r = 4 * part; r < 4 * part + 4; ++r)
+            v[r >> 3][r & 7] = (E)prev[g][r];
+        const auto w = __builtin_bit_cast(uint4x, v[part >> 1]);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {  // the largest magnitude's bits, both halves
+            const unsigned x = w[2 * (part & 1) + k] & 0x7fff7fffu;
+            top = __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(ushort2x, top),
+                                                                         __builtin_bit_cast(ushort2x, x)));
+        }
+        if (part != 3)
+            return;
+        const int h = i / (2 * kBlocksPerSide), rest = i % (2 * kBlocksPerSide);
+        const bool side = rest >= kBlocksPerSide;
+        const bool lane_bad = not_finite<E>((unsigned short)top) || not_finite<E>((unsigned short)(top >> 16));
+        const unsigned long long m = __builtin_amdgcn_ballot_w64(side && lane_bad);
+        if (m != 0) {
+            // V: what is not finite becomes 0 and flags its key, so that a
+            // query that must not see the key can meet it with weight 0
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const E x = v[r >> 3][r & 7];
+                v[r >> 3][r & 7] = not_finite<E>(__builtin_bit_cast(unsigned short, x)) ? (E)0.0f : x;
+            }
+            bad |= (unsigned long long)((unsigned)m | (unsigned)(m >> 32)) << (32 * g);
+        }
+        E *dst = (E *)(side ? a.v : a.k) + ((size_t)h * a.padded + (size_t)tile * kTile + 32 * g + r32) * kNope +
+                 rest % kBlocksPerSide * kWeightRows + 16 * hl;
+        *(E8 *)dst = v[0];
+        *(E8 *)(dst + 8) = v[1];
+        if (side && g == 1) {
+            if (lane == 0)
+                a.flags[((size_t)h * tiles + tile) * kBlocksPerSide + rest % kBlocksPerSide] = bad;
+            bad = 0;
+        }
+    };
+    for (int i = blk0; i < blk1; ++i) {
+        // Block i's 8 loads went out three blocks ago; since then, in order,
+        // those of blocks i + 1 and i + 2 and the stores of three blocks, 4
+        // or 5 each.
+        if (i + 2 < blk1) {
+            if (live && i - blk0 >= 4)
+                MLA_WAIT_VMCNT(2 * (kWeightRows / 4) + 3 * 4);
+            else
+                MLA_WAIT_VMCNT(2 * (kWeightRows / 4));
+        } else if (i + 1 < blk1) {
+            MLA_WAIT_VMCNT(kWeightRows / 4);
+        } else {
+            MLA_WAIT_VMCNT(0);
+        }
+        lds_barrier();  // block i is there, and block i - 1's slot is free
+        if (i + kWeightRing - 1 < blk1)
+            load_block(i + kWeightRing - 1);
+        const unsigned at = ring + ((i - blk0) & (kWeightRing - 1)) * (kWeightElems * 2) + w_lane;
+        const bool have = live && i > blk0;
+        floatx16 acc[2] = {};
+        E8 v[2][2];
+        unsigned top[2] = {0, 0};
+        E8 w[2][4];
+        auto operand = [&](int k) -> E8 { return lds_load<E8>((at ^ (32 * (k & 7))) + 256 * (k >> 3)); };
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            w[0][j] = operand(j);
+#pragma unroll
+        for (int k = 0; k < kLatent / 16; k += 4) {
+            if (k + 4 < kLatent / 16) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    w[(k / 4 + 1) & 1][j] = operand(k + 4 + j);
+                __builtin_amdgcn_sched_barrier(0);  // the reads first: left alone they go out as late as they can
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int g = 0; g < 2; ++g)
+                    acc[g] = mfma32x32x16(w[(k / 4) & 1][j], key[g][k + j], acc[g]);
+            if (have)
+                store(i - 1, k / 16, k / 4 % 4, top[k / 16], v[k / 16]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        prev[0] = acc[0];
+        prev[1] = acc[1];
+    }
+    if (live) {
+        E8 v[2];
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+            unsigned top = 0;
+#pragma unroll
+            for (int part = 0; part < 4; ++part)
+                store(blk1 - 1, g, part, top, v);
+        }
+    }
 }
 
 // ---- attention --------------------------------------------------------------
@@ -263,14 +346,14 @@ __global__ __launch_bounds__(256, 2) void attend_kernel(PrefillArgs a)
     const E *ks = (const E *)a.k + ((size_t)h * a.padded + (size_t)tile0 * kTile) * kNope;
     const E *vs = (const E *)a.v + ((size_t)h * a.padded + (size_t)tile0 * kTile) * kNope;
     const E *rs = (const E *)a.rope + (size_t)tile0 * kTile * kRopeDim;
-    const unsigned long long *flags = a.flags + ((size_t)h * (a.padded / kTile) + tile0) * 2;
+    const ulong4x *flags = (const ulong4x *)a.flags + (size_t)h * (a.padded / kTile) + tile0;
     // 16 units of K and of V (4 rows each), 8 of the rotary parts (8 rows)
     auto load_tile = [&](int j) {
         const unsigned at = lds + (j & 1) * (kStage * 2);
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
             const int r = 16 * wave + 4 * u + (lane >> 4);
-            const int off = r * (kNope * 2) + 16 * ((lane & 15) ^ row_swizzle(r));
+            const int off = r * (kNope * 2) + 16 * ((lane & 15) ^ key_swizzle(r));
             global_to_lds16_at(ks + (size_t)j * kKElems, off, at + (4 * wave + u) * 1024);
             global_to_lds16_at(vs + (size_t)j * kKElems, off, at + 2 * kKElems + (4 * wave + u) * 1024);
         }
@@ -281,15 +364,14 @@ __global__ __launch_bounds__(256, 2) void attend_kernel(PrefillArgs a)
                                at + 4 * kKElems + (2 * wave + u) * 1024);
         }
     };
-    const int key = key_of_row(r32);
-    const unsigned k_lane = key * (kNope * 2) + 16 * (hl ^ row_swizzle(key));
-    const unsigned rope_lane = 4 * kKElems + key * (kRopeDim * 2) + 16 * (hl ^ rope_swizzle(key));
+    const unsigned k_lane = r32 * (kNope * 2) + 16 * (hl ^ key_swizzle(r32));
+    const unsigned rope_lane = 4 * kKElems + r32 * (kRopeDim * 2) + 16 * (hl ^ rope_swizzle(r32));
     unsigned v_lane[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        const int j = lane & 15, r = 8 * hl + 2 * (j >> 2) + i;
+        const int j = lane & 15, r = 8 * i + 4 * hl + (j >> 2);
         v_lane[i] = 2 * kKElems + r * (kNope * 2) +
-                    16 * ((2 * ((lane >> 4) & 1) + ((j & 3) >> 1)) ^ row_swizzle(r)) + 8 * (j & 1);
+                    16 * ((2 * ((lane >> 4) & 1) + ((j & 3) >> 1)) ^ key_swizzle(r)) + 8 * (j & 1);
     }
 
     floatx16 o[4] = {};
@@ -306,16 +388,36 @@ __global__ __launch_bounds__(256, 2) void attend_kernel(PrefillArgs a)
         if (j * kTile > wave_last)
             continue;
         const unsigned at = lds + (j & 1) * (kStage * 2);
-        floatx16 s[2];
+        floatx16 s[2] = {};
+        {
+            // operand k of both 32-key blocks: 8 steps of the head's own part, 4 of the rotary one
+            auto operand = [&](int g, int k) -> E8 {
+                return k < 8 ? lds_load<E8>(((at + k_lane) ^ (32 * k)) + 32 * g * (kNope * 2))
+                             : lds_load<E8>(((at + rope_lane) ^ (32 * (k - 8))) + 32 * g * (kRopeDim * 2));
+            };
+            E8 kv[2][2][2];
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
-            s[g] = floatx16{};
+            for (int g = 0; g < 2; ++g)
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-                s[g] = mfma32x32x16(lds_load<E8>(((at + k_lane) ^ (32 * k)) + 32 * g * (kNope * 2)), q[k], s[g]);
+                for (int i = 0; i < 2; ++i)
+                    kv[0][g][i] = operand(g, i);
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-                s[g] = mfma32x32x16(lds_load<E8>(((at + rope_lane) ^ (32 * k)) + 32 * g * (kRopeDim * 2)), q[8 + k], s[g]);
+            for (int k = 0; k < 12; k += 2) {
+                if (k + 2 < 12) {
+#pragma unroll
+                    for (int g = 0; g < 2; ++g)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+                            kv[(k / 2 + 1) & 1][g][i] = operand(g, k + 2 + i);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int g = 0; g < 2; ++g)
+                        s[g] = mfma32x32x16(kv[(k / 2) & 1][g][i], q[k + i], s[g]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
         if (j * kTile + kTile - 1 > wave_first) {
 #pragma unroll
@@ -345,7 +447,8 @@ __global__ __launch_bounds__(256, 2) void attend_kernel(PrefillArgs a)
             p[r] = fast_exp2(s[r >> 4][r & 15] * a.scale_log2 - ref);
             l += p[r];
         }
-        const unsigned long long bad = scalar_load(flags + 2 * j) | scalar_load(flags + 2 * j + 1);
+        const ulong4x f4 = scalar_load(flags + j);
+        const unsigned long long bad = f4[0] | f4[1] | f4[2] | f4[3];
         if (bad != 0) {  // a query that sees a key whose V is not finite gives NaN
 #pragma unroll
             for (int r = 0; r < 32; ++r) {
@@ -354,17 +457,31 @@ __global__ __launch_bounds__(256, 2) void attend_kernel(PrefillArgs a)
                     l = NAN;
             }
         }
-#pragma unroll
-        for (int ks4 = 0; ks4 < 4; ++ks4) {
-            const E8 pb = p_operand<E>(p + 8 * ks4);
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
+        {
+            auto operand = [&](int ks, int c) -> E8 {  // columns 32 c .. of V^T, keys 16 ks .. +15 in P's order
                 E4 part[2];
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
-                    part[i] = lds_load_tr16<E>(((at + v_lane[i]) ^ (64 * c)) + 16 * ks4 * (kNope * 2));
-                const E8 v = {part[0][0], part[0][1], part[0][2], part[0][3], part[1][0], part[1][1], part[1][2], part[1][3]};
-                o[c] = mfma32x32x16(v, pb, o[c]);
+                    part[i] = lds_load_tr16<E>(((at + v_lane[i]) ^ (64 * c)) + 16 * ks * (kNope * 2));
+                return E8{part[0][0], part[0][1], part[0][2], part[0][3], part[1][0], part[1][1], part[1][2], part[1][3]};
+            };
+            E8 v[2][4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                v[0][c] = operand(0, c);
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) {
+                if (ks + 1 < 4) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+                        v[(ks + 1) & 1][c] = operand(ks + 1, c);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                const E8 pb = p_operand<E>(p + 8 * ks);
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    o[c] = mfma32x32x16(v[ks & 1][c], pb, o[c]);
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
     }
@@ -402,8 +519,36 @@ PrefillPlan prefill_plan(int batch, int num_heads, int total_tokens)
     p.padded = total_tokens / kTile * kTile + kTile * batch;
     p.kv_bytes = align256((size_t)num_heads * p.padded * kNope * 2);
     p.rope_bytes = align256((size_t)p.padded * kRopeDim * 2);
-    p.flag_bytes = align256((size_t)num_heads * (p.padded / kTile) * 16);
+    p.flag_bytes = align256((size_t)num_heads * (p.padded / kTile) * 32);
     return p;
+}
+
+// Weight blocks of an expanding workgroup. It costs its key loads (about as
+// long as kKeyBlocks blocks) and its blocks, and one runs on a CU at a time: of
+// the divisions into a multiple of 8 groups (one XCD's workgroups take the same
+// ones) that fill one round, two rounds, .., the one with the fewest blocks in
+// a row wins.
+constexpr int kKeyBlocks = 6;
+
+int expand_group_blocks(int batch, int total_tokens, int num_heads, int cu_count)
+{
+    // key tiles that hold keys, at most (workgroups without any leave at once)
+    const int64_t tiles = ((int64_t)total_tokens + (int64_t)(kTile - 1) * batch) / kTile;
+    const int64_t quads = std::max<int64_t>(1, (tiles + kExpandTiles - 1) / kExpandTiles);
+    const int blocks = 2 * kBlocksPerSide * num_heads;
+    int best = blocks / 8;
+    int64_t best_cost = (quads * 8 + cu_count - 1) / cu_count * (best + kKeyBlocks);
+    for (int rounds = 1; rounds <= 16; ++rounds) {
+        const int64_t groups = std::min<int64_t>(rounds * (int64_t)cu_count / quads / 8 * 8, blocks);
+        if (groups < 8)
+            continue;
+        const int per = (int)((blocks + groups - 1) / groups);
+        if (rounds * (int64_t)(per + kKeyBlocks) < best_cost) {
+            best = per;
+            best_cost = rounds * (int64_t)(per + kKeyBlocks);
+        }
+    }
+    return best;
 }
 
 bool prefill_sizes_ok(int batch, int num_heads, int total_tokens)
@@ -416,8 +561,9 @@ template <typename E>
 void launch_prefill(const PrefillArgs &a, hipStream_t s)
 {
     if (a.total_tokens > 0) {
-        const int pairs = (a.padded / kTile + 1) / 2;
-        hipLaunchKernelGGL(expand_kernel<E>, dim3((unsigned)pairs * (2 * a.num_heads)), dim3(256), 0, s, a);
+        const int quads = (a.padded / kTile + kExpandTiles - 1) / kExpandTiles;
+        const int groups = (2 * kBlocksPerSide * a.num_heads + a.group_blocks - 1) / a.group_blocks;
+        hipLaunchKernelGGL(expand_kernel<E>, dim3((unsigned)quads * ((groups + 7) / 8 * 8)), dim3(256), 0, s, a);
     }
     hipLaunchKernelGGL(attend_kernel<E>, dim3((unsigned)a.q_slots * a.num_heads), dim3(256), 0, s, a);
 }
@@ -462,6 +608,7 @@ int prefill(bool bf16, const void *q_nope, const void *q_rope, const void *w_uk,
     a.queries = queries;
     a.total_tokens = total_tokens;
     a.padded = p.padded;
+    a.group_blocks = expand_group_blocks(batch, total_tokens, num_heads, current_cu_count());
     a.page_shift = block_table ? __builtin_ctz((unsigned)page_size) : 0;
     a.num_pages = num_pages;
     a.bt_stride = block_table_stride;

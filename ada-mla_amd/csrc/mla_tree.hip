@@ -131,7 +131,7 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
             const int r = 8 * wave + u;
-            global_to_lds16_at(base + (size_t)min(r, lim) * kDK, 16 * (ln ^ row_swizzle(r)), dst + r * (kDV * 2));
+            global_to_lds16_at(base + (size_t)min(r, lim) * kDK, 16 * (ln ^ key_swizzle(r)), dst + r * (kDV * 2));
         }
         const int r = 8 * wave + (ln >> 3);
         global_to_lds16_at(base, min(r, lim) * (kDK * 2) + 2 * (kDV + 8 * ((ln & 7) ^ rope_swizzle(r))),
@@ -162,14 +162,13 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
     // LDS addresses, less the slot's, of the lane's operands. A chunk's place
     // differs from chunk 0's in the same row only by an XOR of its low four
     // bits and an offset of the others, so one address each serves all chunks.
-    const int key = key_of_row(r32);
-    const unsigned k_lane = key * (kDV * 2) + 16 * (hl ^ row_swizzle(key));
-    const unsigned rope_lane = 2 * kRopeElems + key * (kRopeDim * 2) + 16 * (hl ^ rope_swizzle(key));
-    unsigned v_lane[2];  // the two transpose reads: 4 keys of one parity
+    const unsigned k_lane = r32 * (kDV * 2) + 16 * (hl ^ key_swizzle(r32));
+    const unsigned rope_lane = 2 * kRopeElems + r32 * (kRopeDim * 2) + 16 * (hl ^ rope_swizzle(r32));
+    unsigned v_lane[2];  // the two transpose reads that match a P operand, 4 keys each
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        const int j = lane & 15, r = 8 * hl + 2 * (j >> 2) + h;
-        v_lane[h] = r * (kDV * 2) + 16 * ((2 * ((lane >> 4) & 1) + ((j & 3) >> 1)) ^ row_swizzle(r)) + 8 * (j & 1);
+        const int j = lane & 15, r = 8 * h + 4 * hl + (j >> 2);
+        v_lane[h] = r * (kDV * 2) + 16 * ((2 * ((lane >> 4) & 1) + ((j & 3) >> 1)) ^ key_swizzle(r)) + 8 * (j & 1);
     }
     for (int i = 0; i < n_blocks; ++i) {
         if (i + 2 < n_blocks)
@@ -200,6 +199,7 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
                         kv[(k / 4 + 1) & 1][j] = k_operand(k + 4 + j);
+                    __builtin_amdgcn_sched_barrier(0);  // the reads first: left alone they go out as late as they can
                 }
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
@@ -293,6 +293,7 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
                         v[(u / 4 + 1) & 1][j] = v_operand(u + 4 + j);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
