@@ -31,12 +31,51 @@ __device__ __forceinline__ floatx16 mfma32x32x16(bf16x8 a, bf16x8 b, floatx16 c)
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
 
+// The same product accumulated in ordinary registers, for a kernel whose other
+// accumulators fill the accumulation registers (the compiler puts all of a kernel's
+// products there, and moves them back and forth when they do not fit).
+// A chain: first (C = 0), next .., then settle before anything reads the tile:
+// a product's result may be read 11 slots after an 8-pass product (16 here),
+// which the compiler knows of its own products only. Within a chain each
+// product's accumulator is exactly the last one's result, which needs no wait.
+__device__ __forceinline__ void mfma32x32x16_first(floatx16 &d, half8 a, half8 b)
+{
+    asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, 0" : "=&v"(d) : "v"(a), "v"(b));
+}
+
+__device__ __forceinline__ void mfma32x32x16_next(floatx16 &d, half8 a, half8 b)
+{
+    asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+v"(d) : "v"(a), "v"(b));
+}
+
+__device__ __forceinline__ void mfma32x32x16_first(floatx16 &d, bf16x8 a, bf16x8 b)
+{
+    asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(d) : "v"(a), "v"(b));
+}
+
+__device__ __forceinline__ void mfma32x32x16_next(floatx16 &d, bf16x8 a, bf16x8 b)
+{
+    asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(d) : "v"(a), "v"(b));
+}
+
+__device__ __forceinline__ void mfma_settle(floatx16 &d)
+{
+    asm volatile("s_nop 15" : "+v"(d));
+}
+
 // Keeps an accumulator tile in the accumulation registers across this point,
 // so that 16 of them and 144 registers of Q* fit one wave's 512: left to
 // itself the compiler moves them into the 256 others for a rescale and spills.
 __device__ __forceinline__ void in_accumulators(floatx16 &v)
 {
     asm volatile("" : "+a"(v));
+}
+
+// A use of v, whatever it holds: what loads it is waited for here.
+template <typename V>
+__device__ __forceinline__ void in_registers(V &v)
+{
+    asm volatile("" : "+v"(v));
 }
 
 // f over lanes l and l ^ 32, on the VALU (see reduce_over_lane_groups).
@@ -101,6 +140,15 @@ __device__ __forceinline__ void gather_to_lds16(const void *p, unsigned lds)
 __device__ __forceinline__ unsigned lds_address(const void *p)
 {
     return __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(const __attribute__((address_space(3))) void *)p);
+}
+
+// An address that is the same in all lanes, into scalar registers.
+template <typename T>
+__device__ __forceinline__ const T *wave_uniform(const T *p)
+{
+    const uint64_t u = (uint64_t)(uintptr_t)p;
+    const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)u), hi = __builtin_amdgcn_readfirstlane((unsigned)(u >> 32));
+    return (const T *)(uintptr_t)((uint64_t)hi << 32 | lo);
 }
 
 // A load of what the kernel does not write, at a wave-uniform address, by the

@@ -31,6 +31,7 @@ constexpr int kSlotElems = kBlock * kDK;  // 36 KB
 constexpr int kRopeDim = kDK - kDV;
 constexpr int kRopeElems = kBlock * kDV;  // the rope part of a slot, after its C_N rows
 constexpr int kUnitsPerWave = 9;          // 1 KB load units of a block per wave: 8 rows, 1 rope unit
+constexpr int kAhead = 4;                 // products an operand is read ahead
 constexpr int kMaxDrafts = 64;
 
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -54,18 +55,18 @@ struct TreeArgs {
     float scale_log2;
 };
 
-// Request b's tokens [lo, hi) of the packed numbering and its splits. Request
+// Request b's tokens [lo, lo + len) of the packed numbering and its splits. Request
 // b's splits take the slots lo / chunk + b, ..., which never meet those of
 // another request, whatever the lengths.
 struct Request {
     int lo, len, n_splits, slot0, drafts;
     __device__ __forceinline__ void read(const TreeArgs &a, int b)
     {
-        lo = min(max(a.cu_seqlens[b], 0), a.total_tokens);
-        len = min(max(a.cu_seqlens[b + 1], lo), a.total_tokens) - lo;
+        lo = min(max(scalar_load(a.cu_seqlens + b), 0), a.total_tokens);
+        len = min(max(scalar_load(a.cu_seqlens + b + 1), lo), a.total_tokens) - lo;
         n_splits = max(1, (len + a.chunk - 1) / a.chunk);
         slot0 = lo / a.chunk + b;
-        drafts = a.draft_lens ? min(max(a.draft_lens[b], 0), a.drafts) : a.drafts;
+        drafts = a.draft_lens ? min(max(scalar_load(a.draft_lens + b), 0), a.drafts) : a.drafts;
     }
 };
 
@@ -116,26 +117,32 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
     const int t_lo = split * a.chunk, t_hi = min(t_lo + a.chunk, rq.len);
     const int n_blocks = (t_hi - t_lo + kBlock - 1) / kBlock;
 
-    // block i of the split into its ring slot; every block lies in one page.
-    // Page ids and columns are clamped, so a bad table gives wrong results and
-    // no stray access; rows past the request's end re-read its last one.
-    auto load_block = [&](int i) {
-        const int t = t_lo + i * kBlock;
-        const int col = min(t >> a.page_shift, a.bt_stride - 1);
-        const int page = min(max(scalar_load(a.block_table + (size_t)b * a.bt_stride + col), 0), a.num_pages - 1);
-        const E *base = (const E *)a.cache + (((size_t)page << a.page_shift) + (t & ((1 << a.page_shift) - 1))) * kDK;
-        const int lim = min(kBlock - 1, rq.len - 1 - t);
+    // Block i of the split goes into its ring slot in 9 load units a wave: 8
+    // rows, and the rope parts of 8 rows. Every block lies in one page. Page
+    // ids and columns are clamped, so a bad table gives wrong results and no
+    // stray access; rows past the request's end re-read its last one.
+    auto page_of = [&](int i) -> int {
+        const int col = min((t_lo + i * kBlock) >> a.page_shift, a.bt_stride - 1);
+        return scalar_load(a.block_table + (size_t)b * a.bt_stride + col);
+    };
+    auto block_source = [&](int i, int page) -> const E * {
+        page = min(max(page, 0), a.num_pages - 1);
+        return wave_uniform((const E *)a.cache +
+                            (((size_t)page << a.page_shift) + ((t_lo + i * kBlock) & ((1 << a.page_shift) - 1))) * kDK);
+    };
+    auto load_unit = [&](const E *base, int i, int u) {
+        const int lim = min(kBlock - 1, rq.len - 1 - (t_lo + i * kBlock));
         const unsigned dst = ring + (i & (kRing - 1)) * (kSlotElems * 2);
         int ln = lane;  // opaque: the offsets are formed at each load, not kept in registers
         asm volatile("" : "+v"(ln));
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
+        if (u < 8) {
             const int r = 8 * wave + u;
-            global_to_lds16_at(base + (size_t)min(r, lim) * kDK, 16 * (ln ^ key_swizzle(r)), dst + r * (kDV * 2));
+            global_to_lds16_at(base, min(r, lim) * (kDK * 2) + 16 * (ln ^ key_swizzle(r)), dst + r * (kDV * 2));
+        } else {
+            const int r = 8 * wave + (ln >> 3);
+            global_to_lds16_at(base, min(r, lim) * (kDK * 2) + 2 * (kDV + 8 * ((ln & 7) ^ rope_swizzle(r))),
+                               dst + 2 * kRopeElems + 1024 * wave);
         }
-        const int r = 8 * wave + (ln >> 3);
-        global_to_lds16_at(base, min(r, lim) * (kDK * 2) + 2 * (kDV + 8 * ((ln & 7) ^ rope_swizzle(r))),
-                           dst + 2 * kRopeElems + 1024 * wave);
     };
 
     // Q*: the B operand of S^T, whole rows in registers. Rows past the
@@ -147,9 +154,25 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
         for (int k = 0; k < kDK / 16; ++k)
             q[k] = *(const E8 *)(src + 16 * k);
     }
-    const unsigned long long mask = a.tree_mask[(size_t)b * a.drafts + min(row, live - 1) / a.num_heads];
-    for (int i = 0; i < min(kRing - 1, n_blocks); ++i)
+    unsigned long long mask = a.tree_mask[(size_t)b * a.drafts + min(row, live - 1) / a.num_heads];
+    auto load_block = [&](int i) {
+        const E *src = block_source(i, page_of(i));
+#pragma unroll
+        for (int u = 0; u < kUnitsPerWave; ++u)
+            load_unit(src, i, u);
+    };
+    if (n_blocks > 0)
+        load_block(0);
+    // Q* is waited for here, by name: the compiler does not know of the loads
+    // to LDS and would wait for Q* at its uses inside the loop, in every block,
+    // which there means for the blocks in flight.
+#pragma unroll
+    for (int k = 0; k < kDK / 16; ++k)
+        in_registers(q[k]);
+    in_registers(mask);
+    for (int i = 1; i < min(kRing - 1, n_blocks); ++i)
         load_block(i);
+    int next_page = kRing - 1 < n_blocks ? page_of(kRing - 1) : 0;
 
     floatx16 o[kDV / 32];
 #pragma unroll
@@ -170,43 +193,70 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
         const int j = lane & 15, r = 8 * h + 4 * hl + (j >> 2);
         v_lane[h] = r * (kDV * 2) + 16 * ((2 * ((lane >> 4) & 1) + ((j & 3) >> 1)) ^ key_swizzle(r)) + 8 * (j & 1);
     }
-    for (int i = 0; i < n_blocks; ++i) {
-        if (i + 2 < n_blocks)
-            MLA_WAIT_VMCNT(2 * kUnitsPerWave);
-        else if (i + 1 < n_blocks)
-            MLA_WAIT_VMCNT(kUnitsPerWave);
-        else
-            MLA_WAIT_VMCNT(0);
-        lds_barrier();  // block i is there, and block i - 1's slot is free
-        if (i + kRing - 1 < n_blocks)
-            load_block(i + kRing - 1);
+    // S^T of block i, with side(k) between the products: what does not depend
+    // on them, in their shadow (a product takes 32 cycles and one issue slot of
+    // 4). Each operand is read kAhead products before its own. The products go
+    // to ordinary registers: O* fills the accumulation registers.
+    auto logits = [&](int i, auto &&side) -> floatx16 {
         const unsigned blk = ring + (i & (kRing - 1)) * (kSlotElems * 2);
-
         const unsigned k_at = blk + k_lane, rope_at = blk + rope_lane;
         auto k_operand = [&](int k) -> E8 {  // values 16 k + 8 hl .. +7 of the lane's key
             return k < kDV / 16 ? lds_load<E8>((k_at ^ (32 * (k & 7))) + 256 * (k >> 3))
                                 : lds_load<E8>(rope_at ^ (32 * (k - kDV / 16)));
         };
-        floatx16 s = {};
-        {
-            E8 kv[2][4];
+        E8 kv[kAhead + 1];
+        floatx16 s;
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                kv[0][j] = k_operand(j);
+        for (int k = 0; k < kAhead; ++k)
+            kv[k] = k_operand(k);
 #pragma unroll
-            for (int k = 0; k < kDK / 16; k += 4) {
-                if (k + 4 < kDK / 16) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        kv[(k / 4 + 1) & 1][j] = k_operand(k + 4 + j);
-                    __builtin_amdgcn_sched_barrier(0);  // the reads first: left alone they go out as late as they can
-                }
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    s = mfma32x32x16(kv[(k / 4) & 1][j], q[k + j], s);
-                __builtin_amdgcn_sched_barrier(0);
-            }
+        for (int k = 0; k < kDK / 16; ++k) {
+            if (k + kAhead < kDK / 16)
+                kv[(k + kAhead) % (kAhead + 1)] = k_operand(k + kAhead);
+            if (k == 0)
+                mfma32x32x16_first(s, kv[0], q[0]);
+            else
+                mfma32x32x16_next(s, kv[k % (kAhead + 1)], q[k]);
+            side(k);
+            __builtin_amdgcn_sched_barrier(0);
         }
+        mfma_settle(s);
+        return s;
+    };
+    auto largest = [&](const floatx16 &s) {
+        float most = s[0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r)
+            most = fmaxf(most, s[r]);
+        return most;
+    };
+
+    floatx16 s = {};
+    float most = -INFINITY;  // the lane's largest logit of block i
+    if (n_blocks > 0) {
+        if (n_blocks > 2)
+            MLA_WAIT_VMCNT(2 * kUnitsPerWave);
+        else if (n_blocks > 1)
+            MLA_WAIT_VMCNT(kUnitsPerWave);
+        else
+            MLA_WAIT_VMCNT(0);
+        lds_barrier();
+        s = logits(0, [](int) {});
+        most = largest(s);
+    }
+    for (int i = 0; i < n_blocks; ++i) {
+        // Block i: s holds its logits. Those of block i + 1 are computed
+        // while block i's weights are, then O* takes block i.
+        const bool more = i + 1 < n_blocks;
+        if (i + 2 < n_blocks)
+            MLA_WAIT_VMCNT(kUnitsPerWave);
+        else
+            MLA_WAIT_VMCNT(0);
+        lds_barrier();  // block i + 1 is there, every wave has block i's logits, and block i - 1's slot is free
+        const bool feed = i + kRing - 1 < n_blocks;
+        const E *feed_src = block_source(i + kRing - 1, next_page);
+        next_page = i + kRing < n_blocks ? page_of(i + kRing) : 0;
+
         const int t0 = t_lo + i * kBlock;
         const bool edge = t0 + kBlock > context;  // holds drafted tokens, or the end
         if (edge) {
@@ -217,42 +267,14 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
                 const unsigned seen = (unsigned)(t < context) | ((unsigned)(t < rq.len) & bit);
                 s[r] = seen ? s[r] : -INFINITY;
             }
-        }
-        float most = s[0];
-#pragma unroll
-        for (int r = 1; r < 16; ++r)
-            most = fmaxf(most, s[r]);
-        most = reduce_halves(most, [](float x, float y) { return fmaxf(x, y); }) * a.scale_log2;
-        // the reference moves only past kLazyRescale, so P is at most 2^8
-        if (__builtin_amdgcn_ballot_w64(most > m + kLazyRescale) != 0) {
-            const float next = most > m + kLazyRescale ? most : m;  // each row by itself
-            const float f = next == -INFINITY ? 1.0f : fast_exp2(m - next);
-            m = next;
-            l *= f;
-#pragma unroll
-            for (int c = 0; c < kDV / 32; ++c) {
-                in_accumulators(o[c]);
-                o[c] *= f;
-                in_accumulators(o[c]);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-        }
-        const float ref = m == -INFINITY ? 0.0f : m;
-        float p[16];
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            p[r] = fast_exp2(s[r] * a.scale_log2 - ref);
-            l += p[r];
-        }
-        const E8 pb[2] = {p_operand<E>(p), p_operand<E>(p + 8)};
-        if (edge) {
+            most = largest(s);
             // A drafted token that a row does not see meets it with weight 0:
             // 0 times an infinity or NaN in its row would still be NaN, so
             // those become 0 for the second product. A row that does see such
             // a token has its sum l a NaN from the first product already.
-            lds_barrier();  // every wave has its logits
+            E *blk = s_ring + (i & (kRing - 1)) * kSlotElems;
             for (int u = threadIdx.x; u < kBlock * kDV / 8; u += 256) {
-                uint4 *at = (uint4 *)(s_ring + (i & (kRing - 1)) * kSlotElems + 8 * u);
+                uint4 *at = (uint4 *)(blk + 8 * u);
                 uint4 v = *at;
                 unsigned *w = (unsigned *)&v;
                 bool bad = false;
@@ -272,6 +294,43 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
             }
             lds_barrier();
         }
+        most = reduce_halves(most, [](float x, float y) { return fmaxf(x, y); }) * a.scale_log2;
+        // the reference moves only past kLazyRescale, so P is at most 2^8
+        if (__builtin_amdgcn_ballot_w64(most > m + kLazyRescale) != 0) {
+            const float next = most > m + kLazyRescale ? most : m;  // each row by itself
+            const float f = next == -INFINITY ? 1.0f : fast_exp2(m - next);
+            m = next;
+            l *= f;
+#pragma unroll
+            for (int c = 0; c < kDV / 32; ++c) {
+                in_accumulators(o[c]);
+                o[c] *= f;
+                in_accumulators(o[c]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        const float ref = m == -INFINITY ? 0.0f : m;
+        float p[16];
+        auto weight = [&](int r) {
+            p[r] = fast_exp2(s[r] * a.scale_log2 - ref);
+            l += p[r];
+        };
+        floatx16 ahead = {};
+        if (more) {
+            ahead = logits(i + 1, [&](int k) {
+                if (k % 2 == 0 && k < 32)
+                    weight(k / 2);
+                if (k % 4 == 1 && feed)
+                    load_unit(feed_src, i + kRing - 1, k / 4);
+            });
+        } else {
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                weight(r);
+        }
+        const E8 pb[2] = {p_operand<E>(p), p_operand<E>(p + 8)};
+
+        const unsigned blk = ring + (i & (kRing - 1)) * (kSlotElems * 2);
         const unsigned v_at[2] = {blk + v_lane[0], blk + v_lane[1]};
         auto v_operand = [&](int u) -> E8 {  // 32 columns of tile c, keys 16 ks .. +15 in the order of P's registers
             const int ks = u / (kDV / 32), c = u % (kDV / 32);
@@ -281,29 +340,24 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
                 part[h] = lds_load_tr16<E>((v_at[h] ^ (64 * (c & 3))) + 256 * (c >> 2) + 16 * ks * (kDV * 2));
             return E8{part[0][0], part[0][1], part[0][2], part[0][3], part[1][0], part[1][1], part[1][2], part[1][3]};
         };
-        {
-            constexpr int kOps = 2 * kDV / 32;
-            E8 v[2][4];
+        constexpr int kOps = 2 * kDV / 32;
+        E8 v[kAhead + 1];
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                v[0][j] = v_operand(j);
+        for (int u = 0; u < kAhead; ++u)
+            v[u] = v_operand(u);
+        most = ahead[0];
 #pragma unroll
-            for (int u = 0; u < kOps; u += 4) {
-                if (u + 4 < kOps) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        v[(u / 4 + 1) & 1][j] = v_operand(u + 4 + j);
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    floatx16 &acc = o[(u + j) % (kDV / 32)];
-                    acc = mfma32x32x16(v[(u / 4) & 1][j], pb[u / (kDV / 32)], acc);
-                    in_accumulators(acc);
-                }
-                __builtin_amdgcn_sched_barrier(0);
-            }
+        for (int u = 0; u < kOps; ++u) {
+            if (u + kAhead < kOps)
+                v[(u + kAhead) % (kAhead + 1)] = v_operand(u + kAhead);
+            floatx16 &acc = o[u % (kDV / 32)];
+            acc = mfma32x32x16(v[u % (kAhead + 1)], pb[u / (kDV / 32)], acc);
+            in_accumulators(acc);
+            if (u > 0 && u < 16)
+                most = fmaxf(most, ahead[u]);
+            __builtin_amdgcn_sched_barrier(0);
         }
+        s = ahead;
     }
 
 #pragma unroll
@@ -351,7 +405,7 @@ __global__ __launch_bounds__(256) void tree_combine_kernel(TreeArgs a)
     const int lane = threadIdx.x & 63;
     const int item = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = item & 15, w = (item >> 4) & 3, rest = item >> 6;
-    const int rt = rest % a.row_tiles, b = rest / a.row_tiles;
+    const int rt = rest % a.row_tiles, b = rest / a.row_tiles;  // wave-uniform, as Request::read asks
     if (b >= a.batch)
         return;
     Request rq;
