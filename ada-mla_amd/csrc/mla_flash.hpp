@@ -125,6 +125,15 @@ __device__ __forceinline__ bool not_finite(unsigned short bits)
     return (bits & e) == e;
 }
 
+typedef unsigned short ushort2x __attribute__((ext_vector_type(2)));
+
+// The larger of both 16-bit halves, each by itself.
+__device__ __forceinline__ unsigned max_u16x2(unsigned a, unsigned b)
+{
+    return __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(ushort2x, a),
+                                                                  __builtin_bit_cast(ushort2x, b)));
+}
+
 // 16 bytes per lane from a per-lane address into LDS at lds + 16 * lane
 // (lds: a wave-uniform LDS byte address); see global_to_lds16.
 __device__ __forceinline__ void gather_to_lds16(const void *p, unsigned lds)

@@ -27,7 +27,6 @@ constexpr int kNope = 128, kRopeDim = 64, kLatent = 512;
 constexpr int kTile = 64;      // keys per tile; sequences are padded to it in the workspace
 typedef unsigned long long ulong4x __attribute__((ext_vector_type(4)));
 typedef unsigned uint4x __attribute__((ext_vector_type(4)));
-typedef unsigned short ushort2x __attribute__((ext_vector_type(2)));
 constexpr int kQueries = 128;  // queries per workgroup: 32 a wave
 
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -205,8 +204,7 @@ expand_kernel(PrefillArgs a)
 #pragma unroll
         for (int k = 0; k < 2; ++k) {  // the largest magnitude's bits, both halves
             const unsigned x = w[2 * (part & 1) + k] & 0x7fff7fffu;
-            top = __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(ushort2x, top),
-                                                                         __builtin_bit_cast(ushort2x, x)));
+            top = max_u16x2(top, x);
         }
         if (part != 3)
             return;

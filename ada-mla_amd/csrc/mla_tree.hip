@@ -70,9 +70,13 @@ struct Request {
     }
 };
 
-template <typename E>
+// kTiles: 32-column tiles of O* a workgroup computes, 16 (all) or 4. A quarter of
+// the columns computes all logits again but takes a quarter of the second
+// product's and the results' time: for calls that leave most of the CUs idle.
+template <typename E, int kTiles>
 __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_per_eu(1, 1))) void tree_kernel(TreeArgs a)
 {
+    constexpr int kParts = kDV / 32 / kTiles;
     using E8 = typename Vec<E>::v8;
     using E4 = typename Vec<E>::v4;
     __shared__ __attribute__((aligned(1024))) E s_ring[kRing * kSlotElems];
@@ -81,10 +85,12 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
     const int r32 = lane & 31, hl = lane >> 5;
     const unsigned ring = lds_address(s_ring);
 
-    // workgroup -> (slot, row tile): the row tiles of a slot, which read the
-    // same tokens, get ids equal mod 8, i.e. one XCD and its L2
-    const int slot = (blockIdx.x >> 3) / a.row_tiles * 8 + (blockIdx.x & 7);
-    const int rt = (blockIdx.x >> 3) % a.row_tiles;
+    // workgroup -> (slot, row tile, column part): the workgroups of a slot,
+    // which read the same tokens, get ids equal mod 8, i.e. one XCD and its L2
+    const int per_slot = a.row_tiles * kParts;
+    const int slot = (blockIdx.x >> 3) / per_slot * 8 + (blockIdx.x & 7);
+    const int within = (blockIdx.x >> 3) % per_slot;
+    const int rt = within / kParts, part = within % kParts;
     if (slot >= a.n_slots)
         return;
     int b = 0;  // the last request whose first slot is at or before `slot`
@@ -108,7 +114,7 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
     const int row = rt * kRows + 32 * wave + r32; // this lane's
     E *out = (E *)a.out + (size_t)b * rows * kDV;
     if (rt * kRows >= live) {  // only padding rows
-        if (rq.n_splits == 1)
+        if (rq.n_splits == 1 && part == 0)
             for (int i = threadIdx.x; i < min(kRows, rows - rt * kRows) * (kDV / 8); i += 256)
                 *(uint4 *)(out + (size_t)rt * kRows * kDV + 8 * i) = uint4{0, 0, 0, 0};
         return;
@@ -145,43 +151,6 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
         }
     };
 
-    // Q*: the B operand of S^T, whole rows in registers. Rows past the
-    // drafted tokens re-read the last one; their results are never stored.
-    E8 q[kDK / 16];
-    {
-        const E *src = (const E *)a.q + ((size_t)b * rows + min(row, live - 1)) * kDK + 8 * hl;
-#pragma unroll
-        for (int k = 0; k < kDK / 16; ++k)
-            q[k] = *(const E8 *)(src + 16 * k);
-    }
-    unsigned long long mask = a.tree_mask[(size_t)b * a.drafts + min(row, live - 1) / a.num_heads];
-    auto load_block = [&](int i) {
-        const E *src = block_source(i, page_of(i));
-#pragma unroll
-        for (int u = 0; u < kUnitsPerWave; ++u)
-            load_unit(src, i, u);
-    };
-    if (n_blocks > 0)
-        load_block(0);
-    // Q* is waited for here, by name: the compiler does not know of the loads
-    // to LDS and would wait for Q* at its uses inside the loop, in every block,
-    // which there means for the blocks in flight.
-#pragma unroll
-    for (int k = 0; k < kDK / 16; ++k)
-        in_registers(q[k]);
-    in_registers(mask);
-    for (int i = 1; i < min(kRing - 1, n_blocks); ++i)
-        load_block(i);
-    int next_page = kRing - 1 < n_blocks ? page_of(kRing - 1) : 0;
-
-    floatx16 o[kDV / 32];
-#pragma unroll
-    for (int c = 0; c < kDV / 32; ++c) {
-        o[c] = floatx16{};
-        in_accumulators(o[c]);
-    }
-    float m = -INFINITY, l = 0.0f;
-
     // LDS addresses, less the slot's, of the lane's operands. A chunk's place
     // differs from chunk 0's in the same row only by an XOR of its low four
     // bits and an offset of the others, so one address each serves all chunks.
@@ -193,17 +162,121 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
         const int j = lane & 15, r = 8 * h + 4 * hl + (j >> 2);
         v_lane[h] = r * (kDV * 2) + 16 * ((2 * ((lane >> 4) & 1) + ((j & 3) >> 1)) ^ key_swizzle(r)) + 8 * (j & 1);
     }
+    // Operand k of the 32 rows in a ring slot: values 16 k + 8 hl .. +7 of the lane's row.
+    auto row_operand = [&](unsigned slot_at, int k) -> E8 {
+        return k < kDV / 16 ? lds_load<E8>(((slot_at + k_lane) ^ (32 * (k & 7))) + 256 * (k >> 3))
+                            : lds_load<E8>((slot_at + rope_lane) ^ (32 * (k - kDV / 16)));
+    };
+
+    // Q*: the B operand of S^T, whole rows in registers, staged through the
+    // wave's own ring slot by whole rows like a cache block (loaded into
+    // registers at once, every load touched 32 rows of memory).
+    const bool busy = rt * kRows + 32 * wave < live;  // else all the wave's rows are padding
+    E8 q[kDK / 16] = {};
+    unsigned long long mask = 0;
+    if (busy) {
+        const int first = rt * kRows + 32 * wave, lim = min(31, live - 1 - first);  // rows past the drafts re-read the last
+        const E *src = wave_uniform((const E *)a.q + ((size_t)b * rows + first) * kDK);
+        const unsigned own = ring + wave * (kSlotElems * 2);
+#pragma unroll
+        for (int r = 0; r < 32; ++r)
+            global_to_lds16_at(src, min(r, lim) * (kDK * 2) + 16 * (lane ^ key_swizzle(r)), own + r * (kDV * 2));
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int r = 8 * u + (lane >> 3);
+            global_to_lds16_at(src, min(r, lim) * (kDK * 2) + 2 * (kDV + 8 * ((lane & 7) ^ rope_swizzle(r))),
+                               own + 2 * kRopeElems + 1024 * u);
+        }
+        mask = a.tree_mask[(size_t)b * a.drafts + min(row, live - 1) / a.num_heads];
+        MLA_WAIT_VMCNT(0);
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int k = 0; k < kDK / 16; ++k)
+            q[k] = row_operand(own, k);
+    }
+    // waited for here, by name: the compiler does not know of the loads to LDS
+    // and would wait at the uses inside the loop, in every block
+    in_registers(mask);
+#pragma unroll
+    for (int k = 0; k < kDK / 16; ++k)
+        in_registers(q[k]);
+    lds_barrier();  // the ring is free
+    for (int i = 0; i < min(kRing - 1, n_blocks); ++i) {
+        const E *src = block_source(i, page_of(i));
+#pragma unroll
+        for (int u = 0; u < kUnitsPerWave; ++u)
+            load_unit(src, i, u);
+    }
+    // A drafted token that a row does not see meets it with weight 0: 0 times
+    // an infinity or NaN in its row would still be NaN, so those become 0 for
+    // the second product, once every wave has block i's logits. A row that does
+    // see such a token has its sum l a NaN from the first product already.
+    auto drop_not_finite = [&](int i) {
+        constexpr int kEach = kBlock * kDV / 8 / 256;  // 16-byte pieces of a thread
+        uint4 *at = (uint4 *)(s_ring + (i & (kRing - 1)) * kSlotElems) + threadIdx.x;
+        uint4 v[kEach];
+#pragma unroll
+        for (int u = 0; u < kEach; ++u)
+            v[u] = at[256 * u];
+        unsigned top = 0;  // the largest magnitude's bits, both halves
+#pragma unroll
+        for (int u = 0; u < kEach; ++u)
+            for (unsigned w : {v[u].x, v[u].y, v[u].z, v[u].w})
+                top = max_u16x2(top, w & 0x7fff7fffu);
+        if (not_finite<E>((unsigned short)top) || not_finite<E>((unsigned short)(top >> 16))) {
+#pragma unroll
+            for (int u = 0; u < kEach; ++u) {
+                for (unsigned *w : {&v[u].x, &v[u].y, &v[u].z, &v[u].w}) {
+                    *w &= not_finite<E>((unsigned short)*w) ? 0xffff0000u : ~0u;
+                    *w &= not_finite<E>((unsigned short)(*w >> 16)) ? 0xffffu : ~0u;
+                }
+                at[256 * u] = v[u];
+            }
+        }
+        lds_barrier();
+    };
+    // a block that holds drafted tokens, or the request's end
+    auto is_edge = [&](int i) { return t_lo + (i + 1) * kBlock > context; };
+    if (!busy) {  // loads its share, and passes the same barriers
+        if (n_blocks > 0) {
+            MLA_WAIT_VMCNT(0);
+            lds_barrier();
+        }
+        for (int i = 0; i < n_blocks; ++i) {
+            MLA_WAIT_VMCNT(0);
+            lds_barrier();
+            if (i + kRing - 1 < n_blocks) {
+                const E *src = block_source(i + kRing - 1, page_of(i + kRing - 1));
+#pragma unroll
+                for (int u = 0; u < kUnitsPerWave; ++u)
+                    load_unit(src, i + kRing - 1, u);
+            }
+            if (is_edge(i))
+                drop_not_finite(i);
+        }
+        if (rq.n_splits == 1 && part == 0 && row < rows)
+            for (int k = hl; k < kDV / 8; k += 2)
+                *(uint4 *)(out + (size_t)row * kDV + 8 * k) = uint4{0, 0, 0, 0};
+        return;
+    }
+
+    int next_page = kRing - 1 < n_blocks ? page_of(kRing - 1) : 0;
+
+    floatx16 o[kTiles];
+#pragma unroll
+    for (int c = 0; c < kTiles; ++c) {
+        o[c] = floatx16{};
+        in_accumulators(o[c]);
+    }
+    float m = -INFINITY, l = 0.0f;
+
     // S^T of block i, with side(k) between the products: what does not depend
     // on them, in their shadow (a product takes 32 cycles and one issue slot of
     // 4). Each operand is read kAhead products before its own. The products go
     // to ordinary registers: O* fills the accumulation registers.
     auto logits = [&](int i, auto &&side) -> floatx16 {
         const unsigned blk = ring + (i & (kRing - 1)) * (kSlotElems * 2);
-        const unsigned k_at = blk + k_lane, rope_at = blk + rope_lane;
-        auto k_operand = [&](int k) -> E8 {  // values 16 k + 8 hl .. +7 of the lane's key
-            return k < kDV / 16 ? lds_load<E8>((k_at ^ (32 * (k & 7))) + 256 * (k >> 3))
-                                : lds_load<E8>(rope_at ^ (32 * (k - kDV / 16)));
-        };
+        auto k_operand = [&](int k) -> E8 { return row_operand(blk, k); };
         E8 kv[kAhead + 1];
         floatx16 s;
 #pragma unroll
@@ -258,8 +331,7 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
         next_page = i + kRing < n_blocks ? page_of(i + kRing) : 0;
 
         const int t0 = t_lo + i * kBlock;
-        const bool edge = t0 + kBlock > context;  // holds drafted tokens, or the end
-        if (edge) {
+        if (is_edge(i)) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 const int t = t0 + key_of_reg(r, hl);
@@ -268,31 +340,7 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
                 s[r] = seen ? s[r] : -INFINITY;
             }
             most = largest(s);
-            // A drafted token that a row does not see meets it with weight 0:
-            // 0 times an infinity or NaN in its row would still be NaN, so
-            // those become 0 for the second product. A row that does see such
-            // a token has its sum l a NaN from the first product already.
-            E *blk = s_ring + (i & (kRing - 1)) * kSlotElems;
-            for (int u = threadIdx.x; u < kBlock * kDV / 8; u += 256) {
-                uint4 *at = (uint4 *)(blk + 8 * u);
-                uint4 v = *at;
-                unsigned *w = (unsigned *)&v;
-                bool bad = false;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    if (not_finite<E>((unsigned short)w[k])) {
-                        w[k] &= 0xffff0000u;
-                        bad = true;
-                    }
-                    if (not_finite<E>((unsigned short)(w[k] >> 16))) {
-                        w[k] &= 0xffffu;
-                        bad = true;
-                    }
-                }
-                if (bad)
-                    *at = v;
-            }
-            lds_barrier();
+            drop_not_finite(i);
         }
         most = reduce_halves(most, [](float x, float y) { return fmaxf(x, y); }) * a.scale_log2;
         // the reference moves only past kLazyRescale, so P is at most 2^8
@@ -301,12 +349,14 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
             const float f = next == -INFINITY ? 1.0f : fast_exp2(m - next);
             m = next;
             l *= f;
+            if (i > 0) {  // before, O* is zero
 #pragma unroll
-            for (int c = 0; c < kDV / 32; ++c) {
-                in_accumulators(o[c]);
-                o[c] *= f;
-                in_accumulators(o[c]);
-                __builtin_amdgcn_sched_barrier(0);
+                for (int c = 0; c < kTiles; ++c) {
+                    in_accumulators(o[c]);
+                    o[c] *= f;
+                    in_accumulators(o[c]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
             }
         }
         const float ref = m == -INFINITY ? 0.0f : m;
@@ -331,16 +381,16 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
         const E8 pb[2] = {p_operand<E>(p), p_operand<E>(p + 8)};
 
         const unsigned blk = ring + (i & (kRing - 1)) * (kSlotElems * 2);
-        const unsigned v_at[2] = {blk + v_lane[0], blk + v_lane[1]};
+        const unsigned v_at[2] = {blk + v_lane[0] + part * (kTiles * 64), blk + v_lane[1] + part * (kTiles * 64)};
         auto v_operand = [&](int u) -> E8 {  // 32 columns of tile c, keys 16 ks .. +15 in the order of P's registers
-            const int ks = u / (kDV / 32), c = u % (kDV / 32);
+            const int ks = u / kTiles, c = u % kTiles;
             E4 part[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h)
                 part[h] = lds_load_tr16<E>((v_at[h] ^ (64 * (c & 3))) + 256 * (c >> 2) + 16 * ks * (kDV * 2));
             return E8{part[0][0], part[0][1], part[0][2], part[0][3], part[1][0], part[1][1], part[1][2], part[1][3]};
         };
-        constexpr int kOps = 2 * kDV / 32;
+        constexpr int kOps = 2 * kTiles;
         E8 v[kAhead + 1];
 #pragma unroll
         for (int u = 0; u < kAhead; ++u)
@@ -350,18 +400,19 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
         for (int u = 0; u < kOps; ++u) {
             if (u + kAhead < kOps)
                 v[(u + kAhead) % (kAhead + 1)] = v_operand(u + kAhead);
-            floatx16 &acc = o[u % (kDV / 32)];
-            acc = mfma32x32x16(v[u % (kAhead + 1)], pb[u / (kDV / 32)], acc);
+            floatx16 &acc = o[u % kTiles];
+            acc = mfma32x32x16(v[u % (kAhead + 1)], pb[u / kTiles], acc);
             in_accumulators(acc);
-            if (u > 0 && u < 16)
-                most = fmaxf(most, ahead[u]);
+#pragma unroll
+            for (int r = u * 16 / kOps; r < (u + 1) * 16 / kOps; ++r)
+                most = fmaxf(most, ahead[r]);
             __builtin_amdgcn_sched_barrier(0);
         }
         s = ahead;
     }
 
 #pragma unroll
-    for (int c = 0; c < kDV / 32; ++c)
+    for (int c = 0; c < kTiles; ++c)
         in_accumulators(o[c]);
     l = reduce_halves(l, [](float x, float y) { return x + y; });
     if (rq.n_splits == 1) {
@@ -369,45 +420,51 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
         const float inv = l == 0.0f || row >= live ? 0.0f : 1.0f / l;
         if (row < rows) {
 #pragma unroll
-            for (int c = 0; c < kDV / 32; ++c) {
+            for (int c = 0; c < kTiles; ++c) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     E4 v;
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
                         v[j] = row < live ? (E)(o[c][4 * k + j] * inv) : (E)0.0f;
-                    *(E4 *)(out + (size_t)row * kDV + 32 * c + 8 * k + 4 * hl) = v;
+                    *(E4 *)(out + (size_t)row * kDV + 32 * (part * kTiles + c) + 8 * k + 4 * hl) = v;
                 }
             }
         }
         return;
     }
     const size_t tile = (size_t)slot * a.row_tiles + rt;
-    float *po = a.part_o + (tile * kWaves + wave) * (32 * kDV);
+    float *po = a.part_o + (tile * kWaves + wave) * (32 * kDV) + part * (kTiles * 1024);
 #pragma unroll
-    for (int c = 0; c < kDV / 32; ++c)
+    for (int c = 0; c < kTiles; ++c)
 #pragma unroll
         for (int k = 0; k < 4; ++k)
             *(floatx4 *)(po + ((c * 4 + k) * 64 + lane) * 4) =
                 floatx4{o[c][4 * k], o[c][4 * k + 1], o[c][4 * k + 2], o[c][4 * k + 3]};
-    if (hl == 0) {
+    if (hl == 0 && part == 0) {
         a.part_m[tile * kRows + 32 * wave + r32] = m;
         a.part_l[tile * kRows + 32 * wave + r32] = l;
     }
 }
 
-// Merges the splits of a request (those of more than one): a wave takes 32 rows x 32
-// columns, and a lane the 16 values it would hold in the split kernel.
+// Merges the splits of a request (those of more than one). A workgroup takes 32
+// rows x 32 columns; wave w the splits w, w + 4, .., and a lane the 16 values it
+// would hold in the split kernel. The waves' sums meet in LDS. The order of the
+// additions depends on the split count alone.
+constexpr int kMany = 4;  // splits of a wave in flight together
+
 template <typename E>
 __global__ __launch_bounds__(256) void tree_combine_kernel(TreeArgs a)
 {
     using E4 = typename Vec<E>::v4;
+    __shared__ float s_m[kWaves][32];
+    __shared__ float s_l[kWaves][32];
+    __shared__ floatx4 s_o[kWaves][4][64];
     const int lane = threadIdx.x & 63;
-    const int item = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int item = blockIdx.x;
     const int c = item & 15, w = (item >> 4) & 3, rest = item >> 6;
-    const int rt = rest % a.row_tiles, b = rest / a.row_tiles;  // wave-uniform, as Request::read asks
-    if (b >= a.batch)
-        return;
+    const int rt = rest % a.row_tiles, b = rest / a.row_tiles;
     Request rq;
     rq.read(a, b);
     if (rq.n_splits == 1)
@@ -415,52 +472,129 @@ __global__ __launch_bounds__(256) void tree_combine_kernel(TreeArgs a)
     const int rows = a.drafts * a.num_heads, live = rq.drafts * a.num_heads;
     const int r32 = lane & 31, hl = lane >> 5;
     const int row = rt * kRows + 32 * w + r32;
-    E *out = (E *)a.out + ((size_t)b * rows + row) * kDV + 32 * c + 4 * hl;
     floatx4 acc[4] = {};
     float m = -INFINITY, l = 0.0f;
-    if (rt * kRows < live) {
-        for (int s = 0; s < rq.n_splits; ++s)
-            m = fmaxf(m, a.part_m[((size_t)(rq.slot0 + s) * a.row_tiles + rt) * kRows + 32 * w + r32]);
-        const float ref = m == -INFINITY ? 0.0f : m;
-        for (int s = 0; s < rq.n_splits; ++s) {
-            const size_t tile = (size_t)(rq.slot0 + s) * a.row_tiles + rt;
-            const float f = fast_exp2(a.part_m[tile * kRows + 32 * w + r32] - ref);
-            l += f * a.part_l[tile * kRows + 32 * w + r32];
-            const float *po = a.part_o + (tile * kWaves + w) * (32 * kDV);
+    if (rt * kRows + 32 * w < live) {  // else no wave has left partials of these rows
+        // past the last split a wave repeats it with weight 0
+        const size_t tile0 = (size_t)rq.slot0 * a.row_tiles + rt;
+        auto at = [&](int s) { return tile0 + (size_t)min(s, rq.n_splits - 1) * a.row_tiles; };
+        for (int s = wave; s < rq.n_splits; s += kWaves * kMany) {
+            float ms[kMany], ls[kMany];
+            floatx4 po[kMany][4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-                acc[k] += f * *(const floatx4 *)(po + ((c * 4 + k) * 64 + lane) * 4);
+            for (int k = 0; k < kMany; ++k) {
+                const size_t t = at(s + kWaves * k);
+                ms[k] = a.part_m[t * kRows + 32 * w + r32];
+                ls[k] = a.part_l[t * kRows + 32 * w + r32];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    po[k][j] = *(const floatx4 *)(a.part_o + (t * kWaves + w) * (32 * kDV) + ((c * 4 + j) * 64 + lane) * 4);
+            }
+            float next = m;
+#pragma unroll
+            for (int k = 0; k < kMany; ++k)
+                next = fmaxf(next, ms[k]);
+            const float ref = next == -INFINITY ? 0.0f : next;
+            const float f0 = fast_exp2(m - ref);
+            l *= f0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                acc[j] *= f0;
+#pragma unroll
+            for (int k = 0; k < kMany; ++k) {
+                if (s + kWaves * k >= rq.n_splits)
+                    continue;
+                const float f = fast_exp2(ms[k] - ref);
+                l += f * ls[k];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    acc[j] += f * po[k][j];
+            }
+            m = next;
         }
+    }
+    if (hl == 0) {
+        s_m[wave][r32] = m;
+        s_l[wave][r32] = l;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        s_o[wave][j][lane] = acc[j];
+    __syncthreads();
+    // wave j: the 4 columns of quarter j of each lane
+    float top = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < kWaves; ++k)
+        top = fmaxf(top, s_m[k][r32]);
+    const float ref = top == -INFINITY ? 0.0f : top;
+    floatx4 sum = {};
+    l = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kWaves; ++k) {
+        const float f = fast_exp2(s_m[k][r32] - ref);
+        l += f * s_l[k][r32];
+        sum += f * s_o[k][wave][lane];
     }
     if (row >= rows)
         return;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    E4 v;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        E4 v;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            v[j] = row < live ? (E)(acc[k][j] * inv) : (E)0.0f;
-        *(E4 *)(out + 8 * k) = v;
-    }
+    for (int j = 0; j < 4; ++j)
+        v[j] = row < live ? (E)(sum[j] * inv) : (E)0.0f;
+    *(E4 *)((E *)a.out + ((size_t)b * rows + row) * kDV + 32 * c + 8 * wave + 4 * hl) = v;
 }
 
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
 struct TreePlan {
     int row_tiles, chunk, n_slots;
+    int parts;  // column parts: 1 or 4
     size_t o_bytes, ml_bytes;
 };
 
-// Splits: as many workgroups as CUs, no shorter than 4 blocks.
-TreePlan tree_plan(int batch, int drafts, int num_heads, int total_tokens, int num_splits, int cu_count)
+// Splits of a request of mean length, and column parts: those with the least
+// modelled time. A workgroup costs its start and end (Q*, the first block, its
+// results) besides its blocks, and one runs on a CU at a time. Workgroups that fit
+// the CUs at once take one round; else those of one request come in whole
+// rounds, and those of a batch, of unequal lengths, follow each other with about
+// 0.7 of a round to fill at the end (a request's last split is a part of one:
+// half a split more a request). Partials (fp32, written and read) and the second
+// launch are the price of a split.
+struct PartCost {
+    int parts;
+    double start_us, block_us;
+};
+constexpr PartCost kPartCosts[2] = {{1, 7.0, 1.8}, {4, 5.0, 1.0}};
+constexpr double kCombineUs = 3.5, kPartialUsPerByte = 0.2e-6;
+
+TreePlan compute_tree_plan(int batch, int drafts, int num_heads, int total_tokens, int num_splits, int cu_count)
 {
     TreePlan p;
     p.row_tiles = (drafts * num_heads + kRows - 1) / kRows;
-    const int longest = (total_tokens + batch - 1) / batch;  // mean
-    int splits = num_splits;
-    if (splits <= 0)
-        splits = std::max(1, std::min(cu_count / std::max(1, p.row_tiles * batch), longest / (4 * kBlock)));
+    const int longest = (int)(((int64_t)total_tokens + batch - 1) / batch);  // mean
+    const int blocks = std::max(1, (longest + kBlock - 1) / kBlock);
+    int splits = 1;
+    double best = 0.0;
+    for (const PartCost &c : kPartCosts) {
+        const int lo = num_splits > 0 ? num_splits : 1, hi = num_splits > 0 ? num_splits : std::min(blocks, 256);
+        for (int n = lo; n <= hi; ++n) {
+            const int per = (blocks + n - 1) / n;
+            if (n > lo && (blocks + n - 2) / (n - 1) == per)
+                continue;  // no shorter than the one before
+            const double each = batch == 1 ? n : n == 1 ? 1.0 : n + 0.5;
+            const double wgs = each * batch * p.row_tiles * c.parts / cu_count;
+            const double rounds = wgs <= 1.0 ? 1.0 : batch == 1 ? std::ceil(wgs) : wgs + 0.7;
+            double us = rounds * (c.start_us + per * c.block_us);
+            if (n > 1)
+                us += kCombineUs + kPartialUsPerByte * n * batch * drafts * num_heads * (kDV * 4.0);
+            if (best == 0.0 || us < best) {
+                best = us;
+                splits = n;
+                p.parts = c.parts;
+            }
+        }
+    }
     int64_t chunk = (longest + splits - 1) / splits;
     chunk = std::max<int64_t>(kBlock, (chunk + kBlock - 1) / kBlock * kBlock);
     p.chunk = (int)chunk;
@@ -471,6 +605,20 @@ TreePlan tree_plan(int batch, int drafts, int num_heads, int total_tokens, int n
     return p;
 }
 
+// The last plan of each host thread: a call asks for it twice (the workspace's
+// size, then the launch), and a decode loop repeats its sizes.
+TreePlan tree_plan(int batch, int drafts, int num_heads, int total_tokens, int num_splits, int cu_count)
+{
+    thread_local int key[6] = {0, 0, 0, 0, 0, 0};
+    thread_local TreePlan plan;
+    const int now[6] = {batch, drafts, num_heads, total_tokens, num_splits, cu_count};
+    if (!std::equal(key, key + 6, now)) {
+        plan = compute_tree_plan(batch, drafts, num_heads, total_tokens, num_splits, cu_count);
+        std::copy(now, now + 6, key);
+    }
+    return plan;
+}
+
 bool tree_sizes_ok(int batch, int drafts, int num_heads, int total_tokens)
 {
     return batch >= 1 && drafts >= 1 && drafts <= kMaxDrafts && num_heads > 0 && num_heads % 16 == 0 &&
@@ -478,11 +626,12 @@ bool tree_sizes_ok(int batch, int drafts, int num_heads, int total_tokens)
 }
 
 template <typename E>
-void launch_tree(const TreeArgs &a, hipStream_t s)
+void launch_tree(const TreeArgs &a, int parts, hipStream_t s)
 {
-    hipLaunchKernelGGL(tree_kernel<E>, dim3((a.n_slots + 7) / 8 * 8 * a.row_tiles), dim3(256), 0, s, a);
+    auto k = parts == 4 ? tree_kernel<E, 4> : tree_kernel<E, 16>;
+    hipLaunchKernelGGL(k, dim3((unsigned)((a.n_slots + 7) / 8 * 8) * a.row_tiles * parts), dim3(256), 0, s, a);
     if (a.total_tokens > a.chunk)
-        hipLaunchKernelGGL(tree_combine_kernel<E>, dim3(a.batch * a.row_tiles * 16), dim3(256), 0, s, a);
+        hipLaunchKernelGGL(tree_combine_kernel<E>, dim3((unsigned)a.batch * a.row_tiles * (kWaves * kDV / 32)), dim3(256), 0, s, a);
 }
 
 int decode_tree(bool bf16, const void *query, const void *kv_cache, const int *block_table, const int *cu_seqlens,
@@ -497,7 +646,7 @@ int decode_tree(bool bf16, const void *query, const void *kv_cache, const int *b
     if (!aligned16(query) || !aligned16(kv_cache) || !aligned16(out) || !aligned16(workspace))
         return MLA_STATUS_MISALIGNED;
     const TreePlan p = tree_plan(batch, drafts, num_heads, total_tokens, num_splits, current_cu_count());
-    if ((int64_t)(p.n_slots + 7) * p.row_tiles > INT32_MAX / 256 || (int64_t)batch * p.row_tiles > INT32_MAX / 4096)
+    if ((int64_t)(p.n_slots + 7) * p.row_tiles > INT32_MAX / (256 * 4) || (int64_t)batch * p.row_tiles > INT32_MAX / (256 * 64))
         return MLA_STATUS_INVALID_VALUE;
     if (workspace_bytes < p.o_bytes + 2 * p.ml_bytes)
         return MLA_STATUS_WORKSPACE_TOO_SMALL;
@@ -525,9 +674,9 @@ int decode_tree(bool bf16, const void *query, const void *kv_cache, const int *b
     a.bt_stride = block_table_stride;
     a.scale_log2 = (float)(1.4426950408889634 / std::sqrt(192.0));
     if (bf16)
-        launch_tree<__bf16>(a, static_cast<hipStream_t>(stream));
+        launch_tree<__bf16>(a, p.parts, static_cast<hipStream_t>(stream));
     else
-        launch_tree<_Float16>(a, static_cast<hipStream_t>(stream));
+        launch_tree<_Float16>(a, p.parts, static_cast<hipStream_t>(stream));
     const hipError_t e = hipPeekAtLastError();
     return e == hipSuccess ? MLA_STATUS_SUCCESS : record_hip_error(e);
 }
