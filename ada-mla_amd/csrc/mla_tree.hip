@@ -51,6 +51,7 @@ struct TreeArgs {
     int chunk;      // tokens per split
     int row_tiles;  // of 128 rows, per request
     int n_slots;    // total_tokens / chunk + batch
+    int by_xcd;     // 1: the workgroups of a slot share an XCD
     int page_shift, num_pages, bt_stride;
     float scale_log2;
 };
@@ -85,11 +86,12 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
     const int r32 = lane & 31, hl = lane >> 5;
     const unsigned ring = lds_address(s_ring);
 
-    // workgroup -> (slot, row tile, column part): the workgroups of a slot,
-    // which read the same tokens, get ids equal mod 8, i.e. one XCD and its L2
+    // workgroup -> (slot, row tile, column part). With by_xcd the workgroups of
+    // a slot, which read the same tokens, get ids equal mod 8, i.e. one XCD and its L2.
     const int per_slot = a.row_tiles * kParts;
-    const int slot = (blockIdx.x >> 3) / per_slot * 8 + (blockIdx.x & 7);
-    const int within = (blockIdx.x >> 3) % per_slot;
+    const int id = a.by_xcd ? blockIdx.x >> 3 : blockIdx.x;
+    const int slot = a.by_xcd ? id / per_slot * 8 + (blockIdx.x & 7) : id / per_slot;
+    const int within = id % per_slot;
     const int rt = within / kParts, part = within % kParts;
     if (slot >= a.n_slots)
         return;
@@ -566,7 +568,7 @@ struct PartCost {
     double start_us, block_us;
 };
 constexpr PartCost kPartCosts[2] = {{1, 7.0, 1.8}, {4, 5.0, 1.0}};
-constexpr double kCombineUs = 3.5, kPartialUsPerByte = 0.2e-6;
+constexpr double kCombineUs = 3.5, kSplitUs = 0.06, kPartialUsPerByte = 0.2e-6;
 
 TreePlan compute_tree_plan(int batch, int drafts, int num_heads, int total_tokens, int num_splits, int cu_count)
 {
@@ -584,10 +586,10 @@ TreePlan compute_tree_plan(int batch, int drafts, int num_heads, int total_token
                 continue;  // no shorter than the one before
             const double each = batch == 1 ? n : n == 1 ? 1.0 : n + 0.5;
             const double wgs = each * batch * p.row_tiles * c.parts / cu_count;
-            const double rounds = wgs <= 1.0 ? 1.0 : batch == 1 ? std::ceil(wgs) : wgs + 0.7;
+            const double rounds = wgs <= (batch == 1 ? 1.0 : 1.1) ? 1.0 : batch == 1 ? std::ceil(wgs) : wgs + 0.7;
             double us = rounds * (c.start_us + per * c.block_us);
             if (n > 1)
-                us += kCombineUs + kPartialUsPerByte * n * batch * drafts * num_heads * (kDV * 4.0);
+                us += kCombineUs + kSplitUs * n + kPartialUsPerByte * n * batch * drafts * num_heads * (kDV * 4.0);
             if (best == 0.0 || us < best) {
                 best = us;
                 splits = n;
@@ -625,11 +627,18 @@ bool tree_sizes_ok(int batch, int drafts, int num_heads, int total_tokens)
            num_heads <= 4096 && total_tokens >= 0 && total_tokens <= INT32_MAX - 4096;
 }
 
+// Slots from which on a slot's workgroups share an XCD: 16 requests of 16 drafts
+// x 128 heads 222 -> 164 us, 23 of 30 x 64 120 -> 94. With fewer slots the
+// XCDs would take one or two each, or none: 32 drafts x 128 heads over 50021 tokens
+// in 8 splits 441 us against 414, in one split 8.7 ms against 2.1.
+constexpr int kMinSlotsByXcd = 16;
+
 template <typename E>
 void launch_tree(const TreeArgs &a, int parts, hipStream_t s)
 {
     auto k = parts == 4 ? tree_kernel<E, 4> : tree_kernel<E, 16>;
-    hipLaunchKernelGGL(k, dim3((unsigned)((a.n_slots + 7) / 8 * 8) * a.row_tiles * parts), dim3(256), 0, s, a);
+    const unsigned slots = a.by_xcd ? (a.n_slots + 7) / 8 * 8 : a.n_slots;
+    hipLaunchKernelGGL(k, dim3(slots * a.row_tiles * parts), dim3(256), 0, s, a);
     if (a.total_tokens > a.chunk)
         hipLaunchKernelGGL(tree_combine_kernel<E>, dim3((unsigned)a.batch * a.row_tiles * (kWaves * kDV / 32)), dim3(256), 0, s, a);
 }
@@ -669,6 +678,7 @@ int decode_tree(bool bf16, const void *query, const void *kv_cache, const int *b
     a.chunk = p.chunk;
     a.row_tiles = p.row_tiles;
     a.n_slots = p.n_slots;
+    a.by_xcd = p.n_slots >= kMinSlotsByXcd;
     a.page_shift = __builtin_ctz((unsigned)page_size);
     a.num_pages = num_pages;
     a.bt_stride = block_table_stride;
