@@ -367,6 +367,17 @@ int64_t used_stride(const at::Tensor &t, int64_t d, int64_t least)
     return t.size(d) == 1 ? least : t.stride(d);
 }
 
+// A contiguous 1-D tensor of n entries in base's storage, `at` bytes into it: the small
+// outputs of a call share one allocation, which costs a call as much host time as all of them.
+at::Tensor part_of(const at::Tensor &base, size_t at_bytes, int64_t n, at::ScalarType type)
+{
+    at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(base.storage()), base.key_set(),
+                                                            c10::scalarTypeToTypeMeta(type));
+    t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+    t.unsafeGetTensorImpl()->set_storage_offset(static_cast<int64_t>(at_bytes / c10::elementSize(type)));
+    return t;
+}
+
 // No reference counterpart: block table, slots and positions of a step's tokens.
 std::vector<at::Tensor> paged_tables(const at::Tensor &context_in, const at::Tensor &new_in, at::Tensor block_table,
                                          const at::Tensor &free_pages_in, const at::Tensor &free_start_in,
@@ -390,10 +401,14 @@ std::vector<at::Tensor> paged_tables(const at::Tensor &context_in, const at::Ten
     check_devices({&context_in, &new_in, &block_table, &free_pages_in, &free_start_in}, fn);
     const at::OptionalDeviceGuard guard(context_in.device());
     const at::Tensor context = context_in.contiguous(), fresh = new_in.contiguous(), pages = free_pages_in.contiguous();
-    const auto opt = context.options();
-    at::Tensor cu_seqlens = at::empty({batch + 1}, opt), cu_new = at::empty({batch + 1}, opt);
-    at::Tensor slots = at::empty({total_new}, opt.dtype(at::kLong)), positions = at::empty({total_new}, opt);
-    at::Tensor free_next = at::empty({1}, opt);
+    // slots, then positions, cu_seqlens, cu_new and free_next, each from a multiple of 16 bytes on
+    auto up = [](int64_t n) { return static_cast<size_t>((n + 15) / 16 * 16); };
+    const size_t at_pos = up(8 * total_new), at_cu = at_pos + up(4 * total_new), at_new = at_cu + up(4 * (batch + 1));
+    const size_t at_next = at_new + up(4 * (batch + 1));
+    const at::Tensor all = workspace(at_next + 16, context);
+    at::Tensor slots = part_of(all, 0, total_new, at::kLong), positions = part_of(all, at_pos, total_new, at::kInt);
+    at::Tensor cu_seqlens = part_of(all, at_cu, batch + 1, at::kInt), cu_new = part_of(all, at_new, batch + 1, at::kInt);
+    at::Tensor free_next = part_of(all, at_next, 1, at::kInt);
     check_status(mla_paged_tables(context.data_ptr<int>(), fresh.data_ptr<int>(), pages.data_ptr<int>(),
                                     free_start_in.data_ptr<int>(), block_table.data_ptr<int>(),
                                     cu_seqlens.data_ptr<int>(), cu_new.data_ptr<int>(),
