@@ -34,10 +34,12 @@ __device__ __forceinline__ floatx16 mfma32x32x16(bf16x8 a, bf16x8 b, floatx16 c)
 // The same product accumulated in ordinary registers, for a kernel whose other
 // accumulators fill the accumulation registers (the compiler puts all of a kernel's
 // products there, and moves them back and forth when they do not fit).
-// A chain: first (C = 0), next .., then settle before anything reads the tile:
-// a product's result may be read 11 slots after an 8-pass product (16 here),
-// which the compiler knows of its own products only. Within a chain each
-// product's accumulator is exactly the last one's result, which needs no wait.
+// A chain: first (C = 0), next .., then settle, before anything reads the tile: a
+// product's result may be read 11 slots after an 8-pass product (16 here), which
+// the compiler knows of its own products only; nor does it know that an operand
+// which a vector instruction wrote may be read 2 slots later. Operands therefore
+// come from LDS or are never moved, which a test of the assembly checks. Within a chain
+// each product's accumulator is exactly the last one's result, which needs no wait.
 __device__ __forceinline__ void mfma32x32x16_first(floatx16 &d, half8 a, half8 b)
 {
     asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, 0" : "=&v"(d) : "v"(a), "v"(b));
@@ -169,11 +171,17 @@ __device__ __forceinline__ T scalar_load(const T *p)
     return *(const __attribute__((address_space(4))) T *)p;
 }
 
-// A read, and a transpose read (lds_read_tr16), at an LDS byte address.
+// A read, a write, and a transpose read (lds_read_tr16), at an LDS byte address.
 template <typename T>
 __device__ __forceinline__ T lds_load(unsigned addr)
 {
     return *(const MLA_LDS T *)(uintptr_t)addr;
+}
+
+template <typename T>
+__device__ __forceinline__ void lds_store(unsigned addr, T v)
+{
+    *(MLA_LDS T *)(uintptr_t)addr = v;
 }
 
 template <typename E>

@@ -49,22 +49,36 @@ struct PrefillArgs {
 
 __device__ __forceinline__ int clamped(const int *cu, int b, int most) { return min(max(cu[b], 0), most); }
 
+// Sequence b's range in cu, and its range in another one.
+struct Owner {
+    int b, lo, hi, other_lo, other_hi;
+};
+
 // The last b < batch with cu[b] / unit + b <= slot, by the whole wave: the
 // sequence that owns this slot where each takes the slots from cu[b] / unit +
 // b on. That numbering needs no prefix sums of rounded lengths, and no two
-// sequences' slots meet.
-__device__ __forceinline__ int owner_of_slot(const int *cu, int batch, int most, int unit, int slot, int lane)
+// sequences' slots meet. The ranges come with it, in one round trip.
+__device__ __forceinline__ Owner owner_of_slot(const int *cu, int most, const int *other, int other_most, int batch,
+                                               int unit, int slot, int lane)
 {
-    int b = 0;
+    Owner w = {};
     for (int base = 0; base < batch; base += 64) {
-        const int i = base + lane;
-        const unsigned long long m = __builtin_amdgcn_ballot_w64(i < batch && clamped(cu, i, most) / unit + i <= slot);
-        if (m != 0)
-            b = base + 63 - __builtin_clzll(m);
+        const int i = min(base + lane, batch - 1);
+        const int lo = clamped(cu, i, most), hi = max(clamped(cu, i + 1, most), lo);
+        const int other_lo = clamped(other, i, other_most), other_hi = max(clamped(other, i + 1, other_most), other_lo);
+        const unsigned long long m = __builtin_amdgcn_ballot_w64(base + lane < batch && lo / unit + i <= slot);
+        if (m != 0) {
+            const int k = 63 - __builtin_clzll(m);
+            w.b = base + k;
+            w.lo = __builtin_amdgcn_readlane(lo, k);
+            w.hi = __builtin_amdgcn_readlane(hi, k);
+            w.other_lo = __builtin_amdgcn_readlane(other_lo, k);
+            w.other_hi = __builtin_amdgcn_readlane(other_hi, k);
+        }
         if (m != ~0ull)
             break;
     }
-    return __builtin_amdgcn_readfirstlane(b);
+    return w;
 }
 
 // ---- expansion --------------------------------------------------------------
@@ -134,9 +148,8 @@ expand_kernel(PrefillArgs a)
     // ring slot, 32 at a time, then into registers (chunk c of row r at c ^ (r
     // mod 16)). Loaded into registers at once, every load touched 32 rows: 18 us
     // a workgroup with all CUs loading. Rows past the sequence are zeros.
-    const int b = owner_of_slot(a.cu_seqlens, a.batch, a.total_tokens, kTile, tile, lane);
-    const int seq_lo = clamped(a.cu_seqlens, b, a.total_tokens);
-    const int len = max(clamped(a.cu_seqlens, b + 1, a.total_tokens), seq_lo) - seq_lo;
+    const Owner w = owner_of_slot(a.cu_seqlens, a.total_tokens, a.cu_seqlens, a.total_tokens, a.batch, kTile, tile, lane);
+    const int b = w.b, seq_lo = w.lo, len = w.hi - w.lo;
     const int t0 = (tile - seq_lo / kTile - b) * kTile;
     const bool live = tile < tiles && t0 < len;  // else nobody reads this tile
     if (!__syncthreads_or(live))
@@ -293,6 +306,66 @@ expand_kernel(PrefillArgs a)
 
 // ---- attention --------------------------------------------------------------
 
+// A workgroup's queries: q0 .. of one sequence, and its keys.
+struct QueryTile {
+    int q_lo, n_q, q0;  // the sequence's first query, its queries, the tile's first one
+    int n_k, tile0;     // its keys, its first tile in the workspace
+    int rows;           // rows of out from q_lo on: the last sequence's go on to the end of it
+};
+
+__device__ __forceinline__ QueryTile query_tile(const PrefillArgs &a, int slot, int lane)
+{
+    QueryTile t;
+    const Owner w = owner_of_slot(a.cu_q, a.queries, a.cu_seqlens, a.total_tokens, a.batch, kQueries, slot, lane);
+    t.q_lo = w.lo;
+    t.n_q = w.hi - w.lo;
+    t.q0 = (slot - t.q_lo / kQueries - w.b) * kQueries;
+    t.rows = w.b == a.batch - 1 ? a.queries - t.q_lo : t.n_q;
+    t.n_k = w.other_hi - w.other_lo;
+    t.tile0 = w.other_lo / kTile + w.b;
+    return t;
+}
+
+// A tile behind the last sequence's queries: zeros.
+template <typename E>
+__device__ __forceinline__ void zero_rows(const PrefillArgs &a, const QueryTile &t, int h)
+{
+    for (int i = threadIdx.x; i < min(kQueries, t.rows - t.q0) * (kNope / 8); i += 256)
+        *(uint4 *)((E *)a.out + ((size_t)(t.q_lo + t.q0 + i / (kNope / 8)) * a.num_heads + h) * kNope +
+                   8 * (i % (kNope / 8))) = uint4{0, 0, 0, 0};
+}
+
+// The wave's 32 rows from `first` on (relative to the sequence's first query): normalised, rounded, through
+// the wave's 8 KB of LDS at `at`, stored by whole rows (as they lie in the registers, a store would touch 32
+// rows). A query that sees no key (l = 0) gives zeros, as do the rows behind the last sequence's queries.
+template <typename E>
+__device__ __forceinline__ void store_rows(const PrefillArgs &a, const QueryTile &t, int h, int first, int lane, unsigned at,
+                                           const floatx16 (&o)[4], float l)
+{
+    using E4 = typename Vec<E>::v4;
+    const int r32 = lane & 31, hl = lane >> 5;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const unsigned row_at = at + r32 * (kNope * 2) + 16 * key_swizzle(r32) + 8 * hl;
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            E4 v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                v[e] = first + r32 < t.n_q ? (E)(o[c][4 * k + e] * inv) : (E)0.0f;
+            lds_store(row_at ^ (16 * (4 * c + k)), v);
+        }
+    E *out = (E *)a.out + ((size_t)(t.q_lo + first) * a.num_heads + h) * kNope + 8 * (lane & 15);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+        const int r = 4 * u + (lane >> 4);
+        const uint4x v = lds_load<uint4x>(at + r * (kNope * 2) + 16 * ((lane & 15) ^ key_swizzle(r)));
+        if (first + r < t.rows)
+            *(uint4x *)(out + (size_t)r * a.num_heads * kNope) = v;
+    }
+}
+
 template <typename E>
 __global__ __launch_bounds__(256, 2) void attend_kernel(PrefillArgs a)
 {
@@ -311,41 +384,25 @@ __global__ __launch_bounds__(256, 2) void attend_kernel(PrefillArgs a)
     const int slot = a.q_slots - 1 - li % a.q_slots;
     if (h >= a.num_heads)
         return;
-    const int b = owner_of_slot(a.cu_q, a.batch, a.queries, kQueries, slot, lane);
-    const int q_lo = clamped(a.cu_q, b, a.queries);
-    const int n_q = max(clamped(a.cu_q, b + 1, a.queries), q_lo) - q_lo;
-    const int q0 = (slot - q_lo / kQueries - b) * kQueries;
-    // the last sequence's tiles go on to the end of the output: rows behind it are zeros
-    const int rows = b == a.batch - 1 ? a.queries - q_lo : n_q;
-    if (q0 >= n_q) {
-        for (int i = threadIdx.x; i < min(kQueries, rows - q0) * (kNope / 8); i += 256)
-            *(uint4 *)((E *)a.out + ((size_t)(q_lo + q0 + i / (kNope / 8)) * a.num_heads + h) * kNope +
-                       8 * (i % (kNope / 8))) = uint4{0, 0, 0, 0};
+    const QueryTile t = query_tile(a, slot, lane);
+    if (t.q0 >= t.n_q) {
+        zero_rows<E>(a, t, h);
         return;
     }
-    const int k_lo = clamped(a.cu_seqlens, b, a.total_tokens);
-    const int n_k = max(clamped(a.cu_seqlens, b + 1, a.total_tokens), k_lo) - k_lo;
-    const int shift = n_k - n_q;  // query i sees the keys 0 .. i + shift
-    const int tile0 = k_lo / kTile + b;
-    const int n_tiles = (min(n_k, min(q0 + kQueries, n_q) + shift) + kTile - 1) / kTile;
+    const int q0 = t.q0, n_q = t.n_q, tile0 = t.tile0;
+    const int shift = t.n_k - n_q;  // query i sees the keys 0 .. i + shift
+    const int n_tiles = (min(t.n_k, min(q0 + kQueries, n_q) + shift) + kTile - 1) / kTile;
 
     const int row = q0 + 32 * wave + r32;
     const int last = min(row, n_q - 1) + shift;  // the lane's last key
-    const size_t q_at = (size_t)(q_lo + min(row, n_q - 1)) * a.num_heads + h;
-    E8 q[12];
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-        q[k] = *(const E8 *)((const E *)a.q_nope + q_at * kNope + 16 * k + 8 * hl);
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-        q[8 + k] = *(const E8 *)((const E *)a.q_rope + q_at * kRopeDim + 16 * k + 8 * hl);
-
     const unsigned lds = lds_address(s_buf);
+    const unsigned k_lane = r32 * (kNope * 2) + 16 * (hl ^ key_swizzle(r32));
+    const unsigned rope_row = r32 * (kRopeDim * 2) + 16 * (hl ^ rope_swizzle(r32));
     const E *ks = (const E *)a.k + ((size_t)h * a.padded + (size_t)tile0 * kTile) * kNope;
     const E *vs = (const E *)a.v + ((size_t)h * a.padded + (size_t)tile0 * kTile) * kNope;
     const E *rs = (const E *)a.rope + (size_t)tile0 * kTile * kRopeDim;
     const ulong4x *flags = (const ulong4x *)a.flags + (size_t)h * (a.padded / kTile) + tile0;
-    // 16 units of K and of V (4 rows each), 8 of the rotary parts (8 rows)
+    constexpr int kUnits = 10;  // load units of a wave: 4 of K and of V (4 rows each), 2 of the rotary parts (8 rows)
     auto load_tile = [&](int j) {
         const unsigned at = lds + (j & 1) * (kStage * 2);
 #pragma unroll
@@ -362,8 +419,37 @@ __global__ __launch_bounds__(256, 2) void attend_kernel(PrefillArgs a)
                                at + 4 * kKElems + (2 * wave + u) * 1024);
         }
     };
-    const unsigned k_lane = r32 * (kNope * 2) + 16 * (hl ^ key_swizzle(r32));
-    const unsigned rope_lane = 4 * kKElems + r32 * (kRopeDim * 2) + 16 * (hl ^ rope_swizzle(r32));
+    // The queries, the B operand of S^T: their own part comes by whole rows
+    // through the second stage, 8 KB a wave, while the first key tile is on its
+    // way to the first one. Rows past the sequence's queries re-read the last one.
+    E8 q[12];
+    {
+        const int lim = n_q - 1 - q0;
+        const size_t q_at = (size_t)(t.q_lo + q0) * a.num_heads + h;
+        const E *qn = wave_uniform((const E *)a.q_nope + q_at * kNope);
+        const E *qr = (const E *)a.q_rope + (q_at + (size_t)min(32 * wave + r32, lim) * a.num_heads) * kRopeDim + 8 * hl;
+        const unsigned own = lds + kStage * 2 + wave * 8192;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const int r = 4 * u + (lane >> 4);
+            global_to_lds16_at(qn, min(32 * wave + r, lim) * (a.num_heads * (kNope * 2)) + 16 * ((lane & 15) ^ key_swizzle(r)),
+                               own + 1024 * u);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            q[8 + k] = *(const E8 *)(qr + 16 * k);
+        if (n_tiles > 0)
+            load_tile(0);
+        if (n_tiles > 0)
+            MLA_WAIT_VMCNT(kUnits);
+        else
+            MLA_WAIT_VMCNT(0);
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            q[k] = lds_load<E8>((own + k_lane) ^ (32 * k));
+    }
+    const unsigned rope_lane = 4 * kKElems + rope_row;
     unsigned v_lane[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -374,8 +460,6 @@ __global__ __launch_bounds__(256, 2) void attend_kernel(PrefillArgs a)
 
     floatx16 o[4] = {};
     float m = -INFINITY, l = 0.0f;
-    if (n_tiles > 0)
-        load_tile(0);
     const int wave_last = min(q0 + 32 * wave + 31, n_q - 1) + shift;  // of the wave's queries
     const int wave_first = min(q0 + 32 * wave, n_q - 1) + shift;
     for (int j = 0; j < n_tiles; ++j) {
@@ -484,20 +568,8 @@ __global__ __launch_bounds__(256, 2) void attend_kernel(PrefillArgs a)
         }
     }
     l = reduce_halves(l, [](float x, float y) { return x + y; });
-    if (row >= rows)
-        return;
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // a query that sees no key gives zeros
-    E *out = (E *)a.out + ((size_t)(q_lo + row) * a.num_heads + h) * kNope + 4 * hl;
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            E4 v;
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                v[e] = row < n_q ? (E)(o[c][4 * k + e] * inv) : (E)0.0f;
-            *(E4 *)(out + 32 * c + 8 * k) = v;
-        }
+    lds_barrier();  // everyone is done with the last tile
+    store_rows<E>(a, t, h, q0 + 32 * wave, lane, lds + wave * 8192, o, l);
 }
 
 // ---- host -------------------------------------------------------------------
