@@ -10,6 +10,9 @@
 // maximum's factor is one value a lane.
 #pragma once
 
+#include <type_traits>
+#include <utility>
+
 #include "mla_device.hpp"
 #include "mla_internal.hpp"
 #include "mla_ring.hpp"
@@ -31,34 +34,31 @@ __device__ __forceinline__ floatx16 mfma32x32x16(bf16x8 a, bf16x8 b, floatx16 c)
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
 
-// The same product accumulated in ordinary registers, for a kernel whose other
-// accumulators fill the accumulation registers (the compiler puts all of a kernel's
-// products there, and moves them back and forth when they do not fit).
-// A chain: first (C = 0), next .., then settle, before anything reads the tile: a
-// product's result may be read 11 slots after an 8-pass product (16 here), which
-// the compiler knows of its own products only; nor does it know that an operand
-// which a vector instruction wrote may be read 2 slots later. Operands therefore
-// come from LDS or are never moved, which a test of the assembly checks. Within a chain
-// each product's accumulator is exactly the last one's result, which needs no wait.
-__device__ __forceinline__ void mfma32x32x16_first(floatx16 &d, half8 a, half8 b)
-{
-    asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, 0" : "=&v"(d) : "v"(a), "v"(b));
-}
-
-__device__ __forceinline__ void mfma32x32x16_next(floatx16 &d, half8 a, half8 b)
-{
-    asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+v"(d) : "v"(a), "v"(b));
-}
-
-__device__ __forceinline__ void mfma32x32x16_first(floatx16 &d, bf16x8 a, bf16x8 b)
-{
-    asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(d) : "v"(a), "v"(b));
-}
-
-__device__ __forceinline__ void mfma32x32x16_next(floatx16 &d, bf16x8 a, bf16x8 b)
-{
-    asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(d) : "v"(a), "v"(b));
-}
+// The same product accumulated in ordinary registers, for kernels that fill the
+// accumulation registers with something else: other accumulators, or with _acc
+// the B operand itself. (The compiler puts all of a kernel's products into
+// accumulation registers, and moves what does not fit back and forth.)
+// A chain: first (C = 0), next .., then settle, or two products more and
+// in_registers, before anything reads the tile: a product's result may be read 11 slots
+// after an 8-pass product (a product takes 8), which the compiler knows of its own
+// products only; nor does it know that an operand which a vector instruction
+// wrote may be read 2 slots later. Operands therefore come from LDS or are never
+// moved, which a test of the assembly checks. Within a chain each product's
+// accumulator is exactly the last one's result, which needs no wait.
+#define MLA_MFMA_CHAIN(suffix, type, b_class, instruction)                                  \
+    __device__ __forceinline__ void mfma32x32x16_first##suffix(floatx16 &d, type a, type b) \
+    {                                                                                       \
+        asm volatile(instruction " %0, %1, %2, 0" : "=&v"(d) : "v"(a), b_class(b));         \
+    }                                                                                       \
+    __device__ __forceinline__ void mfma32x32x16_next##suffix(floatx16 &d, type a, type b)  \
+    {                                                                                       \
+        asm volatile(instruction " %0, %1, %2, %0" : "+v"(d) : "v"(a), b_class(b));         \
+    }
+MLA_MFMA_CHAIN(, half8, "v", "v_mfma_f32_32x32x16_f16")
+MLA_MFMA_CHAIN(, bf16x8, "v", "v_mfma_f32_32x32x16_bf16")
+MLA_MFMA_CHAIN(_acc, half8, "a", "v_mfma_f32_32x32x16_f16")
+MLA_MFMA_CHAIN(_acc, bf16x8, "a", "v_mfma_f32_32x32x16_bf16")
+#undef MLA_MFMA_CHAIN
 
 __device__ __forceinline__ void mfma_settle(floatx16 &d)
 {
@@ -78,6 +78,13 @@ template <typename V>
 __device__ __forceinline__ void in_registers(V &v)
 {
     asm volatile("" : "+v"(v));
+}
+
+// The same for an operand that stays in accumulation registers.
+template <typename V>
+__device__ __forceinline__ void in_acc_registers(V &v)
+{
+    asm volatile("" : "+a"(v));
 }
 
 // f over lanes l and l ^ 32, on the VALU (see reduce_over_lane_groups).
@@ -136,16 +143,28 @@ __device__ __forceinline__ unsigned max_u16x2(unsigned a, unsigned b)
                                                                   __builtin_bit_cast(ushort2x, b)));
 }
 
-// 16 bytes per lane from a per-lane address into LDS at lds + 16 * lane
-// (lds: a wave-uniform LDS byte address); see global_to_lds16.
-__device__ __forceinline__ void gather_to_lds16(const void *p, unsigned lds)
+// 16 bytes per lane from base + off + kAdd + kOffset into LDS at lds + kLds +
+// kOffset + 16 * lane (the instruction's own offset counts for both), in three
+// instructions: a wave that has a SIMD to itself issues one every 5 to 9
+// cycles, some four beside each 32-cycle product. m0, which carries the LDS address, is
+// left changed: nothing else in a kernel that calls this uses it, which a test of the
+// assembly checks. The addition stands between the write of m0 and its use, which
+// needs one slot there.
+template <int kAdd, int kLds, int kOffset>
+__device__ __forceinline__ void stream_to_lds16(const void *base, int off, unsigned lds)
 {
-    unsigned saved_m0;
-    asm volatile("s_mov_b32 %0, m0\n\t"
-                 "s_mov_b32 m0, %2\n\t"
-                 "global_load_lds_dwordx4 %1, off\n\t"
-                 "s_mov_b32 m0, %0"
-                 : "=&s"(saved_m0) : "v"(p), "s"(lds) : "memory");
+    int at;
+    asm volatile("s_add_u32 m0, %3, %4\n\t"
+                 "v_add_u32 %0, %5, %1\n\t"
+                 "global_load_lds_dwordx4 %0, %2 offset:%6"
+                 : "=&v"(at) : "v"(off), "s"(base), "s"(lds), "n"(kLds), "n"(kAdd), "n"(kOffset) : "memory", "scc");
+}
+
+// f(0), f(1), .., each with its index as a constant.
+template <typename F, int... kIs>
+__device__ __forceinline__ void for_constants(F f, std::integer_sequence<int, kIs...>)
+{
+    (f(std::integral_constant<int, kIs>{}), ...);
 }
 
 __device__ __forceinline__ unsigned lds_address(const void *p)

@@ -129,20 +129,27 @@ expand_kernel(PrefillArgs a)
     if (blk0 >= n_blocks)
         return;
 
-    // block i: rows 32 (i mod 4) .. of side (i / 4) mod 2 of head i / 8
+    // Block i: rows 32 (i mod 4) .. of side (i / 4) mod 2 of head i / 8. The
+    // wave's 8 load units are its rows of 1 KB, which follow each other in
+    // memory and in LDS; a row's swizzle differs from the first one's by an XOR.
     const unsigned ring = lds_address(s_ring);
-    auto load_block = [&](int i) {
+    const int w_off = 16 * (lane ^ weight_swizzle(kWeightRows / 4 * wave));
+    auto block_source = [&](int i) -> const E * {
         const int h = i / (2 * kBlocksPerSide), rest = i % (2 * kBlocksPerSide);
-        const E *w = (const E *)(rest >= kBlocksPerSide ? a.w_uv : a.w_uk) +
-                     ((size_t)h * kNope + rest % kBlocksPerSide * kWeightRows) * kLatent;
-        const unsigned dst = ring + ((i - blk0) & (kWeightRing - 1)) * (kWeightElems * 2);
-        int ln = lane;
-        asm volatile("" : "+v"(ln));
-#pragma unroll
-        for (int u = 0; u < kWeightRows / 4; ++u) {
-            const int r = kWeightRows / 4 * wave + u;
-            global_to_lds16_at(w + (size_t)r * kLatent, 16 * (ln ^ weight_swizzle(r)), dst + r * (kLatent * 2));
-        }
+        return wave_uniform((const E *)(rest >= kBlocksPerSide ? a.w_uv : a.w_uk) +
+                            ((size_t)h * kNope + rest % kBlocksPerSide * kWeightRows + kWeightRows / 4 * wave) * kLatent);
+    };
+    auto slot_of = [&](int i) {
+        return ring + ((i - blk0) & (kWeightRing - 1)) * (kWeightElems * 2) + kWeightRows / 4 * wave * (kLatent * 2);
+    };
+    auto load_unit = [&](const E *src, unsigned dst, auto unit) {
+        constexpr int u = decltype(unit)::value;
+        stream_to_lds16<4096 * (u >> 2), 4096 * (u >> 2), 1024 * (u & 3)>(src, w_off ^ (16 * (u & 3)) ^ (128 * (u >> 2)), dst);
+    };
+    auto load_block = [&](int i) {
+        const E *src = block_source(i);
+        const unsigned dst = slot_of(i);
+        for_constants([&](auto unit) { load_unit(src, dst, unit); }, std::make_integer_sequence<int, kWeightRows / 4>{});
     };
     // The wave's keys: latent rows of 1 KB by direct loads into the wave's own
     // ring slot, 32 at a time, then into registers (chunk c of row r at c ^ (r
@@ -154,7 +161,7 @@ expand_kernel(PrefillArgs a)
     const bool live = tile < tiles && t0 < len;  // else nobody reads this tile
     if (!__syncthreads_or(live))
         return;
-    auto block_source = [&](int t) -> const E * {  // latent row t of the sequence; the 32 rows of a block follow it
+    auto key_source = [&](int t) -> const E * {  // latent row t of the sequence; the 32 rows of a block follow it
         size_t row;
         if (a.block_table) {
             const int col = min(t >> a.page_shift, a.bt_stride - 1);
@@ -170,7 +177,7 @@ expand_kernel(PrefillArgs a)
     for (int g = 0; g < 2; ++g) {
         const int t = t0 + 32 * g;
         if (live && t < len) {
-            const E *src = block_source(t);
+            const E *src = wave_uniform(key_source(t));
             const int lim = min(31, len - 1 - t);
             const unsigned own = ring + wave * (kWeightElems * 2);
 #pragma unroll
@@ -199,6 +206,9 @@ expand_kernel(PrefillArgs a)
             for (int k = 0; k < kLatent / 16; ++k)
                 key[g][k] = E8{};
         }
+#pragma unroll
+        for (int k = 0; k < kLatent / 16; ++k)
+            in_acc_registers(key[g][k]);
     }
     lds_barrier();  // the ring is free
     for (int i = blk0; i < min(blk0 + kWeightRing - 1, blk1); ++i)
@@ -207,18 +217,19 @@ expand_kernel(PrefillArgs a)
     const int row = weight_row(r32);
     const unsigned w_lane = row * (kLatent * 2) + 16 * (hl ^ weight_swizzle(row));
     unsigned long long bad = 0;  // the tile's keys whose V is not finite, in the block of `store`
-    floatx16 prev[2];            // the block before: rounded and stored between this one's products
-    // Rounds and stores quarter `part` of key group g of block i.
-    auto store = [&](int i, int g, int part, unsigned &top, E8 (&v)[2]) {
+    // Rounds and stores quarter `part` of key group g of block i, whose sums
+    // are in acc; v and top gather a group's four quarters.
+    auto store = [&](int i, const floatx16 (&acc)[2], int g, int part, unsigned &top, E8 (&v)[2]) {
+        typedef float floatx4v __attribute__((ext_vector_type(4)));
+        const auto x = __builtin_convertvector(
+            (floatx4v{acc[g][4 * part], acc[g][4 * part + 1], acc[g][4 * part + 2], acc[g][4 * part + 3]}), typename Vec<E>::v4);
 #pragma unroll
-        for (int r = 4 * part; r < 4 * part + 4; ++r)
-            v[r >> 3][r & 7] = (E)prev[g][r];
+        for (int r = 0; r < 4; ++r)
+            v[part >> 1][4 * (part & 1) + r] = x[r];
         const auto w = __builtin_bit_cast(uint4x, v[part >> 1]);
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {  // the largest magnitude's bits, both halves
-            const unsigned x = w[2 * (part & 1) + k] & 0x7fff7fffu;
-            top = max_u16x2(top, x);
-        }
+        for (int k = 0; k < 2; ++k)  // the largest magnitude's bits, both halves
+            top = max_u16x2(top, w[2 * (part & 1) + k] & 0x7fff7fffu);
         if (part != 3)
             return;
         const int h = i / (2 * kBlocksPerSide), rest = i % (2 * kBlocksPerSide);
@@ -230,8 +241,8 @@ expand_kernel(PrefillArgs a)
             // query that must not see the key can meet it with weight 0
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const E x = v[r >> 3][r & 7];
-                v[r >> 3][r & 7] = not_finite<E>(__builtin_bit_cast(unsigned short, x)) ? (E)0.0f : x;
+                const E y = v[r >> 3][r & 7];
+                v[r >> 3][r & 7] = not_finite<E>(__builtin_bit_cast(unsigned short, y)) ? (E)0.0f : y;
             }
             bad |= (unsigned long long)((unsigned)m | (unsigned)(m >> 32)) << (32 * g);
         }
@@ -245,13 +256,16 @@ expand_kernel(PrefillArgs a)
             bad = 0;
         }
     };
-    for (int i = blk0; i < blk1; ++i) {
-        // Block i's 8 loads went out three blocks ago; since then, in order,
-        // those of blocks i + 1 and i + 2 and the stores of three blocks, 4
-        // or 5 each.
+    // Block i into acc, while block i - 1, in prev, is rounded and stored
+    // between the products, a quarter of a group after every 8 of the 64.
+    auto block = [&](int i, floatx16 (&acc)[2], floatx16 (&prev)[2]) {
+        // Block i's 8 loads went out during block i - 3. Behind the last of them
+        // come, in order, 2 stores of that block (half of block i - 4's 4; one more
+        // where it holds flags), then twice 8 loads (of blocks i + 1, i + 2)
+        // and 4 stores: at least 26. The first blocks have fewer stores behind them.
         if (i + 2 < blk1) {
             if (live && i - blk0 >= 4)
-                MLA_WAIT_VMCNT(2 * (kWeightRows / 4) + 3 * 4);
+                MLA_WAIT_VMCNT(2 * (kWeightRows / 4) + 2 * 4 + 2);
             else
                 MLA_WAIT_VMCNT(2 * (kWeightRows / 4));
         } else if (i + 1 < blk1) {
@@ -260,47 +274,66 @@ expand_kernel(PrefillArgs a)
             MLA_WAIT_VMCNT(0);
         }
         lds_barrier();  // block i is there, and block i - 1's slot is free
-        if (i + kWeightRing - 1 < blk1)
-            load_block(i + kWeightRing - 1);
-        const unsigned at = ring + ((i - blk0) & (kWeightRing - 1)) * (kWeightElems * 2) + w_lane;
+        const bool feed = i + kWeightRing - 1 < blk1;
+        const E *feed_src = block_source(min(i + kWeightRing - 1, n_blocks - 1));
+        const unsigned feed_at = slot_of(i + kWeightRing - 1);
         const bool have = live && i > blk0;
-        floatx16 acc[2] = {};
-        E8 v[2][2];
-        unsigned top[2] = {0, 0};
-        E8 w[2][4];
+        const unsigned at = ring + ((i - blk0) & (kWeightRing - 1)) * (kWeightElems * 2) + w_lane;
         auto operand = [&](int k) -> E8 { return lds_load<E8>((at ^ (32 * (k & 7))) + 256 * (k >> 3)); };
+        constexpr int kAhead = 4;  // steps an operand is read ahead
+        E8 w[kAhead + 1], v[2][2];
+        unsigned top[2] = {0, 0};
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            w[0][j] = operand(j);
+        for (int k = 0; k < kAhead; ++k)
+            w[k] = operand(k);
+        for_constants(
+            [&](auto step) {
+                constexpr int k = decltype(step)::value;
+                if constexpr (k + kAhead < kLatent / 16)
+                    w[(k + kAhead) % (kAhead + 1)] = operand(k + kAhead);
 #pragma unroll
-        for (int k = 0; k < kLatent / 16; k += 4) {
-            if (k + 4 < kLatent / 16) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    w[(k / 4 + 1) & 1][j] = operand(k + 4 + j);
-                __builtin_amdgcn_sched_barrier(0);  // the reads first: left alone they go out as late as they can
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int g = 0; g < 2; ++g)
-                    acc[g] = mfma32x32x16(w[(k / 4) & 1][j], key[g][k + j], acc[g]);
-            if (have)
-                store(i - 1, k / 16, k / 4 % 4, top[k / 16], v[k / 16]);
-            __builtin_amdgcn_sched_barrier(0);
-        }
-        prev[0] = acc[0];
-        prev[1] = acc[1];
-    }
-    if (live) {
-        E8 v[2];
+                for (int g = 0; g < 2; ++g) {
+                    if constexpr (k == 0)
+                        mfma32x32x16_first_acc(acc[g], w[0], key[g][0]);
+                    else
+                        mfma32x32x16_next_acc(acc[g], w[k % (kAhead + 1)], key[g][k]);
+                }
+                if constexpr (k == 2) {  // six products behind the last of block i - 1
+                    in_registers(prev[0]);
+                    in_registers(prev[1]);
+                }
+                if constexpr (k % 4 == 1)
+                    if (feed)
+                        load_unit(feed_src, feed_at, std::integral_constant<int, k / 4>{});
+                if constexpr (k % 4 == 3)
+                    if (have)
+                        store(i - 1, prev, k / 16, k / 4 % 4, top[k / 16], v[k / 16]);
+                __builtin_amdgcn_sched_barrier(0);
+            },
+            std::make_integer_sequence<int, kLatent / 16>{});
+    };
+    auto store_last = [&](floatx16 (&acc)[2]) {
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
+            mfma_settle(acc[g]);
+            E8 v[2];
             unsigned top = 0;
 #pragma unroll
             for (int part = 0; part < 4; ++part)
-                store(blk1 - 1, g, part, top, v);
+                store(blk1 - 1, acc, g, part, top, v);
         }
+    };
+    floatx16 even[2] = {}, odd[2] = {};
+    for (int i = blk0; i < blk1; i += 2) {
+        block(i, even, odd);
+        if (i + 1 < blk1)
+            block(i + 1, odd, even);
+    }
+    if (live) {
+        if ((blk1 - blk0) & 1)
+            store_last(even);
+        else
+            store_last(odd);
     }
 }
 
@@ -398,26 +431,28 @@ __global__ __launch_bounds__(256, 2) void attend_kernel(PrefillArgs a)
     const unsigned lds = lds_address(s_buf);
     const unsigned k_lane = r32 * (kNope * 2) + 16 * (hl ^ key_swizzle(r32));
     const unsigned rope_row = r32 * (kRopeDim * 2) + 16 * (hl ^ rope_swizzle(r32));
-    const E *ks = (const E *)a.k + ((size_t)h * a.padded + (size_t)tile0 * kTile) * kNope;
-    const E *vs = (const E *)a.v + ((size_t)h * a.padded + (size_t)tile0 * kTile) * kNope;
-    const E *rs = (const E *)a.rope + (size_t)tile0 * kTile * kRopeDim;
+    const E *ks = wave_uniform((const E *)a.k + ((size_t)h * a.padded + (size_t)tile0 * kTile + 16 * wave) * kNope);
+    const E *vs = wave_uniform((const E *)a.v + ((size_t)h * a.padded + (size_t)tile0 * kTile + 16 * wave) * kNope);
+    const E *rs = wave_uniform((const E *)a.rope + ((size_t)tile0 * kTile + 16 * wave) * kRopeDim);
     const ulong4x *flags = (const ulong4x *)a.flags + (size_t)h * (a.padded / kTile) + tile0;
-    constexpr int kUnits = 10;  // load units of a wave: 4 of K and of V (4 rows each), 2 of the rotary parts (8 rows)
+    // A wave's 10 load units: 4 of K and 4 of V (4 rows of 256 bytes, which follow
+    // each other in memory and in LDS, the swizzle's low bits changing from one to the
+    // next), 2 of the rotary parts (8 rows of 128 bytes).
+    constexpr int kUnits = 10;
+    const int kv_off = (lane >> 4) * (kNope * 2) + 16 * ((lane & 15) ^ key_swizzle(lane >> 4));
+    const int rope_off = (lane >> 3) * (kRopeDim * 2) + 16 * ((lane & 7) ^ rope_swizzle(lane >> 3));
     auto load_tile = [&](int j) {
         const unsigned at = lds + (j & 1) * (kStage * 2);
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int r = 16 * wave + 4 * u + (lane >> 4);
-            const int off = r * (kNope * 2) + 16 * ((lane & 15) ^ key_swizzle(r));
-            global_to_lds16_at(ks + (size_t)j * kKElems, off, at + (4 * wave + u) * 1024);
-            global_to_lds16_at(vs + (size_t)j * kKElems, off, at + 2 * kKElems + (4 * wave + u) * 1024);
-        }
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int r = 16 * wave + 8 * u + (lane >> 3);
-            global_to_lds16_at(rs + (size_t)j * kRElems, r * (kRopeDim * 2) + 16 * ((lane & 7) ^ rope_swizzle(r)),
-                               at + 4 * kKElems + (2 * wave + u) * 1024);
-        }
+        const E *k = ks + (size_t)j * kKElems, *v = vs + (size_t)j * kKElems, *r = rs + (size_t)j * kRElems;
+        for_constants(
+            [&](auto unit) {
+                constexpr int u = decltype(unit)::value;
+                stream_to_lds16<0, 0, 1024 * u>(k, kv_off ^ (16 * u), at + 4096 * wave);
+                stream_to_lds16<0, 2 * kKElems, 1024 * u>(v, kv_off ^ (16 * u), at + 4096 * wave);
+            },
+            std::make_integer_sequence<int, 4>{});
+        stream_to_lds16<0, 4 * kKElems, 0>(r, rope_off, at + 2048 * wave);
+        stream_to_lds16<0, 4 * kKElems, 1024>(r, rope_off ^ 64, at + 2048 * wave);
     };
     // The queries, the B operand of S^T: their own part comes by whole rows
     // through the second stage, 8 KB a wave, while the first key tile is on its

@@ -203,12 +203,13 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
     for (int k = 0; k < kDK / 16; ++k)
         in_registers(q[k]);
     lds_barrier();  // the ring is free
-    for (int i = 0; i < min(kRing - 1, n_blocks); ++i) {
-        const E *src = block_source(i, page_of(i));
+    auto load_block = [&](int i, const E *src) {
 #pragma unroll
         for (int u = 0; u < kUnitsPerWave; ++u)
             load_unit(src, i, u);
-    }
+    };
+    for (int i = 0; i < min(kRing - 1, n_blocks); ++i)
+        load_block(i, block_source(i, page_of(i)));
     // A drafted token that a row does not see meets it with weight 0: 0 times
     // an infinity or NaN in its row would still be NaN, so those become 0 for
     // the second product, once every wave has block i's logits. A row that does
@@ -247,12 +248,8 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
         for (int i = 0; i < n_blocks; ++i) {
             MLA_WAIT_VMCNT(0);
             lds_barrier();
-            if (i + kRing - 1 < n_blocks) {
-                const E *src = block_source(i + kRing - 1, page_of(i + kRing - 1));
-#pragma unroll
-                for (int u = 0; u < kUnitsPerWave; ++u)
-                    load_unit(src, i + kRing - 1, u);
-            }
+            if (i + kRing - 1 < n_blocks)
+                load_block(i + kRing - 1, block_source(i + kRing - 1, page_of(i + kRing - 1)));
             if (is_edge(i))
                 drop_not_finite(i);
         }
@@ -272,6 +269,17 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
     }
     float m = -INFINITY, l = 0.0f;
 
+    // The same units of a block whose 32 rows are all there, in three instructions each.
+    const int row_off = 16 * (lane ^ key_swizzle(8 * wave));
+    const int rope_off = (lane >> 3) * (kDK * 2) + 2 * kDV + 16 * ((lane & 7) ^ rope_swizzle(8 * wave + (lane >> 3)));
+    auto stream_unit = [&](const E *src, unsigned slot, auto unit) {  // src: the wave's first row
+        constexpr int u = decltype(unit)::value;
+        if constexpr (u < 8)
+            stream_to_lds16<u * kDK * 2, u * kDV * 2, 0>(src, row_off ^ (64 * (u & 3)) ^ (16 * (u >> 2)), slot + 8192 * wave);
+        else
+            stream_to_lds16<0, 2 * kRopeElems, 0>(src, rope_off, slot + 1024 * wave);
+    };
+
     // S^T of block i, with side(k) between the products: what does not depend
     // on them, in their shadow (a product takes 32 cycles and one issue slot of
     // 4). Each operand is read kAhead products before its own. The products go
@@ -284,17 +292,19 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
 #pragma unroll
         for (int k = 0; k < kAhead; ++k)
             kv[k] = k_operand(k);
-#pragma unroll
-        for (int k = 0; k < kDK / 16; ++k) {
-            if (k + kAhead < kDK / 16)
-                kv[(k + kAhead) % (kAhead + 1)] = k_operand(k + kAhead);
-            if (k == 0)
-                mfma32x32x16_first(s, kv[0], q[0]);
-            else
-                mfma32x32x16_next(s, kv[k % (kAhead + 1)], q[k]);
-            side(k);
-            __builtin_amdgcn_sched_barrier(0);
-        }
+        for_constants(
+            [&](auto product) {
+                constexpr int k = decltype(product)::value;
+                if constexpr (k + kAhead < kDK / 16)
+                    kv[(k + kAhead) % (kAhead + 1)] = k_operand(k + kAhead);
+                if constexpr (k == 0)
+                    mfma32x32x16_first(s, kv[0], q[0]);
+                else
+                    mfma32x32x16_next(s, kv[k % (kAhead + 1)], q[k]);
+                side(product);
+                __builtin_amdgcn_sched_barrier(0);
+            },
+            std::make_integer_sequence<int, kDK / 16>{});
         mfma_settle(s);
         return s;
     };
@@ -316,7 +326,7 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
         else
             MLA_WAIT_VMCNT(0);
         lds_barrier();
-        s = logits(0, [](int) {});
+        s = logits(0, [](auto) {});
         most = largest(s);
     }
     for (int i = 0; i < n_blocks; ++i) {
@@ -367,13 +377,26 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
             p[r] = fast_exp2(s[r] * a.scale_log2 - ref);
             l += p[r];
         };
+        // block i + 3, requested between the products where it is whole
+        const bool whole = feed && t0 + kRing * kBlock <= rq.len;
+        if (feed && !whole)
+            load_block(i + kRing - 1, feed_src);
         floatx16 ahead = {};
-        if (more) {
-            ahead = logits(i + 1, [&](int k) {
-                if (k % 2 == 0 && k < 32)
+        if (more && whole) {
+            const E *src = feed_src + 8 * wave * kDK;
+            const unsigned slot_at = ring + ((i + kRing - 1) & (kRing - 1)) * (kSlotElems * 2);
+            ahead = logits(i + 1, [&](auto product) {
+                constexpr int k = decltype(product)::value;
+                if constexpr (k % 2 == 0 && k < 32)
                     weight(k / 2);
-                if (k % 4 == 1 && feed)
-                    load_unit(feed_src, i + kRing - 1, k / 4);
+                if constexpr (k % 4 == 1)
+                    stream_unit(src, slot_at, std::integral_constant<int, k / 4>{});
+            });
+        } else if (more) {
+            ahead = logits(i + 1, [&](auto product) {
+                constexpr int k = decltype(product)::value;
+                if constexpr (k % 2 == 0 && k < 32)
+                    weight(k / 2);
             });
         } else {
 #pragma unroll
