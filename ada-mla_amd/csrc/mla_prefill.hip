@@ -36,7 +36,7 @@ struct PrefillArgs {
     const int *block_table;  // nullptr: a packed cache
     const int *cu_q, *cu_seqlens;
     void *out;
-    void *k, *v;                // [head][padded key][128]
+    void *k, *v;                // [head][tile][4 column blocks][64 keys][32]
     void *rope;                 // [padded key][64]
     unsigned long long *flags;  // [head][tile][4]: keys whose V holds an infinity or NaN, by 32 of its columns
     int batch, num_heads, queries, total_tokens;
@@ -89,7 +89,10 @@ __device__ __forceinline__ Owner owner_of_slot(const int *cu, int most, const in
 // and the weights stream past in blocks of 32 rows through an LDS ring, each
 // block read once for 256 keys (two products a LDS read). With the weights as
 // the A operand a lane owns a key and, with the rows of a block read in the
-// order of weight_row, 16 adjacent columns of it: two 16-byte stores.
+// order of weight_row, two times 8 adjacent columns of it, the lane 32 on the 8
+// beside them. The workspace holds a tile's 64 keys x 32 columns of a block in one
+// piece, so that a block's four stores a wave fill 4 KB of whole lines: in rows of 256
+// bytes they were what bound this kernel (8192 keys at 64 heads 156 us, 124 without them).
 constexpr int kWeightRows = 32;                       // rows of W a block
 constexpr int kWeightElems = kWeightRows * kLatent;   // 32 KB
 constexpr int kWeightRing = 4;
@@ -97,17 +100,18 @@ constexpr int kExpandTiles = 4;                       // key tiles a workgroup: 
 constexpr int kBlocksPerSide = kNope / kWeightRows;   // blocks of one head's W_UK or W_UV
 
 // The row of a weight block in row rho = 8 q + 4 c + j of the product's tile:
-// lane half c then holds columns 16 c .. 16 c + 15 in register order.
+// lane half c then holds columns 8 c .. 8 c + 7 in its registers 0 .. 7 and 16 + 8 c ..
+// in the others.
 __device__ __forceinline__ int weight_row(int rho)
 {
-    return 16 * ((rho >> 2) & 1) + 4 * (rho >> 3) + (rho & 3);
+    return 16 * (rho >> 4) + 8 * ((rho >> 2) & 1) + 4 * ((rho >> 3) & 1) + (rho & 3);
 }
 
 // 16-byte chunk c of row r sits at c ^ weight_swizzle(r): rho mod 16, so that
 // 16 lanes that read one chunk of 16 successive rho meet 16 places.
 __device__ __forceinline__ int weight_swizzle(int r)
 {
-    return 8 * ((r >> 2) & 1) + 4 * (r >> 4) + (r & 3);
+    return 8 * ((r >> 2) & 1) + 4 * ((r >> 3) & 1) + (r & 3);
 }
 
 template <typename E>
@@ -134,7 +138,10 @@ expand_kernel(PrefillArgs a)
     // memory and in LDS; a row's swizzle differs from the first one's by an XOR.
     const unsigned ring = lds_address(s_ring);
     const int w_off = 16 * (lane ^ weight_swizzle(kWeightRows / 4 * wave));
+    // Past the group's last block it is loaded again, into a slot that nobody
+    // reads: every block then has the same instructions and the same counts.
     auto block_source = [&](int i) -> const E * {
+        i = min(i, blk1 - 1);
         const int h = i / (2 * kBlocksPerSide), rest = i % (2 * kBlocksPerSide);
         return wave_uniform((const E *)(rest >= kBlocksPerSide ? a.w_uv : a.w_uk) +
                             ((size_t)h * kNope + rest % kBlocksPerSide * kWeightRows + kWeightRows / 4 * wave) * kLatent);
@@ -211,12 +218,13 @@ expand_kernel(PrefillArgs a)
             in_acc_registers(key[g][k]);
     }
     lds_barrier();  // the ring is free
-    for (int i = blk0; i < min(blk0 + kWeightRing - 1, blk1); ++i)
+    for (int i = blk0; i < blk0 + kWeightRing - 1; ++i)
         load_block(i);
 
     const int row = weight_row(r32);
     const unsigned w_lane = row * (kLatent * 2) + 16 * (hl ^ weight_swizzle(row));
     unsigned long long bad = 0;  // the tile's keys whose V is not finite, in the block of `store`
+    const unsigned row_at = r32 * (kWeightRows * 2) + 16 * hl;  // the lane's first 8 values in the block's rows
     // Rounds and stores quarter `part` of key group g of block i, whose sums
     // are in acc; v and top gather a group's four quarters.
     auto store = [&](int i, const floatx16 (&acc)[2], int g, int part, unsigned &top, E8 (&v)[2]) {
@@ -246,15 +254,17 @@ expand_kernel(PrefillArgs a)
             }
             bad |= (unsigned long long)((unsigned)m | (unsigned)(m >> 32)) << (32 * g);
         }
-        E *dst = (E *)(side ? a.v : a.k) + ((size_t)h * a.padded + (size_t)tile * kTile + 32 * g + r32) * kNope +
-                 rest % kBlocksPerSide * kWeightRows + 16 * hl;
-        *(E8 *)dst = v[0];
-        *(E8 *)(dst + 8) = v[1];
-        if (side && g == 1) {
-            if (lane == 0)
+        char *dst = (char *)wave_uniform((const char *)(side ? a.v : a.k) +
+                                         (((size_t)h * tiles + tile) * kBlocksPerSide + rest % kBlocksPerSide) *
+                                             (kTile * kWeightRows * 2));
+        if (i >= blk0 && live) {
+            *(E8 *)(dst + (row_at + 32 * g * (kWeightRows * 2))) = v[0];
+            *(E8 *)(dst + (row_at + 32 * g * (kWeightRows * 2) + 32)) = v[1];
+            if (side && g == 1 && lane == 0)
                 a.flags[((size_t)h * tiles + tile) * kBlocksPerSide + rest % kBlocksPerSide] = bad;
-            bad = 0;
         }
+        if (side && g == 1)
+            bad = 0;
     };
     // Block i into acc, while block i - 1, in prev, is rounded and stored
     // between the products, a quarter of a group after every 8 of the 64.
@@ -263,21 +273,13 @@ expand_kernel(PrefillArgs a)
         // come, in order, 2 stores of that block (half of block i - 4's 4; one more
         // where it holds flags), then twice 8 loads (of blocks i + 1, i + 2)
         // and 4 stores: at least 26. The first blocks have fewer stores behind them.
-        if (i + 2 < blk1) {
-            if (live && i - blk0 >= 4)
-                MLA_WAIT_VMCNT(2 * (kWeightRows / 4) + 2 * 4 + 2);
-            else
-                MLA_WAIT_VMCNT(2 * (kWeightRows / 4));
-        } else if (i + 1 < blk1) {
-            MLA_WAIT_VMCNT(kWeightRows / 4);
-        } else {
-            MLA_WAIT_VMCNT(0);
-        }
+        if (live && i - blk0 >= 4)
+            MLA_WAIT_VMCNT(2 * (kWeightRows / 4) + 2 * 4 + 2);
+        else
+            MLA_WAIT_VMCNT(2 * (kWeightRows / 4));
         lds_barrier();  // block i is there, and block i - 1's slot is free
-        const bool feed = i + kWeightRing - 1 < blk1;
-        const E *feed_src = block_source(min(i + kWeightRing - 1, n_blocks - 1));
+        const E *feed_src = block_source(i + kWeightRing - 1);
         const unsigned feed_at = slot_of(i + kWeightRing - 1);
-        const bool have = live && i > blk0;
         const unsigned at = ring + ((i - blk0) & (kWeightRing - 1)) * (kWeightElems * 2) + w_lane;
         auto operand = [&](int k) -> E8 { return lds_load<E8>((at ^ (32 * (k & 7))) + 256 * (k >> 3)); };
         constexpr int kAhead = 4;  // steps an operand is read ahead
@@ -303,11 +305,9 @@ expand_kernel(PrefillArgs a)
                     in_registers(prev[1]);
                 }
                 if constexpr (k % 4 == 1)
-                    if (feed)
-                        load_unit(feed_src, feed_at, std::integral_constant<int, k / 4>{});
+                    load_unit(feed_src, feed_at, std::integral_constant<int, k / 4>{});
                 if constexpr (k % 4 == 3)
-                    if (have)
-                        store(i - 1, prev, k / 16, k / 4 % 4, top[k / 16], v[k / 16]);
+                    store(i - 1, prev, k / 16, k / 4 % 4, top[k / 16], v[k / 16]);
                 __builtin_amdgcn_sched_barrier(0);
             },
             std::make_integer_sequence<int, kLatent / 16>{});
@@ -329,12 +329,11 @@ expand_kernel(PrefillArgs a)
         if (i + 1 < blk1)
             block(i + 1, odd, even);
     }
-    if (live) {
-        if ((blk1 - blk0) & 1)
-            store_last(even);
-        else
-            store_last(odd);
-    }
+    if ((blk1 - blk0) & 1)
+        store_last(even);
+    else
+        store_last(odd);
+    MLA_WAIT_VMCNT(0);  // no load to LDS outlives the workgroup
 }
 
 // ---- attention --------------------------------------------------------------
@@ -431,15 +430,16 @@ __global__ __launch_bounds__(256, 2) void attend_kernel(PrefillArgs a)
     const unsigned lds = lds_address(s_buf);
     const unsigned k_lane = r32 * (kNope * 2) + 16 * (hl ^ key_swizzle(r32));
     const unsigned rope_row = r32 * (kRopeDim * 2) + 16 * (hl ^ rope_swizzle(r32));
-    const E *ks = wave_uniform((const E *)a.k + ((size_t)h * a.padded + (size_t)tile0 * kTile + 16 * wave) * kNope);
-    const E *vs = wave_uniform((const E *)a.v + ((size_t)h * a.padded + (size_t)tile0 * kTile + 16 * wave) * kNope);
+    const E *ks = wave_uniform((const E *)a.k + ((size_t)h * a.padded + (size_t)tile0 * kTile) * kNope + 16 * wave * kWeightRows);
+    const E *vs = wave_uniform((const E *)a.v + ((size_t)h * a.padded + (size_t)tile0 * kTile) * kNope + 16 * wave * kWeightRows);
     const E *rs = wave_uniform((const E *)a.rope + ((size_t)tile0 * kTile + 16 * wave) * kRopeDim);
     const ulong4x *flags = (const ulong4x *)a.flags + (size_t)h * (a.padded / kTile) + tile0;
-    // A wave's 10 load units: 4 of K and 4 of V (4 rows of 256 bytes, which follow
-    // each other in memory and in LDS, the swizzle's low bits changing from one to the
-    // next), 2 of the rotary parts (8 rows of 128 bytes).
+    // A wave's 10 load units: 4 of K and 4 of V (4 keys of 256 bytes in LDS, 4 times
+    // 64 bytes in the workspace, the swizzle's low bits changing from one unit to
+    // the next), 2 of the rotary parts (8 rows of 128 bytes).
     constexpr int kUnits = 10;
-    const int kv_off = (lane >> 4) * (kNope * 2) + 16 * ((lane & 15) ^ key_swizzle(lane >> 4));
+    const int kv_chunk = (lane & 15) ^ key_swizzle(lane >> 4);
+    const int kv_off = (kv_chunk >> 2) * (kTile * kWeightRows * 2) + (lane >> 4) * (kWeightRows * 2) + 16 * (kv_chunk & 3);
     const int rope_off = (lane >> 3) * (kRopeDim * 2) + 16 * ((lane & 7) ^ rope_swizzle(lane >> 3));
     auto load_tile = [&](int j) {
         const unsigned at = lds + (j & 1) * (kStage * 2);
@@ -447,8 +447,8 @@ __global__ __launch_bounds__(256, 2) void attend_kernel(PrefillArgs a)
         for_constants(
             [&](auto unit) {
                 constexpr int u = decltype(unit)::value;
-                stream_to_lds16<0, 0, 1024 * u>(k, kv_off ^ (16 * u), at + 4096 * wave);
-                stream_to_lds16<0, 2 * kKElems, 1024 * u>(v, kv_off ^ (16 * u), at + 4096 * wave);
+                stream_to_lds16<4 * u * kWeightRows * 2, 1024 * u, 0>(k, kv_off ^ (16 * u), at + 4096 * wave);
+                stream_to_lds16<4 * u * kWeightRows * 2, 2 * kKElems + 1024 * u, 0>(v, kv_off ^ (16 * u), at + 4096 * wave);
             },
             std::make_integer_sequence<int, 4>{});
         stream_to_lds16<0, 4 * kKElems, 0>(r, rope_off, at + 2048 * wave);
