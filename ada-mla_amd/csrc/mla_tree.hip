@@ -473,13 +473,13 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
 }
 
 // Merges the splits of a request (those of more than one). A workgroup takes 32
-// rows x 32 columns; wave w the splits w, w + 4, .., and a lane the 16 values it
+// rows x `tiles` times 32 columns; wave w the splits w, w + 4, .., and a lane the 16 values it
 // would hold in the split kernel. The waves' sums meet in LDS. The order of the
 // additions depends on the split count alone.
 constexpr int kMany = 4;  // splits of a wave in flight together
 
 template <typename E>
-__global__ __launch_bounds__(256) void tree_combine_kernel(TreeArgs a)
+__global__ __launch_bounds__(256) void tree_combine_kernel(TreeArgs a, int tiles)
 {
     using E4 = typename Vec<E>::v4;
     __shared__ float s_m[kWaves][32];
@@ -487,8 +487,8 @@ __global__ __launch_bounds__(256) void tree_combine_kernel(TreeArgs a)
     __shared__ floatx4 s_o[kWaves][4][64];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int item = blockIdx.x;
-    const int c = item & 15, w = (item >> 4) & 3, rest = item >> 6;
+    const int per_row = kDV / 32 / tiles;  // workgroups of 32 rows
+    const int c0 = blockIdx.x % per_row * tiles, w = blockIdx.x / per_row & 3, rest = blockIdx.x / per_row >> 2;
     const int rt = rest % a.row_tiles, b = rest / a.row_tiles;
     Request rq;
     rq.read(a, b);
@@ -497,77 +497,80 @@ __global__ __launch_bounds__(256) void tree_combine_kernel(TreeArgs a)
     const int rows = a.drafts * a.num_heads, live = rq.drafts * a.num_heads;
     const int r32 = lane & 31, hl = lane >> 5;
     const int row = rt * kRows + 32 * w + r32;
-    floatx4 acc[4] = {};
-    float m = -INFINITY, l = 0.0f;
-    if (rt * kRows + 32 * w < live) {  // else no wave has left partials of these rows
-        // past the last split a wave repeats it with weight 0
-        const size_t tile0 = (size_t)rq.slot0 * a.row_tiles + rt;
-        auto at = [&](int s) { return tile0 + (size_t)min(s, rq.n_splits - 1) * a.row_tiles; };
-        for (int s = wave; s < rq.n_splits; s += kWaves * kMany) {
-            float ms[kMany], ls[kMany];
-            floatx4 po[kMany][4];
+    for (int c = c0; c < c0 + tiles; ++c) {
+        if (c > c0)
+            __syncthreads();  // everyone has read the sums of the tile before
+        floatx4 acc[4] = {};
+        float m = -INFINITY, l = 0.0f;
+        if (rt * kRows + 32 * w < live) {  // else no wave has left partials of these rows
+            // past the last split a wave repeats it with weight 0
+            const size_t tile0 = (size_t)rq.slot0 * a.row_tiles + rt;
+            auto at = [&](int s) { return tile0 + (size_t)min(s, rq.n_splits - 1) * a.row_tiles; };
+            for (int s = wave; s < rq.n_splits; s += kWaves * kMany) {
+                float ms[kMany], ls[kMany];
+                floatx4 po[kMany][4];
 #pragma unroll
-            for (int k = 0; k < kMany; ++k) {
-                const size_t t = at(s + kWaves * k);
-                ms[k] = a.part_m[t * kRows + 32 * w + r32];
-                ls[k] = a.part_l[t * kRows + 32 * w + r32];
+                for (int k = 0; k < kMany; ++k) {
+                    const size_t t = at(s + kWaves * k);
+                    ms[k] = a.part_m[t * kRows + 32 * w + r32];
+                    ls[k] = a.part_l[t * kRows + 32 * w + r32];
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    po[k][j] = *(const floatx4 *)(a.part_o + (t * kWaves + w) * (32 * kDV) + ((c * 4 + j) * 64 + lane) * 4);
-            }
-            float next = m;
+                    for (int j = 0; j < 4; ++j)
+                        po[k][j] = *(const floatx4 *)(a.part_o + (t * kWaves + w) * (32 * kDV) + ((c * 4 + j) * 64 + lane) * 4);
+                }
+                float next = m;
 #pragma unroll
-            for (int k = 0; k < kMany; ++k)
-                next = fmaxf(next, ms[k]);
-            const float ref = next == -INFINITY ? 0.0f : next;
-            const float f0 = fast_exp2(m - ref);
-            l *= f0;
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                acc[j] *= f0;
-#pragma unroll
-            for (int k = 0; k < kMany; ++k) {
-                if (s + kWaves * k >= rq.n_splits)
-                    continue;
-                const float f = fast_exp2(ms[k] - ref);
-                l += f * ls[k];
+                for (int k = 0; k < kMany; ++k)
+                    next = fmaxf(next, ms[k]);
+                const float ref = next == -INFINITY ? 0.0f : next;
+                const float f0 = fast_exp2(m - ref);
+                l *= f0;
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    acc[j] += f * po[k][j];
+                    acc[j] *= f0;
+#pragma unroll
+                for (int k = 0; k < kMany; ++k) {
+                    if (s + kWaves * k >= rq.n_splits)
+                        continue;
+                    const float f = fast_exp2(ms[k] - ref);
+                    l += f * ls[k];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        acc[j] += f * po[k][j];
+                }
+                m = next;
             }
-            m = next;
         }
+        if (hl == 0) {
+            s_m[wave][r32] = m;
+            s_l[wave][r32] = l;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            s_o[wave][j][lane] = acc[j];
+        __syncthreads();
+        // wave j: the 4 columns of quarter j of each lane
+        float top = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < kWaves; ++k)
+            top = fmaxf(top, s_m[k][r32]);
+        const float ref = top == -INFINITY ? 0.0f : top;
+        floatx4 sum = {};
+        l = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kWaves; ++k) {
+            const float f = fast_exp2(s_m[k][r32] - ref);
+            l += f * s_l[k][r32];
+            sum += f * s_o[k][wave][lane];
+        }
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        E4 v;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            v[j] = row < live ? (E)(sum[j] * inv) : (E)0.0f;
+        if (row < rows)
+            *(E4 *)((E *)a.out + ((size_t)b * rows + row) * kDV + 32 * c + 8 * wave + 4 * hl) = v;
     }
-    if (hl == 0) {
-        s_m[wave][r32] = m;
-        s_l[wave][r32] = l;
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-        s_o[wave][j][lane] = acc[j];
-    __syncthreads();
-    // wave j: the 4 columns of quarter j of each lane
-    float top = -INFINITY;
-#pragma unroll
-    for (int k = 0; k < kWaves; ++k)
-        top = fmaxf(top, s_m[k][r32]);
-    const float ref = top == -INFINITY ? 0.0f : top;
-    floatx4 sum = {};
-    l = 0.0f;
-#pragma unroll
-    for (int k = 0; k < kWaves; ++k) {
-        const float f = fast_exp2(s_m[k][r32] - ref);
-        l += f * s_l[k][r32];
-        sum += f * s_o[k][wave][lane];
-    }
-    if (row >= rows)
-        return;
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    E4 v;
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-        v[j] = row < live ? (E)(sum[j] * inv) : (E)0.0f;
-    *(E4 *)((E *)a.out + ((size_t)b * rows + row) * kDV + 32 * c + 8 * wave + 4 * hl) = v;
 }
 
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
@@ -662,8 +665,14 @@ void launch_tree(const TreeArgs &a, int parts, hipStream_t s)
     auto k = parts == 4 ? tree_kernel<E, 4> : tree_kernel<E, 16>;
     const unsigned slots = a.by_xcd ? (a.n_slots + 7) / 8 * 8 : a.n_slots;
     hipLaunchKernelGGL(k, dim3(slots * a.row_tiles * parts), dim3(256), 0, s, a);
-    if (a.total_tokens > a.chunk)
-        hipLaunchKernelGGL(tree_combine_kernel<E>, dim3((unsigned)a.batch * a.row_tiles * (kWaves * kDV / 32)), dim3(256), 0, s, a);
+    if (a.total_tokens > a.chunk) {
+        // one 32 x 32 tile a workgroup, 4 where there are many rows: 16 requests of 16
+        // drafts x 128 heads 18.0 us (most of 16384 workgroups find nothing to do)
+        // against 16.0
+        const unsigned groups = (unsigned)a.batch * a.row_tiles * kWaves;
+        const int tiles = groups >= 512 ? 4 : 1;
+        hipLaunchKernelGGL(tree_combine_kernel<E>, dim3(groups * (kDV / 32 / tiles)), dim3(256), 0, s, a, tiles);
+    }
 }
 
 int decode_tree(bool bf16, const void *query, const void *kv_cache, const int *block_table, const int *cu_seqlens,
