@@ -604,8 +604,9 @@ TreePlan compute_tree_plan(int batch, int drafts, int num_heads, int total_token
     const int blocks = std::max(1, (longest + kBlock - 1) / kBlock);
     int splits = 1;
     double best = 0.0;
+    const int asked = std::min(num_splits, blocks);
     for (const PartCost &c : kPartCosts) {
-        const int lo = num_splits > 0 ? num_splits : 1, hi = num_splits > 0 ? num_splits : std::min(blocks, 256);
+        const int lo = asked > 0 ? asked : 1, hi = asked > 0 ? asked : std::min(blocks, 256);
         for (int n = lo; n <= hi; ++n) {
             const int per = (blocks + n - 1) / n;
             if (n > lo && (blocks + n - 2) / (n - 1) == per)

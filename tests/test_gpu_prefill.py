@@ -201,3 +201,63 @@ def test_agrees_with_the_absorbed_form():
     # norms: 2 u for the expanded form; the absorbed one rounds q*, p, its partials and o*: below 2 u again
     err = (expanded - absorbed).norm() / absorbed.norm()
     assert err <= 4 * half_step(torch.float16), err
+
+
+def test_cache_rows_past_2_to_31_elements():
+    gen = torch.Generator()
+    gen.manual_seed(13)
+    page, n = 64, 150
+    pages = 2 ** 31 // (576 * page) + 6
+    cache = torch.zeros(pages, page, 576, dtype=torch.bfloat16, device="cuda")
+    ids = [pages - 1, 2, pages - 4]
+    for i in ids:
+        cache[i] = torch.randn(page, 576, generator=gen).bfloat16().cuda()
+    qn, qr, uk, uv = _inputs(gen, n, 16, torch.bfloat16)
+    cu = _cu([n])
+    got = ada_mla.mla_prefill(qn, qr, uk, uv, cache, cu, cu, torch.tensor([ids], dtype=torch.int32, device="cuda"), n)
+    rows = cache[ids].view(-1, 576)[:n].contiguous()
+    assert torch.equal(got, ada_mla.mla_prefill(qn, qr, uk, uv, rows, cu, cu))
+    _check(got, qn, qr, uk, uv, lambda b: rows.double().cpu(), [n], [n], torch.bfloat16, "far pages")
+
+
+def test_page_ids_out_of_range_stay_inside_the_cache():
+    gen = torch.Generator()
+    gen.manual_seed(14)
+    qn, qr, uk, uv = _inputs(gen, 100, 16, torch.float16)
+    cache = torch.randn(4, 32, 576, generator=gen).half().cuda()
+    cu = _cu([100])
+    table = torch.tensor([[0, -9, 2 ** 31 - 1, 3]], dtype=torch.int32, device="cuda")
+    got = ada_mla.mla_prefill(qn, qr, uk, uv, cache, cu, cu, table, 100)
+    same = ada_mla.mla_prefill(qn, qr, uk, uv, cache, cu, cu, table.clamp(0, 3), 100)
+    assert torch.equal(got, same)
+
+
+def test_a_row_is_the_same_whatever_runs_beside_it():
+    # a request's results do not depend on the others of the batch, nor on where its tiles begin
+    gen = torch.Generator()
+    gen.manual_seed(15)
+    qn, qr, uk, uv = _inputs(gen, 300, 16, torch.float16)
+    cache = torch.randn(300, 576, generator=gen).half().cuda()
+    alone = ada_mla.mla_prefill(qn[90:], qr[90:], uk, uv, cache[90:], _cu([210]), _cu([210]))
+    both = ada_mla.mla_prefill(qn, qr, uk, uv, cache, _cu([90, 210]), _cu([90, 210]))
+    assert torch.equal(both[90:], alone)
+
+
+def test_two_streams_at_once():
+    gen = torch.Generator()
+    gen.manual_seed(16)
+    cases = []
+    for n in (400, 700):
+        qn, qr, uk, uv = _inputs(gen, n, 16, torch.bfloat16)
+        cache, cu = torch.randn(n, 576, generator=gen).bfloat16().cuda(), _cu([n])
+        cases.append((qn, qr, uk, uv, cache, cu, cu))
+    want = [ada_mla.mla_prefill(*c) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    got = []
+    for c, stream in zip(cases * 2, streams * 2):
+        with torch.cuda.stream(stream):
+            got.append(ada_mla.mla_prefill(*c))
+    torch.cuda.synchronize()
+    for g, w in zip(got, want * 2):
+        assert torch.equal(g, w)

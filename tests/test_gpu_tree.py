@@ -253,3 +253,34 @@ def test_another_stream():
         got = ada_mla.mla_decode_tree(q, cache, table, cu, mask, total_tokens=500)
     side.synchronize()
     assert torch.equal(got, want)
+
+
+def test_cache_rows_past_2_to_31_elements():
+    # a pool of more than 2^32 bytes whose last pages hold the request
+    gen = torch.Generator()
+    gen.manual_seed(17)
+    page, n = 64, 200
+    pages = 2 ** 31 // (576 * page) + 6
+    cache = torch.zeros(pages, page, 576, dtype=torch.bfloat16, device="cuda")
+    ids = [pages - 1, 3, pages - 2, pages - 3]
+    for i in ids:
+        cache[i] = torch.randn(page, 576, generator=gen).bfloat16().cuda()
+    table = torch.tensor([ids], dtype=torch.int32, device="cuda")
+    cu = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    q = torch.randn(1, 3, 16, 576, generator=gen).bfloat16().cuda()
+    masks = [chain_mask(3)]
+    mask = torch.tensor(masks, dtype=torch.int64, device="cuda")
+    got = ada_mla.mla_decode_tree(q, cache, table, cu, mask, total_tokens=n)
+    small = cache[ids].contiguous()
+    order = torch.arange(4, dtype=torch.int32, device="cuda")[None]
+    assert torch.equal(got, ada_mla.mla_decode_tree(q, small, order, cu, mask, total_tokens=n))
+    _check(got, q, small, order, [n], [3], masks, torch.bfloat16, "far pages")
+
+
+def test_one_long_request_among_empty_ones():
+    lengths = [0] * 30 + [4000] + [0, 3] * 10
+    _run(16, 3, lengths, [min(3, n) for n in lengths], 64, torch.float16, seed=18)
+
+
+def test_most_drafts_and_heads():
+    _run(256, 64, [100], [64], 32, torch.bfloat16, seed=19)

@@ -99,6 +99,15 @@ def test_workspace_sizes():
         assert lib.mla_prefill_workspace_size(*a) <= lib.mla_prefill_workspace_size(*b)
 
 
+def test_tree_splits_are_clamped_to_blocks():
+    lib = capi.load()
+    size = lib.mla_decode_tree_workspace_size
+    # 100 tokens are 4 blocks of 32, whatever is asked for
+    assert size(1, 4, 16, 100, 4) == size(1, 4, 16, 100, 5) == size(1, 4, 16, 100, 2 ** 31 - 1)
+    assert size(3, 4, 16, 2 ** 31 - 5000, 2 ** 31 - 1) > 0
+    assert size(1, 64, 4096, 0, 0) > 0
+
+
 def test_extension_refusals_tables():
     m = _ext()
     i = lambda *s: torch.zeros(*s, dtype=torch.int32)  # noqa: E731
