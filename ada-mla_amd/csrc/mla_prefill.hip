@@ -495,7 +495,8 @@ __global__ __launch_bounds__(256, 2) void attend_kernel(PrefillArgs a)
 
     floatx16 o[4] = {};
     float m = -INFINITY, l = 0.0f;
-    const int wave_last = min(q0 + 32 * wave + 31, n_q - 1) + shift;  // of the wave's queries
+    // the last key of the wave's queries; a wave without queries only loads
+    const int wave_last = q0 + 32 * wave < n_q ? min(q0 + 32 * wave + 31, n_q - 1) + shift : -1;
     const int wave_first = min(q0 + 32 * wave, n_q - 1) + shift;
     for (int j = 0; j < n_tiles; ++j) {
         MLA_WAIT_VMCNT(0);
