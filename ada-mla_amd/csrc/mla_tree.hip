@@ -81,6 +81,7 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
     using E8 = typename Vec<E>::v8;
     using E4 = typename Vec<E>::v4;
     __shared__ __attribute__((aligned(1024))) E s_ring[kRing * kSlotElems];
+    __shared__ unsigned s_bad[kWaves];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r32 = lane & 31, hl = lane >> 5;
@@ -212,9 +213,9 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
         load_block(i, block_source(i, page_of(i)));
     // A drafted token that a row does not see meets it with weight 0: 0 times
     // an infinity or NaN in its row would still be NaN, so those become 0 for
-    // the second product, once every wave has block i's logits. A row that does
-    // see such a token has its sum l a NaN from the first product already.
-    auto drop_not_finite = [&](int i) {
+    // the second product, once every wave has block i's logits. Returns the
+    // block's tokens that had one: a row that sees such a token gives NaN.
+    auto drop_not_finite = [&](int i) -> unsigned {
         constexpr int kEach = kBlock * kDV / 8 / 256;  // 16-byte pieces of a thread
         uint4 *at = (uint4 *)(s_ring + (i & (kRing - 1)) * kSlotElems) + threadIdx.x;
         uint4 v[kEach];
@@ -226,17 +227,26 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
         for (int u = 0; u < kEach; ++u)
             for (unsigned w : {v[u].x, v[u].y, v[u].z, v[u].w})
                 top = max_u16x2(top, w & 0x7fff7fffu);
-        if (not_finite<E>((unsigned short)top) || not_finite<E>((unsigned short)(top >> 16))) {
+        const bool lane_bad = not_finite<E>((unsigned short)top) || not_finite<E>((unsigned short)(top >> 16));
+        unsigned bad = 0;
+        if (__builtin_amdgcn_ballot_w64(lane_bad) != 0) {
 #pragma unroll
-            for (int u = 0; u < kEach; ++u) {
+            for (int u = 0; u < kEach; ++u) {  // the wave's pieces u are token 4 u + wave
+                bool found = false;
                 for (unsigned *w : {&v[u].x, &v[u].y, &v[u].z, &v[u].w}) {
-                    *w &= not_finite<E>((unsigned short)*w) ? 0xffff0000u : ~0u;
-                    *w &= not_finite<E>((unsigned short)(*w >> 16)) ? 0xffffu : ~0u;
+                    const unsigned keep = (not_finite<E>((unsigned short)*w) ? 0u : 0xffffu) |
+                                          (not_finite<E>((unsigned short)(*w >> 16)) ? 0u : 0xffff0000u);
+                    found |= keep != ~0u;
+                    *w &= keep;
                 }
                 at[256 * u] = v[u];
+                bad |= __builtin_amdgcn_ballot_w64(found) != 0 ? 1u << (4 * u + wave) : 0u;
             }
         }
+        if (lane == 0)
+            s_bad[wave] = bad;
         lds_barrier();
+        return s_bad[0] | s_bad[1] | s_bad[2] | s_bad[3];
     };
     // a block that holds drafted tokens, or the request's end
     auto is_edge = [&](int i) { return t_lo + (i + 1) * kBlock > context; };
@@ -344,15 +354,20 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
 
         const int t0 = t_lo + i * kBlock;
         if (is_edge(i)) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int t = t0 + key_of_reg(r, hl);
+            auto sees = [&](int t) -> bool {
                 const unsigned bit = (unsigned)(mask >> ((t - context) & 63)) & 1u;
-                const unsigned seen = (unsigned)(t < context) | ((unsigned)(t < rq.len) & bit);
-                s[r] = seen ? s[r] : -INFINITY;
-            }
+                return ((unsigned)(t < context) | ((unsigned)(t < rq.len) & bit)) != 0;
+            };
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                s[r] = sees(t0 + key_of_reg(r, hl)) ? s[r] : -INFINITY;
             most = largest(s);
-            drop_not_finite(i);
+            const unsigned bad = drop_not_finite(i);
+            if (bad != 0) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    l = ((bad >> key_of_reg(r, hl)) & 1u) != 0 && sees(t0 + key_of_reg(r, hl)) ? NAN : l;
+            }
         }
         most = reduce_halves(most, [](float x, float y) { return fmaxf(x, y); }) * a.scale_log2;
         // the reference moves only past kLazyRescale, so P is at most 2^8

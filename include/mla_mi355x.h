@@ -410,9 +410,9 @@ int mla_append_kv_bf16(const void *kv, const void *norm_weight,
  * drafts x num_heads x 512]. Drafted token i sees the request's whole context
  * and drafted token j where bit j of tree_mask[b][i] ([batch x drafts]) is set:
  * its ancestors and itself, or, with masks 2^(i+1) - 1, a plain chain. A row
- * that sees nothing, and the rows from draft_lens[b] on, are zeros. Infinities
- * and NaN in a drafted token's row reach only the rows that see it (NaN there). drafts
- * is at most 64. num_splits <= 0 picks the splits of each request's tokens. */
+ * that sees nothing, and the rows from draft_lens[b] on, are zeros. A row that
+ * sees a drafted token with an infinity or NaN in its first 512 values is NaN;
+ * what it does not see never reaches it. drafts is at most 64. num_splits <= 0 picks the splits of each request's tokens. */
 size_t mla_decode_tree_workspace_size(int batch, int drafts, int num_heads,
                                       int total_tokens, int num_splits);
 int mla_decode_tree_fp16(const void *query, const void *kv_cache,
