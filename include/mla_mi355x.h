@@ -4,7 +4,9 @@
  *     O*[h, :] = softmax_t( Q*[h, :] . C[t, :] / sqrt(192) ) . C[t, :512]
  *
  * with Q* [num_heads x 576], the latent cache C [N x 576] (first 512 columns
- * are C_N, the last 64 the rope part) and O* [num_heads x 512].
+ * are C_N, the last 64 the rope part) and O* [num_heads x 512], and of what a
+ * serving loop runs around it on a paged cache: block tables, cache rows,
+ * prompts, drafted tokens.
  *
  * This is the drop-in boundary below the PyTorch extension: the reference's
  * extension (csrc/mla_api.cpp) calls raw-pointer launchers declared in
@@ -26,7 +28,7 @@
  *    count and a per-device cache of the allocation-free entry point's
  *    scratch address (each written once per device). Per host thread: the
  *    last HIP error and the last few split plans.
- *  - num_heads must be a positive multiple of 16.
+ *  - num_heads must be a positive multiple of 16 (mla_append_kv_*: 0 to 4096).
  */
 #ifndef MLA_MI355X_H
 #define MLA_MI355X_H
