@@ -69,7 +69,7 @@ _SIGNATURES = {
     "mla_decode_tree_workspace_size": (_sz, [_i] * 5),
     "mla_decode_tree_fp16": (_i, [_vp] * 8 + [_sz] + [_i] * 8 + [_vp]),
     "mla_decode_tree_bf16": (_i, [_vp] * 8 + [_sz] + [_i] * 8 + [_vp]),
-    "mla_prefill_workspace_size": (_sz, [_i] * 3),
+    "mla_prefill_workspace_size": (_sz, [_i] * 4),
     "mla_prefill_fp16": (_i, [_vp] * 10 + [_sz] + [_i] * 7 + [_vp]),
     "mla_prefill_bf16": (_i, [_vp] * 10 + [_sz] + [_i] * 7 + [_vp]),
 }
@@ -397,7 +397,7 @@ def prefill(q_nope, q_rope, w_uk, w_uv, kv_cache, cu_q, cu_seqlens, total_tokens
         assert t.is_contiguous()
     if out is None:
         out = torch.empty((queries, n_h, 128), dtype=q_nope.dtype, device=q_nope.device)
-    ws_bytes = lib.mla_prefill_workspace_size(b, n_h, total_tokens)
+    ws_bytes = lib.mla_prefill_workspace_size(b, n_h, queries, total_tokens)
     if ws_bytes == 0:
         raise MlaError("mla_prefill_workspace_size", STATUS_INVALID_VALUE)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q_nope.device) if workspace is None else workspace

@@ -588,7 +588,8 @@ at::Tensor mla_prefill(const at::Tensor &q_nope_in, const at::Tensor &q_rope_in,
     const at::Tensor bt = block_table_in ? block_table_in->contiguous() : at::Tensor();
     const int total = static_cast<int>(given_total(total_tokens, cu, fn));
     at::Tensor out = at::empty({queries, heads, 128}, qn.options());
-    const size_t ws_bytes = mla_prefill_workspace_size(static_cast<int>(batch), static_cast<int>(heads), total);
+    const size_t ws_bytes = mla_prefill_workspace_size(static_cast<int>(batch), static_cast<int>(heads),
+                                                       static_cast<int>(queries), total);
     TORCH_CHECK(ws_bytes > 0, fn, ": unsupported sizes");
     at::Tensor ws = workspace(ws_bytes, qn);
     auto f = dt == at::kHalf ? mla_prefill_fp16 : mla_prefill_bf16;

@@ -10,7 +10,8 @@
 //
 // Two launches: expand_kernel writes K, V and the rotary parts to the
 // workspace, tile by tile of 64 keys (each sequence starts a tile of its own);
-// attend_kernel is one pass over them with a running maximum and sum.
+// attend_kernel is one pass over them with a running maximum and sum. Where few
+// queries see long contexts it splits the keys, and merge_kernel joins the parts.
 // K and V are held in the inputs' 16-bit type, as a cache of expanded heads
 // would hold them: a rounding of half a step on each, the sums in fp32. (In fp32
 // they would double the workspace and take three products of split operands
@@ -44,10 +45,14 @@ struct PrefillArgs {
     void *out;
     void *k, *v;                // [head][tile][4 column blocks][64 keys][32]
     void *rope;                 // [padded key][64]
+    float *part_o;              // [query tile][head][split][wave][4 column tiles][4][64 lanes][4]
+    float *part_m, *part_l;     // [query tile][head][split][128]
     unsigned long long *flags;  // [head][tile][4]: keys whose V holds an infinity or NaN, by 32 of its columns
     int batch, num_heads, queries, total_tokens;
     int padded;  // keys of the workspace: whole tiles
     int q_slots;
+    int splits;        // of a query tile's keys, at most
+    int split_tiles;   // key tiles a split, at least
     int group_blocks;  // weight blocks of an expanding workgroup
     int page_shift, num_pages, bt_stride;
     float scale_log2;
@@ -355,6 +360,8 @@ expand_kernel(PrefillArgs a)
 struct QueryTile {
     int q_lo, n_q, q0;  // the sequence's first query, its queries, the tile's first one
     int n_k, tile0;     // its keys, its first tile in the workspace
+    int n_tiles;        // tiles with keys that the queries see (0 or less: none)
+    int per, n_splits;  // key tiles a split, and the splits
     int rows;           // rows of out from q_lo on: the last sequence's go on to the end of it
 };
 
@@ -368,6 +375,9 @@ __device__ __forceinline__ QueryTile query_tile(const PrefillArgs &a, int slot, 
     t.rows = w.b == a.batch - 1 ? a.queries - t.q_lo : t.n_q;
     t.n_k = w.other_hi - w.other_lo;
     t.tile0 = w.other_lo / kTile + w.b;
+    t.n_tiles = (min(t.n_k, min(t.q0 + kQueries, t.n_q) + t.n_k - t.n_q) + kTile - 1) / kTile;
+    t.per = max(a.split_tiles, (t.n_tiles + a.splits - 1) / a.splits);
+    t.n_splits = max(1, (t.n_tiles + t.per - 1) / t.per);
     return t;
 }
 
@@ -422,21 +432,24 @@ __global__ __launch_bounds__(256, 2) void attend_kernel(PrefillArgs a)
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r32 = lane & 31, hl = lane >> 5;
-    // workgroup -> (head, query tile): all tiles of a head on one XCD, whose L2
+    // workgroup -> (head, query tile, split): all tiles of a head on one XCD, whose L2
     // then holds its K and V, the last (longest) first
     const int li = blockIdx.x >> 3;
-    const int h = li / a.q_slots * 8 + (blockIdx.x & 7);
-    const int slot = a.q_slots - 1 - li % a.q_slots;
+    const int h = li / (a.q_slots * a.splits) * 8 + (blockIdx.x & 7);
+    const int slot = a.q_slots - 1 - li / a.splits % a.q_slots, split = li % a.splits;
     if (h >= a.num_heads)
         return;
     const QueryTile t = query_tile(a, slot, lane);
+    if (split >= t.n_splits)
+        return;
     if (t.q0 >= t.n_q) {
-        zero_rows<E>(a, t, h);
+        if (split == 0)
+            zero_rows<E>(a, t, h);
         return;
     }
     const int q0 = t.q0, n_q = t.n_q, tile0 = t.tile0;
     const int shift = t.n_k - n_q;  // query i sees the keys 0 .. i + shift
-    const int n_tiles = (min(t.n_k, min(q0 + kQueries, n_q) + shift) + kTile - 1) / kTile;
+    const int j0 = split * t.per, j1 = min(j0 + t.per, t.n_tiles);  // the split's key tiles
 
     const int row = q0 + 32 * wave + r32;
     const int last = min(row, n_q - 1) + shift;  // the lane's last key
@@ -455,7 +468,7 @@ __global__ __launch_bounds__(256, 2) void attend_kernel(PrefillArgs a)
     const int kv_off = (kv_chunk >> 2) * (kTile * kWeightRows * 2) + (lane >> 4) * (kWeightRows * 2) + 16 * (kv_chunk & 3);
     const int rope_off = (lane >> 3) * (kRopeDim * 2) + 16 * ((lane & 7) ^ rope_swizzle(lane >> 3));
     auto load_tile = [&](int j) {
-        const unsigned at = lds + (j & 1) * (kStage * 2);
+        const unsigned at = lds + ((j - j0) & 1) * (kStage * 2);
         const E *k = ks + (size_t)j * kKElems, *v = vs + (size_t)j * kKElems, *r = rs + (size_t)j * kRElems;
         for_constants(
             [&](auto unit) {
@@ -486,9 +499,9 @@ __global__ __launch_bounds__(256, 2) void attend_kernel(PrefillArgs a)
 #pragma unroll
         for (int k = 0; k < 4; ++k)
             q[8 + k] = *(const E8 *)(qr + 16 * k);
-        if (n_tiles > 0)
-            load_tile(0);
-        if (n_tiles > 0)
+        if (j0 < j1)
+            load_tile(j0);
+        if (j0 < j1)
             MLA_WAIT_VMCNT(kUnits);
         else
             MLA_WAIT_VMCNT(0);
@@ -511,14 +524,14 @@ __global__ __launch_bounds__(256, 2) void attend_kernel(PrefillArgs a)
     // the last key of the wave's queries; a wave without queries only loads
     const int wave_last = q0 + 32 * wave < n_q ? min(q0 + 32 * wave + 31, n_q - 1) + shift : -1;
     const int wave_first = min(q0 + 32 * wave, n_q - 1) + shift;
-    for (int j = 0; j < n_tiles; ++j) {
+    for (int j = j0; j < j1; ++j) {
         MLA_WAIT_VMCNT(0);
         lds_barrier();  // tile j is there, and everyone is done with tile j - 1
-        if (j + 1 < n_tiles)
+        if (j + 1 < j1)
             load_tile(j + 1);
         if (j * kTile > wave_last)
             continue;
-        const unsigned at = lds + (j & 1) * (kStage * 2);
+        const unsigned at = lds + ((j - j0) & 1) * (kStage * 2);
         floatx16 s[2] = {};
         {
             // operand k of both 32-key blocks: 8 steps of the head's own part, 4 of the rotary one
@@ -617,8 +630,91 @@ __global__ __launch_bounds__(256, 2) void attend_kernel(PrefillArgs a)
         }
     }
     l = reduce_halves(l, [](float x, float y) { return x + y; });
+    if (t.n_splits > 1) {
+        const size_t part = ((size_t)slot * a.num_heads + h) * a.splits + split;
+        float *po = a.part_o + (part * 4 + wave) * (32 * kNope);
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                *(floatx4 *)(po + ((c * 4 + k) * 64 + lane) * 4) =
+                    floatx4{o[c][4 * k], o[c][4 * k + 1], o[c][4 * k + 2], o[c][4 * k + 3]};
+        if (hl == 0) {
+            a.part_m[part * kQueries + 32 * wave + r32] = m;
+            a.part_l[part * kQueries + 32 * wave + r32] = l;
+        }
+        return;
+    }
     lds_barrier();  // everyone is done with the last tile
     store_rows<E>(a, t, h, q0 + 32 * wave, lane, lds + wave * 8192, o, l);
+}
+
+// Merges the splits of the query tiles that have more than one. A workgroup takes 32
+// rows of a head, wave c their columns 32 c .., and a lane the 16 values it would hold in
+// attend_kernel. The splits are added in their order.
+template <typename E>
+__global__ __launch_bounds__(256) void merge_kernel(PrefillArgs a)
+{
+    using E4 = typename Vec<E>::v4;
+    const int lane = threadIdx.x & 63;
+    const int c = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int w = blockIdx.x & 3, h = (blockIdx.x >> 2) % a.num_heads, slot = (blockIdx.x >> 2) / a.num_heads;
+    const QueryTile t = query_tile(a, slot, lane);
+    const int first = t.q0 + 32 * w;
+    if (t.n_splits == 1 || t.q0 >= t.n_q || first >= t.rows)
+        return;
+    const int r32 = lane & 31, hl = lane >> 5;
+    const size_t part0 = ((size_t)slot * a.num_heads + h) * a.splits;
+    constexpr int kMany = 4;  // splits in flight together
+    floatx4 acc[4] = {};
+    float m = -INFINITY, l = 0.0f;
+    for (int s = 0; first < t.n_q && s < t.n_splits; s += kMany) {
+        float ms[kMany], ls[kMany];
+        floatx4 po[kMany][4];
+#pragma unroll
+        for (int k = 0; k < kMany; ++k) {  // past the last split it is read again, and not used
+            const size_t part = part0 + min(s + k, t.n_splits - 1);
+            ms[k] = a.part_m[part * kQueries + 32 * w + r32];
+            ls[k] = a.part_l[part * kQueries + 32 * w + r32];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                po[k][j] = *(const floatx4 *)(a.part_o + (part * 4 + w) * (32 * kNope) + ((c * 4 + j) * 64 + lane) * 4);
+        }
+        float next = m;
+#pragma unroll
+        for (int k = 0; k < kMany; ++k)
+            next = fmaxf(next, ms[k]);
+        const float ref = next == -INFINITY ? 0.0f : next;
+        const float f0 = fast_exp2(m - ref);
+        l *= f0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            acc[j] *= f0;
+#pragma unroll
+        for (int k = 0; k < kMany; ++k) {
+            if (s + k >= t.n_splits)
+                continue;
+            const float f = fast_exp2(ms[k] - ref);
+            l += f * ls[k];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                acc[j] += f * po[k][j];
+        }
+        m = next;
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const int row = first + r32;
+    if (row >= t.rows)
+        return;
+    E *out = (E *)a.out + ((size_t)(t.q_lo + row) * a.num_heads + h) * kNope + 32 * c + 4 * hl;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        E4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            v[e] = row < t.n_q ? (E)(acc[j][e] * inv) : (E)0.0f;
+        *(E4 *)(out + 8 * j) = v;
+    }
 }
 
 // ---- host -------------------------------------------------------------------
@@ -627,14 +723,53 @@ size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
 struct PrefillPlan {
     int padded;
-    size_t kv_bytes, rope_bytes, flag_bytes;
-    size_t bytes() const { return 2 * kv_bytes + rope_bytes + flag_bytes; }
+    int q_slots, splits, split_tiles;
+    size_t kv_bytes, rope_bytes, flag_bytes, o_bytes, ml_bytes;
+    size_t bytes() const { return 2 * kv_bytes + rope_bytes + flag_bytes + o_bytes + 2 * ml_bytes; }
 };
 
+// Splits of the keys, where few query tiles see long contexts: those with the least
+// modelled time, for requests of mean lengths. A workgroup costs its start and end
+// and its tiles, more each where two run on a CU; partials (fp32, written and read) and a
+// third launch are the price. A split has a given number of tiles, more where a request is
+// longer than the splits then reach. Calls in one split and as planned: 1 query behind
+// 8000 tokens at 16 heads 225 us and 71, 500 queries there 274 and 138, 1000 at 32
+// heads 336 and 311, 100 behind 2000 at 16 heads 76 and 38.
+constexpr double kStartUs = 4.0, kTileUs = 1.3, kSharedTileUs = 1.8, kMergeUs = 4.0, kPartialUsPerByte = 0.4e-6;
+
+void plan_splits(PrefillPlan &p, int batch, int num_heads, int queries, int total_tokens, int cu_count)
+{
+    const int64_t mean_q = ((int64_t)queries + batch - 1) / batch, mean_k = ((int64_t)total_tokens + batch - 1) / batch;
+    const int64_t wgs = (mean_q + kQueries - 1) / kQueries * batch * num_heads;
+    const int tiles = (int)std::max<int64_t>(1, (mean_k + kTile - 1) / kTile);
+    p.splits = 1;
+    p.split_tiles = INT32_MAX / 2;
+    double best = 0.0;
+    for (int n = 1; n <= std::min(tiles, 128); ++n) {
+        const int per = (tiles + n - 1) / n;
+        if (n > 1 && (tiles + n - 2) / (n - 1) == per)
+            continue;  // no shorter than the one before
+        const int64_t rounds = std::max<int64_t>(1, (wgs * n + 2 * cu_count - 1) / (2 * cu_count));
+        double us = rounds * (kStartUs + per * (wgs * n > cu_count ? kSharedTileUs : kTileUs));
+        if (n > 1)
+            us += kMergeUs + kPartialUsPerByte * wgs * n * (kQueries * kNope * 4.0);
+        if (n == 1 || us < best) {
+            best = us;
+            p.splits = n;
+            p.split_tiles = n == 1 ? INT32_MAX / 2 : per;
+        }
+    }
+}
+
 // Sequence b's keys start at tile cu[b] / 64 + b of the workspace.
-PrefillPlan prefill_plan(int batch, int num_heads, int total_tokens)
+PrefillPlan prefill_plan(int batch, int num_heads, int queries, int total_tokens)
 {
     PrefillPlan p;
+    p.q_slots = queries / kQueries + batch;
+    plan_splits(p, batch, num_heads, queries, total_tokens, current_cu_count());
+    const size_t parts = p.splits > 1 ? (size_t)p.q_slots * num_heads * p.splits : 0;
+    p.o_bytes = align256(parts * kQueries * kNope * sizeof(float));
+    p.ml_bytes = align256(parts * kQueries * sizeof(float));
     p.padded = total_tokens / kTile * kTile + kTile * batch;
     p.kv_bytes = align256((size_t)num_heads * p.padded * kNope * 2);
     p.rope_bytes = align256((size_t)p.padded * kRopeDim * 2);
@@ -670,9 +805,9 @@ int expand_group_blocks(int batch, int total_tokens, int num_heads, int cu_count
     return best;
 }
 
-bool prefill_sizes_ok(int batch, int num_heads, int total_tokens)
+bool prefill_sizes_ok(int batch, int num_heads, int queries, int total_tokens)
 {
-    return batch >= 1 && num_heads > 0 && num_heads % 16 == 0 && num_heads <= 4096 && total_tokens >= 0 &&
+    return batch >= 1 && queries >= 1 && queries <= INT32_MAX - 4096 && num_heads > 0 && num_heads % 16 == 0 && num_heads <= 4096 && total_tokens >= 0 &&
            (int64_t)total_tokens + (int64_t)kTile * batch <= INT32_MAX - 4096;
 }
 
@@ -684,7 +819,9 @@ void launch_prefill(const PrefillArgs &a, hipStream_t s)
         const int groups = (2 * kBlocksPerSide * a.num_heads + a.group_blocks - 1) / a.group_blocks;
         hipLaunchKernelGGL(expand_kernel<E>, dim3((unsigned)quads * ((groups + 7) / 8 * 8)), dim3(256), 0, s, a);
     }
-    hipLaunchKernelGGL(attend_kernel<E>, dim3((unsigned)a.q_slots * a.num_heads), dim3(256), 0, s, a);
+    hipLaunchKernelGGL(attend_kernel<E>, dim3((unsigned)a.q_slots * a.num_heads * a.splits), dim3(256), 0, s, a);
+    if (a.splits > 1)
+        hipLaunchKernelGGL(merge_kernel<E>, dim3((unsigned)a.q_slots * a.num_heads * 4), dim3(256), 0, s, a);
 }
 
 int prefill(bool bf16, const void *q_nope, const void *q_rope, const void *w_uk, const void *w_uv, const void *kv_cache,
@@ -692,19 +829,21 @@ int prefill(bool bf16, const void *q_nope, const void *q_rope, const void *w_uk,
             size_t workspace_bytes, int batch, int num_heads, int queries, int total_tokens, int page_size,
             int num_pages, int block_table_stride, void *stream)
 {
-    if (!prefill_sizes_ok(batch, num_heads, total_tokens) || queries < 1 || queries > INT32_MAX - 4096 || !q_nope ||
-        !q_rope || !w_uk || !w_uv || (!kv_cache && total_tokens > 0) || !cu_q || !cu_seqlens || !out || !workspace ||
+    if (!prefill_sizes_ok(batch, num_heads, queries, total_tokens) || !q_nope || !q_rope || !w_uk || !w_uv ||
+        (!kv_cache && total_tokens > 0) || !cu_q || !cu_seqlens || !out || !workspace ||
         (block_table && (page_size < 32 || page_size > (1 << 20) || (page_size & (page_size - 1)) != 0 ||
                          num_pages < 1 || block_table_stride < 1)))
         return MLA_STATUS_INVALID_VALUE;
     if (!aligned16(q_nope) || !aligned16(q_rope) || !aligned16(w_uk) || !aligned16(w_uv) || !aligned16(kv_cache) ||
         !aligned16(out) || !aligned16(workspace))
         return MLA_STATUS_MISALIGNED;
-    const PrefillPlan p = prefill_plan(batch, num_heads, total_tokens);
+    const PrefillPlan p = prefill_plan(batch, num_heads, queries, total_tokens);
     PrefillArgs a;
-    a.q_slots = queries / kQueries + batch;
+    a.q_slots = p.q_slots;
+    a.splits = p.splits;
+    a.split_tiles = p.split_tiles;
     if ((int64_t)(p.padded / kTile + 1) * num_heads > INT32_MAX / 256 ||
-        (int64_t)a.q_slots * num_heads > INT32_MAX / 256)
+        (int64_t)a.q_slots * num_heads > INT32_MAX / 256 / std::max(4, p.splits))
         return MLA_STATUS_INVALID_VALUE;
     if (workspace_bytes < p.bytes())
         return MLA_STATUS_WORKSPACE_TOO_SMALL;
@@ -722,6 +861,9 @@ int prefill(bool bf16, const void *q_nope, const void *q_rope, const void *w_uk,
     a.v = ws + p.kv_bytes;
     a.rope = ws + 2 * p.kv_bytes;
     a.flags = reinterpret_cast<unsigned long long *>(ws + 2 * p.kv_bytes + p.rope_bytes);
+    a.part_o = reinterpret_cast<float *>(ws + 2 * p.kv_bytes + p.rope_bytes + p.flag_bytes);
+    a.part_m = a.part_o + p.o_bytes / sizeof(float);
+    a.part_l = a.part_m + p.ml_bytes / sizeof(float);
     a.batch = batch;
     a.num_heads = num_heads;
     a.queries = queries;
@@ -745,10 +887,10 @@ int prefill(bool bf16, const void *q_nope, const void *q_rope, const void *w_uk,
 
 extern "C" {
 
-size_t mla_prefill_workspace_size(int batch, int num_heads, int total_tokens)
+size_t mla_prefill_workspace_size(int batch, int num_heads, int queries, int total_tokens)
 {
-    return mla::prefill_sizes_ok(batch, num_heads, total_tokens)
-               ? mla::prefill_plan(batch, num_heads, total_tokens).bytes()
+    return mla::prefill_sizes_ok(batch, num_heads, queries, total_tokens)
+               ? mla::prefill_plan(batch, num_heads, queries, total_tokens).bytes()
                : 0;
 }
 

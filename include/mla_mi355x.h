@@ -449,8 +449,10 @@ int mla_decode_tree_bf16(const void *query, const void *kv_cache,
  * mla_absorb_query_* / mla_project_output_*. K and V are rounded to the
  * inputs' type; a query that sees a key whose V is not finite gives NaN, and
  * what it does not see never reaches it. The workspace holds K and V: 512
- * bytes a key and head. Two launches. */
-size_t mla_prefill_workspace_size(int batch, int num_heads, int total_tokens);
+ * bytes a key and head, and partial results where few queries see many keys.
+ * Two launches, three with partials. */
+size_t mla_prefill_workspace_size(int batch, int num_heads, int queries,
+                                  int total_tokens);
 int mla_prefill_fp16(const void *q_nope, const void *q_rope, const void *w_uk,
                      const void *w_uv, const void *kv_cache,
                      const int *block_table, const int *cu_q,

@@ -154,7 +154,7 @@ def test_workspace_of_nans():
     gen = torch.Generator()
     gen.manual_seed(10)
     lib = capi.load()
-    ws = torch.full((lib.mla_prefill_workspace_size(4, 16, 500),), 255, dtype=torch.uint8, device="cuda")
+    ws = torch.full((lib.mla_prefill_workspace_size(4, 16, 231, 500),), 255, dtype=torch.uint8, device="cuda")
     for lengths in ([100, 3, 64, 65], [1, 1, 1, 1], [0, 200, 0, 31]):
         qn, qr, uk, uv = _inputs(gen, sum(lengths), 16, torch.float16)
         cache = torch.randn(sum(lengths), 576, generator=gen).half().cuda()
@@ -261,3 +261,67 @@ def test_two_streams_at_once():
     torch.cuda.synchronize()
     for g, w in zip(got, want * 2):
         assert torch.equal(g, w)
+
+
+def _partials(batch, heads, queries, total):
+    """Whether a call splits its keys: its workspace then holds more than K, V, rotary parts and flags."""
+    tiles = total // 64 + batch
+    up = lambda n: (n + 255) // 256 * 256  # noqa: E731
+    plain = 2 * up(heads * tiles * 64 * 256) + up(tiles * 64 * 128) + up(heads * tiles * 32)
+    return capi.load().mla_prefill_workspace_size(batch, heads, queries, total) > plain
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("queries,context,page", [
+    ([1], [6000], 64), ([33], [4063], 0), ([7, 1, 0, 140, 3], [5000, 1, 900, 1337, 64], 32), ([200], [3900], 128)])
+def test_few_queries_behind_long_contexts(queries, context, page, dtype):
+    # keys split over workgroups; a short request among long ones, tiles that end inside a split
+    total = sum(queries) + sum(context)
+    assert _partials(len(queries), 16, sum(queries), total)
+    _run(queries, context, 16, dtype, page, seed=total)
+
+
+def test_split_keys_padded_rows_and_values_that_are_not_finite():
+    gen = torch.Generator()
+    gen.manual_seed(17)
+    n, m, rows = 5000, 40, 170
+    assert _partials(1, 16, rows, n)
+    qn, qr, uk, uv = _inputs(gen, rows, 16, torch.bfloat16)
+    cache = torch.randn(n, 576, generator=gen).bfloat16().cuda()
+    call = lambda: capi.prefill(qn, qr, uk, uv, cache, _cu([m]), _cu([n]), n,  # noqa: E731
+                                out=torch.full((rows, 16, 128), float("nan"), dtype=torch.bfloat16, device="cuda"))
+    want = call()
+    assert torch.isfinite(want).all() and not want[m:].any()
+    assert torch.equal(call(), want)
+    cache[n - 20, 7] = float("inf")  # seen by the last 20 queries
+    got = call()
+    assert torch.equal(got[:20], want[:20]) and torch.isnan(got[20:m]).all() and not got[m:].any()
+    cache[n - 20, 7] = 0
+    cache[100, 3] = float("nan")  # seen by all
+    got = call()
+    assert torch.isnan(got[:m]).all() and not got[m:].any()
+
+
+def test_split_keys_captured_and_replayed():
+    gen = torch.Generator()
+    gen.manual_seed(18)
+    n = 3500
+    qn, qr, uk, uv = _inputs(gen, 60, 16, torch.float16)
+    cache = torch.randn(n, 576, generator=gen).half().cuda()
+    cu_q, cu = _cu([10, 50]), _cu([500, n - 500])
+    assert _partials(2, 16, 60, n)
+    call = lambda: ada_mla.mla_prefill(qn, qr, uk, uv, cache, cu_q, cu, total_tokens=n)  # noqa: E731
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for r in range(4):
+        qn.normal_()
+        cache.normal_()
+        cu[1:2].add_(200)
+        want = call().clone()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.isfinite(want).all() and torch.equal(out, want), r

@@ -90,12 +90,12 @@ def test_workspace_sizes():
     assert lib.mla_decode_tree_workspace_size(1, 65, 16, 100, 0) == 0
     assert lib.mla_decode_tree_workspace_size(1, 4, 24, 100, 0) == 0
     assert lib.mla_decode_tree_workspace_size(1, 4, 16, 0, 0) > 0
-    assert lib.mla_prefill_workspace_size(1, 24, 100) == 0
-    assert lib.mla_prefill_workspace_size(0, 16, 100) == 0
+    assert lib.mla_prefill_workspace_size(1, 24, 50, 100) == 0
+    assert lib.mla_prefill_workspace_size(0, 16, 50, 100) == 0
     # K and V of whole tiles of 64 keys, at least 512 bytes a key and head
-    assert lib.mla_prefill_workspace_size(3, 16, 1000) >= 1000 * 16 * 512
+    assert lib.mla_prefill_workspace_size(3, 16, 1000, 1000) >= 1000 * 16 * 512
     # it never falls as the batch or the tokens grow
-    for a, b in (((1, 16, 100), (2, 16, 100)), ((4, 32, 100), (4, 32, 101)), ((4, 32, 127), (4, 32, 128))):
+    for a, b in (((1, 16, 50, 100), (2, 16, 50, 100)), ((4, 32, 50, 100), (4, 32, 50, 101)), ((4, 32, 50, 127), (4, 32, 50, 128))):
         assert lib.mla_prefill_workspace_size(*a) <= lib.mla_prefill_workspace_size(*b)
 
 
