@@ -53,6 +53,7 @@ struct PrefillArgs {
     int q_slots;
     int splits;        // of a query tile's keys, at most
     int split_tiles;   // key tiles a split, at least
+    int key_groups;    // of 32 keys a wave in expand_kernel, 1 or 2
     int group_blocks;  // weight blocks of an expanding workgroup
     int page_shift, num_pages, bt_stride;
     float scale_log2;
@@ -104,10 +105,12 @@ __device__ __forceinline__ Owner owner_of_slot(const int *cu, int most, const in
 // beside them. The workspace holds a tile's 64 keys x 32 columns of a block in one
 // piece, so that a block's four stores a wave fill 4 KB of whole lines: in rows of 256
 // bytes they were what bound this kernel (8192 keys at 64 heads 156 us, 124 without them).
+// kGroups: groups of 32 keys a wave, 2 or, for calls that leave most of the CUs
+// idle, 1: half the time to load the keys, and one product a LDS read.
 constexpr int kWeightRows = 32;                       // rows of W a block
 constexpr int kWeightElems = kWeightRows * kLatent;   // 32 KB
 constexpr int kWeightRing = 4;
-constexpr int kExpandTiles = 4;                       // key tiles a workgroup: one a wave
+constexpr int kExpandWaves = 4;
 constexpr int kBlocksPerSide = kNope / kWeightRows;   // blocks of one head's W_UK or W_UV
 
 // The row of a weight block in row rho = 8 q + 4 c + j of the product's tile:
@@ -125,7 +128,7 @@ __device__ __forceinline__ int weight_swizzle(int r)
     return 8 * ((r >> 2) & 1) + 4 * ((r >> 3) & 1) + (r & 3);
 }
 
-template <typename E>
+template <typename E, int kGroups>
 __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_per_eu(1, 1))) void
 expand_kernel(PrefillArgs a)
 {
@@ -136,9 +139,11 @@ expand_kernel(PrefillArgs a)
     const int r32 = lane & 31, hl = lane >> 5;
     // workgroup -> (group of weight blocks, four key tiles): the key tiles of a
     // group get ids that differ by 8, one XCD, whose L2 then holds the group's weights
-    const int tiles = a.padded / kTile, quads = (tiles + kExpandTiles - 1) / kExpandTiles;
+    constexpr int kPerTile = 2 / kGroups;  // waves
+    const int tiles = a.padded / kTile, quads = (tiles * kPerTile + kExpandWaves - 1) / kExpandWaves;
     const int group = (blockIdx.x >> 3) / quads * 8 + (blockIdx.x & 7);
-    const int tile = (blockIdx.x >> 3) % quads * kExpandTiles + wave;
+    const int unit = (blockIdx.x >> 3) % quads * kExpandWaves + wave;
+    const int tile = unit / kPerTile, key0 = 32 * (unit % kPerTile);  // the wave's tile, and its first key there
     const int n_blocks = 2 * kBlocksPerSide * a.num_heads;
     const int blk0 = group * a.group_blocks, blk1 = min(blk0 + a.group_blocks, n_blocks);
     if (blk0 >= n_blocks)
@@ -175,8 +180,8 @@ expand_kernel(PrefillArgs a)
     // a workgroup with all CUs loading. Rows past the sequence are zeros.
     const Owner w = owner_of_slot(a.cu_seqlens, a.total_tokens, a.cu_seqlens, a.total_tokens, a.batch, kTile, tile, lane);
     const int b = w.b, seq_lo = w.lo, len = w.hi - w.lo;
-    const int t0 = (tile - seq_lo / kTile - b) * kTile;
-    const bool live = tile < tiles && t0 < len;  // else nobody reads this tile
+    const int t0 = (tile - seq_lo / kTile - b) * kTile + key0;
+    const bool live = tile < tiles && t0 - key0 < len;  // else nobody reads this tile
     if (!__syncthreads_or(live))
         return;
     auto key_source = [&](int t) -> const E * {  // latent row t of the sequence; the 32 rows of a block follow it
@@ -190,9 +195,9 @@ expand_kernel(PrefillArgs a)
         }
         return (const E *)a.cache + row * kDK;
     };
-    E8 key[2][kLatent / 16];
+    E8 key[kGroups][kLatent / 16];
 #pragma unroll
-    for (int g = 0; g < 2; ++g) {
+    for (int g = 0; g < kGroups; ++g) {
         const int t = t0 + 32 * g;
         if (live && t < len) {
             const E *src = wave_uniform(key_source(t));
@@ -205,7 +210,7 @@ expand_kernel(PrefillArgs a)
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
                     const int r = 8 * u + (lane >> 3);
-                    *(uint4 *)((E *)a.rope + ((size_t)tile * kTile + 32 * g + r) * kRopeDim + 8 * (lane & 7)) =
+                    *(uint4 *)((E *)a.rope + ((size_t)tile * kTile + key0 + 32 * g + r) * kRopeDim + 8 * (lane & 7)) =
                         *(const uint4 *)(src + (size_t)min(r, lim) * kDK + kLatent + 8 * (lane & 7));
                 }
             }
@@ -234,11 +239,11 @@ expand_kernel(PrefillArgs a)
 
     const int row = weight_row(r32);
     const unsigned w_lane = row * (kLatent * 2) + 16 * (hl ^ weight_swizzle(row));
-    unsigned long long bad = 0;  // the tile's keys whose V is not finite, in the block of `store`
-    const unsigned row_at = r32 * (kWeightRows * 2) + 16 * hl;  // the lane's first 8 values in the block's rows
+    unsigned bad[kGroups] = {};  // the wave's keys whose V is not finite, in the block of `store`
+    const unsigned row_at = (key0 + r32) * (kWeightRows * 2) + 16 * hl;  // the lane's first 8 values in the block's rows
     // Rounds and stores quarter `part` of key group g of block i, whose sums
     // are in acc; v and top gather a group's four quarters.
-    auto store = [&](int i, const floatx16 (&acc)[2], int g, int part, unsigned &top, E8 (&v)[2]) {
+    auto store = [&](int i, const floatx16 (&acc)[kGroups], int g, int part, unsigned &top, E8 (&v)[2]) {
         typedef float floatx4v __attribute__((ext_vector_type(4)));
         const auto x = __builtin_convertvector(
             (floatx4v{acc[g][4 * part], acc[g][4 * part + 1], acc[g][4 * part + 2], acc[g][4 * part + 3]}), typename Vec<E>::v4);
@@ -263,7 +268,7 @@ expand_kernel(PrefillArgs a)
                 const E y = v[r >> 3][r & 7];
                 v[r >> 3][r & 7] = not_finite<E>(__builtin_bit_cast(unsigned short, y)) ? (E)0.0f : y;
             }
-            bad |= (unsigned long long)((unsigned)m | (unsigned)(m >> 32)) << (32 * g);
+            bad[g] |= (unsigned)m | (unsigned)(m >> 32);
         }
         char *dst = (char *)wave_uniform((const char *)(side ? a.v : a.k) +
                                          (((size_t)h * tiles + tile) * kBlocksPerSide + rest % kBlocksPerSide) *
@@ -271,21 +276,22 @@ expand_kernel(PrefillArgs a)
         if (i >= blk0 && live) {
             *(E8 *)(dst + (row_at + 32 * g * (kWeightRows * 2))) = v[0];
             *(E8 *)(dst + (row_at + 32 * g * (kWeightRows * 2) + 32)) = v[1];
-            if (side && g == 1 && lane == 0)
-                a.flags[((size_t)h * tiles + tile) * kBlocksPerSide + rest % kBlocksPerSide] = bad;
+            if (side && lane == 0)
+                ((unsigned *)a.flags)[2 * (((size_t)h * tiles + tile) * kBlocksPerSide + rest % kBlocksPerSide) + key0 / 32 + g] =
+                    bad[g];
         }
-        if (side && g == 1)
-            bad = 0;
+        bad[g] = 0;
     };
     // Block i into acc, while block i - 1, in prev, is rounded and stored
     // between the products, a quarter of a group after every 8 of the 64.
-    auto block = [&](int i, floatx16 (&acc)[2], floatx16 (&prev)[2]) {
+    auto block = [&](int i, floatx16 (&acc)[kGroups], floatx16 (&prev)[kGroups]) {
         // Block i's 8 loads went out during block i - 3. Behind the last of them
-        // come, in order, 2 stores of that block (half of block i - 4's 4; one more
-        // where it holds flags), then twice 8 loads (of blocks i + 1, i + 2)
-        // and 4 stores: at least 26. The first blocks have fewer stores behind them.
+        // come, in order, that block's 2 stores of a second group (half of block i - 4's;
+        // one more where it holds flags), then twice 8 loads (of blocks i + 1, i + 2)
+        // and 2 stores a group: at least 26, or 20 of one group. The first blocks have fewer
+        // stores behind them.
         if (live && i - blk0 >= 4)
-            MLA_WAIT_VMCNT(2 * (kWeightRows / 4) + 2 * 4 + 2);
+            MLA_WAIT_VMCNT(2 * (kWeightRows / 4) + 2 * 2 * kGroups + 2 * (kGroups - 1));
         else
             MLA_WAIT_VMCNT(2 * (kWeightRows / 4));
         lds_barrier();  // block i is there, and block i - 1's slot is free
@@ -294,8 +300,8 @@ expand_kernel(PrefillArgs a)
         const unsigned at = ring + ((i - blk0) & (kWeightRing - 1)) * (kWeightElems * 2) + w_lane;
         auto operand = [&](int k) -> E8 { return lds_load<E8>((at ^ (32 * (k & 7))) + 256 * (k >> 3)); };
         constexpr int kAhead = 4;  // steps an operand is read ahead
-        E8 w[kAhead + 1], v[2][2];
-        unsigned top[2] = {0, 0};
+        E8 w[kAhead + 1], v[kGroups][2];
+        unsigned top[kGroups] = {};
 #pragma unroll
         for (int k = 0; k < kAhead; ++k)
             w[k] = operand(k);
@@ -305,27 +311,27 @@ expand_kernel(PrefillArgs a)
                 if constexpr (k + kAhead < kLatent / 16)
                     w[(k + kAhead) % (kAhead + 1)] = operand(k + kAhead);
 #pragma unroll
-                for (int g = 0; g < 2; ++g) {
+                for (int g = 0; g < kGroups; ++g) {
                     if constexpr (k == 0)
                         mfma32x32x16_first_acc(acc[g], w[0], key[g][0]);
                     else
                         mfma32x32x16_next_acc(acc[g], w[k % (kAhead + 1)], key[g][k]);
                 }
-                if constexpr (k == 2) {  // six products behind the last of block i - 1
-                    in_registers(prev[0]);
-                    in_registers(prev[1]);
-                }
+                if constexpr (k == 2)  // three products at least behind the last of block i - 1
+#pragma unroll
+                    for (int g = 0; g < kGroups; ++g)
+                        in_registers(prev[g]);
                 if constexpr (k % 4 == 1)
                     load_unit(feed_src, feed_at, std::integral_constant<int, k / 4>{});
-                if constexpr (k % 4 == 3)
+                if constexpr (k % 4 == 3 && k / 16 < kGroups)
                     store(i - 1, prev, k / 16, k / 4 % 4, top[k / 16], v[k / 16]);
                 __builtin_amdgcn_sched_barrier(0);
             },
             std::make_integer_sequence<int, kLatent / 16>{});
     };
-    auto store_last = [&](floatx16 (&acc)[2]) {
+    auto store_last = [&](floatx16 (&acc)[kGroups]) {
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
+        for (int g = 0; g < kGroups; ++g) {
             mfma_settle(acc[g]);
             E8 v[2];
             unsigned top = 0;
@@ -334,7 +340,7 @@ expand_kernel(PrefillArgs a)
                 store(blk1 - 1, acc, g, part, top, v);
         }
     };
-    floatx16 even[2] = {}, odd[2] = {};
+    floatx16 even[kGroups] = {}, odd[kGroups] = {};
     for (int i = blk0; i < blk1; i += 2) {
         block(i, even, odd);
         if (i + 1 < blk1)
@@ -777,32 +783,37 @@ PrefillPlan prefill_plan(int batch, int num_heads, int queries, int total_tokens
     return p;
 }
 
-// Weight blocks of an expanding workgroup. It costs its key loads (about as
-// long as kKeyBlocks blocks) and its blocks, and one runs on a CU at a time: of
-// the divisions into a multiple of 8 groups (one XCD's workgroups take the same
-// ones) that fill one round, two rounds, .., the one with the fewest blocks in
-// a row wins.
-constexpr int kKeyBlocks = 6;
+// Weight blocks of an expanding workgroup, and its key groups a wave. It costs its key
+// loads (about as long as kKeyBlocks blocks, half with one group) and its blocks (kOneGroupBlock
+// of the time with one group), and one runs on a CU at a time: of the divisions into a multiple of 8
+// groups of blocks (one XCD's workgroups take the same ones) that fill one round, two
+// rounds, .., the one with the least time wins.
+constexpr double kKeyBlocks = 6.0, kOneGroupBlock = 0.65;
 
-int expand_group_blocks(int batch, int total_tokens, int num_heads, int cu_count)
+void plan_expansion(PrefillArgs &a, int cu_count)
 {
     // key tiles that hold keys, at most (workgroups without any leave at once)
-    const int64_t tiles = ((int64_t)total_tokens + (int64_t)(kTile - 1) * batch) / kTile;
-    const int64_t quads = std::max<int64_t>(1, (tiles + kExpandTiles - 1) / kExpandTiles);
-    const int blocks = 2 * kBlocksPerSide * num_heads;
-    int best = blocks / 8;
-    int64_t best_cost = (quads * 8 + cu_count - 1) / cu_count * (best + kKeyBlocks);
-    for (int rounds = 1; rounds <= 16; ++rounds) {
-        const int64_t groups = std::min<int64_t>(rounds * (int64_t)cu_count / quads / 8 * 8, blocks);
-        if (groups < 8)
-            continue;
-        const int per = (int)((blocks + groups - 1) / groups);
-        if (rounds * (int64_t)(per + kKeyBlocks) < best_cost) {
-            best = per;
-            best_cost = rounds * (int64_t)(per + kKeyBlocks);
+    const int64_t tiles = ((int64_t)a.total_tokens + (int64_t)(kTile - 1) * a.batch) / kTile;
+    const int blocks = 2 * kBlocksPerSide * a.num_heads;
+    double best = 0.0;
+    for (int key_groups = 2; key_groups >= 1; --key_groups) {
+        const int64_t quads = std::max<int64_t>(1, (tiles * 2 / key_groups + kExpandWaves - 1) / kExpandWaves);
+        const double start = kKeyBlocks / 2 * key_groups, each = key_groups == 2 ? 1.0 : kOneGroupBlock;
+        auto consider = [&](int64_t rounds, int per) {
+            const double cost = rounds * (per * each + start);
+            if (best == 0.0 || cost < best) {
+                best = cost;
+                a.key_groups = key_groups;
+                a.group_blocks = per;
+            }
+        };
+        consider((quads * 8 + cu_count - 1) / cu_count, blocks / 8);
+        for (int rounds = 1; rounds <= 16; ++rounds) {
+            const int64_t groups = std::min<int64_t>(rounds * (int64_t)cu_count / quads / 8 * 8, blocks);
+            if (groups >= 8)
+                consider(rounds, (int)((blocks + groups - 1) / groups));
         }
     }
-    return best;
 }
 
 bool prefill_sizes_ok(int batch, int num_heads, int queries, int total_tokens)
@@ -815,9 +826,10 @@ template <typename E>
 void launch_prefill(const PrefillArgs &a, hipStream_t s)
 {
     if (a.total_tokens > 0) {
-        const int quads = (a.padded / kTile + kExpandTiles - 1) / kExpandTiles;
+        const int quads = (a.padded / kTile * (2 / a.key_groups) + kExpandWaves - 1) / kExpandWaves;
         const int groups = (2 * kBlocksPerSide * a.num_heads + a.group_blocks - 1) / a.group_blocks;
-        hipLaunchKernelGGL(expand_kernel<E>, dim3((unsigned)quads * ((groups + 7) / 8 * 8)), dim3(256), 0, s, a);
+        auto k = a.key_groups == 2 ? expand_kernel<E, 2> : expand_kernel<E, 1>;
+        hipLaunchKernelGGL(k, dim3((unsigned)quads * ((groups + 7) / 8 * 8)), dim3(256), 0, s, a);
     }
     hipLaunchKernelGGL(attend_kernel<E>, dim3((unsigned)a.q_slots * a.num_heads * a.splits), dim3(256), 0, s, a);
     if (a.splits > 1)
@@ -842,7 +854,7 @@ int prefill(bool bf16, const void *q_nope, const void *q_rope, const void *w_uk,
     a.q_slots = p.q_slots;
     a.splits = p.splits;
     a.split_tiles = p.split_tiles;
-    if ((int64_t)(p.padded / kTile + 1) * num_heads > INT32_MAX / 256 ||
+    if ((int64_t)(p.padded / kTile + 4) * num_heads > INT32_MAX / 512 ||
         (int64_t)a.q_slots * num_heads > INT32_MAX / 256 / std::max(4, p.splits))
         return MLA_STATUS_INVALID_VALUE;
     if (workspace_bytes < p.bytes())
@@ -869,7 +881,7 @@ int prefill(bool bf16, const void *q_nope, const void *q_rope, const void *w_uk,
     a.queries = queries;
     a.total_tokens = total_tokens;
     a.padded = p.padded;
-    a.group_blocks = expand_group_blocks(batch, total_tokens, num_heads, current_cu_count());
+    plan_expansion(a, current_cu_count());
     a.page_shift = block_table ? __builtin_ctz((unsigned)page_size) : 0;
     a.num_pages = num_pages;
     a.bt_stride = block_table_stride;
