@@ -51,6 +51,7 @@ struct PrefillArgs {
     int batch, num_heads, queries, total_tokens;
     int padded;  // keys of the workspace: whole tiles
     int q_slots;
+    int narrow;        // 1: narrow_kernel
     int splits;        // of a query tile's keys, at most
     int split_tiles;   // key tiles a split, at least
     int key_groups;    // of 32 keys a wave in expand_kernel, 1 or 2
@@ -371,27 +372,32 @@ struct QueryTile {
     int rows;           // rows of out from q_lo on: the last sequence's go on to the end of it
 };
 
+template <int kUnit>  // queries of a tile
 __device__ __forceinline__ QueryTile query_tile(const PrefillArgs &a, int slot, int lane)
 {
     QueryTile t;
-    const Owner w = owner_of_slot(a.cu_q, a.queries, a.cu_seqlens, a.total_tokens, a.batch, kQueries, slot, lane);
+    const Owner w = owner_of_slot(a.cu_q, a.queries, a.cu_seqlens, a.total_tokens, a.batch, kUnit, slot, lane);
     t.q_lo = w.lo;
     t.n_q = w.hi - w.lo;
-    t.q0 = (slot - t.q_lo / kQueries - w.b) * kQueries;
+    t.q0 = (slot - t.q_lo / kUnit - w.b) * kUnit;
     t.rows = w.b == a.batch - 1 ? a.queries - t.q_lo : t.n_q;
     t.n_k = w.other_hi - w.other_lo;
     t.tile0 = w.other_lo / kTile + w.b;
-    t.n_tiles = (min(t.n_k, min(t.q0 + kQueries, t.n_q) + t.n_k - t.n_q) + kTile - 1) / kTile;
-    t.per = max(a.split_tiles, (t.n_tiles + a.splits - 1) / a.splits);
-    t.n_splits = max(1, (t.n_tiles + t.per - 1) / t.per);
+    t.n_tiles = (min(t.n_k, min(t.q0 + kUnit, t.n_q) + t.n_k - t.n_q) + kTile - 1) / kTile;
+    t.per = INT32_MAX / 2;
+    t.n_splits = 1;
+    if (a.splits > 1) {
+        t.per = max(a.split_tiles, (t.n_tiles + a.splits - 1) / a.splits);
+        t.n_splits = max(1, (t.n_tiles + t.per - 1) / t.per);
+    }
     return t;
 }
 
 // A tile behind the last sequence's queries: zeros.
-template <typename E>
+template <typename E, int kUnit>
 __device__ __forceinline__ void zero_rows(const PrefillArgs &a, const QueryTile &t, int h)
 {
-    for (int i = threadIdx.x; i < min(kQueries, t.rows - t.q0) * (kNope / 8); i += 256)
+    for (int i = threadIdx.x; i < min(kUnit, t.rows - t.q0) * (kNope / 8); i += 256)
         *(uint4 *)((E *)a.out + ((size_t)(t.q_lo + t.q0 + i / (kNope / 8)) * a.num_heads + h) * kNope +
                    8 * (i % (kNope / 8))) = uint4{0, 0, 0, 0};
 }
@@ -427,64 +433,198 @@ __device__ __forceinline__ void store_rows(const PrefillArgs &a, const QueryTile
     }
 }
 
+constexpr int kVAt = kTile * kNope * 2, kRopeAt = 2 * kVAt;         // bytes of a stage before V, before the rotary parts
+constexpr int kStageBytes = kRopeAt + kTile * kRopeDim * 2;         // 40 KB
+
+// One wave's work on a tile of 64 keys in LDS, for its 32 queries.
+
+// S^T: the lane's logits. k_at and rope_at: the lane's operand 0 of the keys' own
+// parts and of the rotary ones.
+template <typename E>
+__device__ __forceinline__ void tile_logits(unsigned k_at, unsigned rope_at, const typename Vec<E>::v8 (&q)[12], floatx16 (&s)[2])
+{
+    using E8 = typename Vec<E>::v8;
+    // operand k of both 32-key blocks: 8 steps of the head's own part, 4 of the rotary one
+    auto operand = [&](int g, int k) -> E8 {
+        return k < 8 ? lds_load<E8>((k_at ^ (32 * k)) + 32 * g * (kNope * 2))
+                     : lds_load<E8>((rope_at ^ (32 * (k - 8))) + 32 * g * (kRopeDim * 2));
+    };
+    E8 kv[2][2][2];
+#pragma unroll
+    for (int g = 0; g < 2; ++g)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            kv[0][g][i] = operand(g, i);
+#pragma unroll
+    for (int k = 0; k < 12; k += 2) {
+        if (k + 2 < 12) {
+#pragma unroll
+            for (int g = 0; g < 2; ++g)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    kv[(k / 2 + 1) & 1][g][i] = operand(g, k + 2 + i);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int g = 0; g < 2; ++g)
+                s[g] = mfma32x32x16(kv[(k / 2) & 1][g][i], q[k + i], s[g]);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+
+// The weights p of keys t0 .. t0 + 63 from their logits, and the running maximum
+// m, sum l and output o moved on. The lane's query sees the keys up to `last`, every
+// query of the wave those up to `wave_first`.
+template <typename E>
+__device__ __forceinline__ void tile_weights(const PrefillArgs &a, int t0, int wave_first, int last, int hl, const ulong4x *flags,
+                                             floatx16 (&s)[2], float (&p)[32], float &m, float &l, floatx16 (&o)[4])
+{
+    if (t0 + kTile - 1 > wave_first) {
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                s[g][r] = t0 + 32 * g + key_of_reg(r, hl) <= last ? s[g][r] : -INFINITY;
+    }
+    float most = s[0][0];
+#pragma unroll
+    for (int r = 1; r < 32; ++r)
+        most = fmaxf(most, s[r >> 4][r & 15]);
+    most = reduce_halves(most, [](float x, float y) { return fmaxf(x, y); }) * a.scale_log2;
+    if (__builtin_amdgcn_ballot_w64(most > m + kLazyRescale) != 0) {
+        const float next = most > m + kLazyRescale ? most : m;  // each row by itself
+        const float f = next == -INFINITY ? 1.0f : fast_exp2(m - next);
+        m = next;
+        l *= f;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+            o[c] *= f;
+    }
+    const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+    for (int r = 0; r < 32; ++r) {
+        p[r] = fast_exp2(s[r >> 4][r & 15] * a.scale_log2 - ref);
+        l += p[r];
+    }
+    const ulong4x f4 = scalar_load(flags);
+    const unsigned long long bad = f4[0] | f4[1] | f4[2] | f4[3];
+    if (bad != 0) {  // a query that sees a key whose V is not finite gives NaN
+#pragma unroll
+        for (int r = 0; r < 32; ++r) {
+            const int t = 32 * (r >> 4) + key_of_reg(r & 15, hl);
+            if (((bad >> t) & 1) != 0 && t0 + t <= last)
+                l = NAN;
+        }
+    }
+}
+
+// O^T += V^T P^T. v_at0, v_at1: the lane's two transpose reads of the first operand.
+template <typename E>
+__device__ __forceinline__ void tile_values(unsigned v_at0, unsigned v_at1, const float (&p)[32], floatx16 (&o)[4])
+{
+    using E8 = typename Vec<E>::v8;
+    using E4 = typename Vec<E>::v4;
+    auto operand = [&](int ks, int c) -> E8 {  // columns 32 c .. of V^T, keys 16 ks .. +15 in P's order
+        E4 part[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            part[i] = lds_load_tr16<E>(((i ? v_at1 : v_at0) ^ (64 * c)) + 16 * ks * (kNope * 2));
+        return E8{part[0][0], part[0][1], part[0][2], part[0][3], part[1][0], part[1][1], part[1][2], part[1][3]};
+    };
+    E8 v[2][4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+        v[0][c] = operand(0, c);
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+        if (ks + 1 < 4) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                v[(ks + 1) & 1][c] = operand(ks + 1, c);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        const E8 pb = p_operand<E>(p + 8 * ks);
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+            o[c] = mfma32x32x16(v[ks & 1][c], pb, o[c]);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+
+// The lane's LDS addresses in a stage (K at 0, V, the rotary parts), and its part
+// of the load units' offsets in the workspace: 4 keys of 256 bytes in LDS are
+// 4 times 64 bytes there, the swizzle's low bits changing from one unit to the next.
+struct TileLanes {
+    unsigned k, rope, v[2];
+    int kv_off, rope_off;
+    __device__ __forceinline__ explicit TileLanes(int lane)
+    {
+        const int r32 = lane & 31, hl = lane >> 5, j = lane & 15;
+        k = r32 * (kNope * 2) + 16 * (hl ^ key_swizzle(r32));
+        rope = kRopeAt + r32 * (kRopeDim * 2) + 16 * (hl ^ rope_swizzle(r32));
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int r = 8 * i + 4 * hl + (j >> 2);
+            v[i] = kVAt + r * (kNope * 2) + 16 * ((2 * ((lane >> 4) & 1) + ((j & 3) >> 1)) ^ key_swizzle(r)) + 8 * (j & 1);
+        }
+        const int chunk = j ^ key_swizzle(lane >> 4);
+        kv_off = (chunk >> 2) * (kTile * kWeightRows * 2) + (lane >> 4) * (kWeightRows * 2) + 16 * (chunk & 3);
+        rope_off = (lane >> 3) * (kRopeDim * 2) + 16 * ((lane & 7) ^ rope_swizzle(lane >> 3));
+    }
+};
+
 template <typename E>
 __global__ __launch_bounds__(256, 2) void attend_kernel(PrefillArgs a)
 {
     using E8 = typename Vec<E>::v8;
-    using E4 = typename Vec<E>::v4;
-    constexpr int kKElems = kTile * kNope, kRElems = kTile * kRopeDim;
-    constexpr int kStage = 2 * kKElems + kRElems;  // K, V, rotary parts: 40 KB
-    __shared__ __attribute__((aligned(1024))) E s_buf[2][kStage];
+    __shared__ __attribute__((aligned(1024))) char s_buf[2][kStageBytes];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r32 = lane & 31, hl = lane >> 5;
     // workgroup -> (head, query tile, split): all tiles of a head on one XCD, whose L2
     // then holds its K and V, the last (longest) first
-    const int li = blockIdx.x >> 3;
-    const int h = li / (a.q_slots * a.splits) * 8 + (blockIdx.x & 7);
-    const int slot = a.q_slots - 1 - li / a.splits % a.q_slots, split = li % a.splits;
+    const int li = blockIdx.x >> 3, tile = a.splits > 1 ? li / a.splits : li, split = li - tile * a.splits;
+    const int h = tile / a.q_slots * 8 + (blockIdx.x & 7);
+    const int slot = a.q_slots - 1 - tile % a.q_slots;
     if (h >= a.num_heads)
         return;
-    const QueryTile t = query_tile(a, slot, lane);
+    const QueryTile t = query_tile<kQueries>(a, slot, lane);
     if (split >= t.n_splits)
         return;
     if (t.q0 >= t.n_q) {
         if (split == 0)
-            zero_rows<E>(a, t, h);
+            zero_rows<E, kQueries>(a, t, h);
         return;
     }
     const int q0 = t.q0, n_q = t.n_q, tile0 = t.tile0;
     const int shift = t.n_k - n_q;  // query i sees the keys 0 .. i + shift
-    const int j0 = split * t.per, j1 = min(j0 + t.per, t.n_tiles);  // the split's key tiles
+    const int j0 = split == 0 ? 0 : split * t.per, j1 = min(j0 + t.per, t.n_tiles);  // the split's key tiles
 
     const int row = q0 + 32 * wave + r32;
     const int last = min(row, n_q - 1) + shift;  // the lane's last key
     const unsigned lds = lds_address(s_buf);
-    const unsigned k_lane = r32 * (kNope * 2) + 16 * (hl ^ key_swizzle(r32));
-    const unsigned rope_row = r32 * (kRopeDim * 2) + 16 * (hl ^ rope_swizzle(r32));
+    const TileLanes at_lane(lane);
     const E *ks = wave_uniform((const E *)a.k + ((size_t)h * a.padded + (size_t)tile0 * kTile) * kNope + 16 * wave * kWeightRows);
     const E *vs = wave_uniform((const E *)a.v + ((size_t)h * a.padded + (size_t)tile0 * kTile) * kNope + 16 * wave * kWeightRows);
     const E *rs = wave_uniform((const E *)a.rope + ((size_t)tile0 * kTile + 16 * wave) * kRopeDim);
     const ulong4x *flags = (const ulong4x *)a.flags + (size_t)h * (a.padded / kTile) + tile0;
-    // A wave's 10 load units: 4 of K and 4 of V (4 keys of 256 bytes in LDS, 4 times
-    // 64 bytes in the workspace, the swizzle's low bits changing from one unit to
-    // the next), 2 of the rotary parts (8 rows of 128 bytes).
+    // A wave's 10 load units: 4 of K, 4 of V and 2 of the rotary parts (8 rows of 128 bytes).
     constexpr int kUnits = 10;
-    const int kv_chunk = (lane & 15) ^ key_swizzle(lane >> 4);
-    const int kv_off = (kv_chunk >> 2) * (kTile * kWeightRows * 2) + (lane >> 4) * (kWeightRows * 2) + 16 * (kv_chunk & 3);
-    const int rope_off = (lane >> 3) * (kRopeDim * 2) + 16 * ((lane & 7) ^ rope_swizzle(lane >> 3));
     auto load_tile = [&](int j) {
-        const unsigned at = lds + ((j - j0) & 1) * (kStage * 2);
-        const E *k = ks + (size_t)j * kKElems, *v = vs + (size_t)j * kKElems, *r = rs + (size_t)j * kRElems;
+        const unsigned at = lds + ((j - j0) & 1) * kStageBytes;
+        const E *k = ks + (size_t)j * (kTile * kNope), *v = vs + (size_t)j * (kTile * kNope);
+        const E *r = rs + (size_t)j * (kTile * kRopeDim);
         for_constants(
             [&](auto unit) {
                 constexpr int u = decltype(unit)::value;
-                stream_to_lds16<4 * u * kWeightRows * 2, 1024 * u, 0>(k, kv_off ^ (16 * u), at + 4096 * wave);
-                stream_to_lds16<4 * u * kWeightRows * 2, 2 * kKElems + 1024 * u, 0>(v, kv_off ^ (16 * u), at + 4096 * wave);
+                stream_to_lds16<4 * u * kWeightRows * 2, 1024 * u, 0>(k, at_lane.kv_off ^ (16 * u), at + 4096 * wave);
+                stream_to_lds16<4 * u * kWeightRows * 2, kVAt + 1024 * u, 0>(v, at_lane.kv_off ^ (16 * u), at + 4096 * wave);
             },
             std::make_integer_sequence<int, 4>{});
-        stream_to_lds16<0, 4 * kKElems, 0>(r, rope_off, at + 2048 * wave);
-        stream_to_lds16<0, 4 * kKElems, 1024>(r, rope_off ^ 64, at + 2048 * wave);
+        stream_to_lds16<0, kRopeAt, 0>(r, at_lane.rope_off, at + 2048 * wave);
+        stream_to_lds16<0, kRopeAt, 1024>(r, at_lane.rope_off ^ 64, at + 2048 * wave);
     };
     // The queries, the B operand of S^T: their own part comes by whole rows
     // through the second stage, 8 KB a wave, while the first key tile is on its
@@ -495,7 +635,7 @@ __global__ __launch_bounds__(256, 2) void attend_kernel(PrefillArgs a)
         const size_t q_at = (size_t)(t.q_lo + q0) * a.num_heads + h;
         const E *qn = wave_uniform((const E *)a.q_nope + q_at * kNope);
         const E *qr = (const E *)a.q_rope + (q_at + (size_t)min(32 * wave + r32, lim) * a.num_heads) * kRopeDim + 8 * hl;
-        const unsigned own = lds + kStage * 2 + wave * 8192;
+        const unsigned own = lds + kStageBytes + wave * 8192;
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
             const int r = 4 * u + (lane >> 4);
@@ -514,17 +654,8 @@ __global__ __launch_bounds__(256, 2) void attend_kernel(PrefillArgs a)
         asm volatile("" ::: "memory");
 #pragma unroll
         for (int k = 0; k < 8; ++k)
-            q[k] = lds_load<E8>((own + k_lane) ^ (32 * k));
+            q[k] = lds_load<E8>((own + at_lane.k) ^ (32 * k));
     }
-    const unsigned rope_lane = 4 * kKElems + rope_row;
-    unsigned v_lane[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int j = lane & 15, r = 8 * i + 4 * hl + (j >> 2);
-        v_lane[i] = 2 * kKElems + r * (kNope * 2) +
-                    16 * ((2 * ((lane >> 4) & 1) + ((j & 3) >> 1)) ^ key_swizzle(r)) + 8 * (j & 1);
-    }
-
     floatx16 o[4] = {};
     float m = -INFINITY, l = 0.0f;
     // the last key of the wave's queries; a wave without queries only loads
@@ -537,103 +668,12 @@ __global__ __launch_bounds__(256, 2) void attend_kernel(PrefillArgs a)
             load_tile(j + 1);
         if (j * kTile > wave_last)
             continue;
-        const unsigned at = lds + ((j - j0) & 1) * (kStage * 2);
+        const unsigned at = lds + ((j - j0) & 1) * kStageBytes;
         floatx16 s[2] = {};
-        {
-            // operand k of both 32-key blocks: 8 steps of the head's own part, 4 of the rotary one
-            auto operand = [&](int g, int k) -> E8 {
-                return k < 8 ? lds_load<E8>(((at + k_lane) ^ (32 * k)) + 32 * g * (kNope * 2))
-                             : lds_load<E8>(((at + rope_lane) ^ (32 * (k - 8))) + 32 * g * (kRopeDim * 2));
-            };
-            E8 kv[2][2][2];
-#pragma unroll
-            for (int g = 0; g < 2; ++g)
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    kv[0][g][i] = operand(g, i);
-#pragma unroll
-            for (int k = 0; k < 12; k += 2) {
-                if (k + 2 < 12) {
-#pragma unroll
-                    for (int g = 0; g < 2; ++g)
-#pragma unroll
-                        for (int i = 0; i < 2; ++i)
-                            kv[(k / 2 + 1) & 1][g][i] = operand(g, k + 2 + i);
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int g = 0; g < 2; ++g)
-                        s[g] = mfma32x32x16(kv[(k / 2) & 1][g][i], q[k + i], s[g]);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-        }
-        if (j * kTile + kTile - 1 > wave_first) {
-#pragma unroll
-            for (int g = 0; g < 2; ++g)
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    s[g][r] = j * kTile + 32 * g + key_of_reg(r, hl) <= last ? s[g][r] : -INFINITY;
-        }
-        float most = s[0][0];
-#pragma unroll
-        for (int r = 1; r < 32; ++r)
-            most = fmaxf(most, s[r >> 4][r & 15]);
-        most = reduce_halves(most, [](float x, float y) { return fmaxf(x, y); }) * a.scale_log2;
-        if (__builtin_amdgcn_ballot_w64(most > m + kLazyRescale) != 0) {
-            const float next = most > m + kLazyRescale ? most : m;  // each row by itself
-            const float f = next == -INFINITY ? 1.0f : fast_exp2(m - next);
-            m = next;
-            l *= f;
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-                o[c] *= f;
-        }
-        const float ref = m == -INFINITY ? 0.0f : m;
         float p[32];
-#pragma unroll
-        for (int r = 0; r < 32; ++r) {
-            p[r] = fast_exp2(s[r >> 4][r & 15] * a.scale_log2 - ref);
-            l += p[r];
-        }
-        const ulong4x f4 = scalar_load(flags + j);
-        const unsigned long long bad = f4[0] | f4[1] | f4[2] | f4[3];
-        if (bad != 0) {  // a query that sees a key whose V is not finite gives NaN
-#pragma unroll
-            for (int r = 0; r < 32; ++r) {
-                const int t = 32 * (r >> 4) + key_of_reg(r & 15, hl);
-                if (((bad >> t) & 1) != 0 && j * kTile + t <= last)
-                    l = NAN;
-            }
-        }
-        {
-            auto operand = [&](int ks, int c) -> E8 {  // columns 32 c .. of V^T, keys 16 ks .. +15 in P's order
-                E4 part[2];
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    part[i] = lds_load_tr16<E>(((at + v_lane[i]) ^ (64 * c)) + 16 * ks * (kNope * 2));
-                return E8{part[0][0], part[0][1], part[0][2], part[0][3], part[1][0], part[1][1], part[1][2], part[1][3]};
-            };
-            E8 v[2][4];
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-                v[0][c] = operand(0, c);
-#pragma unroll
-            for (int ks = 0; ks < 4; ++ks) {
-                if (ks + 1 < 4) {
-#pragma unroll
-                    for (int c = 0; c < 4; ++c)
-                        v[(ks + 1) & 1][c] = operand(ks + 1, c);
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-                const E8 pb = p_operand<E>(p + 8 * ks);
-#pragma unroll
-                for (int c = 0; c < 4; ++c)
-                    o[c] = mfma32x32x16(v[ks & 1][c], pb, o[c]);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-        }
+        tile_logits<E>(at + at_lane.k, at + at_lane.rope, q, s);
+        tile_weights<E>(a, j * kTile, wave_first, last, hl, flags + j, s, p, m, l, o);
+        tile_values<E>(at + at_lane.v[0], at + at_lane.v[1], p, o);
     }
     l = reduce_halves(l, [](float x, float y) { return x + y; });
     if (t.n_splits > 1) {
@@ -655,6 +695,172 @@ __global__ __launch_bounds__(256, 2) void attend_kernel(PrefillArgs a)
     store_rows<E>(a, t, h, q0 + 32 * wave, lane, lds + wave * 8192, o, l);
 }
 
+// The same for calls so small that 128 queries a workgroup leave most of the CUs idle:
+// 32 queries a workgroup, and its waves take the key tiles in turn, each a stage of its own
+// and its own running maximum and sum, which meet at the end. A wave's next K is on
+// its way while the weights and O take a tile, its next V while the logits do.
+constexpr int kNarrow = 32;
+
+template <typename E>
+__global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_per_eu(1, 1))) void
+narrow_kernel(PrefillArgs a)
+{
+    using E8 = typename Vec<E>::v8;
+    using E4 = typename Vec<E>::v4;
+    __shared__ __attribute__((aligned(1024))) char s_buf[4][kStageBytes];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r32 = lane & 31, hl = lane >> 5;
+    const int li = blockIdx.x >> 3;
+    const int h = li / a.q_slots * 8 + (blockIdx.x & 7);
+    const int slot = a.q_slots - 1 - li % a.q_slots;
+    if (h >= a.num_heads)
+        return;
+    const QueryTile t = query_tile<kNarrow>(a, slot, lane);
+    if (t.q0 >= t.n_q) {
+        zero_rows<E, kNarrow>(a, t, h);
+        return;
+    }
+    const int shift = t.n_k - t.n_q;  // query i sees the keys 0 .. i + shift
+    const int last = min(t.q0 + r32, t.n_q - 1) + shift, first = t.q0 + shift;
+    const unsigned at = lds_address(s_buf) + wave * kStageBytes;
+    const TileLanes at_lane(lane);
+    const E *ks = wave_uniform((const E *)a.k + ((size_t)h * a.padded + (size_t)t.tile0 * kTile) * kNope);
+    const E *vs = wave_uniform((const E *)a.v + ((size_t)h * a.padded + (size_t)t.tile0 * kTile) * kNope);
+    const E *rs = wave_uniform((const E *)a.rope + (size_t)t.tile0 * kTile * kRopeDim);
+    const ulong4x *flags = (const ulong4x *)a.flags + (size_t)h * (a.padded / kTile) + t.tile0;
+    // a tile's load units: 16 of K and 8 of the rotary parts, then 16 of V
+    constexpr int kKeyUnits = 24, kValueUnits = 16;
+    auto load_keys = [&](int j) {
+        const E *k = ks + (size_t)j * (kTile * kNope), *r = rs + (size_t)j * (kTile * kRopeDim);
+        for_constants(
+            [&](auto unit) {
+                constexpr int u = decltype(unit)::value;
+                stream_to_lds16<4 * u * kWeightRows * 2, 1024 * u, 0>(k, at_lane.kv_off ^ (16 * (u & 3)), at);
+            },
+            std::make_integer_sequence<int, 16>{});
+        for_constants(
+            [&](auto unit) {
+                constexpr int u = decltype(unit)::value;
+                stream_to_lds16<1024 * u, kRopeAt + 1024 * u, 0>(r, at_lane.rope_off ^ (64 * (u & 1)), at);
+            },
+            std::make_integer_sequence<int, 8>{});
+    };
+    auto load_values = [&](int j) {
+        const E *v = vs + (size_t)j * (kTile * kNope);
+        for_constants(
+            [&](auto unit) {
+                constexpr int u = decltype(unit)::value;
+                stream_to_lds16<4 * u * kWeightRows * 2, kVAt + 1024 * u, 0>(v, at_lane.kv_off ^ (16 * (u & 3)), at);
+            },
+            std::make_integer_sequence<int, 16>{});
+    };
+    // the wave's reads of LDS have ended: what they read may be loaded over
+    auto reads_done = [] { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); };
+
+    floatx16 o[4] = {};
+    float m = -INFINITY, l = 0.0f;
+    if (wave < t.n_tiles) {
+        // the queries through V's place, whole rows: 8 KB of their own part, 4 KB of the rotary one
+        E8 q[12];
+        const int lim = t.n_q - 1 - t.q0;
+        const size_t q_at = (size_t)(t.q_lo + t.q0) * a.num_heads + h;
+        const E *qn = wave_uniform((const E *)a.q_nope + q_at * kNope);
+        const E *qr = wave_uniform((const E *)a.q_rope + q_at * kRopeDim);
+        constexpr int kQRopeAt = 32 * kNope * 2;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const int r = 4 * u + (lane >> 4);
+            global_to_lds16_at(qn, min(r, lim) * (a.num_heads * (kNope * 2)) + 16 * ((lane & 15) ^ key_swizzle(r)),
+                               at + kVAt + 1024 * u);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int r = 8 * u + (lane >> 3);
+            global_to_lds16_at(qr, min(r, lim) * (a.num_heads * (kRopeDim * 2)) + 16 * ((lane & 7) ^ rope_swizzle(r)),
+                               at + kVAt + kQRopeAt + 1024 * u);
+        }
+        load_keys(wave);
+        MLA_WAIT_VMCNT(kKeyUnits);
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int k = 0; k < 12; ++k)
+            q[k] = k < 8 ? lds_load<E8>((at + kVAt + at_lane.k) ^ (32 * k))
+                         : lds_load<E8>((at + kVAt + kQRopeAt + at_lane.rope - kRopeAt) ^ (32 * (k - 8)));
+#pragma unroll
+        for (int k = 0; k < 12; ++k)
+            in_registers(q[k]);
+        reads_done();
+        load_values(wave);
+        for (int j = wave; j < t.n_tiles; j += 4) {
+            const bool more = j + 4 < t.n_tiles;
+            MLA_WAIT_VMCNT(kValueUnits);  // K and the rotary parts are there, V may not be
+            asm volatile("" ::: "memory");
+            floatx16 s[2] = {};
+            float p[32];
+            tile_logits<E>(at + at_lane.k, at + at_lane.rope, q, s);
+            reads_done();
+            if (more)
+                load_keys(j + 4);
+            tile_weights<E>(a, j * kTile, first, last, hl, flags + j, s, p, m, l, o);
+            if (more)
+                MLA_WAIT_VMCNT(kKeyUnits);
+            else
+                MLA_WAIT_VMCNT(0);
+            asm volatile("" ::: "memory");
+            tile_values<E>(at + at_lane.v[0], at + at_lane.v[1], p, o);
+            reads_done();
+            if (more)
+                load_values(j + 4);
+        }
+    }
+    l = reduce_halves(l, [](float x, float y) { return x + y; });
+    // the waves' parts, each in its own stage: O as it lies in the registers (16 KB), m and l
+    constexpr int kMAt = 32 * kNope * 4;
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            lds_store(at + (4 * c + k) * 1024 + 16 * lane,
+                      floatx4{o[c][4 * k], o[c][4 * k + 1], o[c][4 * k + 2], o[c][4 * k + 3]});
+    if (hl == 0) {
+        lds_store(at + kMAt + 4 * r32, m);
+        lds_store(at + kMAt + 128 + 4 * r32, l);
+    }
+    lds_barrier();
+    // wave c: columns 32 c .. of the 32 rows
+    const unsigned all = at - wave * kStageBytes;
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < 4; ++w)
+        top = fmaxf(top, lds_load<float>(all + w * kStageBytes + kMAt + 4 * r32));
+    const float ref = top == -INFINITY ? 0.0f : top;
+    floatx4 sum[4] = {};
+    l = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const unsigned from = all + w * kStageBytes;
+        const float f = fast_exp2(lds_load<float>(from + kMAt + 4 * r32) - ref);
+        l += f * lds_load<float>(from + kMAt + 128 + 4 * r32);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            sum[k] += f * lds_load<floatx4>(from + (4 * wave + k) * 1024 + 16 * lane);
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const int row = t.q0 + r32;
+    if (row >= t.rows)
+        return;
+    E *out = (E *)a.out + ((size_t)(t.q_lo + row) * a.num_heads + h) * kNope + 32 * wave + 4 * hl;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        E4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            v[e] = row < t.n_q ? (E)(sum[k][e] * inv) : (E)0.0f;
+        *(E4 *)(out + 8 * k) = v;
+    }
+}
+
 // Merges the splits of the query tiles that have more than one. A workgroup takes 32
 // rows of a head, wave c their columns 32 c .., and a lane the 16 values it would hold in
 // attend_kernel. The splits are added in their order.
@@ -665,7 +871,7 @@ __global__ __launch_bounds__(256) void merge_kernel(PrefillArgs a)
     const int lane = threadIdx.x & 63;
     const int c = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int w = blockIdx.x & 3, h = (blockIdx.x >> 2) % a.num_heads, slot = (blockIdx.x >> 2) / a.num_heads;
-    const QueryTile t = query_tile(a, slot, lane);
+    const QueryTile t = query_tile<kQueries>(a, slot, lane);
     const int first = t.q0 + 32 * w;
     if (t.n_splits == 1 || t.q0 >= t.n_q || first >= t.rows)
         return;
@@ -730,6 +936,7 @@ size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 struct PrefillPlan {
     int padded;
     int q_slots, splits, split_tiles;
+    bool narrow;  // narrow_kernel, and its query tiles
     size_t kv_bytes, rope_bytes, flag_bytes, o_bytes, ml_bytes;
     size_t bytes() const { return 2 * kv_bytes + rope_bytes + flag_bytes + o_bytes + 2 * ml_bytes; }
 };
@@ -741,9 +948,14 @@ struct PrefillPlan {
 // longer than the splits then reach. Calls in one split and as planned: 1 query behind
 // 8000 tokens at 16 heads 225 us and 71, 500 queries there 274 and 138, 1000 at 32
 // heads 336 and 311, 100 behind 2000 at 16 heads 76 and 38.
-constexpr double kStartUs = 4.0, kTileUs = 1.3, kSharedTileUs = 1.8, kMergeUs = 4.0, kPartialUsPerByte = 0.4e-6;
+//
+// narrow_kernel competes with them: one workgroup a CU at a time, four tiles in each
+// kNarrowTileUs; only the first round is taken to see all the keys. 197 queries at
+// 16 heads 10.2 -> 7.0 us, 500 16.9 -> 9.8, 1000 29.4 -> 20.9; 200 at 128 heads 12.6 stay (23.5).
+constexpr double kNarrowStartUs = 4.7, kNarrowTileUs = 2.2;
+constexpr double kStartUs = 4.8, kTileUs = 1.5, kSharedTileUs = 2.0, kMergeUs = 4.0, kPartialUsPerByte = 0.4e-6;
 
-void plan_splits(PrefillPlan &p, int batch, int num_heads, int queries, int total_tokens, int cu_count)
+void plan_attention(PrefillPlan &p, int batch, int num_heads, int queries, int total_tokens, int cu_count)
 {
     const int64_t mean_q = ((int64_t)queries + batch - 1) / batch, mean_k = ((int64_t)total_tokens + batch - 1) / batch;
     const int64_t wgs = (mean_q + kQueries - 1) / kQueries * batch * num_heads;
@@ -765,14 +977,20 @@ void plan_splits(PrefillPlan &p, int batch, int num_heads, int queries, int tota
             p.split_tiles = n == 1 ? INT32_MAX / 2 : per;
         }
     }
+    const int64_t small = (mean_q + kNarrow - 1) / kNarrow * batch * num_heads;
+    const int64_t rounds = (small + cu_count - 1) / cu_count;
+    const int steps = (tiles + 3) / 4, mean_steps = (int)(std::max<int64_t>(0, mean_k - mean_q / 2) / (4 * kTile) + 1);
+    p.narrow = rounds * kNarrowStartUs + (steps + (rounds - 1) * std::min(steps, mean_steps)) * kNarrowTileUs < best;
+    p.q_slots = queries / (p.narrow ? kNarrow : kQueries) + batch;
+    if (p.narrow)
+        p.splits = 1;
 }
 
 // Sequence b's keys start at tile cu[b] / 64 + b of the workspace.
 PrefillPlan prefill_plan(int batch, int num_heads, int queries, int total_tokens)
 {
     PrefillPlan p;
-    p.q_slots = queries / kQueries + batch;
-    plan_splits(p, batch, num_heads, queries, total_tokens, current_cu_count());
+    plan_attention(p, batch, num_heads, queries, total_tokens, current_cu_count());
     const size_t parts = p.splits > 1 ? (size_t)p.q_slots * num_heads * p.splits : 0;
     p.o_bytes = align256(parts * kQueries * kNope * sizeof(float));
     p.ml_bytes = align256(parts * kQueries * sizeof(float));
@@ -831,7 +1049,8 @@ void launch_prefill(const PrefillArgs &a, hipStream_t s)
         auto k = a.key_groups == 2 ? expand_kernel<E, 2> : expand_kernel<E, 1>;
         hipLaunchKernelGGL(k, dim3((unsigned)quads * ((groups + 7) / 8 * 8)), dim3(256), 0, s, a);
     }
-    hipLaunchKernelGGL(attend_kernel<E>, dim3((unsigned)a.q_slots * a.num_heads * a.splits), dim3(256), 0, s, a);
+    auto k = a.narrow ? narrow_kernel<E> : attend_kernel<E>;
+    hipLaunchKernelGGL(k, dim3((unsigned)a.q_slots * a.num_heads * a.splits), dim3(256), 0, s, a);
     if (a.splits > 1)
         hipLaunchKernelGGL(merge_kernel<E>, dim3((unsigned)a.q_slots * a.num_heads * 4), dim3(256), 0, s, a);
 }
@@ -852,6 +1071,7 @@ int prefill(bool bf16, const void *q_nope, const void *q_rope, const void *w_uk,
     const PrefillPlan p = prefill_plan(batch, num_heads, queries, total_tokens);
     PrefillArgs a;
     a.q_slots = p.q_slots;
+    a.narrow = p.narrow;
     a.splits = p.splits;
     a.split_tiles = p.split_tiles;
     if ((int64_t)(p.padded / kTile + 4) * num_heads > INT32_MAX / 512 ||

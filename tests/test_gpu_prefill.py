@@ -272,12 +272,13 @@ def _partials(batch, heads, queries, total):
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
-@pytest.mark.parametrize("queries,context,page", [
-    ([1], [6000], 64), ([33], [4063], 0), ([7, 1, 0, 140, 3], [5000, 1, 900, 1337, 64], 32), ([200], [3900], 128)])
-def test_few_queries_behind_long_contexts(queries, context, page, dtype):
+@pytest.mark.parametrize("queries,context,page,split", [
+    ([1], [6000], 64, True), ([33], [4063], 0, True), ([200], [3900], 128, True), ([7, 3, 130], [11000, 12, 900], 32, True),
+    ([7, 1, 0, 140, 3], [5000, 1, 900, 1337, 64], 32, False)])
+def test_few_queries_behind_long_contexts(queries, context, page, split, dtype):
     # keys split over workgroups; a short request among long ones, tiles that end inside a split
     total = sum(queries) + sum(context)
-    assert _partials(len(queries), 16, sum(queries), total)
+    assert _partials(len(queries), 16, sum(queries), total) == split
     _run(queries, context, 16, dtype, page, seed=total)
 
 
@@ -305,7 +306,7 @@ def test_split_keys_padded_rows_and_values_that_are_not_finite():
 def test_split_keys_captured_and_replayed():
     gen = torch.Generator()
     gen.manual_seed(18)
-    n = 3500
+    n = 9000
     qn, qr, uk, uv = _inputs(gen, 60, 16, torch.float16)
     cache = torch.randn(n, 576, generator=gen).half().cuda()
     cu_q, cu = _cu([10, 50]), _cu([500, n - 500])
@@ -325,3 +326,29 @@ def test_split_keys_captured_and_replayed():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.isfinite(want).all() and torch.equal(out, want), r
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("queries,context", [
+    ([1], [0]), ([1], [64]), ([31], [33]), ([32], [31]), ([33], [224]), ([65], [192]), ([197], [0]), ([5, 0, 40], [700, 9, 3])])
+def test_small_calls(queries, context, dtype):
+    # 32 queries a workgroup whose waves take the key tiles in turn: from none of them to three each
+    _run(queries, context, 16, dtype, 32, seed=sum(queries) + sum(context))
+
+
+def test_many_requests_with_rows_behind_the_last():
+    # enough query tiles to fill the chip by themselves
+    gen = torch.Generator()
+    gen.manual_seed(19)
+    lengths = [70] * 40
+    n, rows = sum(lengths), sum(lengths) + 150
+    qn, qr, uk, uv = _inputs(gen, rows, 16, torch.float16)
+    cache, cu = torch.randn(n, 576, generator=gen).half().cuda(), _cu(lengths)
+    out = torch.full((rows, 16, 128), float("nan"), dtype=torch.float16, device="cuda")
+    got = capi.prefill(qn, qr, uk, uv, cache, cu, cu, n, out=out)
+    assert torch.isfinite(got).all() and not got[n:].any()
+    _check(got[:n], qn, qr, uk, uv, lambda b: cache[int(cu[b]):int(cu[b + 1])].double().cpu(), lengths, lengths,
+           torch.float16, "many, padded")
+    cache[n - 30, 9] = float("nan")  # of the last request, seen by its last 30 queries
+    bad = capi.prefill(qn, qr, uk, uv, cache, cu, cu, n)
+    assert torch.equal(bad[:n - 30], got[:n - 30]) and torch.isnan(bad[n - 30:n]).all() and not bad[n:].any()
