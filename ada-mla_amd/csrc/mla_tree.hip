@@ -57,7 +57,7 @@ struct TreeArgs {
     int chunk;      // tokens per split
     int row_tiles;  // of 128 rows, per request
     int n_slots;    // total_tokens / chunk + batch
-    int by_xcd;     // 1: the workgroups of a slot share an XCD
+    int by_xcd;     // 1: the workgroups of a split share an XCD
     int page_shift, num_pages, bt_stride;
     float scale_log2;
 };
@@ -93,31 +93,43 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
     const int r32 = lane & 31, hl = lane >> 5;
     const unsigned ring = lds_address(s_ring);
 
-    // workgroup -> (slot, row tile, column part). With by_xcd the workgroups of
-    // a slot, which read the same tokens, get ids equal mod 8, i.e. one XCD and its L2.
-    const int per_slot = a.row_tiles * kParts;
+    // workgroup -> (split of a request, row tile, column part), the splits counted through
+    // the batch. With by_xcd the workgroups of a split, which read the same tokens, get ids
+    // equal mod 8, i.e. one XCD and its L2, and the splits go to the XCDs in turn. (Taken by
+    // slot, of which requests leave some empty, 15 requests of 32 drafts x 128 heads fell on
+    // half of the XCDs: 625 us, 24 of 16 x 64 632.)
+    const int per_split = a.row_tiles * kParts;
     const int id = a.by_xcd ? blockIdx.x >> 3 : blockIdx.x;
-    const int slot = a.by_xcd ? id / per_slot * 8 + (blockIdx.x & 7) : id / per_slot;
-    const int within = id % per_slot;
+    const int nth = a.by_xcd ? id / per_split * 8 + (blockIdx.x & 7) : id / per_split;
+    const int within = id % per_split;
     const int rt = within / kParts, part = within % kParts;
-    if (slot >= a.n_slots)
-        return;
-    int b = 0;  // the last request whose first slot is at or before `slot`
+    int b = -1, split = 0, before = 0;  // the nth split's request, its place there, the splits of the requests before
     for (int base = 0; base < a.batch; base += 64) {
-        const int i = base + lane;
-        const bool in = i < a.batch && min(max(a.cu_seqlens[i], 0), a.total_tokens) / a.chunk + i <= slot;
-        const unsigned long long m = __builtin_amdgcn_ballot_w64(in);
-        if (m != 0)
-            b = base + 63 - __builtin_clzll(m);
-        if (m != ~0ull)
+        const int i = min(base + lane, a.batch - 1);
+        const int lo = min(max(a.cu_seqlens[i], 0), a.total_tokens);
+        const int len = min(max(a.cu_seqlens[i + 1], lo), a.total_tokens) - lo;
+        const int n = base + lane < a.batch ? max(1, (len + a.chunk - 1) / a.chunk) : 0;
+        int sum = n;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const int u = __shfl_up(sum, d);
+            sum += lane >= d ? u : 0;
+        }
+        const unsigned long long m = __builtin_amdgcn_ballot_w64(before + sum > nth);
+        if (m != 0) {
+            const int k = __builtin_ctzll(m);
+            b = base + k;
+            split = nth - before - (__builtin_amdgcn_readlane(sum, k) - __builtin_amdgcn_readlane(n, k));
             break;
+        }
+        before += __builtin_amdgcn_readlane(sum, 63);
     }
+    if (b < 0)
+        return;
     b = __builtin_amdgcn_readfirstlane(b);
     Request rq;
     rq.read(a, b);
-    const int split = slot - rq.slot0;
-    if (split < 0 || split >= rq.n_splits)
-        return;
+    const int slot = rq.slot0 + split;
     const int rows = a.drafts * a.num_heads;      // of the request's output
     const int live = rq.drafts * a.num_heads;     // of its drafted tokens
     const int row = rt * kRows + 32 * wave + r32; // this lane's
@@ -676,8 +688,8 @@ bool tree_sizes_ok(int batch, int drafts, int num_heads, int total_tokens)
            num_heads <= 4096 && total_tokens >= 0 && total_tokens <= INT32_MAX - 4096;
 }
 
-// Slots from which on a slot's workgroups share an XCD: 16 requests of 16 drafts
-// x 128 heads 222 -> 164 us, 23 of 30 x 64 120 -> 94. With fewer slots the
+// Slots from which on a split's workgroups share an XCD: 16 requests of 16 drafts
+// x 128 heads 222 -> 164 us, 23 of 30 x 64 120 -> 94. With fewer splits the
 // XCDs would take one or two each, or none: 32 drafts x 128 heads over 50021 tokens
 // in 8 splits 441 us against 414, in one split 8.7 ms against 2.1.
 constexpr int kMinSlotsByXcd = 16;
