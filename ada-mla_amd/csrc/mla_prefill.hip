@@ -8,18 +8,19 @@
 // instead of 576 + 512, for 2 x 128 x 512 once per key and head: with more
 // than some 170 queries a key (a prompt of 340 tokens) the expanded form needs fewer.
 //
-// Two launches: expand_kernel writes K, V and the rotary parts to the
+// Two launches mostly: expand_kernel writes K, V and the rotary parts to the
 // workspace, tile by tile of 64 keys (each sequence starts a tile of its own);
 // attend_kernel is one pass over them with a running maximum and sum. Where few
-// queries see long contexts it splits the keys, and merge_kernel joins the parts.
+// queries see long contexts it splits the keys, and merge_kernel joins the parts;
+// small calls take narrow_kernel instead.
 // K and V are held in the inputs' 16-bit type, as a cache of expanded heads
 // would hold them: a rounding of half a step on each, the sums in fp32. (In fp32
 // they would double the workspace and take three products of split operands
 // for each one.)
 //
-// Measured: 8192 queries at 64 heads 151 us + 1286 us (137 and 1375 GF: 0.9 and
-// 1.07 PFLOP/s, where a large matrix product reaches 1.3); 6 prompts of up to 1500
-// tokens at 128 heads 182 + 291 us; 197 queries at 16 heads 12 + 10 us.
+// Measured: 8192 queries at 64 heads 155 us + 1317 us (137 and 1375 GF: 0.9 and
+// 1.04 PFLOP/s, where a large matrix product reaches 1.3); 6 prompts of up to 1500
+// tokens at 128 heads 190 + 303 us; 197 queries at 16 heads 8 + 7 us.
 #include <algorithm>
 #include <cmath>
 #include <cstdint>

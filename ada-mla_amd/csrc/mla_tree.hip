@@ -14,11 +14,11 @@
 // whole (Q* 144 registers, O* 256 accumulators, P in registers, see
 // mla_flash.hpp), so the waves meet only to hand over cache blocks.
 //
-// Measured: 32 drafts x 128 heads over 50021 tokens 390 us + 14 of merging (446
-// GF: 1.15 PFLOP/s; a large matrix product reaches 1.3), bound by the LDS reads of
+// Measured: 32 drafts x 128 heads over 50021 tokens 399 us + 15 of merging (446
+// GF: 1.12 PFLOP/s; a large matrix product reaches 1.3), bound by the LDS reads of
 // the first product (16 bytes a lane each: 40 cycles a product instead of 32) and
-// a clock of some 1.6 GHz; 48 requests of 5 x 16 rows over 12000 tokens 92 + 10 us,
-// the cache at 4.1 TB/s; 7 x 16 rows over 1003 tokens 10 + 4 us, round trips.
+// a clock of some 1.6 GHz; 48 requests of 5 x 16 rows over 12000 tokens 84 + 10 us,
+// the cache at 4.5 TB/s; 7 x 16 rows over 1003 tokens 10 + 4 us, round trips.
 #include <algorithm>
 #include <cmath>
 #include <cstdint>

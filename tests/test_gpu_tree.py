@@ -282,3 +282,14 @@ def test_one_long_request_among_empty_ones():
 
 def test_most_drafts_and_heads():
     _run(256, 64, [100], [64], 32, torch.bfloat16, seed=19)
+
+
+def test_splits_counted_through_many_requests():
+    # more requests than lanes, several splits each, empty requests between
+    rng = random.Random(23)
+    lengths = [rng.choice([0, 1, 32, 200, 333, 700]) for _ in range(150)]
+    drafts = [min(2, n) for n in lengths]
+    _run(16, 2, lengths, drafts, 32, torch.float16, 23, splits=3)
+    # equal lengths, whose splits leave every request's last slot empty
+    _run(16, 3, [160] * 40, [3] * 40, 32, torch.bfloat16, 24, splits=1)
+    _run(16, 3, [448] * 24, [3] * 24, 64, torch.float16, 25, splits=7)
