@@ -1041,14 +1041,19 @@ bool prefill_sizes_ok(int batch, int num_heads, int queries, int total_tokens)
            (int64_t)total_tokens + (int64_t)kTile * batch <= INT32_MAX - 4096;
 }
 
+int64_t expand_workgroups(const PrefillArgs &a)
+{
+    const int64_t quads = ((int64_t)a.padded / kTile * (2 / a.key_groups) + kExpandWaves - 1) / kExpandWaves;
+    const int groups = (2 * kBlocksPerSide * a.num_heads + a.group_blocks - 1) / a.group_blocks;
+    return quads * ((groups + 7) / 8 * 8);
+}
+
 template <typename E>
 void launch_prefill(const PrefillArgs &a, hipStream_t s)
 {
     if (a.total_tokens > 0) {
-        const int quads = (a.padded / kTile * (2 / a.key_groups) + kExpandWaves - 1) / kExpandWaves;
-        const int groups = (2 * kBlocksPerSide * a.num_heads + a.group_blocks - 1) / a.group_blocks;
         auto k = a.key_groups == 2 ? expand_kernel<E, 2> : expand_kernel<E, 1>;
-        hipLaunchKernelGGL(k, dim3((unsigned)quads * ((groups + 7) / 8 * 8)), dim3(256), 0, s, a);
+        hipLaunchKernelGGL(k, dim3((unsigned)expand_workgroups(a)), dim3(256), 0, s, a);
     }
     auto k = a.narrow ? narrow_kernel<E> : attend_kernel<E>;
     hipLaunchKernelGGL(k, dim3((unsigned)a.q_slots * a.num_heads * a.splits), dim3(256), 0, s, a);
@@ -1075,8 +1080,8 @@ int prefill(bool bf16, const void *q_nope, const void *q_rope, const void *w_uk,
     a.narrow = p.narrow;
     a.splits = p.splits;
     a.split_tiles = p.split_tiles;
-    if ((int64_t)(p.padded / kTile + 4) * num_heads > INT32_MAX / 512 ||
-        (int64_t)a.q_slots * num_heads > INT32_MAX / 256 / std::max(4, p.splits))
+    if ((int64_t)(p.padded / kTile + 1) * num_heads > INT32_MAX / 256 ||
+        (int64_t)a.q_slots * num_heads * (p.splits > 1 ? std::max(4, p.splits) : 1) > INT32_MAX / 256)
         return MLA_STATUS_INVALID_VALUE;
     if (workspace_bytes < p.bytes())
         return MLA_STATUS_WORKSPACE_TOO_SMALL;
@@ -1103,6 +1108,8 @@ int prefill(bool bf16, const void *q_nope, const void *q_rope, const void *w_uk,
     a.total_tokens = total_tokens;
     a.padded = p.padded;
     plan_expansion(a, current_cu_count());
+    if (expand_workgroups(a) > INT32_MAX / 256)
+        return MLA_STATUS_INVALID_VALUE;
     a.page_shift = block_table ? __builtin_ctz((unsigned)page_size) : 0;
     a.num_pages = num_pages;
     a.bt_stride = block_table_stride;
