@@ -58,40 +58,37 @@ __device__ __forceinline__ void lds_barrier()
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
-// 16 bytes per lane from base + off (bytes) into LDS at lds + 16 * lane
-// (global_load_lds_dwordx4; lds must be wave-uniform). Issued as inline asm
-// so that the compiler does not model it: it would otherwise wait for every
-// such load before each LDS read. The kernel orders these loads itself with
-// MLA_WAIT_VMCNT; the compiler's own vmcnt waits stay correct because
-// vector-memory loads retire in order, so loads it does not count only make
-// its waits more conservative.
-__device__ __forceinline__ void global_to_lds16(const void *base, int off, const void *lds)
+// 16 bytes per lane from base + off (bytes) into LDS at lds_addr + 16 * lane
+// (global_load_lds_dwordx4; lds_addr, an LDS byte address, must be
+// wave-uniform). Issued as inline asm so that the compiler does not model it:
+// it would otherwise wait for every such load before each LDS read. The kernel
+// orders these loads itself with MLA_WAIT_VMCNT; the compiler's own vmcnt waits
+// stay correct because vector-memory loads retire in order, so loads it does
+// not count only make its waits more conservative. Two waits are left to the
+// code, as the compiler does not see a load here:
+//  - m0, which carries the LDS address, may be read one slot after it is
+//    written: the s_nop. m0 is left changed, and nothing outside inline
+//    assembly uses it.
+//  - base may be read 5 slots after a vector instruction (v_readfirstlane)
+//    wrote it.
+// A test of the assembly checks all three in every kernel.
+__device__ __forceinline__ void global_to_lds16_at(const void *base, int off, unsigned lds_addr)
 {
-    const unsigned l = __builtin_amdgcn_readfirstlane(
-        (unsigned)(uintptr_t)(const __attribute__((address_space(3))) void *)lds);
-    unsigned saved_m0;
-    // m0 carries the LDS address; its previous value is restored so the asm
-    // leaves the (compiler-reserved) register unchanged.
-    asm volatile("s_mov_b32 %0, m0\n\t"
-                 "s_mov_b32 m0, %3\n\t"
-                 "global_load_lds_dwordx4 %1, %2\n\t"
-                 "s_mov_b32 m0, %0"
-                 : "=&s"(saved_m0) : "v"(off), "s"(base), "s"(l) : "memory");
+    asm volatile("s_mov_b32 m0, %2\n\t"
+                 "s_nop 0\n\t"
+                 "global_load_lds_dwordx4 %0, %1"
+                 : : "v"(off), "s"(base), "s"(lds_addr) : "memory");
 }
 
-// The same load with the LDS destination given as a wave-uniform LDS byte
-// address, for the steady-state feeding: its lane offsets are formed once and
+// The same load with the LDS destination given as a pointer. The steady-state
+// feeding takes the address instead: its lane offsets are formed once and
 // kept in registers of their own. Offsets recomputed into one shared register
 // before every load made each load's address arithmetic wait until the
 // previous load had read that register.
-__device__ __forceinline__ void global_to_lds16_at(const void *base, int off, unsigned lds_addr)
+__device__ __forceinline__ void global_to_lds16(const void *base, int off, const void *lds)
 {
-    unsigned saved_m0;
-    asm volatile("s_mov_b32 %0, m0\n\t"
-                 "s_mov_b32 m0, %3\n\t"
-                 "global_load_lds_dwordx4 %1, %2\n\t"
-                 "s_mov_b32 m0, %0"
-                 : "=&s"(saved_m0) : "v"(off), "s"(base), "s"(lds_addr) : "memory");
+    global_to_lds16_at(base, off, __builtin_amdgcn_readfirstlane(
+                                      (unsigned)(uintptr_t)(const __attribute__((address_space(3))) void *)lds));
 }
 
 }  // namespace mla
