@@ -38,8 +38,8 @@ __device__ __forceinline__ floatx16 mfma32x32x16(bf16x8 a, bf16x8 b, floatx16 c)
 // accumulation registers with something else: other accumulators, or with _acc
 // the B operand itself. (The compiler puts all of a kernel's products into
 // accumulation registers, and moves what does not fit back and forth.)
-// A chain: first (C = 0), next .., then settle, or 11 instructions more and
-// in_registers, before anything reads the tile: a product's result may be read 11 issue
+// A chain: first (C = 0), next .., then settle, or 12 instructions more and
+// in_registers, before anything reads the tile: a product's result may be read 12 issue
 // slots after an 8-pass product, which the compiler knows of its own
 // products only; nor does it know that an operand which a vector instruction
 // wrote may be read 2 slots later. Operands therefore come from LDS or are never

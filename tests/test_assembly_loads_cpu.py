@@ -5,6 +5,8 @@ every source of the library. Every instruction is a slot, s_nop n is n + 1:
     instruction wrote it;
   * the scalar base may be read 5 slots after a vector instruction (v_readfirstlane) wrote it;
   * m0 is left changed, so nothing outside inline assembly may use it.
+And of the products in inline assembly: a result may be read 12 slots after an
+8-pass product on gfx950, the distance that the compiler keeps for its own.
 All paths to a load count, jumps among them.
 """
 import os
@@ -18,8 +20,9 @@ from conftest import PKG
 
 sys.path.insert(0, PKG)
 import build as pkg_build  # noqa: E402  -- ada-mla_amd/build.py
+import test_assembly_waits_cpu as products  # noqa: E402
 
-M0_SLOTS, BASE_SLOTS = 1, 5
+M0_SLOTS, BASE_SLOTS, RESULT_SLOTS = 1, 5, 12
 
 
 class _Code:
@@ -115,3 +118,41 @@ def test_waits_of_direct_loads(source, tmp_path):
     with open(os.path.join(pkg_build.CSRC, source)) as f:
         assert (loads > 0) == bool(re.search(r"global_to_lds16|stream_to_lds16", f.read()))
     assert not faults, (len(faults), faults[:5])
+
+
+def test_the_compiler_keeps_12_slots_itself(tmp_path):
+    # the distance that the inline products below are held to, from a product the compiler knows
+    src, out = tmp_path / "product.hip", tmp_path / "product.s"
+    src.write_text("""#include <hip/hip_runtime.h>
+typedef float f16x __attribute__((ext_vector_type(16)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+__global__ void k(const h8 *p, float *o, float n)
+{
+    f16x c = {};
+    c = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[threadIdx.x], p[threadIdx.x + 64], c, 0, 0, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    o[0] = c[0] * n;
+}
+""")
+    hipcc = os.path.join(pkg_build.ROCM, "bin", "hipcc")
+    subprocess.run([hipcc, *pkg_build.HIPCC_FLAGS, "--cuda-device-only", "-S", str(src), "-o", str(out)], check=True,
+                   capture_output=True)
+    lines = products._lines(out.read_text())
+    at = next(i for i, l in enumerate(lines) if l.product)
+    result, slots = products._registers(lines[at].args[0]), 0
+    for other in lines[at + 1:]:
+        if products._registers(other.text) & result:
+            break
+        slots += other.slots
+    assert slots == RESULT_SLOTS
+
+
+@pytest.mark.parametrize("source", ["mla_tree.hip", "mla_prefill.hip"])
+def test_results_of_inline_products(source, tmp_path, monkeypatch):
+    out = tmp_path / "kernels.s"
+    hipcc = os.path.join(pkg_build.ROCM, "bin", "hipcc")
+    subprocess.run([hipcc, *pkg_build.HIPCC_FLAGS, "--cuda-device-only", "-S", os.path.join(pkg_build.CSRC, source),
+                    "-o", str(out)], check=True, capture_output=True)
+    monkeypatch.setattr(products, "RESULT_SLOTS", RESULT_SLOTS)
+    found, faults = products._faults(products._lines(out.read_text()))
+    assert found >= 100 and not faults, faults[:5]
