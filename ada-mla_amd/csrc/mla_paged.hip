@@ -295,17 +295,34 @@ __global__ __launch_bounds__(256) void append_kv_kernel(const E *__restrict__ kv
     Pairs<E> p;
     if (lane < 4)
         p.template load<kHalves>(row + kLatent, lane);
-    float x[8], sum = 0.0f;
+    float x[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 8; ++i)
         x[i] = (float)xv[i];
-        sum += x[i] * x[i];
-    }
-    sum = sum_over_lane_groups(sum);
+    auto mean_square = [&](float f) {  // of f x, the same in every lane
+        float sum = 0.0f;
 #pragma unroll
-    for (int d = 8; d > 0; d /= 2)
-        sum += __shfl_xor(sum, d);
-    const float norm = 1.0f / sqrtf(sum * (1.0f / kLatent) + eps);
+        for (int i = 0; i < 8; ++i)
+            sum += (f * x[i]) * (f * x[i]);
+        sum = sum_over_lane_groups(sum);
+#pragma unroll
+        for (int d = 8; d > 0; d /= 2)
+            sum += __shfl_xor(sum, d);
+        return sum * (1.0f / kLatent);
+    };
+    float under_root = mean_square(1.0f) + eps, norm = 1.0f / sqrtf(under_root);
+    // bf16 reaches further than its squares do in fp32. Where they may have left fp32's
+    // range, rows and epsilon are squared again times a power of two: what then
+    // vanishes is below 2^-24 of the sum.
+    if (!(under_root > 0x1p-100f && under_root < 0x1p100f)) {
+        const bool tiny = under_root < 1.0f;
+        const float f = tiny ? 0x1p100f : 0x1p-100f;
+        under_root = mean_square(f) + eps * f * f;
+        norm = 1.0f / sqrtf(under_root) * (tiny ? 1.0f : f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            x[i] *= tiny ? f : 1.0f;  // 1 / norm may pass 2^128, each factor does not
+    }
 #pragma unroll
     for (int i = 0; i < 8; ++i)
         x[i] = x[i] * norm * (float)wv[i];

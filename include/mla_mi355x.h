@@ -375,7 +375,8 @@ int mla_paged_tables(const int *context_lens, const int *new_lens,
  *   kv_cache[slots[t]][:512] = kv[t][:512] norm_weight / sqrt(mean(kv[t][:512]^2) + eps)
  *   kv_cache[slots[t]][512:] = rotated kv[t][512:]
  *   q_rope_out[t][h]         = rotated q_rope[t][h]
- * computed in fp32 and rounded once. The rotation turns pair i (values 2 i and
+ * computed in fp32 and rounded once; rows of any finite values, also such whose
+ * squares leave fp32's range. The rotation turns pair i (values 2 i and
  * 2 i + 1, or i and i + 32 with MLA_FLAG_ROPE_HALVES) by the angle whose
  * cosine and sine are cos_sin[positions[t]][i] and [32 + i] (fp32
  * [num_positions][64]; positions are clamped to it). kv [tokens] rows of 576

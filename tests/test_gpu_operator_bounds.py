@@ -1,0 +1,86 @@
+"""The operators around the decode at the bounds of their types and buffers: rows whose
+squares pass fp32's range, keys whose expansion passes fp16's, saturated fp8 rows,
+inputs that begin off 16 bytes, workspaces of exactly the size that is asked for.
+Tolerances: test_gpu_append_kv.py and operators_reference."""
+import random
+
+import pytest
+import torch
+
+import ada_mla
+from ada_mla import capi
+from operators_reference import attention_check, gather_paged, half_step, latent_rows, paged_case, random_tree, signed
+
+pytestmark = pytest.mark.gpu
+
+
+def _angles(positions=64):
+    i = torch.arange(32, dtype=torch.float64)
+    angle = torch.arange(positions, dtype=torch.float64)[:, None] * 10000.0 ** (-i / 32)
+    return torch.cat([angle.cos(), angle.sin()], 1).float()
+
+
+def _rows(kv, w, eps, interleaved=True, fp8_scale=None):
+    """kv's rows appended to an empty cache, and the same in float64."""
+    n = kv.shape[0]
+    cs, pos = _angles(), torch.arange(n, dtype=torch.int32)
+    cache = torch.zeros(n, 576, dtype=kv.dtype if fp8_scale is None else torch.float8_e4m3fn, device="cuda")
+    ada_mla.mla_append_kv(kv.cuda(), w.cuda(), cs.cuda(), pos.cuda(), torch.arange(n).cuda(), cache, eps=eps,
+                          cache_scale=1.0 if fp8_scale is None else fp8_scale, interleaved=interleaved)
+    angle = cs[:n].double()
+    return cache.cpu().double(), latent_rows(kv, w, angle[:, :32], angle[:, 32:], eps, interleaved)
+
+
+@pytest.mark.parametrize("eps", [1e-6, 0.0])
+@pytest.mark.parametrize("largest", [2.0 ** 62, 2.0 ** 100, 2.0 ** 126])
+def test_rows_whose_squares_pass_fp32(largest, eps):
+    # bf16 reaches 2^128: the mean of the squares is past fp32's range, the normalised row is an ordinary one
+    gen = torch.Generator()
+    gen.manual_seed(1)
+    kv = torch.randn(6, 576, generator=gen)
+    kv[:, :512] *= largest / 4
+    kv[1, 7:512] = 0        # one value alone
+    kv[2, :256] *= 2.0 ** -40
+    kv[3, :512] = largest * 1.5
+    kv = kv.bfloat16()
+    assert torch.isfinite(kv).all()
+    w = (1 + 0.3 * torch.randn(512, generator=gen)).bfloat16()
+    got, ref = _rows(kv, w, eps)
+    bound = ref[:, :512].abs() * (half_step(torch.bfloat16) + 2.0 ** -14)
+    assert ((got[:, :512] - ref[:, :512]).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("scale", [2.0 ** -60, 2.0 ** -75, 2.0 ** -120])
+def test_rows_whose_squares_vanish_in_fp32(scale):
+    # without an epsilon a row of tiny values is normalised like any other
+    gen = torch.Generator()
+    gen.manual_seed(2)
+    kv = torch.randn(4, 576, generator=gen)
+    kv[:, :512] *= scale
+    kv = kv.bfloat16()
+    w = (1 + 0.3 * torch.randn(512, generator=gen)).bfloat16()
+    got, ref = _rows(kv, w, 0.0)
+    bound = ref[:, :512].abs() * (half_step(torch.bfloat16) + 2.0 ** -14)
+    assert ((got[:, :512] - ref[:, :512]).abs() <= bound).all()
+    # with one they stay tiny: the epsilon is all there is under the root
+    got, ref = _rows(kv, w, 1e-6)
+    bound = ref[:, :512].abs() * (half_step(torch.bfloat16) + 2.0 ** -14) + 2.0 ** -134  # half a step of subnormals
+    assert ((got[:, :512] - ref[:, :512]).abs() <= bound).all()
+
+
+def test_rows_with_infinities_among_large_values():
+    kv = torch.full((3, 576), 2.0 ** 100)
+    kv[0, 5], kv[1, 6] = float("inf"), float("nan")
+    got, _ = _rows(kv.bfloat16(), torch.ones(512).bfloat16(), 1e-6)
+    assert torch.isnan(got[0, 5]) and not got[0, :5].any() and not got[0, 6:512].any()
+    assert torch.isnan(got[1, :512]).all()
+    assert (got[2, :512] == 1).all()
+
+
+def _off(t, by=1):
+    """The same values, contiguous, `by` entries into another buffer."""
+    flat = torch.full((t.numel() + by,), 7.0, dtype=t.dtype, device="cuda")
+    flat[by:] = t.flatten().cuda()
+    view = flat[by:].view(t.shape)
+    assert view.is_contiguous() and view.data_ptr() % 16 != 0
+    return view
