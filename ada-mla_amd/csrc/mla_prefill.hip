@@ -261,14 +261,17 @@ expand_kernel(PrefillArgs a)
         const int h = i / (2 * kBlocksPerSide), rest = i % (2 * kBlocksPerSide);
         const bool side = rest >= kBlocksPerSide;
         const bool lane_bad = not_finite<E>((unsigned short)top) || not_finite<E>((unsigned short)(top >> 16));
-        const unsigned long long m = __builtin_amdgcn_ballot_w64(side && lane_bad);
+        const unsigned long long m = __builtin_amdgcn_ballot_w64(lane_bad);
         if (m != 0) {
             // V: what is not finite becomes 0 and flags its key, so that a
-            // query that must not see the key can meet it with weight 0
+            // query that must not see the key can meet it with weight 0. K: it
+            // becomes NaN, as an infinity that was a finite value before its rounding
+            // to fp16 could make a logit of -inf, and the key would count for nothing.
+            const E put = side ? (E)0.0f : (E)NAN;
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 const E y = v[r >> 3][r & 7];
-                v[r >> 3][r & 7] = not_finite<E>(__builtin_bit_cast(unsigned short, y)) ? (E)0.0f : y;
+                v[r >> 3][r & 7] = not_finite<E>(__builtin_bit_cast(unsigned short, y)) ? put : y;
             }
             bad[g] |= (unsigned)m | (unsigned)(m >> 32);
         }

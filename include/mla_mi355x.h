@@ -448,8 +448,8 @@ int mla_decode_tree_bf16(const void *query, const void *kv_cache,
  * start at 0 and are clamped to [0, queries] and [0, total_tokens]; rows of out
  * behind the last request's are zeros. w_uk, w_uv as for
  * mla_absorb_query_* / mla_project_output_*. K and V are rounded to the
- * inputs' type; a query that sees a key whose V is not finite gives NaN, and
- * what it does not see never reaches it. The workspace holds K and V: 512
+ * inputs' type; a query that sees a key whose K or V is not finite then (fp16:
+ * past 65504) gives NaN, and what it does not see never reaches it. The workspace holds K and V: 512
  * bytes a key and head, and partial results where few queries see many keys.
  * Two launches, three with partials. */
 size_t mla_prefill_workspace_size(int batch, int num_heads, int queries,

@@ -77,6 +77,34 @@ def test_rows_with_infinities_among_large_values():
     assert (got[2, :512] == 1).all()
 
 
+@pytest.mark.parametrize("queries", [100, 1500])
+def test_a_key_that_overflows_fp16(queries):
+    # A finite latent row whose key passes 65504 in one value. Its logit is large and positive; as an
+    # infinity times a negative query value it would be -inf, and the key would silently count for nothing.
+    gen = torch.Generator()
+    gen.manual_seed(4)
+    heads, t, h = 16, 50, 3
+    qn = torch.randn(queries, heads, 128, generator=gen).half()
+    qr = torch.randn(queries, heads, 64, generator=gen).half()
+    uk, uv = ((torch.randn(heads, 128, 512, generator=gen) * 512 ** -0.5).half() for _ in range(2))
+    cache = torch.randn(queries, 576, generator=gen).half()
+    uk[h] = 0
+    uk[h, 17], uk[h, 18] = 2.0, 0.5
+    qn[:, h] = 0
+    qn[:, h, 17], qn[:, h, 18] = -0.01, 1.0
+    cu = torch.tensor([0, queries], dtype=torch.int32, device="cuda")
+    args = [x.cuda() for x in (qn, qr, uk, uv)]
+    want = ada_mla.mla_prefill(*args, cache.cuda(), cu, cu)
+    cache[t, :512] = 128.0
+    k = cache[t, :512].double() @ uk[h].double().T
+    assert k[17] > 65504 and k[18] < 65504 and qn[0, h].double() @ k > 1000
+    got = ada_mla.mla_prefill(*args, cache.cuda(), cu, cu)
+    assert torch.equal(got[:t], want[:t])
+    assert torch.isnan(got[t:, h]).all()
+    others = [i for i in range(heads) if i != h]
+    assert torch.isfinite(got[:, others]).all()
+
+
 def _off(t, by=1):
     """The same values, contiguous, `by` entries into another buffer."""
     flat = torch.full((t.numel() + by,), 7.0, dtype=t.dtype, device="cuda")
