@@ -350,15 +350,26 @@ int64_t given_total(int64_t total_tokens, const at::Tensor &cu, const char *fn)
     return total_tokens;
 }
 
+bool starts_aligned(const at::Tensor &t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
+
+// A contiguous tensor that starts at a multiple of 16 bytes: the same one, else a
+// copy. (A contiguous view into a buffer may start anywhere, and contiguous()
+// returns it as it is.)
+at::Tensor readable(const at::Tensor &t)
+{
+    const at::Tensor c = t.contiguous();
+    return starts_aligned(c) ? c : c.clone(at::MemoryFormat::Contiguous);
+}
+
 // A tensor whose rows the kernels can read in place: the last dimension
 // contiguous, the others' strides multiples of 16 bytes, the start aligned;
 // else a contiguous copy.
 at::Tensor readable_rows(const at::Tensor &t)
 {
-    bool ok = reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && t.stride(-1) == 1;
+    bool ok = starts_aligned(t) && t.stride(-1) == 1;
     for (int64_t d = 0; d + 1 < t.dim(); ++d)
         ok = ok && (t.size(d) == 1 || t.stride(d) % 8 == 0);
-    return ok ? t : t.contiguous();
+    return ok ? t : readable(t);
 }
 
 // A stride that the C ABI takes: that of a dimension of one entry is never used.
@@ -469,7 +480,7 @@ c10::optional<at::Tensor> mla_append_kv(const at::Tensor &kv_in, const at::Tenso
         out = at::empty({tokens, heads, 64}, q_rope_in->options().memory_format(at::MemoryFormat::Contiguous));
     if (tokens == 0)
         return out;
-    const at::Tensor kv = readable_rows(kv_in), weight = readable_rows(weight_in), cos_sin = cos_sin_in.contiguous();
+    const at::Tensor kv = readable_rows(kv_in), weight = readable_rows(weight_in), cos_sin = readable(cos_sin_in);
     const at::Tensor positions = positions_in.contiguous(), slots = slots_in.contiguous();
     const at::Tensor q = q_rope_in ? readable_rows(*q_rope_in) : at::Tensor();
     auto f = dt == at::kHalf ? mla_append_kv_fp16 : mla_append_kv_bf16;
@@ -517,7 +528,7 @@ at::Tensor mla_decode_tree(const at::Tensor &query_in, const at::Tensor &kv_in, 
     check_devices({&query_in, &kv_in, &block_table_in, &cu_seqlens_in, &tree_mask_in,
                    draft_lens_in ? &*draft_lens_in : &query_in}, fn);
     const at::OptionalDeviceGuard guard(query_in.device());
-    const at::Tensor query = query_in.contiguous(), kv = kv_in.contiguous(), bt = block_table_in.contiguous();
+    const at::Tensor query = readable(query_in), kv = readable(kv_in), bt = block_table_in.contiguous();
     const at::Tensor cu = cu_seqlens_in.contiguous(), mask = tree_mask_in.contiguous();
     const at::Tensor lens = draft_lens_in ? draft_lens_in->contiguous() : at::Tensor();
     const int total = static_cast<int>(given_total(total_tokens, cu, fn));
@@ -582,8 +593,8 @@ at::Tensor mla_prefill(const at::Tensor &q_nope_in, const at::Tensor &q_rope_in,
     check_devices({&q_nope_in, &q_rope_in, &w_uk_in, &w_uv_in, &kv_in, &cu_q_in, &cu_seqlens_in,
                    block_table_in ? &*block_table_in : &q_nope_in}, fn);
     const at::OptionalDeviceGuard guard(q_nope_in.device());
-    const at::Tensor qn = q_nope_in.contiguous(), qr = q_rope_in.contiguous();
-    const at::Tensor wuk = w_uk_in.contiguous(), wuv = w_uv_in.contiguous(), kv = kv_in.contiguous();
+    const at::Tensor qn = readable(q_nope_in), qr = readable(q_rope_in);
+    const at::Tensor wuk = readable(w_uk_in), wuv = readable(w_uv_in), kv = readable(kv_in);
     const at::Tensor cu_q = cu_q_in.contiguous(), cu = cu_seqlens_in.contiguous();
     const at::Tensor bt = block_table_in ? block_table_in->contiguous() : at::Tensor();
     const int total = static_cast<int>(given_total(total_tokens, cu, fn));

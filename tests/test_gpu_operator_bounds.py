@@ -112,3 +112,50 @@ def _off(t, by=1):
     view = flat[by:].view(t.shape)
     assert view.is_contiguous() and view.data_ptr() % 16 != 0
     return view
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_append_inputs_that_begin_off_16_bytes(dtype):
+    gen = torch.Generator()
+    gen.manual_seed(5)
+    kv, q = torch.randn(21, 576, generator=gen).to(dtype), torch.randn(21, 16, 64, generator=gen).to(dtype)
+    w, cs = (1 + 0.3 * torch.randn(512, generator=gen)).to(dtype), _angles()
+    pos, slots = torch.arange(21, dtype=torch.int32).cuda(), torch.arange(21).cuda()
+
+    def call(kv, w, cs, q):
+        cache = torch.zeros(32, 576, dtype=dtype, device="cuda")
+        return ada_mla.mla_append_kv(kv, w, cs, pos, slots, cache, q_rope=q), cache
+    good = [kv.cuda(), w.cuda(), cs.cuda(), q.cuda()]
+    want = call(*good)
+    for i in range(4):
+        got = call(*[_off(x) if i == k else x for k, x in enumerate(good)])
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), i
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_tree_inputs_that_begin_off_16_bytes(dtype):
+    gen = torch.Generator()
+    gen.manual_seed(6)
+    cache, table, cu = paged_case(gen, random.Random(6), [100, 33], 32, dtype)
+    q = torch.randn(2, 3, 16, 576, generator=gen).to(dtype).cuda()
+    mask = torch.tensor([[1, 3, 5]] * 2, dtype=torch.int64, device="cuda")
+    want = ada_mla.mla_decode_tree(q, cache, table, cu, mask)
+    assert torch.equal(ada_mla.mla_decode_tree(_off(q), cache, table, cu, mask), want)
+    assert torch.equal(ada_mla.mla_decode_tree(q, _off(cache), table, cu, mask), want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("paged", [False, True])
+def test_prefill_inputs_that_begin_off_16_bytes(dtype, paged):
+    gen = torch.Generator()
+    gen.manual_seed(7)
+    qn, qr = torch.randn(70, 16, 128, generator=gen).to(dtype), torch.randn(70, 16, 64, generator=gen).to(dtype)
+    uk, uv = ((torch.randn(16, 128, 512, generator=gen) * 512 ** -0.5).to(dtype) for _ in range(2))
+    cache, table, cu = paged_case(gen, random.Random(7), [50, 20], 32, dtype)
+    if not paged:
+        cache, table = torch.randn(70, 576, generator=gen).to(dtype).cuda(), None
+    good = [qn.cuda(), qr.cuda(), uk.cuda(), uv.cuda(), cache]
+    want = ada_mla.mla_prefill(*good, cu, cu, table)
+    for i in range(5):
+        got = ada_mla.mla_prefill(*[_off(x) if i == k else x for k, x in enumerate(good)], cu, cu, table)
+        assert torch.equal(got, want), i
