@@ -50,21 +50,25 @@ struct TreeArgs {
     const unsigned long long *tree_mask;
     const int *draft_lens;
     void *out;
-    float *part_o;  // [slot][row tile][wave][16 column tiles][4][64 lanes][4]
-    float *part_m;  // [slot][row tile * 128]
+    float *part_o;  // [part slot][row tile][wave][16 column tiles][4][64 lanes][4]
+    float *part_m;  // [part slot][row tile * 128]
     float *part_l;
     int batch, drafts, num_heads, total_tokens;
     int chunk;      // tokens per split
     int row_tiles;  // of 128 rows, per request
-    int n_slots;    // total_tokens / chunk + batch
+    int n_slots;    // splits of the batch, at most: total_tokens / chunk + batch
+    int pairs;      // how the splits' partials are numbered, see Request
     int by_xcd;     // 1: the workgroups of a split share an XCD
     int page_shift, num_pages, bt_stride;
     float scale_log2;
 };
 
-// Request b's tokens [lo, lo + len) of the packed numbering and its splits. Request
-// b's splits take the slots lo / chunk + b, ..., which never meet those of
-// another request, whatever the lengths.
+// Request b's tokens [lo, lo + len) of the packed numbering and its splits. The
+// partials of a request of several splits take the part slots lo / chunk + b, ..., or
+// with `pairs` 2 lo / chunk, ...: neither meets those of another request, whatever the
+// lengths. (A request of several splits has len > chunk, so 2 len / chunk rounded
+// down is at least len / chunk rounded up.) The second has fewer slots where most
+// requests are shorter than a split.
 struct Request {
     int lo, len, n_splits, slot0, drafts;
     __device__ __forceinline__ void read(const TreeArgs &a, int b)
@@ -72,7 +76,7 @@ struct Request {
         lo = min(max(scalar_load(a.cu_seqlens + b), 0), a.total_tokens);
         len = min(max(scalar_load(a.cu_seqlens + b + 1), lo), a.total_tokens) - lo;
         n_splits = max(1, (len + a.chunk - 1) / a.chunk);
-        slot0 = lo / a.chunk + b;
+        slot0 = (int)(((unsigned)lo << a.pairs) / (unsigned)a.chunk) + (a.pairs ? 0 : b);
         drafts = a.draft_lens ? min(max(scalar_load(a.draft_lens + b), 0), a.drafts) : a.drafts;
     }
 };
@@ -609,9 +613,10 @@ __global__ __launch_bounds__(256) void tree_combine_kernel(TreeArgs a, int tiles
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
 struct TreePlan {
-    int row_tiles, chunk, n_slots;
+    int row_tiles, chunk, n_slots, pairs;
     int parts;  // column parts: 1 or 4
     size_t o_bytes, ml_bytes;
+    size_t bytes() const { return std::max<size_t>(256, o_bytes + 2 * ml_bytes); }  // 0 would say: unsupported
 };
 
 // Splits of a request of mean length, and column parts: those with the least
@@ -669,7 +674,11 @@ TreePlan compute_tree_plan(int batch, int drafts, int num_heads, int total_token
         chunk = std::max<int64_t>(chunk, kWholeTokens);
     p.chunk = (int)chunk;
     p.n_slots = total_tokens / p.chunk + batch;
-    const size_t tiles = (size_t)p.n_slots * p.row_tiles;
+    // partials: none where no request can be longer than a split
+    const int64_t by_pairs = 2 * (int64_t)total_tokens / p.chunk;
+    p.pairs = by_pairs < p.n_slots;
+    const size_t part_slots = total_tokens <= p.chunk ? 0 : p.pairs ? (size_t)by_pairs : (size_t)p.n_slots;
+    const size_t tiles = part_slots * p.row_tiles;
     p.o_bytes = align256(tiles * kRows * kDV * sizeof(float));
     p.ml_bytes = align256(tiles * kRows * sizeof(float));
     return p;
@@ -731,7 +740,7 @@ int decode_tree(bool bf16, const void *query, const void *kv_cache, const int *b
     const TreePlan p = tree_plan(batch, drafts, num_heads, total_tokens, num_splits, current_cu_count());
     if ((int64_t)(p.n_slots + 7) * p.row_tiles > INT32_MAX / (256 * 4) || (int64_t)batch * p.row_tiles > INT32_MAX / (256 * 64))
         return MLA_STATUS_INVALID_VALUE;
-    if (workspace_bytes < p.o_bytes + 2 * p.ml_bytes)
+    if (workspace_bytes < p.bytes())
         return MLA_STATUS_WORKSPACE_TOO_SMALL;
     TreeArgs a;
     a.q = query;
@@ -752,6 +761,7 @@ int decode_tree(bool bf16, const void *query, const void *kv_cache, const int *b
     a.chunk = p.chunk;
     a.row_tiles = p.row_tiles;
     a.n_slots = p.n_slots;
+    a.pairs = p.pairs;
     a.by_xcd = p.n_slots >= kMinSlotsByXcd;
     a.page_shift = __builtin_ctz((unsigned)page_size);
     a.num_pages = num_pages;
@@ -774,8 +784,7 @@ size_t mla_decode_tree_workspace_size(int batch, int drafts, int num_heads, int 
 {
     if (!mla::tree_sizes_ok(batch, drafts, num_heads, total_tokens))
         return 0;
-    const mla::TreePlan p = mla::tree_plan(batch, drafts, num_heads, total_tokens, num_splits, mla::current_cu_count());
-    return p.o_bytes + 2 * p.ml_bytes;
+    return mla::tree_plan(batch, drafts, num_heads, total_tokens, num_splits, mla::current_cu_count()).bytes();
 }
 
 int mla_decode_tree_fp16(const void *query, const void *kv_cache, const int *block_table, const int *cu_seqlens,

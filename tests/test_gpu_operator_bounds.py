@@ -159,3 +159,36 @@ def test_prefill_inputs_that_begin_off_16_bytes(dtype, paged):
     for i in range(5):
         got = ada_mla.mla_prefill(*[_off(x) if i == k else x for k, x in enumerate(good)], cu, cu, table)
         assert torch.equal(got, want), i
+
+
+@pytest.mark.parametrize("heads,m,lengths,splits", [
+    # rows that fill the chip, most requests far below a split's tokens and a few past it
+    (64, 16, [5, 30, 1025, 16, 700, 2049, 40, 1, 0, 1024] + [20 + i for i in range(30)], 0),
+    # the same lengths in every request, and splits that one request asks for among short ones
+    (16, 4, [300] * 7, 4), (16, 4, [4] * 20 + [900] + [4] * 20, 5),
+    # no request can be split
+    (128, 8, [7, 90, 13] * 20, 0)])
+def test_tree_workspace_of_exactly_its_size(heads, m, lengths, splits):
+    rng, gen = random.Random(8), torch.Generator()
+    gen.manual_seed(8)
+    dtype = torch.bfloat16
+    cache, table, cu = paged_case(gen, rng, lengths, 32, dtype)
+    q = torch.randn(len(lengths), m, heads, 576, generator=gen).to(dtype).cuda()
+    masks = [random_tree(rng, m) for _ in lengths]
+    mask = torch.tensor([signed(x) for x in masks], dtype=torch.int64, device="cuda")
+    drafts = [min(m, n) for n in lengths]
+    size = capi.load().mla_decode_tree_workspace_size(len(lengths), m, heads, sum(lengths), splits)
+    room = torch.full((size + 4096,), 255, dtype=torch.uint8, device="cuda")
+    got = capi.decode_tree(q, cache, table, cu, mask, sum(lengths), draft_lens=torch.tensor(drafts, dtype=torch.int32).cuda(),
+                           num_splits=splits, workspace=room[:size]).cpu()
+    assert (room[size:] == 255).all()
+    for b, (n, k) in enumerate(zip(lengths, drafts)):
+        c = gather_paged(cache, table[b], n)
+        for i in range(m):
+            seen = torch.zeros(1, n, dtype=torch.bool)
+            if i < k:
+                seen[0, :n - k] = True
+                for j in range(k):
+                    seen[0, n - k + j] = bool(masks[b][i] >> j & 1)
+            attention_check(got[b, i], q[b, i].double().cpu(), c, c[:, :512], seen.expand(heads, n), dtype,
+                            what=f"request {b} draft {i}")
