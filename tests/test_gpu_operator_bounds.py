@@ -77,6 +77,31 @@ def test_rows_with_infinities_among_large_values():
     assert (got[2, :512] == 1).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("interleaved", [True, False])
+def test_fp8_rows_saturate_at_448(dtype, interleaved):
+    # every value past 448 scales is 448 of its sign, every other one within half a step of E4M3
+    gen = torch.Generator()
+    gen.manual_seed(3)
+    kv = torch.randn(9, 576, generator=gen)
+    kv[:, 512:] *= 3
+    w = 1 + 0.3 * torch.randn(512, generator=gen)
+    kv, w, scale = kv.to(dtype), w.to(dtype), 2.0 ** -8  # 448 scales are 1.75
+    got, ref = _rows(kv, w, 1e-6, interleaved, scale)
+    want = ref / scale
+    # fp32 before the rounding: 2^-14 |ref| for latents, 2^-22 of the rotated pair's values
+    slack = want.abs() * 2.0 ** -14
+    slack[:, 512:] += 2.0 ** -21 * kv[:, 512:].double().abs().amax(1, keepdim=True) / scale
+    past = want.abs() - slack > 448
+    for part in (slice(0, 512), slice(512, 576)):
+        for sign in (1.0, -1.0):
+            assert (past[:, part] & (want[:, part].sign() == sign)).sum() >= 10
+    assert torch.equal(got[past], 448 * want[past].sign())
+    inside = want.clamp(-448, 448)
+    bound = inside.abs() * 2.0 ** -4 + 2.0 ** -10 + slack * (1 + 2.0 ** -4)
+    assert ((got - inside).abs() <= bound).all()
+
+
 @pytest.mark.parametrize("queries", [100, 1500])
 def test_a_key_that_overflows_fp16(queries):
     # A finite latent row whose key passes 65504 in one value. Its logit is large and positive; as an
