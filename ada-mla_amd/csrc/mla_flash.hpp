@@ -115,7 +115,8 @@ __device__ __forceinline__ int key_swizzle(int r)
 
 // P's registers 8 a .. 8 a + 7, rounded to the type of V: the B operand of keys 16 a ..
 // 16 a + 15 of its block. P is in [0, 2^8] and the rounding at most half a
-// step of each term; the sums of P that normalise the result stay in fp32.
+// step of each term; the sums of P that normalise the result stay in fp32. (The
+// rest of P as a second operand would double the second product.)
 template <typename E>
 __device__ __forceinline__ typename Vec<E>::v8 p_operand(const float *p)
 {

@@ -13,14 +13,17 @@
 // attend_kernel is one pass over them with a running maximum and sum. Where few
 // queries see long contexts it splits the keys, and merge_kernel joins the parts;
 // small calls take narrow_kernel instead.
-// K and V are held in the inputs' 16-bit type, as a cache of expanded heads
-// would hold them: a rounding of half a step on each, the sums in fp32. (In fp32
-// they would double the workspace and take three products of split operands
-// for each one.)
+// K and V are held in the inputs' 16-bit type, as a model that expands its keys
+// with a matrix product holds them: a rounding of half a step on each, the sums in
+// fp32. With P's (p_operand) that makes three roundings before the result's own.
+// Against 64 bits, in units of the error that rounding the result alone has, V's makes
+// 1.37, K's 1.2, P's 1.2, all of them 1.35 (some keys) to 1.67 (hundreds). A second 16 bits of V
+// would take 16 products more to a tile's 40 and half as much workspace again, fp32 K and
+// V twice the workspace and three products for each one.
 //
-// Measured: 8192 queries at 64 heads 155 us + 1317 us (137 and 1375 GF: 0.9 and
+// Measured: 8192 queries at 64 heads 154 us + 1320 us (137 and 1375 GF: 0.9 and
 // 1.04 PFLOP/s, where a large matrix product reaches 1.3); 6 prompts of up to 1500
-// tokens at 128 heads 190 + 303 us; 197 queries at 16 heads 8 + 7 us.
+// tokens at 128 heads 187 + 301 us; 197 queries at 16 heads 7.5 + 7.2 us.
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
@@ -950,8 +953,8 @@ struct PrefillPlan {
 // and its tiles, more each where two run on a CU; partials (fp32, written and read) and a
 // third launch are the price. A split has a given number of tiles, more where a request is
 // longer than the splits then reach. Calls in one split and as planned: 1 query behind
-// 8000 tokens at 16 heads 225 us and 71, 500 queries there 274 and 138, 1000 at 32
-// heads 336 and 311, 100 behind 2000 at 16 heads 76 and 38.
+// 8000 tokens at 16 heads 225 us and 76, 500 queries there 274 and 134, 1000 at 32
+// heads 336 and 317, 100 behind 2000 at 16 heads 76 and 39.
 //
 // narrow_kernel competes with them: one workgroup a CU at a time, four tiles in each
 // kNarrowTileUs; only the first round is taken to see all the keys. 197 queries at

@@ -68,7 +68,8 @@ __device__ __forceinline__ void lds_barrier()
 // code, as the compiler does not see a load here:
 //  - m0, which carries the LDS address, may be read one slot after it is
 //    written: the s_nop. m0 is left changed, and nothing outside inline
-//    assembly uses it.
+//    assembly uses it. (Saved and restored, two instructions more: 128 heads, N =
+//    4096 10.87 us a call against 10.82, N = 65536 32.8 against 32.9.)
 //  - base may be read 5 slots after a vector instruction (v_readfirstlane)
 //    wrote it.
 // A test of the assembly checks all three in every kernel.

@@ -14,11 +14,13 @@
 // whole (Q* 144 registers, O* 256 accumulators, P in registers, see
 // mla_flash.hpp), so the waves meet only to hand over cache blocks.
 //
-// Measured: 32 drafts x 128 heads over 50021 tokens 399 us + 15 of merging (446
-// GF: 1.12 PFLOP/s; a large matrix product reaches 1.3), bound by the LDS reads of
+// Measured: 32 drafts x 128 heads over 50021 tokens 403 us + 14 of merging (446
+// GF: 1.11 PFLOP/s; a large matrix product reaches 1.3), bound by the LDS reads of
 // the first product (16 bytes a lane each: 40 cycles a product instead of 32) and
-// a clock of some 1.6 GHz; 48 requests of 5 x 16 rows over 12000 tokens 84 + 10 us,
+// a clock of some 1.6 GHz; 48 requests of 5 x 16 rows over 12000 tokens 85 + 10 us,
 // the cache at 4.5 TB/s; 7 x 16 rows over 1003 tokens 10 + 4 us, round trips.
+// Rounded to 16 bits on the way: P, for the second product (p_operand). The error
+// against 64 bits is then up to a quarter above that of rounding the result alone.
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
@@ -101,7 +103,7 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
     // the batch. With by_xcd the workgroups of a split, which read the same tokens, get ids
     // equal mod 8, i.e. one XCD and its L2, and the splits go to the XCDs in turn. (Taken by
     // slot, of which requests leave some empty, 15 requests of 32 drafts x 128 heads fell on
-    // half of the XCDs: 625 us, 24 of 16 x 64 632.)
+    // half of the XCDs: 642 us against 379, 24 of 16 x 64 628 against 329.)
     const int per_split = a.row_tiles * kParts;
     const int id = a.by_xcd ? blockIdx.x >> 3 : blockIdx.x;
     const int nth = a.by_xcd ? id / per_split * 8 + (blockIdx.x & 7) : id / per_split;
@@ -667,7 +669,7 @@ TreePlan compute_tree_plan(int batch, int drafts, int num_heads, int total_token
     chunk = std::max<int64_t>(kBlock, (chunk + kBlock - 1) / kBlock * kBlock);
     // Where the rows alone fill the CUs, requests up to kWholeTokens are not split for being
     // longer than the mean: 60 requests of 24 drafts x 128 heads over 1 to 40 tokens 284 ->
-    // 167 us, 40 of 16 x 128 over up to 716 186 -> 136. (Twice the mean for longer ones
+    // 165 us, 40 of 16 x 128 over up to 716 186 -> 142. (Twice the mean for longer ones
     // gained on some batches, 257 -> 214, and lost on others, 161 -> 187.)
     constexpr int kWholeTokens = 1024;
     if (splits == 1 && asked <= 0 && (int64_t)batch * p.row_tiles * p.parts >= cu_count)
