@@ -20,7 +20,8 @@
 //  * mla_decode_split and mla_decode_split_batched also take a float8_e4m3fn
 //    cache with a float16 query: the cache holds C / cache_scale (keyword
 //    cache_scale, default 1) and is read at one byte per value (fp8 is
-//    future work in the reference too, README.md:408).
+//    future work in the reference too, README.md:408); mla_decode_paged takes
+//    such a cache with float16 and bfloat16 queries.
 #include <torch/extension.h>
 
 #include <cmath>
@@ -207,12 +208,16 @@ at::Tensor mla_decode_split_batched(const at::Tensor &query_in, const at::Tensor
 // the split plan.
 at::Tensor mla_decode_paged(const at::Tensor &query_in, const at::Tensor &kv_in,
                             const at::Tensor &block_table_in, const at::Tensor &cu_seqlens_in,
-                            int64_t total_tokens, int64_t num_splits)
+                            int64_t total_tokens, int64_t num_splits, double cache_scale)
 {
     const char *fn = "mla_decode_paged";
-    TORCH_CHECK(query_in.scalar_type() == kv_in.scalar_type() &&
+    const bool fp8 = kv_in.scalar_type() == at::kFloat8_e4m3fn;
+    TORCH_CHECK((fp8 || query_in.scalar_type() == kv_in.scalar_type()) &&
                     (query_in.scalar_type() == at::kHalf || query_in.scalar_type() == at::kBFloat16),
-                fn, ": query and kv_cache must both be float16 or both bfloat16");
+                fn, ": query and kv_cache must both be float16 or both bfloat16 (or a float8_e4m3fn kv_cache with "
+                "either)");
+    check_cache_scale(cache_scale, fn);
+    TORCH_CHECK(fp8 || cache_scale == 1.0, fn, ": cache_scale is for a float8_e4m3fn cache");
     TORCH_CHECK(block_table_in.scalar_type() == at::kInt && block_table_in.dim() == 2, fn,
                 ": block_table must be a 2-D int32 tensor");
     TORCH_CHECK(cu_seqlens_in.scalar_type() == at::kInt && cu_seqlens_in.dim() == 1, fn,
@@ -247,13 +252,23 @@ at::Tensor mla_decode_paged(const at::Tensor &query_in, const at::Tensor &kv_in,
     const int total = static_cast<int>(total_tokens);
     const int splits = static_cast<int>(num_splits);
     at::Tensor out = at::empty({batch, nh, MLA_HEAD_DIM_V}, query.options());
-    const size_t ws_bytes = mla_decode_paged_workspace_size(static_cast<int>(batch), nh, total, splits);
+    const size_t ws_bytes = (fp8 ? mla_decode_paged_fp8_workspace_size
+                                 : mla_decode_paged_workspace_size)(static_cast<int>(batch), nh, total, splits);
     TORCH_CHECK(ws_bytes > 0, fn, ": unsupported sizes");
     at::Tensor ws = workspace(ws_bytes, query);
-    auto f = query.scalar_type() == at::kHalf ? mla_decode_paged_fp16 : mla_decode_paged_bf16;
-    const int st = f(query.data_ptr(), kv.data_ptr(), bt.data_ptr<int>(), cu.data_ptr<int>(), out.data_ptr(),
-                     ws.data_ptr(), ws_bytes, static_cast<int>(batch), nh, total, static_cast<int>(page),
-                     static_cast<int>(kv.size(0)), static_cast<int>(bt.size(1)), splits, stream_of(query));
+    const bool half = query.scalar_type() == at::kHalf;
+    int st;
+    if (fp8) {
+        auto f = half ? mla_decode_paged_fp8_fp16 : mla_decode_paged_fp8_bf16;
+        st = f(query.data_ptr(), kv.data_ptr(), static_cast<float>(cache_scale), bt.data_ptr<int>(), cu.data_ptr<int>(),
+               out.data_ptr(), ws.data_ptr(), ws_bytes, static_cast<int>(batch), nh, total, static_cast<int>(page),
+               static_cast<int>(kv.size(0)), static_cast<int>(bt.size(1)), splits, stream_of(query));
+    } else {
+        auto f = half ? mla_decode_paged_fp16 : mla_decode_paged_bf16;
+        st = f(query.data_ptr(), kv.data_ptr(), bt.data_ptr<int>(), cu.data_ptr<int>(), out.data_ptr(),
+               ws.data_ptr(), ws_bytes, static_cast<int>(batch), nh, total, static_cast<int>(page),
+               static_cast<int>(kv.size(0)), static_cast<int>(bt.size(1)), splits, stream_of(query));
+    }
     check_status(st, fn);
     return out;
 }
@@ -634,9 +649,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
           "paged-KV fp16 / bf16 MLA decode (query [B,n_h,576], kv_cache [pages,page_size,576], "
           "block_table [B,max_pages] int32, cu_seqlens [B+1] int32); total_tokens=-1 reads cu_seqlens[B] "
           "(synchronising); a given total_tokens is not checked: one below cu_seqlens[B] silently "
-          "truncates the trailing sequences",
+          "truncates the trailing sequences. kv_cache of the query's dtype, or float8_e4m3fn holding C / cache_scale",
           pybind11::arg("query"), pybind11::arg("kv_cache"), pybind11::arg("block_table"),
-          pybind11::arg("cu_seqlens"), pybind11::arg("total_tokens") = -1, pybind11::arg("num_splits") = 0);
+          pybind11::arg("cu_seqlens"), pybind11::arg("total_tokens") = -1, pybind11::arg("num_splits") = 0,
+          pybind11::arg("cache_scale") = 1.0);
     m.def("mla_absorb_query", &mla_absorb_query,
           "Q* [B,n_h,576] = [q_nope W_UK[h], q_rope] (q_nope [B,n_h,128], q_rope [B,n_h,64], w_uk [n_h,128,512])",
           pybind11::arg("q_nope"), pybind11::arg("q_rope"), pybind11::arg("w_uk"));

@@ -207,7 +207,9 @@ int most_chunks(int cu_count, int n_head_tiles)
 Plan compute_plan(bool fp32, int num_heads, int total_tokens, int batch, bool seqlens,
                   int num_splits, int cu_count, CacheKind cache, bool f32_partials)
 {
-    const bool paged = cache == CacheKind::kPaged;  // pieces start page-aligned: one more block
+    // paged: pieces start page-aligned, one more block
+    const bool paged = cache == CacheKind::kPaged || cache == CacheKind::kPagedF8;
+    const bool f8 = cache == CacheKind::kF8 || cache == CacheKind::kPagedF8;
     Plan p{};
     if (total_tokens <= 0) {
         p.head_tile = fp32 ? 16 : (num_heads % 64 == 0) ? 64 : (num_heads % 32 == 0) ? 32 : 16;
@@ -282,7 +284,7 @@ Plan compute_plan(bool fp32, int num_heads, int total_tokens, int batch, bool se
             for (int w = w_lo; w <= w_hi; ++w) {
                 set_chunks(c, total_v, batch, w);
                 const double us = modelled_us(c, num_heads, total_tokens, batch, cu_count, paged,
-                                              !seqlens && cache != CacheKind::kPaged, c_bytes);
+                                              !seqlens && !paged, c_bytes);
                 if (best_us == 0.0 || us < best_us) {
                     best = c;
                     best_us = us;
@@ -305,7 +307,7 @@ Plan compute_plan(bool fp32, int num_heads, int total_tokens, int batch, bool se
         if (live * p16.block_tokens * kDK * 2 / kStreamBytesPerUs > step_us)
             set_chunks(p16, total_tokens + p16.seq_cost * batch, batch, most_chunks(cu_count, p16.n_head_tiles));
     }
-    if (cache != CacheKind::kF8 || num_splits > 0)
+    if (!f8 || num_splits > 0)
         return p16;
     // fp8 cache: its blocks stream half the bytes, so with few heads more
     // chunks than the 16-bit plan's pay -- but only long ones (measured on
@@ -317,7 +319,7 @@ Plan compute_plan(bool fp32, int num_heads, int total_tokens, int batch, bool se
     double us8 = 0.0;
     const Plan p8 = search(1, [](int ht, int) { return ht == 16 ? 4 : 16; }, us8);
     const double us16_as8 = modelled_us(p16, num_heads, total_tokens, batch, cu_count, paged,
-                                        !seqlens && cache != CacheKind::kPaged, 1);
+                                        !seqlens && !paged, 1);
     return us8 < us16_as8 ? p8 : p16;
 }
 
@@ -434,7 +436,7 @@ int choose_part_plain(const Plan &p, int batch, int num_heads, int cu_count)
 
 // Shared body of every entry point; `phases` selects the split kernel, the
 // combine, or both (in that order, on one stream).
-enum class Dtype { kF16, kBF16, kF32, kF8Cache };
+enum class Dtype { kF16, kBF16, kF32, kF8Cache, kF8CacheBF16 };  // kF8Cache*: query and out fp16 or bf16
 
 int run_decode(Dtype dt, const void *query, const void *cache, const int *cu_seqlens,
                void *out, void *workspace, size_t workspace_bytes, int batch,
@@ -450,9 +452,10 @@ int run_decode(Dtype dt, const void *query, const void *cache, const int *cu_seq
         (combine && !aligned16(out)))
         return MLA_STATUS_MISALIGNED;
     const bool fp32 = dt == Dtype::kF32;
-    const bool f32_part = !fp32 && !paging && dt != Dtype::kF8Cache && (flags & MLA_FLAG_FP32_PARTIALS) != 0;
-    const CacheKind kind = paging != nullptr ? CacheKind::kPaged
-                           : dt == Dtype::kF8Cache ? CacheKind::kF8 : CacheKind::kPacked;
+    const bool fp8 = dt == Dtype::kF8Cache || dt == Dtype::kF8CacheBF16;
+    const bool f32_part = !fp32 && !paging && !fp8 && (flags & MLA_FLAG_FP32_PARTIALS) != 0;
+    const CacheKind kind = paging != nullptr ? (fp8 ? CacheKind::kPagedF8 : CacheKind::kPaged)
+                                             : (fp8 ? CacheKind::kF8 : CacheKind::kPacked);
     const int cu = current_cu_count();
     Plan p = make_plan(fp32, num_heads, total_tokens, batch, cu_seqlens != nullptr, num_splits, cu, kind, f32_part);
     if (workspace_bytes < partials_bytes(p, num_heads))
@@ -470,10 +473,10 @@ int run_decode(Dtype dt, const void *query, const void *cache, const int *cu_seq
     pb.batch = batch;
     pb.num_heads = num_heads;
     pb.total_tokens = total_tokens;
-    pb.fp8 = dt == Dtype::kF8Cache;
+    pb.fp8 = fp8;
     pb.out_scale = pb.fp8 ? c_scale : 1.0f;
     pb.scale_log2 = scale_log2() * pb.out_scale;  // fp8: logits of the dequantised cache
-    pb.bf16 = dt == Dtype::kBF16;
+    pb.bf16 = dt == Dtype::kBF16 || dt == Dtype::kF8CacheBF16;
     pb.fp32 = fp32;
     pb.paging = paging ? *paging : Paging{nullptr, 0, 0, 0};
     const Partials w = carve_partials(workspace, p, num_heads);
@@ -715,9 +718,10 @@ namespace {
 int paged_decode(mla::Dtype dt, const void *query, const void *kv_cache, const int *block_table,
                  const int *cu_seqlens, void *out, void *workspace, size_t workspace_bytes, int batch,
                  int num_heads, int total_tokens, int page_size, int num_pages, int block_table_stride,
-                 int num_splits, void *stream)
+                 int num_splits, void *stream, float cache_scale = 1.0f)
 {
     if (!mla::heads_ok(num_heads) || batch < 1 || total_tokens < 0 || !cu_seqlens || !block_table ||
+        !(cache_scale > 0.0f && cache_scale < INFINITY) ||
         page_size < 32 || page_size > (1 << 20) || (page_size & (page_size - 1)) != 0 || num_pages < 1 ||
         block_table_stride < 1)
         return MLA_STATUS_INVALID_VALUE;
@@ -726,7 +730,7 @@ int paged_decode(mla::Dtype dt, const void *query, const void *kv_cache, const i
     mla::Paging pg{block_table, __builtin_ctz((unsigned)page_size), block_table_stride, num_pages};
     return mla::run_decode(dt, query, kv_cache, cu_seqlens, out, workspace, workspace_bytes, batch,
                            num_heads, total_tokens, num_splits, 0u, stream,
-                           mla::kPhaseSplit | mla::kPhaseCombine, &pg);
+                           mla::kPhaseSplit | mla::kPhaseCombine, &pg, cache_scale);
 }
 
 }  // namespace
@@ -749,6 +753,35 @@ int mla_decode_paged_bf16(const void *query, const void *kv_cache, const int *bl
     return paged_decode(mla::Dtype::kBF16, query, kv_cache, block_table, cu_seqlens, out, workspace,
                         workspace_bytes, batch, num_heads, total_tokens, page_size, num_pages,
                         block_table_stride, num_splits, stream);
+}
+
+size_t mla_decode_paged_fp8_workspace_size(int batch, int num_heads, int total_tokens, int num_splits)
+{
+    if (!mla::heads_ok(num_heads) || batch < 1 || total_tokens < 0)
+        return 0;
+    const mla::Plan p = mla::make_plan(false, num_heads, total_tokens, batch, true, num_splits,
+                                       mla::current_cu_count(), mla::CacheKind::kPagedF8);
+    return mla::partials_bytes(p, num_heads);
+}
+
+int mla_decode_paged_fp8_fp16(const void *query, const void *kv_cache_fp8, float cache_scale, const int *block_table,
+                              const int *cu_seqlens, void *out, void *workspace, size_t workspace_bytes, int batch,
+                              int num_heads, int total_tokens, int page_size, int num_pages, int block_table_stride,
+                              int num_splits, void *stream)
+{
+    return paged_decode(mla::Dtype::kF8Cache, query, kv_cache_fp8, block_table, cu_seqlens, out, workspace,
+                        workspace_bytes, batch, num_heads, total_tokens, page_size, num_pages,
+                        block_table_stride, num_splits, stream, cache_scale);
+}
+
+int mla_decode_paged_fp8_bf16(const void *query, const void *kv_cache_fp8, float cache_scale, const int *block_table,
+                              const int *cu_seqlens, void *out, void *workspace, size_t workspace_bytes, int batch,
+                              int num_heads, int total_tokens, int page_size, int num_pages, int block_table_stride,
+                              int num_splits, void *stream)
+{
+    return paged_decode(mla::Dtype::kF8CacheBF16, query, kv_cache_fp8, block_table, cu_seqlens, out, workspace,
+                        workspace_bytes, batch, num_heads, total_tokens, page_size, num_pages,
+                        block_table_stride, num_splits, stream, cache_scale);
 }
 
 size_t mla_decode_split_fp8_workspace_size(int batch, int num_heads, int total_tokens, int num_splits)

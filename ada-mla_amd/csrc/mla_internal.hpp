@@ -85,14 +85,14 @@ struct Problem {
     bool fp32;              // fp32 path (q, c, out fp32; unnormalised fp32 partials)
     bool bf16;              // 16-bit path: q, c, out (and the partial O) in bf16, not fp16
     Paging paging;          // c is a paged cache when paging.block_table != nullptr
-    bool fp8;               // c is OCP fp8 (E4M3FN) with per-tensor scale c_scale (q, out fp16)
+    bool fp8;               // c is OCP fp8 (E4M3FN) with per-tensor scale c_scale (q, out fp16, paged also bf16)
     float out_scale;        // multiplies the normalised partial O (c_scale for fp8, else 1)
 };
 
 // Layout of the cache the plan is for. kPaged: one extra block per piece in
-// the cost model (pieces start page-aligned). kF8: charged the same extra
-// block, a stand-in for the operand conversions that lengthen its steps.
-enum class CacheKind { kPacked, kPaged, kF8 };
+// the cost model (pieces start page-aligned). kF8: an fp8 cache (also tried with the
+// chunks that its halved stream allows); kPagedF8: both.
+enum class CacheKind { kPacked, kPaged, kF8, kPagedF8 };
 
 // CUs of the current device (cached per device); 256 if it cannot be queried.
 int current_cu_count();

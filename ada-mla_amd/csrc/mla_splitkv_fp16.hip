@@ -88,6 +88,45 @@ __device__ unsigned long long mla_timeline_stamps[kTimelineWorkgroups * 16];
 
 namespace {
 
+// Two values of E and E4M3 bytes: value(w, s) is the low (or high) two bytes of w
+// times s, bytes(a, b, s) the four bytes of a / s and b / s (to nearest even;
+// s a power of two).
+template <typename E>
+struct F8Pair;
+typedef short s16x2 __attribute__((ext_vector_type(2)));
+template <>
+struct F8Pair<_Float16> {
+    typedef half2v V;
+    template <bool kHigh>
+    static __device__ __forceinline__ V value(int w, float s, std::integral_constant<bool, kHigh>)
+    {
+        return __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, s, kHigh);
+    }
+    static __device__ __forceinline__ int bytes(V a, V b, float s)
+    {
+        // the first conversion writes the register's low half; the old value
+        // passed for the high half is overwritten by the second
+        s16x2 h = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(__builtin_bit_cast(s16x2, b), a, s, false);
+        h = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(h, b, s, true);
+        return __builtin_bit_cast(int, h);
+    }
+};
+template <>
+struct F8Pair<__bf16> {
+    typedef __bf16 V __attribute__((ext_vector_type(2)));
+    template <bool kHigh>
+    static __device__ __forceinline__ V value(int w, float s, std::integral_constant<bool, kHigh>)
+    {
+        return __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, kHigh);
+    }
+    static __device__ __forceinline__ int bytes(V a, V b, float s)
+    {
+        s16x2 h = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(__builtin_bit_cast(s16x2, b), a, s, false);
+        h = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(h, b, s, true);
+        return __builtin_bit_cast(int, h);
+    }
+};
+
 template <int HT>
 struct F16Tile {
     // kTen: 32-head tiles run 10 waves -- four 16-head S waves (head group,
@@ -131,12 +170,12 @@ struct F16Tile {
 
 // kF32Part: the partial O is stored in fp32 (still normalised) instead of E.
 // kF8: the cache C is OCP fp8 (E4M3FN) [tokens][576] bytes and c points to
-// it (E is then fp16 for Q* and P). The ring holds the fp8 bytes as loaded
+// it (E is the type of Q* and P: fp16, with a paged cache also bf16). The ring holds the fp8 bytes as loaded
 // (a block takes the first 18 KB of its slot; the load units are 512 bytes,
 // 32 lanes of a global->LDS load, except for the feeders' 1 KB units of
 // two rows), so a CU fills half the bytes of a 16-bit
-// cache; the S and O waves convert their operands to fp16 after each LDS
-// read, exactly (every E4M3 value is an fp16 value). The per-tensor cache
+// cache; the S and O waves convert their operands to E after each LDS
+// read, exactly (every E4M3 value is an fp16 and a bf16 value). The per-tensor cache
 // scale is folded into scale_log2 and out_scale.
 // kMode: kModeBatch (cu_seqlens: a chunk may hold pieces of several
 // sequences), kModeSingle (one sequence: the chunk is one piece, whose
@@ -184,7 +223,7 @@ void splitkv_fp16_kernel(const E *__restrict__ q,
     // fp8 N = 65536 29.9 against 30.5).
     constexpr bool kSharedRef = __is_same(E, __bf16) && HT >= 32;
     static_assert(kMode == kModeBatch || !kPaged, "a paged cache comes with cu_seqlens");
-    static_assert(!(kF8 && (kPaged || !__is_same(E, _Float16))), "fp8 cache: packed layout, fp16 query");
+    static_assert(!kF8 || kPaged || __is_same(E, _Float16), "a packed fp8 cache comes with fp16 queries");
     using E8 = typename Vec<E>::v8;
     using E4 = typename Vec<E>::v4;
     __shared__ __attribute__((aligned(1024))) E s_ring[T::kRing * T::kSlot];
@@ -317,8 +356,8 @@ void splitkv_fp16_kernel(const E *__restrict__ q,
     };
     // Global address of token t0 of sequence b (first token seq_lo), in two
     // steps so that a paged cache's block-table read can be issued early:
-    // page_of reads the page id (0 for the packed layout), src_at forms the
-    // address. The rows of a block that starts at t0 follow it contiguously
+    // page_of reads the page id (0 for the packed layout), row_at forms the
+    // cache row. The rows of a block that starts at t0 follow it contiguously
     // (same page).
     auto page_of = [&](int b, int seq_lo, int t0) -> int {
         if constexpr (kPaged) {
@@ -333,13 +372,13 @@ void splitkv_fp16_kernel(const E *__restrict__ q,
             return 0;
         }
     };
-    auto src_at = [&](int page, int seq_lo, int t0) -> const E * {
+    auto row_at = [&](int page, int seq_lo, int t0) -> size_t {
         if constexpr (kPaged) {
             page = min(max(page, 0), pg.num_pages - 1);
             const int l = t0 - seq_lo;
-            return c + (((size_t)page << pg.page_shift) + (l & ((1 << pg.page_shift) - 1))) * kDK;
+            return ((size_t)page << pg.page_shift) + (l & ((1 << pg.page_shift) - 1));
         } else {
-            return c + (size_t)t0 * kDK;
+            return (size_t)t0;
         }
     };
     // fp8 ring slot (first 18 KB of a slot): the 512-byte C_N part of row r
@@ -386,20 +425,20 @@ void splitkv_fp16_kernel(const E *__restrict__ q,
         global_to_lds16(base, min(rrow, lim) * kDK + kDV + 16 * ((ln & 3) ^ ((rrow >> 2) & 3)),
                         ring8 + slot * (T::kSlot * 2) + kF8Rope + 1024 * rr);
     };
-    // 8 fp8 values -> 8 fp16 values (byte k -> element k)
-    auto f8_to_f16 = [](uint2 v) -> half8 {
-        const half2v a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v.x, 1.0f, false);
-        const half2v b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v.x, 1.0f, true);
-        const half2v d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v.y, 1.0f, false);
-        const half2v e = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v.y, 1.0f, true);
-        return half8{a[0], a[1], b[0], b[1], d[0], d[1], e[0], e[1]};
+    // 8 fp8 values -> 8 values of E (byte k -> element k)
+    auto f8_to_e = [](uint2 v) -> E8 {
+        const auto a = F8Pair<E>::value(v.x, 1.0f, std::false_type{});
+        const auto b = F8Pair<E>::value(v.x, 1.0f, std::true_type{});
+        const auto d = F8Pair<E>::value(v.y, 1.0f, std::false_type{});
+        const auto e = F8Pair<E>::value(v.y, 1.0f, std::true_type{});
+        return E8{a[0], a[1], b[0], b[1], d[0], d[1], e[0], e[1]};
     };
     // a block's load units for either cache type: src is its first row
     auto block_src = [&](int page, int seq_lo, int t0) -> const void * {
         if constexpr (kF8)
-            return c8 + (size_t)t0 * kDK;
+            return c8 + row_at(page, seq_lo, t0) * kDK;
         else
-            return src_at(page, seq_lo, t0);
+            return c + row_at(page, seq_lo, t0) * kDK;
     };
     auto blk_row = [&](const void *src, int lim, int slot, int row) {
         if constexpr (kF8)
@@ -492,42 +531,36 @@ void splitkv_fp16_kernel(const E *__restrict__ q,
     // goes subnormal). The S waves accumulate the products with hi and with
     // lo separately, combine them as hi + lo / 16 and scale by 2^-e_h in the
     // softmax (s_qsc[h] = scale_log2 2^-e_h).
-    // 8 fp16 values -> 8 bytes of hi and of lo (byte k <- value k), two
+    // 8 values -> 8 bytes of hi and of lo (byte k <- value k), two
     // values per instruction: the scaled conversions compute fp8(v / s)
     // and fp8 * s (round to nearest even, checked on gfx950), so with
     // si = 2^-e and sl = 2^-(e+4):
-    //   hi = fp8(q / si),  r = q - hi * si (fp16, exact: hi * si is q
+    //   hi = fp8(q / si),  r = q - hi * si (exact in E: hi * si is q
     //   rounded to 4 significant bits, within a factor 2 of q),
     //   lo = fp8(r / sl) = fp8(16 (2^e q - hi)).
-    // kHalf: for heads whose largest |q| is 2^15 or more. Rounded to 4
-    // significant bits, an entry of 63488 or more becomes 65536, which fp16
+    // kHalf: for heads whose largest |q| is 2^15 or more (bf16: 2^127). Rounded to 4
+    // significant bits, an fp16 entry of 63488 or more becomes 65536, which fp16
     // cannot hold (hi * si would be inf), so such heads form the residual at
-    // half scale: r / 2 = q / 2 - hi * (si / 2), both terms exact in fp16
-    // (q / 2 loses nothing for |q| >= 2^-14, and smaller entries are below
+    // half scale: r / 2 = q / 2 - hi * (si / 2), both terms exact in E
+    // (fp16: q / 2 loses nothing for |q| >= 2^-14, and smaller entries are below
     // 2^-29 of the head's maximum), and lo = fp8((r / 2) / (sl / 2)).
-    auto q_split8 = [](half8 x, float si, float sl, uint2 &hi, uint2 &lo, auto kHalf) {
-        typedef short s16x2 __attribute__((ext_vector_type(2)));
+    auto q_split8 = [](E8 x, float si, float sl, uint2 &hi, uint2 &lo, auto kHalf) {
+        using P = F8Pair<E>;
         constexpr bool kH = decltype(kHalf)::value;
         const float sb = kH ? 0.5f * si : si, slb = kH ? 0.5f * sl : sl;
         unsigned hv[2], lv[2];
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
-            half2v q0 = half2v{x[4 * p], x[4 * p + 1]}, q1 = half2v{x[4 * p + 2], x[4 * p + 3]};
-            // (the first conversion of each register writes its low half; the
-            // old value passed for the high half is overwritten by the second)
-            s16x2 h = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(__builtin_bit_cast(s16x2, q1), q0, si, false);
-            h = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(h, q1, si, true);
-            const int hw = __builtin_bit_cast(int, h);
-            const half2v b0 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hw, sb, false);
-            const half2v b1 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hw, sb, true);
+            auto q0 = typename P::V{x[4 * p], x[4 * p + 1]}, q1 = typename P::V{x[4 * p + 2], x[4 * p + 3]};
+            const int hw = P::bytes(q0, q1, si);
+            const auto b0 = P::value(hw, sb, std::false_type{});
+            const auto b1 = P::value(hw, sb, std::true_type{});
             if constexpr (kH) {
-                q0 *= (_Float16)0.5f;
-                q1 *= (_Float16)0.5f;
+                q0 *= (E)0.5f;
+                q1 *= (E)0.5f;
             }
-            s16x2 l = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(__builtin_bit_cast(s16x2, q1), q0 - b0, slb, false);
-            l = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(l, q1 - b1, slb, true);
-            hv[p] = __builtin_bit_cast(unsigned, h);
-            lv[p] = __builtin_bit_cast(unsigned, l);
+            hv[p] = (unsigned)hw;
+            lv[p] = (unsigned)P::bytes(q0 - b0, q1 - b1, slb);
         }
         hi = uint2{hv[0], hv[1]};
         lo = uint2{lv[0], lv[1]};
@@ -556,18 +589,18 @@ void splitkv_fp16_kernel(const E *__restrict__ q,
         const int rr = h % 32;
         E *const qrow = s_ring + (T::kPre + h / 32) * T::kSlot + rr * kDV;
         E *const qrope = s_ring + (T::kPre + h / 32) * T::kSlot + T::kRope + rr * (kDK - kDV);
-        half8 v[kQCpl];
-        // max |q| over the lane's values: packed over the fp16 bit patterns
+        E8 v[kQCpl];
+        // max |q| over the lane's values: packed over the 16-bit patterns
         // with the sign cleared (their unsigned order is the order of |q|)
         typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
         u16x2 mb = {0, 0};
 #pragma unroll
         for (int i = 0; i < kQCpl; ++i) {
             const int ch = j + kQAct * i;
-            v[i] = half8{};
+            v[i] = E8{};
             if (j < kQAct)
-                v[i] = ch < 64 ? *(const half8 *)(qrow + 8 * (ch ^ row_swizzle(rr)))
-                               : *(const half8 *)(qrope + 8 * ((ch - 64) ^ rope_swizzle(rr)));
+                v[i] = ch < 64 ? *(const E8 *)(qrow + 8 * (ch ^ row_swizzle(rr)))
+                               : *(const E8 *)(qrope + 8 * ((ch - 64) ^ rope_swizzle(rr)));
             const uint4 u = __builtin_bit_cast(uint4, v[i]);
             mb = __builtin_elementwise_max(mb, __builtin_bit_cast(u16x2, u.x & 0x7fff7fffu));
             mb = __builtin_elementwise_max(mb, __builtin_bit_cast(u16x2, u.y & 0x7fff7fffu));
@@ -588,11 +621,15 @@ void splitkv_fp16_kernel(const E *__restrict__ q,
             const auto sw = __builtin_amdgcn_permlane16_swap(mi, mi, false, false);
             mi = max((int)sw[0], (int)sw[1]);
         }
-        const float amax = (float)__builtin_bit_cast(_Float16, (unsigned short)mi);
-        // amax = m 2^x, m in [0.5, 1): 2^(8 - x) amax in [128, 256)
-        const int e = 8 - __builtin_amdgcn_frexp_expf(amax);
+        const float amax = (float)__builtin_bit_cast(E, (unsigned short)mi);
+        // amax = m 2^x, m in [0.5, 1): 2^(8 - x) amax in [128, 256). A bf16 head below
+        // 2^-92 keeps e = 100, as the conversions take scales of normal exponents: what
+        // its logits lose is below 2^-99 of the cache's entries.
+        int e = 8 - __builtin_amdgcn_frexp_expf(amax);
+        if constexpr (__is_same(E, __bf16))
+            e = min(e, 100);
         const float si = __builtin_ldexpf(1.f, -e);
-        const bool big = amax >= 32768.f;  // the half-scale residual (q_split8)
+        const bool big = amax >= (__is_same(E, __bf16) ? 0x1p127f : 32768.f);  // the half-scale residual (q_split8)
         if (j == 0)
             s_qsc[h] = scale_log2 * si;
         unsigned char *const q8 = reinterpret_cast<unsigned char *>(qrow);
@@ -857,7 +894,7 @@ void splitkv_fp16_kernel(const E *__restrict__ q,
                     // and every MFMA for its operand)
                     E8 cv[2];
                     if constexpr (kF8)
-                        cv[0] = f8_to_f16(ab[0][0]);
+                        cv[0] = f8_to_e(ab[0][0]);
 #pragma unroll
                     for (int bi = 0; bi < kNB; ++bi) {
                         if (bi + 2 < kNB)
@@ -870,7 +907,7 @@ void splitkv_fp16_kernel(const E *__restrict__ q,
                                 const int j = bi * kB + k;  // K-step
                                 a = cv[j & 1];
                                 if (j + 1 < kDK / 32)
-                                    cv[(j + 1) & 1] = f8_to_f16(ab[((j + 1) / kB) % 3][(j + 1) % kB]);
+                                    cv[(j + 1) & 1] = f8_to_e(ab[((j + 1) / kB) % 3][(j + 1) % kB]);
                             } else {
                                 a = ab[bi % 3][k];
                             }
@@ -980,8 +1017,11 @@ void splitkv_fp16_kernel(const E *__restrict__ q,
                     // the partial's max is the O waves' reference (finite, at
                     // most kLazyRescale below the halves' maxima), so that m, l
                     // and O share one scale
-                    const float mr = s_mref[h];
+                    float mr = s_mref[h];
                     const float ls = s_l[0][h] * fast_exp2(s_m[0][m_at(h, 0)] - mr) + s_l[1][h] * fast_exp2(s_m[0][m_at(h, 1)] - mr);
+                    // a query with a NaN leaves its max at -inf, which the combine takes
+                    // for a piece without tokens: its sum, NaN, has to count
+                    mr = ls != ls ? 0.f : mr;
                     float *const mp = m_part + (size_t)slot_out * num_heads + head0 + h;
                     float *const lp = l_part + (size_t)slot_out * num_heads + head0 + h;
                     if (part_plain) {
@@ -1278,14 +1318,14 @@ void splitkv_fp16_kernel(const E *__restrict__ q,
                         // register sets (as in the S waves)
                         E8 cva[2];
                         if constexpr (kF8)
-                            cva[0] = f8_to_f16(av[0]);
+                            cva[0] = f8_to_e(av[0]);
 #pragma unroll
                         for (int dt = 0; dt < 8; ++dt) {
                             E8 a;
                             if constexpr (kF8) {
                                 a = cva[dt & 1];
                                 if (dt + 1 < 8)
-                                    cva[(dt + 1) & 1] = f8_to_f16(av[dt + 1]);
+                                    cva[(dt + 1) & 1] = f8_to_e(av[dt + 1]);
                             } else {
                                 a = av[dt];
                             }
@@ -1476,6 +1516,11 @@ hipError_t launch_splitkv_fp16(const Problem &pb, const Plan &p, const Partials 
                         : launch_tiles<false, _Float16, false, false, false>(pb, p, w, s);
     }
     if (!tr_load || f32_part)
+        return hipErrorInvalidValue;
+    if (pb.fp8 && pb.paging.block_table)
+        return pb.bf16 ? launch_tiles<true, __bf16, true, false, true>(pb, p, w, s)
+                       : launch_tiles<true, _Float16, true, false, true>(pb, p, w, s);
+    if (pb.fp8 && pb.bf16)
         return hipErrorInvalidValue;
     if (pb.fp8)  // fp16 query, fp8 cache, fp16 partials
         return single ? launch_tiles<true, _Float16, false, false, true, kModeSingle>(pb, p, w, s)

@@ -281,6 +281,28 @@ int mla_decode_paged_bf16(const void *query, const void *kv_cache,
                           int block_table_stride, int num_splits,
                           void *stream);
 
+/* mla_decode_paged_* over a paged cache of OCP fp8 E4M3FN bytes that hold
+ * C / cache_scale (a per-tensor scale > 0), as mla_append_kv_* writes it with
+ * MLA_FLAG_FP8_CACHE: query and out in fp16 or bf16, everything else as there.
+ * The cache is read at one byte per value; every E4M3FN value is a value of the
+ * query's type, so the products see the cache as it stands. */
+size_t mla_decode_paged_fp8_workspace_size(int batch, int num_heads,
+                                           int total_tokens, int num_splits);
+int mla_decode_paged_fp8_fp16(const void *query, const void *kv_cache_fp8,
+                              float cache_scale, const int *block_table,
+                              const int *cu_seqlens, void *out, void *workspace,
+                              size_t workspace_bytes, int batch, int num_heads,
+                              int total_tokens, int page_size, int num_pages,
+                              int block_table_stride, int num_splits,
+                              void *stream);
+int mla_decode_paged_fp8_bf16(const void *query, const void *kv_cache_fp8,
+                              float cache_scale, const int *block_table,
+                              const int *cu_seqlens, void *out, void *workspace,
+                              size_t workspace_bytes, int batch, int num_heads,
+                              int total_tokens, int page_size, int num_pages,
+                              int block_table_stride, int num_splits,
+                              void *stream);
+
 /* fp8 KV cache (no reference counterpart: the reference lists it as future
  * work, README.md:408): query [.. x num_heads x 576] fp16, cache
  * [tokens x 576] OCP fp8 E4M3FN bytes holding C / cache_scale (a per-tensor
