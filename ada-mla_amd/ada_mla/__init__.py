@@ -16,6 +16,11 @@ and what a serving loop runs around it on the paged cache:
     q_rope = ada_mla.mla_append_kv(kv, norm_weight, cos_sin, positions, slots, kv_pages, q_rope=q_rope)
     o = ada_mla.mla_prefill(q_nope, q_rope, w_uk, w_uv, kv_pages, cu_new, cu, block_table=block_table)
     out = ada_mla.mla_decode_tree(q, kv_pages, block_table, cu, tree_mask)  # drafted tokens
+    block_table, lens, copies, free = ada_mla.mla_fork_tables(  # requests copied, reordered, rolled back, ended
+        block_table, lens, parents, free_pages, free, page_size, num_pages, kept_lens=kept_lens)
+    block_table, copies, free_pages = ada_mla.mla_compact_tables(  # used pages to the lowest ids
+        block_table, lens, free_pages, free, page_size, num_pages)
+    ada_mla.mla_copy_pages(kv_pages, copies)               # what either asks for
 
 The functions live in the compiled extension ``ada_mla._C`` (built by
 ada-mla_amd/build.py), which calls the HIP library through its C ABI
@@ -28,11 +33,11 @@ import importlib
 
 __all__ = ["mla_decode_split", "mla_decode_fused", "mla_decode_split_batched", "mla_decode_paged",
            "mla_absorb_query", "mla_project_output", "mla_paged_tables", "mla_append_kv", "mla_decode_tree",
-           "mla_prefill", "HEAD_DIM_C", "HEAD_DIM_ROPE", "HEAD_DIM_K", "extension"]
+           "mla_prefill", "mla_fork_tables", "mla_compact_tables", "mla_copy_pages", "HEAD_DIM_C", "HEAD_DIM_ROPE", "HEAD_DIM_K", "extension"]
 
 _EXPORTS = {"mla_decode_split", "mla_decode_fused", "mla_decode_split_batched", "mla_decode_paged",
             "mla_absorb_query", "mla_project_output", "mla_paged_tables", "mla_append_kv", "mla_decode_tree",
-           "mla_prefill", "HEAD_DIM_C", "HEAD_DIM_ROPE", "HEAD_DIM_K"}
+           "mla_prefill", "mla_fork_tables", "mla_compact_tables", "mla_copy_pages", "HEAD_DIM_C", "HEAD_DIM_ROPE", "HEAD_DIM_K"}
 
 
 def extension():

@@ -67,6 +67,10 @@ _SIGNATURES = {
     "mla_decode_paged_fp8_fp16": (_i, [_vp, _vp, _f] + [_vp] * 4 + [_sz] + [_i] * 7 + [_vp]),
     "mla_decode_paged_fp8_bf16": (_i, [_vp, _vp, _f] + [_vp] * 4 + [_sz] + [_i] * 7 + [_vp]),
     "mla_paged_tables": (_i, [_vp] * 10 + [_i] * 5 + [_vp]),
+    "mla_page_tables_workspace_size": (_sz, [_i]),
+    "mla_fork_tables": (_i, [_vp] * 12 + [_sz] + [_i] * 6 + [_vp]),
+    "mla_compact_tables": (_i, [_vp] * 9 + [_sz] + [_i] * 5 + [_vp]),
+    "mla_copy_pages": (_i, [_vp, _vp] + [_i] * 5 + [_vp]),
     "mla_append_kv_fp16": (_i, [_vp] * 8 + [_f, _f, _i, _i, _i, _ll, _ll, _ll, _ll, _u, _vp]),
     "mla_append_kv_bf16": (_i, [_vp] * 8 + [_f, _f, _i, _i, _i, _ll, _ll, _ll, _ll, _u, _vp]),
     "mla_decode_tree_workspace_size": (_sz, [_i] * 5),
@@ -343,6 +347,63 @@ def paged_tables(context_lens, new_lens, block_table, free_pages, free_start, pa
                                 _ptr(free_next), b, total_new, free_pages.shape[0], page_size, block_table.shape[1],
                                 _stream(context_lens)))
     return cu_seqlens, cu_new, slots, positions, free_next
+
+
+def fork_tables(block_table, lens, parents, free_pages, free_start, page_size: int, num_pages: int, kept_lens=None,
+                pinned=None, workspace=None):
+    """mla_fork_tables: int32 device tensors block_table [R, max_pages], lens [R], parents [B], free_pages [F]
+    (written in place), free_start [1], kept_lens [B] or None, pinned [num_pages] or None -> (block_table
+    [B, max_pages], lens [B], copies [B, 3], free_next [1])."""
+    import torch
+    lib = load()
+    for t in (block_table, lens, parents, free_pages, free_start, kept_lens, pinned):
+        assert t is None or (t.dtype == torch.int32 and t.is_contiguous())
+    (rows, width), b = block_table.shape, parents.shape[0]
+    assert lens.shape == (rows,) and free_start.shape == (1,) and (kept_lens is None or kept_lens.shape == (b,))
+    assert pinned is None or pinned.shape == (num_pages,)
+    i32 = dict(dtype=torch.int32, device=block_table.device)
+    table, new_lens, copies, nxt = (torch.empty(s, **i32) for s in ((b, width), (b,), (b, 3), (1,)))
+    ws_bytes = lib.mla_page_tables_workspace_size(num_pages)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=block_table.device) if workspace is None else workspace
+    _check("mla_fork_tables",
+           lib.mla_fork_tables(_ptr(block_table), _ptr(lens), _ptr(parents), _ptr(kept_lens), _ptr(pinned),
+                               _ptr(free_pages), _ptr(free_start), _ptr(table), _ptr(new_lens), _ptr(copies), _ptr(nxt),
+                               _ptr(ws), ws.numel(), rows, b, num_pages, free_pages.shape[0], page_size, width,
+                               _stream(block_table)))
+    return table, new_lens, copies, nxt
+
+
+def compact_tables(block_table, lens, free_pages, free_start, page_size: int, num_pages: int, pinned=None,
+                   workspace=None):
+    """mla_compact_tables: int32 device tensors as for fork_tables -> (block_table, copies [min(F, num_pages // 2), 3],
+    free_pages)."""
+    import torch
+    lib = load()
+    for t in (block_table, lens, free_pages, free_start, pinned):
+        assert t is None or (t.dtype == torch.int32 and t.is_contiguous())
+    rows, width = block_table.shape
+    assert lens.shape == (rows,) and free_start.shape == (1,) and (pinned is None or pinned.shape == (num_pages,))
+    table, new_free = torch.empty_like(block_table), torch.empty_like(free_pages)
+    copies = torch.empty((min(free_pages.shape[0], num_pages // 2), 3), dtype=torch.int32, device=block_table.device)
+    ws_bytes = lib.mla_page_tables_workspace_size(num_pages)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=block_table.device) if workspace is None else workspace
+    _check("mla_compact_tables",
+           lib.mla_compact_tables(_ptr(block_table), _ptr(lens), _ptr(pinned), _ptr(free_pages), _ptr(free_start),
+                                  _ptr(table), _ptr(copies), _ptr(new_free), _ptr(ws), ws.numel(), rows, num_pages,
+                                  free_pages.shape[0], page_size, width, _stream(block_table)))
+    return table, copies, new_free
+
+
+def copy_pages(kv_cache, copies):
+    """mla_copy_pages: kv_cache [num_pages, page_size, 576] or [layers, num_pages, page_size, 576], written in place;
+    copies [n, 3] int32 (page, page, rows)."""
+    import torch
+    lib = load()
+    assert kv_cache.is_contiguous() and kv_cache.shape[-1] == HEAD_DIM_K and kv_cache.dim() in (3, 4)
+    assert copies.dtype == torch.int32 and copies.is_contiguous() and copies.shape[1] == 3
+    layers = kv_cache.shape[0] if kv_cache.dim() == 4 else 1
+    _check("mla_copy_pages", lib.mla_copy_pages(_ptr(kv_cache), _ptr(copies), copies.shape[0], layers, kv_cache.shape[-3],
+                                                kv_cache.shape[-2], kv_cache.element_size(), _stream(kv_cache)))
 
 
 def append_kv(kv, norm_weight, cos_sin, positions, slots, kv_cache, q_rope=None, eps: float = 1e-6,

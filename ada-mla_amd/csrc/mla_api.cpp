@@ -446,6 +446,118 @@ std::vector<at::Tensor> paged_tables(const at::Tensor &context_in, const at::Ten
     return {cu_seqlens, cu_new, slots, positions, free_next};
 }
 
+// What fork and compaction check of a table and its pool.
+void check_pool(const at::Tensor &table, const at::Tensor &lens, const at::Tensor &free_pages, const at::Tensor &free_start,
+                const c10::optional<at::Tensor> &pinned, int64_t page_size, int64_t num_pages, const char *fn)
+{
+    check_int32(table, 2, fn, "block_table");
+    check_int32(lens, 1, fn, "lens");
+    check_int32(free_pages, 1, fn, "free_pages");
+    check_int32(free_start, 1, fn, "free_start");
+    TORCH_CHECK(table.size(0) >= 1 && table.size(0) <= 8192 && lens.size(0) == table.size(0), fn,
+                ": lens and block_table must have one entry or row per request, 8192 at most");
+    TORCH_CHECK(table.size(1) >= 1 && table.size(1) <= INT32_MAX, fn, ": block_table needs at least one column");
+    TORCH_CHECK(free_pages.size(0) <= INT32_MAX, fn, ": too many free pages");
+    TORCH_CHECK(free_start.size(0) == 1, fn, ": free_start must have one entry");
+    check_page_size(page_size, fn);
+    TORCH_CHECK(num_pages >= 1 && num_pages <= (1 << 18), fn, ": num_pages must be 1 to 2^18, got ", num_pages);
+    if (pinned) {
+        check_int32(*pinned, 1, fn, "pinned");
+        TORCH_CHECK(pinned->size(0) == num_pages, fn, ": pinned must have one entry per page");
+    }
+    check_devices({&table, &lens, &free_pages, &free_start, pinned ? &*pinned : &table}, fn);
+}
+
+// No reference counterpart: rows of a block table taken over from others.
+std::vector<at::Tensor> fork_tables(const at::Tensor &table_in, const at::Tensor &lens_in, const at::Tensor &parents_in,
+                                    at::Tensor free_pages, const at::Tensor &free_start, int64_t page_size,
+                                    int64_t num_pages, const c10::optional<at::Tensor> &kept_in,
+                                    const c10::optional<at::Tensor> &pinned_in)
+{
+    const char *fn = "mla_fork_tables";
+    check_int32(parents_in, 1, fn, "parents");
+    const int64_t batch = parents_in.size(0);
+    TORCH_CHECK(batch >= 1 && batch <= INT32_MAX / 4, fn, ": parents must have at least one entry");
+    if (kept_in) {
+        check_int32(*kept_in, 1, fn, "kept_lens");
+        TORCH_CHECK(kept_in->size(0) == batch, fn, ": kept_lens must have one entry per parent");
+    }
+    TORCH_CHECK(free_pages.is_contiguous(), fn, ": free_pages must be contiguous (it is written in place)");
+    check_pool(table_in, lens_in, free_pages, free_start, pinned_in, page_size, num_pages, fn);
+    check_devices({&table_in, &parents_in, kept_in ? &*kept_in : &table_in}, fn);
+    const at::OptionalDeviceGuard guard(table_in.device());
+    const at::Tensor table = table_in.contiguous(), lens = lens_in.contiguous(), parents = parents_in.contiguous();
+    const at::Tensor kept = kept_in ? kept_in->contiguous() : at::Tensor();
+    const at::Tensor pinned = pinned_in ? pinned_in->contiguous() : at::Tensor();
+    const int64_t width = table.size(1);
+    // the outputs and the workspace share one allocation, each from a multiple of 16 bytes on
+    auto up = [](int64_t n) { return static_cast<size_t>((n + 15) / 16 * 16); };
+    const size_t ws_bytes = mla_page_tables_workspace_size(static_cast<int>(num_pages));
+    const size_t at_lens = up(4 * batch * width), at_copies = at_lens + up(4 * batch), at_next = at_copies + up(12 * batch);
+    const at::Tensor all = workspace(at_next + 16, table), ws = workspace(ws_bytes, table);
+    at::Tensor new_table = part_of(all, 0, batch * width, at::kInt).view({batch, width});
+    at::Tensor new_lens = part_of(all, at_lens, batch, at::kInt);
+    at::Tensor copies = part_of(all, at_copies, 3 * batch, at::kInt).view({batch, 3});
+    at::Tensor free_next = part_of(all, at_next, 1, at::kInt);
+    check_status(mla_fork_tables(table.data_ptr<int>(), lens.data_ptr<int>(), parents.data_ptr<int>(),
+                                 kept_in ? kept.data_ptr<int>() : nullptr, pinned_in ? pinned.data_ptr<int>() : nullptr,
+                                 free_pages.data_ptr<int>(), free_start.data_ptr<int>(), new_table.data_ptr<int>(),
+                                 new_lens.data_ptr<int>(), copies.data_ptr<int>(), free_next.data_ptr<int>(), ws.data_ptr(),
+                                 ws_bytes, static_cast<int>(table.size(0)), static_cast<int>(batch),
+                                 static_cast<int>(num_pages), static_cast<int>(free_pages.size(0)),
+                                 static_cast<int>(page_size), static_cast<int>(width), stream_of(table)),
+                 fn);
+    return {new_table, new_lens, copies, free_next};
+}
+
+// No reference counterpart: a pool's used pages moved to its lowest ids.
+std::vector<at::Tensor> compact_tables(const at::Tensor &table_in, const at::Tensor &lens_in, const at::Tensor &free_in,
+                                       const at::Tensor &free_start, int64_t page_size, int64_t num_pages,
+                                       const c10::optional<at::Tensor> &pinned_in)
+{
+    const char *fn = "mla_compact_tables";
+    check_pool(table_in, lens_in, free_in, free_start, pinned_in, page_size, num_pages, fn);
+    const at::OptionalDeviceGuard guard(table_in.device());
+    const at::Tensor table = table_in.contiguous(), lens = lens_in.contiguous(), free_pages = free_in.contiguous();
+    const at::Tensor pinned = pinned_in ? pinned_in->contiguous() : at::Tensor();
+    const int64_t num_free = free_pages.size(0), moves = std::min(num_free, num_pages / 2);
+    at::Tensor new_table = at::empty(table.sizes(), table.options()), copies = at::empty({moves, 3}, table.options());
+    at::Tensor new_free = at::empty({num_free}, table.options());
+    const size_t ws_bytes = mla_page_tables_workspace_size(static_cast<int>(num_pages));
+    const at::Tensor ws = workspace(ws_bytes, table);
+    check_status(mla_compact_tables(table.data_ptr<int>(), lens.data_ptr<int>(), pinned_in ? pinned.data_ptr<int>() : nullptr,
+                                    free_pages.data_ptr<int>(), free_start.data_ptr<int>(), new_table.data_ptr<int>(),
+                                    copies.data_ptr<int>(), new_free.data_ptr<int>(), ws.data_ptr(), ws_bytes,
+                                    static_cast<int>(table.size(0)), static_cast<int>(num_pages),
+                                    static_cast<int>(num_free), static_cast<int>(page_size),
+                                    static_cast<int>(table.size(1)), stream_of(table)),
+                 fn);
+    return {new_table, copies, new_free};
+}
+
+// No reference counterpart: the copies that either asks for, in every layer's cache.
+void copy_pages(at::Tensor kv_cache, const at::Tensor &copies_in)
+{
+    const char *fn = "mla_copy_pages";
+    TORCH_CHECK((kv_cache.dim() == 3 || kv_cache.dim() == 4) && kv_cache.size(-1) == MLA_HEAD_DIM_K && kv_cache.numel() > 0,
+                fn, ": kv_cache must be [num_pages, page_size, ", MLA_HEAD_DIM_K, "] or [layers, num_pages, page_size, ",
+                MLA_HEAD_DIM_K, "], got ", kv_cache.sizes());
+    TORCH_CHECK(kv_cache.is_contiguous(), fn, ": kv_cache must be contiguous (it is written in place)");
+    const int64_t size = kv_cache.element_size(), layers = kv_cache.dim() == 4 ? kv_cache.size(0) : 1;
+    TORCH_CHECK(size == 1 || size == 2 || size == 4, fn, ": kv_cache must have elements of 1, 2 or 4 bytes");
+    check_page_size(kv_cache.size(-2), fn);
+    TORCH_CHECK(layers <= INT32_MAX && kv_cache.size(-3) <= INT32_MAX, fn, ": too many pages or layers");
+    check_int32(copies_in, 2, fn, "copies");
+    TORCH_CHECK(copies_in.size(1) == 3 && copies_in.size(0) <= INT32_MAX / 4, fn, ": copies must be [n, 3]");
+    check_devices({&kv_cache, &copies_in}, fn);
+    const at::OptionalDeviceGuard guard(kv_cache.device());
+    const at::Tensor copies = copies_in.contiguous();
+    check_status(mla_copy_pages(kv_cache.data_ptr(), copies.data_ptr<int>(), static_cast<int>(copies.size(0)),
+                                static_cast<int>(layers), static_cast<int>(kv_cache.size(-3)),
+                                static_cast<int>(kv_cache.size(-2)), static_cast<int>(size), stream_of(kv_cache)),
+                 fn);
+}
+
 // No reference counterpart: a step's latent rows normalised, rotated and
 // written to their slots of the cache, its queries' rotary parts rotated.
 c10::optional<at::Tensor> mla_append_kv(const at::Tensor &kv_in, const at::Tensor &weight_in,
@@ -668,6 +780,23 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
           pybind11::arg("context_lens"), pybind11::arg("new_lens"), pybind11::arg("block_table"),
           pybind11::arg("free_pages"), pybind11::arg("free_start"), pybind11::arg("page_size"),
           pybind11::arg("total_new"));
+    m.def("mla_fork_tables", &fork_tables,
+          "(block_table [B,max_pages], lens [B], copies [B,3], free_next [1]): row b holds the first kept_lens[b] tokens "
+          "(None: all) of row parents[b] of block_table (lens [R]); whole pages are shared, a last page that another row "
+          "goes on writing is copied (copies: page, page taken, rows; for mla_copy_pages), pages that no row holds any "
+          "more are pushed to free_pages in place, below free_start[0]. pinned [num_pages]: pages that others hold",
+          pybind11::arg("block_table"), pybind11::arg("lens"), pybind11::arg("parents"), pybind11::arg("free_pages"),
+          pybind11::arg("free_start"), pybind11::arg("page_size"), pybind11::arg("num_pages"),
+          pybind11::arg("kept_lens") = pybind11::none(), pybind11::arg("pinned") = pybind11::none());
+    m.def("mla_compact_tables", &compact_tables,
+          "(block_table, copies [n,3], free_pages): the highest used pages that are not pinned moved to the lowest free "
+          "ids (free_pages from free_start[0] on), as long as those are lower; copies for mla_copy_pages",
+          pybind11::arg("block_table"), pybind11::arg("lens"), pybind11::arg("free_pages"), pybind11::arg("free_start"),
+          pybind11::arg("page_size"), pybind11::arg("num_pages"), pybind11::arg("pinned") = pybind11::none());
+    m.def("mla_copy_pages", &copy_pages,
+          "the first copies[i][2] rows of page copies[i][0] of kv_cache [pages,page_size,576] or "
+          "[layers,pages,page_size,576] to page copies[i][1], in place (copies [n,3] int32; ids out of range: nothing)",
+          pybind11::arg("kv_cache"), pybind11::arg("copies"));
     m.def("mla_append_kv", &mla_append_kv,
           "latent rows kv [T,576] RMS-normalised (first 512 values, norm_weight [512]) and rotated (last 64, "
           "cos_sin [P,64] float32 at positions [T] int32), written to rows slots [T] int64 of kv_cache in place "

@@ -5,8 +5,8 @@
  *
  * with Q* [num_heads x 576], the latent cache C [N x 576] (first 512 columns
  * are C_N, the last 64 the rope part) and O* [num_heads x 512], and of what a
- * serving loop runs around it on a paged cache: block tables, cache rows,
- * prompts, drafted tokens.
+ * serving loop runs around it on a paged cache: block tables, shared pages,
+ * cache rows, prompts, drafted tokens.
  *
  * This is the drop-in boundary below the PyTorch extension: the reference's
  * extension (csrc/mla_api.cpp) calls raw-pointer launchers declared in
@@ -391,6 +391,67 @@ int mla_paged_tables(const int *context_lens, const int *new_lens,
                      long long *slots, int *positions, int *free_next,
                      int batch, int total_new, int num_free, int page_size,
                      int block_table_stride, void *stream);
+
+/* Rows of a block table taken over from others: requests sampled several times,
+ * beams reordered, drafts rolled back, requests ended (no reference
+ * counterpart). All pointers are on the device and aligned to their type.
+ *
+ * Row b of new_table [batch][block_table_stride] holds the first kept_lens[b]
+ * tokens (NULL: all; clamped to 0 and what is there) of row parents[b] of
+ * block_table [rows][block_table_stride], whose rows hold lens [rows] tokens
+ * (clamped to 0 and the columns' room); a parent outside [0, rows) makes
+ * an empty row. new_lens [batch] gets the tokens, columns behind a row's
+ * last page -1. Rows share their whole pages. Of the rows that end inside a page the
+ * lowest goes on writing it, if no new row holds the page whole and pinned
+ * ([num_pages], NULL: none) is not positive for it; every other one takes
+ * the next page of the free list, row after row, and copies [batch][3] gets
+ * (page, page taken, rows to copy); (-1, -1, 0) for the other rows.
+ * Pages that a row of block_table holds, no row of new_table holds and that
+ * are not pinned are pushed to the free list before: with f of them,
+ * free_pages [num_free] gets their ids, lowest first, from index
+ * *free_start - f on, and pages are taken from there on. free_next gets
+ * *free_start - f + pages taken. Where the list ends (below 0 or at num_free) nothing is
+ * written, and a page taken is -1. Ids outside [0, num_pages) are passed on
+ * and neither freed nor copied. pinned marks pages that others hold, a prompt
+ * cache or another table. rows is at most 8192, num_pages at most 2^18,
+ * page_size a power of two from 32 to 2^20. new_table, new_lens and
+ * free_next must not be their inputs. One launch. */
+size_t mla_page_tables_workspace_size(int num_pages);
+int mla_fork_tables(const int *block_table, const int *lens,
+                    const int *parents, const int *kept_lens,
+                    const int *pinned, int *free_pages, const int *free_start,
+                    int *new_table, int *new_lens, int *copies, int *free_next,
+                    void *workspace, size_t workspace_bytes, int rows,
+                    int batch, int num_pages, int num_free, int page_size,
+                    int block_table_stride, void *stream);
+
+/* The used pages of a pool moved to its lowest ids, so that its tail can be given
+ * back (no reference counterpart). Of the pages that a row of block_table
+ * holds (not pinned) and the ids of free_pages [num_free] from *free_start on
+ * (not held, not pinned, each counted once), the k-th highest held one moves to the
+ * k-th lowest free one as long as that is lower: copies
+ * [min(num_free, num_pages / 2)][3] gets (from, to, page_size) in that order,
+ * (-1, -1, 0) behind the last move. new_table gets block_table with every page
+ * where it went (columns behind a row's last page: -1), new_free_pages the
+ * free ids in ascending order from *free_start on, -1 elsewhere. Workspace,
+ * limits and other conditions as for mla_fork_tables. Two launches. */
+int mla_compact_tables(const int *block_table, const int *lens,
+                       const int *pinned, const int *free_pages,
+                       const int *free_start, int *new_table, int *copies,
+                       int *new_free_pages, void *workspace,
+                       size_t workspace_bytes, int rows, int num_pages,
+                       int num_free, int page_size, int block_table_stride,
+                       void *stream);
+
+/* The rows that mla_fork_tables and mla_compact_tables ask for: in each of
+ * `layers` caches [num_pages][page_size][576] back to back, of elements of
+ * 1, 2 or 4 bytes, the first copies[i][2] rows of page copies[i][0] go to page
+ * copies[i][1]. Entries with an id outside [0, num_pages) or no rows copy
+ * nothing, more rows than page_size are page_size. A page must not be copied to twice,
+ * nor both to and from (the tables above never ask for that). One launch. */
+int mla_copy_pages(void *kv_cache, const int *copies, int count, int layers,
+                   int num_pages, int page_size, int element_size,
+                   void *stream);
 
 /* A step's latent rows into the cache, and its queries' rotary parts (no
  * reference counterpart; the reference's cache comes ready made). Token t:

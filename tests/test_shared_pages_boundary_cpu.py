@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from ada_mla import capi
+from pages_reference import compact, fork
 from test_operators_boundary_cpu import FAKE, _caller, _ext
 
 
@@ -44,3 +45,83 @@ def test_extension_refusals_paged_fp8():
                      (dict(query=h(2, 16, 576).bfloat16()), "GPU tensors")):
         with pytest.raises(RuntimeError, match=msg):
             m.mla_decode_paged(**{**ok, **bad})
+
+
+def test_fork_argument_errors():
+    names = ("table lens parents kept pinned free start new new_lens copies next ws wsb rows batch pages num_free page "
+             "stride stream")
+    ok = {n: FAKE + 64 * i for i, n in enumerate(names.split())} | dict(
+        wsb=1 << 30, rows=4, batch=4, pages=100, num_free=10, page=64, stride=4, stream=None)
+    call = _caller("mla_fork_tables", names, ok)
+    for bad in (dict(table=None), dict(lens=None), dict(parents=None), dict(free=None), dict(start=None), dict(new=None),
+                dict(new_lens=None), dict(copies=None), dict(next=None), dict(ws=None), dict(rows=0), dict(rows=8193),
+                dict(batch=0), dict(batch=2 ** 31 - 1), dict(pages=0), dict(pages=2 ** 18 + 1), dict(num_free=-1),
+                dict(page=16), dict(page=48), dict(page=1 << 21), dict(stride=0), dict(new=ok["table"]),
+                dict(new_lens=ok["lens"]), dict(next=ok["start"])):
+        assert call(**bad) == capi.STATUS_INVALID_VALUE, bad
+    assert call(ws=FAKE + 4) == capi.STATUS_MISALIGNED
+    assert call(wsb=399) == capi.STATUS_WORKSPACE_TOO_SMALL
+
+
+def test_compact_argument_errors():
+    names = "table lens pinned free start new copies new_free ws wsb rows pages num_free page stride stream"
+    ok = {n: FAKE + 64 * i for i, n in enumerate(names.split())} | dict(
+        wsb=1 << 30, rows=4, pages=100, num_free=10, page=64, stride=4, stream=None)
+    call = _caller("mla_compact_tables", names, ok)
+    for bad in (dict(table=None), dict(lens=None), dict(free=None), dict(start=None), dict(new=None), dict(copies=None),
+                dict(new_free=None), dict(ws=None), dict(rows=0), dict(rows=8193), dict(pages=0), dict(pages=2 ** 18 + 1),
+                dict(num_free=-1), dict(page=16), dict(page=48), dict(stride=0), dict(new=ok["table"]),
+                dict(new_free=ok["free"])):
+        assert call(**bad) == capi.STATUS_INVALID_VALUE, bad
+    assert call(ws=FAKE + 4) == capi.STATUS_MISALIGNED
+    assert call(wsb=399) == capi.STATUS_WORKSPACE_TOO_SMALL
+    size = capi.load().mla_page_tables_workspace_size
+    assert size(0) == size(2 ** 18 + 1) == 0 and size(1) >= 12 and size(2 ** 18) >= 4 * 2 ** 18 + 8
+
+
+def test_copy_argument_errors():
+    names = "cache copies count layers pages page size stream"
+    ok = dict(cache=FAKE, copies=FAKE, count=3, layers=1, pages=10, page=64, size=2, stream=None)
+    call = _caller("mla_copy_pages", names, ok)
+    for bad in (dict(cache=None), dict(copies=None), dict(count=-1), dict(layers=0), dict(pages=0), dict(page=16),
+                dict(page=96), dict(size=3), dict(size=8)):
+        assert call(**bad) == capi.STATUS_INVALID_VALUE, bad
+    assert call(cache=FAKE + 8) == capi.STATUS_MISALIGNED
+    assert call(count=0, copies=None) == capi.STATUS_SUCCESS
+
+
+def test_extension_refusals_pages():
+    m = _ext()
+    i = lambda *s: torch.zeros(*s, dtype=torch.int32)  # noqa: E731
+    pool = dict(block_table=i(2, 3), lens=i(2), free_pages=i(4), free_start=i(1), page_size=32, num_pages=9)
+    for bad, msg in ((dict(block_table=i(2, 3).long()), "block_table must be"), (dict(block_table=i(2, 0)), "one column"),
+                     (dict(lens=i(3)), "per request"), (dict(lens=i(2).long()), "lens must be"),
+                     (dict(free_pages=i(4, 1)), "free_pages must be"), (dict(free_start=i(2)), "one entry"),
+                     (dict(page_size=48), "power of two"), (dict(num_pages=0), "2\\^18"), (dict(num_pages=2 ** 18 + 1), "2\\^18"),
+                     (dict(pinned=i(8)), "per page"), (dict(pinned=i(9).bool()), "pinned must be"),
+                     (dict(block_table=i(8193, 3), lens=i(8193)), "8192"), (dict(), "GPU tensors")):
+        with pytest.raises(RuntimeError, match=msg):
+            m.mla_compact_tables(**{**pool, **bad})
+        with pytest.raises(RuntimeError, match=msg):
+            m.mla_fork_tables(**{**pool, "parents": i(5), **bad})
+    for bad, msg in ((dict(parents=i(0)), "at least one"), (dict(parents=i(5).long()), "parents must be"),
+                     (dict(kept_lens=i(4)), "per parent"), (dict(free_pages=i(8)[::2]), "contiguous")):
+        with pytest.raises(RuntimeError, match=msg):
+            m.mla_fork_tables(**{**pool, "parents": i(5), **bad})
+    h = lambda *s: torch.zeros(*s, dtype=torch.float16)  # noqa: E731
+    for cache, copies, msg in ((h(4, 64, 512), i(3, 3), "kv_cache must be"), (h(4, 576), i(3, 3), "kv_cache must be"),
+                               (h(0, 64, 576), i(3, 3), "kv_cache must be"), (h(4, 48, 576), i(3, 3), "power of two"),
+                               (h(4, 64, 1152)[..., :576], i(3, 3), "contiguous"),
+                               (h(4, 64, 576).double(), i(3, 3), "1, 2 or 4"), (h(4, 64, 576), i(3, 2), "copies must be"),
+                               (h(4, 64, 576), i(3, 3).long(), "copies must be"), (h(4, 64, 576), i(3, 3), "GPU tensors")):
+        with pytest.raises(RuntimeError, match=msg):
+            m.mla_copy_pages(cache, copies)
+
+
+def test_pages_oracle_on_small_cases():
+    # two rows share page 4; the first ends, the second is rolled back into its second page and forked
+    t, lens, copies, nxt, free = fork([[4, 1], [4, 7]], [40, 64], [1, 1], [50, 50], [0] * 9, [-1, -1, -1, 8], 3, 32, 9)
+    assert t == [[4, 7], [4, 1]] and lens == [50, 50] and copies == [[-1, -1, 0], [7, 1, 18]]
+    assert nxt == 3 - 1 + 1 and free == [-1, -1, 1, 8]
+    t, copies, free = compact([[8, 2], [5, -1]], [64, 3], [0] * 9, [-1, 0, 7, 3], 1, 32, 9)
+    assert copies[:2] == [[8, 0, 32], [5, 3, 32]] and t == [[0, 2], [3, -1]] and free == [-1, 5, 7, 8]
