@@ -8,6 +8,8 @@ reference's ``ada_mla`` extension module (csrc/mla_api.cpp:115-120).
     out = ada_mla.mla_decode_paged(q, kv_pages, block_table, cu_seqlens)  # paged KV cache
     q = ada_mla.mla_absorb_query(q_nope, q_rope, w_uk)     # the projections around
     y = ada_mla.mla_project_output(o_star, w_uv, w_o)      # the decode (MLA block)
+    y = ada_mla.mla_linear_fp8(x, weight, weight_scale)    # x W^T, W in e4m3 with a scale a 128 x 128
+    xq, x_scale = ada_mla.mla_quantize_fp8(x)              # rows quantised once for several such products
 
 and what a serving loop runs around it on the paged cache:
 
@@ -33,11 +35,13 @@ import importlib
 
 __all__ = ["mla_decode_split", "mla_decode_fused", "mla_decode_split_batched", "mla_decode_paged",
            "mla_absorb_query", "mla_project_output", "mla_paged_tables", "mla_append_kv", "mla_decode_tree",
-           "mla_prefill", "mla_fork_tables", "mla_compact_tables", "mla_copy_pages", "HEAD_DIM_C", "HEAD_DIM_ROPE", "HEAD_DIM_K", "extension"]
+           "mla_prefill", "mla_fork_tables", "mla_compact_tables", "mla_copy_pages",
+           "mla_quantize_fp8", "mla_linear_fp8", "HEAD_DIM_C", "HEAD_DIM_ROPE", "HEAD_DIM_K", "extension"]
 
 _EXPORTS = {"mla_decode_split", "mla_decode_fused", "mla_decode_split_batched", "mla_decode_paged",
             "mla_absorb_query", "mla_project_output", "mla_paged_tables", "mla_append_kv", "mla_decode_tree",
-           "mla_prefill", "mla_fork_tables", "mla_compact_tables", "mla_copy_pages", "HEAD_DIM_C", "HEAD_DIM_ROPE", "HEAD_DIM_K"}
+           "mla_prefill", "mla_fork_tables", "mla_compact_tables", "mla_copy_pages",
+           "mla_quantize_fp8", "mla_linear_fp8", "HEAD_DIM_C", "HEAD_DIM_ROPE", "HEAD_DIM_K"}
 
 
 def extension():

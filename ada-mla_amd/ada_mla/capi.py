@@ -67,6 +67,13 @@ _SIGNATURES = {
     "mla_decode_paged_fp8_fp16": (_i, [_vp, _vp, _f] + [_vp] * 4 + [_sz] + [_i] * 7 + [_vp]),
     "mla_decode_paged_fp8_bf16": (_i, [_vp, _vp, _f] + [_vp] * 4 + [_sz] + [_i] * 7 + [_vp]),
     "mla_paged_tables": (_i, [_vp] * 10 + [_i] * 5 + [_vp]),
+    "mla_quantize_fp8_fp16": (_i, [_vp] * 3 + [_i, _i, _ll, _vp]),
+    "mla_quantize_fp8_bf16": (_i, [_vp] * 3 + [_i, _i, _ll, _vp]),
+    "mla_linear_fp8_workspace_size": (_sz, [_i] * 3),
+    "mla_linear_fp8_fp16": (_i, [_vp] * 5 + [_sz] + [_i] * 3 + [_ll, _ll, _vp]),
+    "mla_linear_fp8_bf16": (_i, [_vp] * 5 + [_sz] + [_i] * 3 + [_ll, _ll, _vp]),
+    "mla_linear_fp8_quantized_fp16": (_i, [_vp] * 5 + [_i] * 3 + [_ll, _ll, _vp]),
+    "mla_linear_fp8_quantized_bf16": (_i, [_vp] * 5 + [_i] * 3 + [_ll, _ll, _vp]),
     "mla_page_tables_workspace_size": (_sz, [_i]),
     "mla_fork_tables": (_i, [_vp] * 12 + [_sz] + [_i] * 6 + [_vp]),
     "mla_compact_tables": (_i, [_vp] * 9 + [_sz] + [_i] * 5 + [_vp]),
@@ -404,6 +411,47 @@ def copy_pages(kv_cache, copies):
     layers = kv_cache.shape[0] if kv_cache.dim() == 4 else 1
     _check("mla_copy_pages", lib.mla_copy_pages(_ptr(kv_cache), _ptr(copies), copies.shape[0], layers, kv_cache.shape[-3],
                                                 kv_cache.shape[-2], kv_cache.element_size(), _stream(kv_cache)))
+
+
+def quantize_fp8(x):
+    """mla_quantize_fp8_*: x [M, K] (last dimension contiguous) -> (float8_e4m3fn [M, K], scales [M, ceil(K / 128)])."""
+    import torch
+    lib = load()
+    m, k = x.shape
+    assert x.stride(1) == 1
+    q = torch.empty((m, k), dtype=torch.float8_e4m3fn, device=x.device)
+    scales = torch.empty((m, -(-k // 128)), dtype=torch.float32, device=x.device)
+    fn = "mla_quantize_fp8_" + _suffix(x)
+    _check(fn, getattr(lib, fn)(_ptr(x), _ptr(q), _ptr(scales), m, k, x.stride(0), _stream(x)))
+    return q, scales
+
+
+def linear_fp8(x, w, w_scale, x_scale=None, dtype=None, out=None, workspace=None):
+    """mla_linear_fp8_*: x [M, K] 16-bit, or float8_e4m3fn with x_scale [M, ceil(K / 128)]; w [N, K] float8_e4m3fn with
+    w_scale [ceil(N / 128), ceil(K / 128)] -> [M, N]."""
+    import torch
+    lib = load()
+    (m, k), n = x.shape, w.shape[0]
+    assert w.shape == (n, k) and x.stride(1) == 1 and w.stride(1) == 1 and w_scale.is_contiguous()
+    assert w_scale.shape == (-(-n // 128), -(-k // 128)) and w_scale.dtype == torch.float32
+    if x_scale is None:
+        if out is None:
+            out = torch.empty((m, n), dtype=x.dtype, device=x.device)
+        ws_bytes = lib.mla_linear_fp8_workspace_size(m, k, n)
+        if ws_bytes == 0:
+            raise MlaError("mla_linear_fp8_workspace_size", STATUS_INVALID_VALUE)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device) if workspace is None else workspace
+        fn = "mla_linear_fp8_" + _suffix(x)
+        _check(fn, getattr(lib, fn)(_ptr(x), _ptr(w), _ptr(w_scale), _ptr(out), _ptr(ws), ws.numel(), m, k, n, x.stride(0),
+                                    w.stride(0), _stream(x)))
+        return out
+    assert x_scale.is_contiguous() and x_scale.shape == (m, -(-k // 128)) and x_scale.dtype == torch.float32
+    if out is None:
+        out = torch.empty((m, n), dtype=dtype or torch.bfloat16, device=x.device)
+    fn = "mla_linear_fp8_quantized_" + _suffix(out)
+    _check(fn, getattr(lib, fn)(_ptr(x), _ptr(x_scale), _ptr(w), _ptr(w_scale), _ptr(out), m, k, n, x.stride(0), w.stride(0),
+                                _stream(x)))
+    return out
 
 
 def append_kv(kv, norm_weight, cos_sin, positions, slots, kv_cache, q_rope=None, eps: float = 1e-6,

@@ -28,7 +28,7 @@ INCLUDE = os.path.join(REPO, "include")
 ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 
 HIP_SOURCES = ["mla_splitkv_fp16.hip", "mla_splitkv_fp32.hip", "mla_combine.hip", "mla_capi.hip",
-               "mla_block.hip", "mla_paged.hip", "mla_pages.hip", "mla_tree.hip", "mla_prefill.hip"]
+               "mla_block.hip", "mla_linear.hip", "mla_paged.hip", "mla_pages.hip", "mla_tree.hip", "mla_prefill.hip"]
 LIB_NAME = "libmla_mi355x.so"
 TIMELINE_LIB_NAME = "libmla_mi355x_timeline.so"
 

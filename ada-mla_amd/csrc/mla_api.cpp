@@ -740,6 +740,105 @@ at::Tensor mla_prefill(const at::Tensor &q_nope_in, const at::Tensor &q_rope_in,
     return out;
 }
 
+void check_inputs(int64_t inputs, const char *fn)
+{
+    TORCH_CHECK(inputs >= 16 && inputs % 16 == 0 && inputs <= (1 << 22), fn,
+                ": the last dimension must be a positive multiple of 16 (<= 2^22), got ", inputs);
+}
+
+// x as rows [m, inputs] that the kernels can read in place (else a copy): the last dimension contiguous, rows `unit`
+// values apart or a multiple of that.
+at::Tensor as_rows(const at::Tensor &x, int64_t unit)
+{
+    const at::Tensor rows = x.dim() == 2 ? x : x.reshape({-1, x.size(-1)});
+    const bool ok = starts_aligned(rows) && rows.stride(1) == 1 &&
+                    (rows.size(0) == 1 || (rows.stride(0) % unit == 0 && rows.stride(0) <= (1 << 22)));
+    return ok ? rows : readable(rows);
+}
+
+std::vector<int64_t> with_last(const at::Tensor &x, int64_t last)
+{
+    std::vector<int64_t> sizes = x.sizes().vec();
+    sizes.back() = last;
+    return sizes;
+}
+
+// No reference code: rows in e4m3 with a scale for each 128 values.
+std::vector<at::Tensor> quantize_fp8(const at::Tensor &x_in)
+{
+    const char *fn = "mla_quantize_fp8";
+    const auto dt = x_in.scalar_type();
+    TORCH_CHECK(dt == at::kHalf || dt == at::kBFloat16, fn, ": x must be float16 or bfloat16");
+    TORCH_CHECK(x_in.dim() >= 1, fn, ": x must be [..., inputs]");
+    const int64_t inputs = x_in.size(-1), blocks = (inputs + 127) / 128, rows = inputs ? x_in.numel() / inputs : 0;
+    check_inputs(inputs, fn);
+    TORCH_CHECK(rows <= (1 << 26), fn, ": too many rows");
+    check_devices({&x_in}, fn);
+    const at::OptionalDeviceGuard guard(x_in.device());
+    const auto options = x_in.options().memory_format(at::MemoryFormat::Contiguous);
+    at::Tensor q = at::empty(x_in.sizes(), options.dtype(at::kFloat8_e4m3fn));
+    at::Tensor scales = at::empty(with_last(x_in, blocks), options.dtype(at::kFloat));
+    if (rows == 0)
+        return {q, scales};
+    const at::Tensor x = as_rows(x_in, 8);
+    auto f = dt == at::kHalf ? mla_quantize_fp8_fp16 : mla_quantize_fp8_bf16;
+    check_status(f(x.data_ptr(), q.data_ptr(), scales.data_ptr<float>(), static_cast<int>(rows), static_cast<int>(inputs),
+                   used_stride(x, 0, inputs), stream_of(x)),
+                 fn);
+    return {q, scales};
+}
+
+// No reference code: y = x W^T with W in e4m3 and a scale for each 128 x 128 values.
+at::Tensor linear_fp8(const at::Tensor &x_in, const at::Tensor &w_in, const at::Tensor &ws_in,
+                      const c10::optional<at::Tensor> &xs_in, const c10::optional<at::ScalarType> &dtype)
+{
+    const char *fn = "mla_linear_fp8";
+    const bool quantised = x_in.scalar_type() == at::kFloat8_e4m3fn;
+    TORCH_CHECK(quantised || x_in.scalar_type() == at::kHalf || x_in.scalar_type() == at::kBFloat16, fn,
+                ": x must be float16, bfloat16 or float8_e4m3fn");
+    TORCH_CHECK(quantised == xs_in.has_value(), fn, ": x_scale comes with a float8_e4m3fn x, and only with one");
+    const auto dt = dtype ? *dtype : quantised ? at::kBFloat16 : x_in.scalar_type();
+    TORCH_CHECK(dt == at::kHalf || dt == at::kBFloat16, fn, ": dtype must be float16 or bfloat16");
+    TORCH_CHECK(quantised || dt == x_in.scalar_type(), fn, ": dtype is for a float8_e4m3fn x (else out has x's)");
+    TORCH_CHECK(x_in.dim() >= 1, fn, ": x must be [..., inputs]");
+    const int64_t inputs = x_in.size(-1), blocks = (inputs + 127) / 128, rows = inputs ? x_in.numel() / inputs : 0;
+    check_inputs(inputs, fn);
+    TORCH_CHECK(w_in.scalar_type() == at::kFloat8_e4m3fn && w_in.dim() == 2 && w_in.size(1) == inputs && w_in.size(0) >= 1, fn,
+                ": weight must be a float8_e4m3fn tensor [outputs, ", inputs, "], got ", w_in.sizes());
+    const int64_t outputs = w_in.size(0);
+    TORCH_CHECK(rows <= (1 << 26) && outputs <= (1 << 26), fn, ": too many rows or outputs");
+    TORCH_CHECK(ws_in.scalar_type() == at::kFloat && ws_in.dim() == 2 && ws_in.size(0) == (outputs + 127) / 128 &&
+                    ws_in.size(1) == blocks,
+                fn, ": weight_scale must be a float32 tensor [", (outputs + 127) / 128, ", ", blocks, "], got ", ws_in.sizes());
+    if (xs_in)
+        TORCH_CHECK(xs_in->scalar_type() == at::kFloat && xs_in->sizes().vec() == with_last(x_in, blocks), fn,
+                    ": x_scale must be a float32 tensor of x's shape with ", blocks, " in the last place, got ", xs_in->sizes());
+    check_devices({&x_in, &w_in, &ws_in, xs_in ? &*xs_in : &x_in}, fn);
+    const at::OptionalDeviceGuard guard(x_in.device());
+    at::Tensor out = at::empty(with_last(x_in, outputs), x_in.options().dtype(dt).memory_format(at::MemoryFormat::Contiguous));
+    if (rows == 0)
+        return out;
+    const at::Tensor x = as_rows(x_in, quantised ? 16 : 8), w = as_rows(w_in, 16), ws = ws_in.contiguous();
+    const int m = static_cast<int>(rows), k = static_cast<int>(inputs), n = static_cast<int>(outputs);
+    const int64_t x_stride = used_stride(x, 0, inputs), w_stride = used_stride(w, 0, inputs);
+    if (quantised) {
+        const at::Tensor xs = xs_in->contiguous();
+        auto f = dt == at::kHalf ? mla_linear_fp8_quantized_fp16 : mla_linear_fp8_quantized_bf16;
+        check_status(f(x.data_ptr(), xs.data_ptr<float>(), w.data_ptr(), ws.data_ptr<float>(), out.data_ptr(), m, k, n,
+                       x_stride, w_stride, stream_of(x)),
+                     fn);
+        return out;
+    }
+    const size_t ws_bytes = mla_linear_fp8_workspace_size(m, k, n);
+    TORCH_CHECK(ws_bytes > 0, fn, ": unsupported sizes");
+    const at::Tensor space = workspace(ws_bytes, x);
+    auto f = dt == at::kHalf ? mla_linear_fp8_fp16 : mla_linear_fp8_bf16;
+    check_status(f(x.data_ptr(), w.data_ptr(), ws.data_ptr<float>(), out.data_ptr(), space.data_ptr(), ws_bytes, m, k, n,
+                   x_stride, w_stride, stream_of(x)),
+                 fn);
+    return out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
@@ -772,6 +871,16 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
           "out [B,d_model] = concat_h(O*[:,h] W_UV[h]^T) W_O^T (o_star [B,n_h,512], w_uv [n_h,128,512], "
           "w_o [d_model,n_h*128])",
           pybind11::arg("o_star"), pybind11::arg("w_uv"), pybind11::arg("w_o"));
+    m.def("mla_quantize_fp8", &quantize_fp8,
+          "(x in float8_e4m3fn, scales float32 [..., ceil(inputs/128)]) of float16 or bfloat16 x [..., inputs]: each 128 "
+          "values' largest at 448",
+          pybind11::arg("x"));
+    m.def("mla_linear_fp8", &linear_fp8,
+          "x W^T [..., outputs] of x [..., inputs] (float16 or bfloat16, quantised as mla_quantize_fp8 does; or "
+          "float8_e4m3fn with x_scale, the result then in dtype, bfloat16 by default) and weight [outputs, inputs] "
+          "float8_e4m3fn with weight_scale float32 [ceil(outputs/128), ceil(inputs/128)]; inputs a multiple of 16",
+          pybind11::arg("x"), pybind11::arg("weight"), pybind11::arg("weight_scale"),
+          pybind11::arg("x_scale") = pybind11::none(), pybind11::arg("dtype") = pybind11::none());
     m.def("mla_paged_tables", &paged_tables,
           "(cu_seqlens [B+1], cu_new [B+1], slots [total_new] int64, positions [total_new], free_next [1]) of a "
           "step's tokens from int32 context_lens and new_lens [B]; the pages that the new tokens start come from "

@@ -363,6 +363,49 @@ int mla_project_output_bf16(const void *o_star, const void *w_uv,
                             size_t workspace_bytes, int batch, int num_heads,
                             int d_model, void *stream);
 
+/* Products in OCP fp8 (E4M3FN) with a scale for each block of 128, as the
+ * projections before and after the attention hold their weights (no reference
+ * code).
+ *
+ * mla_quantize_fp8_*: rows x [rows][inputs] (x_stride values apart) in fp16 or bf16 ->
+ *   xq [rows][inputs] and scales [rows][ceil(inputs / 128)]: a block's scale is
+ *   top / 448 with top = max(max |x|, 2^-100), its values xq = e4m3(448 x / top)
+ *   (to nearest even). An infinity makes its block's values NaN and its scale
+ *   infinite, a NaN stays one.
+ * mla_linear_fp8_*: out [rows][outputs], in x's type, = x W^T:
+ *   out[m][n] = sum_b xs[m][b] w_scale[n / 128][b] sum_{k in b} xq[m][k] w[n][k]
+ *   with x quantised so, w [outputs][inputs] E4M3FN (w_stride bytes apart) and
+ *   w_scale [ceil(outputs / 128)][ceil(inputs / 128)]; sums in fp32, rounded
+ *   once. The workspace holds the quantised rows.
+ * mla_linear_fp8_quantized_*: the same of rows that are quantised already, xq
+ *   (x_stride bytes apart) with x_scale [rows][ceil(inputs / 128)], and out in fp16 or bf16.
+ * A NaN or infinity in a row of x makes its row of out NaN, a NaN in a row of w its
+ * column. inputs must be a multiple of 16, strides of 8 values (16-bit rows) or 16 bytes, and
+ * inputs and strides at most 2^22; rows and outputs at most 2^26. */
+int mla_quantize_fp8_fp16(const void *x, void *xq, float *scales, int rows,
+                          int inputs, long long x_stride, void *stream);
+int mla_quantize_fp8_bf16(const void *x, void *xq, float *scales, int rows,
+                          int inputs, long long x_stride, void *stream);
+size_t mla_linear_fp8_workspace_size(int rows, int inputs, int outputs);
+int mla_linear_fp8_fp16(const void *x, const void *w, const float *w_scale,
+                        void *out, void *workspace, size_t workspace_bytes,
+                        int rows, int inputs, int outputs, long long x_stride,
+                        long long w_stride, void *stream);
+int mla_linear_fp8_bf16(const void *x, const void *w, const float *w_scale,
+                        void *out, void *workspace, size_t workspace_bytes,
+                        int rows, int inputs, int outputs, long long x_stride,
+                        long long w_stride, void *stream);
+int mla_linear_fp8_quantized_fp16(const void *xq, const float *x_scale,
+                                  const void *w, const float *w_scale,
+                                  void *out, int rows, int inputs, int outputs,
+                                  long long x_stride, long long w_stride,
+                                  void *stream);
+int mla_linear_fp8_quantized_bf16(const void *xq, const float *x_scale,
+                                  const void *w, const float *w_scale,
+                                  void *out, int rows, int inputs, int outputs,
+                                  long long x_stride, long long w_stride,
+                                  void *stream);
+
 /* Block table, slots and positions of one step's tokens, from the requests'
  * lengths (no reference counterpart). All pointers are on the device and
  * aligned to their type.

@@ -125,3 +125,57 @@ def test_pages_oracle_on_small_cases():
     assert nxt == 3 - 1 + 1 and free == [-1, -1, 1, 8]
     t, copies, free = compact([[8, 2], [5, -1]], [64, 3], [0] * 9, [-1, 0, 7, 3], 1, 32, 9)
     assert copies[:2] == [[8, 0, 32], [5, 3, 32]] and t == [[0, 2], [3, -1]] and free == [-1, 5, 7, 8]
+
+
+@pytest.mark.parametrize("t", ["fp16", "bf16"])
+def test_linear_argument_errors(t):
+    call = _caller("mla_quantize_fp8_" + t, "x q s rows k stride stream",
+                   dict(x=FAKE, q=FAKE, s=FAKE, rows=3, k=256, stride=256, stream=None))
+    for bad in (dict(x=None), dict(q=None), dict(s=None), dict(rows=0), dict(rows=2 ** 26 + 1), dict(k=0), dict(k=24),
+                dict(k=2 ** 22 + 16), dict(stride=-8), dict(stride=2 ** 22 + 8)):
+        assert call(**bad) == capi.STATUS_INVALID_VALUE, bad
+    for bad in (dict(x=FAKE + 2), dict(q=FAKE + 8), dict(stride=257)):
+        assert call(**bad) == capi.STATUS_MISALIGNED, bad
+    names = "x w ws out space bytes rows k n xstride wstride stream"
+    ok = dict.fromkeys(names.split(), FAKE) | dict(bytes=1 << 40, rows=3, k=256, n=100, xstride=256, wstride=256, stream=None)
+    common = (dict(x=None), dict(w=None), dict(ws=None), dict(out=None), dict(rows=0), dict(k=0), dict(k=24), dict(n=0),
+              dict(n=2 ** 26 + 1), dict(rows=2 ** 26, n=2 ** 26), dict(xstride=-16), dict(wstride=-16),
+              dict(wstride=2 ** 22 + 16))
+    call = _caller("mla_linear_fp8_" + t, names, ok)
+    for bad in (*common, dict(space=None)):
+        assert call(**bad) == capi.STATUS_INVALID_VALUE, bad
+    for bad in (dict(x=FAKE + 2), dict(w=FAKE + 8), dict(out=FAKE + 2), dict(space=FAKE + 4), dict(xstride=257), dict(wstride=264)):
+        assert call(**bad) == capi.STATUS_MISALIGNED, bad
+    assert call(bytes=16) == capi.STATUS_WORKSPACE_TOO_SMALL
+    size = capi.load().mla_linear_fp8_workspace_size
+    assert size(3, 256, 100) >= 3 * 256 + 3 * 2 * 4 and size(0, 256, 100) == size(3, 24, 100) == size(3, 256, 0) == 0
+    names = "x xs w ws out rows k n xstride wstride stream"
+    call = _caller("mla_linear_fp8_quantized_" + t, names, {n: ok.get(n, FAKE) for n in names.split()})
+    for bad in (*common, dict(xs=None)):
+        assert call(**bad) == capi.STATUS_INVALID_VALUE, bad
+    for bad in (dict(x=FAKE + 8), dict(w=FAKE + 8), dict(out=FAKE + 2), dict(xstride=264), dict(wstride=264)):
+        assert call(**bad) == capi.STATUS_MISALIGNED, bad
+
+
+def test_extension_refusals_linear():
+    m = _ext()
+    f8 = torch.float8_e4m3fn
+    h = lambda *s: torch.zeros(*s, dtype=torch.float16)  # noqa: E731
+    ok = dict(x=h(3, 272), weight=h(200, 272).to(f8), weight_scale=torch.zeros(2, 3))
+    for bad, msg in ((dict(x=h(3, 272).float()), "x must be float16"), (dict(x=h(3, 264)), "multiple of 16"),
+                     (dict(x=h(3, 256)), "weight must be"), (dict(weight=h(200, 272)), "weight must be"),
+                     (dict(weight=h(0, 272).to(f8)), "weight must be"), (dict(weight_scale=torch.zeros(2, 2)), "weight_scale must be"),
+                     (dict(weight_scale=torch.zeros(3, 3)), "weight_scale must be"),
+                     (dict(weight_scale=torch.zeros(2, 3).double()), "weight_scale must be"),
+                     (dict(x_scale=torch.zeros(3, 3)), "x_scale comes with"), (dict(x=h(3, 272).to(f8)), "x_scale comes with"),
+                     (dict(x=h(3, 272).to(f8), x_scale=torch.zeros(3, 2)), "x_scale must be"),
+                     (dict(x=h(3, 272).to(f8), x_scale=torch.zeros(3, 3).half()), "x_scale must be"),
+                     (dict(x=h(3, 272).to(f8), x_scale=torch.zeros(3, 3), dtype=torch.float32), "dtype must be"),
+                     (dict(dtype=torch.bfloat16), "dtype is for"), (dict(x=torch.zeros((), dtype=torch.float16)), "inputs"),
+                     (dict(), "GPU tensors"), (dict(x=h(3, 272).to(f8), x_scale=torch.zeros(3, 3)), "GPU tensors")):
+        with pytest.raises(RuntimeError, match=msg):
+            m.mla_linear_fp8(**{**ok, **bad})
+    for x, msg in ((h(3, 272).float(), "float16 or bfloat16"), (h(3, 24), "multiple of 16"), (h(3, 0), "multiple of 16"),
+                   (torch.zeros((), dtype=torch.float16), "inputs"), (h(3, 272), "GPU tensors")):
+        with pytest.raises(RuntimeError, match=msg):
+            m.mla_quantize_fp8(x)
