@@ -17,6 +17,7 @@
 #include "mla_device.hpp"
 #include "mla_internal.hpp"
 #include "mla_mi355x.h"
+#include "mla_ring.hpp"
 
 namespace mla {
 namespace {
@@ -112,72 +113,157 @@ struct Linear {
     long long x_stride, w_stride, xs_row, xs_block;
 };
 
-constexpr int kTile = 128;
+// A BN x BM tile of y (BN outputs, BM rows): 8 waves, kWN x kWM of them, each with its outputs as the A
+// operand and its rows as B, so that a lane holds four outputs of one row and one scale serves them
+// all. Blocks of 128 inputs go through two LDS slots by direct loads: block b + 1 is on its way
+// while b is multiplied. 16-byte chunk c of row r sits at c ^ (r / 2 mod 8): rows are 128 bytes, two of them an
+// LDS bank period, so 16 rows' chunks are in 16 different places.
+template <int BN, int BM, int kWN, int kWM>
+struct Tile {
+    static constexpr int kThreads = 64 * kWN * kWM;
+    static constexpr int kN = BN / kWN, kM = BM / kWM;          // a wave's outputs and rows
+    static constexpr int kNT = kN / 16, kMT = kM / 16;
+    static constexpr int kWUnits = BN / 8 / (kWN * kWM);        // loads of 8 rows, a wave and block: of W
+    static constexpr int kUnits = kWUnits + BM / 8 / (kWN * kWM);  // and of x
+    static constexpr int kSlot = (BN + BM) * kBlock;
+    static constexpr int kScales = BM * 4;
+    static_assert(BN / 8 % (kWN * kWM) == 0 && BM / 8 % (kWN * kWM) == 0 && kBlock % kN == 0 && BM % 64 == 0, "tile split");
+};
 
-// A 128 x 128 tile of y: 4 waves of 64 x 64, one block of 128 inputs at a time through LDS. 16-byte
-// chunk c of row r sits at c ^ (r / 2 mod 8): rows are 128 bytes, two of them an LDS bank period.
-template <typename E>
-__global__ __launch_bounds__(256) void linear_kernel(Linear p)
+template <typename E, int BN, int BM, int kWN, int kWM>
+__global__ __launch_bounds__((Tile<BN, BM, kWN, kWM>::kThreads)) void linear_kernel(Linear p)
 {
-    __shared__ __attribute__((aligned(16))) unsigned char s_w[kTile * kBlock], s_x[kTile * kBlock];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, g = lane >> 4;
-    const int n_tiles = (p.outputs + kTile - 1) / kTile;
-    const int n0 = (int)(blockIdx.x % n_tiles) * kTile, m0 = (int)(blockIdx.x / n_tiles) * kTile;
-    const int wn = (wave & 1) * 64, wm = (wave >> 1) * 64;
-    floatx4 acc[4][4] = {};
-    for (int b = 0; b < p.blocks; ++b) {
-        __syncthreads();
+    using T = Tile<BN, BM, kWN, kWM>;
+    using E4 = typename Vec<E>::v4;
+    __shared__ __attribute__((aligned(1024))) unsigned char s_slot[2][T::kSlot];
+    __shared__ __attribute__((aligned(16))) float s_xs[2][BM];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int l16 = lane & 15, g = lane >> 4;
+    const int n_tiles = (p.outputs + BN - 1) / BN;
+    const int n0 = (int)(blockIdx.x % n_tiles) * BN, m0 = (int)(blockIdx.x / n_tiles) * BM;
+    const int wn = wave % kWN * T::kN, wm = wave / kWN * T::kM;
+
+    // Unit u of a block: rows 8 u .. 8 u + 7 of the slot (its BN weight rows, then its BM x rows); lane -> row
+    // lane / 8, stored chunk lane % 8. Rows past the last re-read it.
+    const unsigned slot_lds = (unsigned)(uintptr_t)(const MLA_LDS unsigned char *)&s_slot[0][0];
+    const unsigned scale_lds = (unsigned)(uintptr_t)(const MLA_LDS float *)&s_xs[0][0];
+    const unsigned char *w_tile = p.w + n0 * p.w_stride, *x_tile = p.x + m0 * p.x_stride;
+    auto unit = [&](int i) { return i < T::kWUnits ? wave * T::kWUnits + i : BN / 8 + wave * (T::kUnits - T::kWUnits) + i - T::kWUnits; };
+    auto chunk_of = [&](int u) { return (lane & 7) ^ (((8 * u + (lane >> 3)) >> 1) & 7); };
+    int off[T::kUnits];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int r = 32 * i + (threadIdx.x >> 3), c = threadIdx.x & 7, k = b * kBlock + 16 * c;
-            const int at = r * kBlock + 16 * (c ^ ((r >> 1) & 7));
-            uint4 a = {0, 0, 0, 0}, v = {0, 0, 0, 0};
-            if (k < p.inputs) {
-                a = *(const uint4 *)(p.w + min(n0 + r, p.outputs - 1) * p.w_stride + k);
-                v = *(const uint4 *)(p.x + min(m0 + r, p.rows - 1) * p.x_stride + k);
+    for (int i = 0; i < T::kUnits; ++i) {
+        const int u = unit(i), r = 8 * u + (lane >> 3);
+        off[i] = (i < T::kWUnits ? min(r, p.outputs - 1 - n0) * (int)p.w_stride : min(r - BN, p.rows - 1 - m0) * (int)p.x_stride) +
+                 16 * chunk_of(u);
+    }
+    int scale_off = 0;
+    if (wave < BM / 64)
+        scale_off = 4 * min(64 * wave + lane, p.rows - 1 - m0) * (int)p.xs_row;
+    const int tail = p.inputs % kBlock / 16;  // whole chunks of the last block (0: all 8)
+    auto issue = [&](int b) {
+        const unsigned lds = slot_lds + (b & 1) * T::kSlot;
+        const bool ragged = tail != 0 && b == p.blocks - 1;
+#pragma unroll
+        for (int i = 0; i < T::kUnits; ++i) {
+            const int u = unit(i);
+            int o = off[i];
+            if (ragged) {  // chunks behind the inputs' end read the block's first, and are cleared afterwards
+                const int c = chunk_of(u);
+                o -= c >= tail ? 16 * c : 0;
             }
-            *(uint4 *)(s_w + at) = a;
-            *(uint4 *)(s_x + at) = v;
+            global_to_lds16_at((i < T::kWUnits ? w_tile : x_tile) + (size_t)b * kBlock, o, lds + 1024 * u);
         }
-        __syncthreads();
-        auto operand = [&](const unsigned char *s, int r) {
-            const uint4 lo = *(const uint4 *)(s + r * kBlock + 16 * ((2 * g) ^ ((r >> 1) & 7)));
-            const uint4 hi = *(const uint4 *)(s + r * kBlock + 16 * ((2 * g + 1) ^ ((r >> 1) & 7)));
+        if (wave < BM / 64)
+            global_to_lds4_at(p.xs + m0 * p.xs_row + b * p.xs_block, scale_off, scale_lds + (b & 1) * T::kScales + 256 * wave);
+    };
+    // the wave's loads of block b have landed
+    auto landed = [&](int b) {
+        MLA_WAIT_VMCNT(0);
+        if (tail != 0 && b == p.blocks - 1) {
+#pragma unroll
+            for (int i = 0; i < T::kUnits; ++i) {
+                const int u = unit(i);
+                if (chunk_of(u) >= tail)
+                    *(uint4 *)(&s_slot[b & 1][0] + 1024 * u + 16 * lane) = uint4{0, 0, 0, 0};
+            }
+        }
+    };
+    const auto *ws = (const __attribute__((address_space(4))) float *)p.ws +
+                     (size_t)min((n0 + wn) / kBlock, (p.outputs - 1) / kBlock) * p.blocks;
+
+    // a lane's 32 bytes of a row: chunks 2 g and 2 g + 1
+    const int lo_off = l16 * kBlock + 16 * ((2 * g) ^ (l16 >> 1)), hi_off = l16 * kBlock + 16 * ((2 * g + 1) ^ (l16 >> 1));
+    float acc[T::kNT][T::kMT][4] = {};
+    issue(0);
+    landed(0);
+    lds_barrier();
+    for (int b = 0; b < p.blocks; ++b) {
+        if (b + 1 < p.blocks)
+            issue(b + 1);
+        const unsigned char *slot = &s_slot[b & 1][0];
+        // row l16 of the 16 rows from row0 (a multiple of 16) on
+        auto operand = [&](int row0) {
+            const uint4 lo = *(const uint4 *)(slot + row0 * kBlock + lo_off);
+            const uint4 hi = *(const uint4 *)(slot + row0 * kBlock + hi_off);
             return intx8{(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w, (int)hi.x, (int)hi.y, (int)hi.z, (int)hi.w};
         };
-        const float ws = p.ws[(size_t)((n0 + wn) / kBlock) * p.blocks + b];
-        intx8 a[4], v[4];
-        float s[4];
+        const float wscale = ws[b];
+        intx8 v[T::kMT], a[2];
+        float s[T::kMT];
+        a[0] = operand(wn);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            a[i] = operand(s_w, wn + 16 * i + l16);
-            v[i] = operand(s_x, wm + 16 * i + l16);
-            s[i] = p.xs[min(m0 + wm + 16 * i + l16, p.rows - 1) * p.xs_row + b * p.xs_block] * ws;
-        }
+        for (int j = 0; j < T::kMT; ++j)
+            v[j] = operand(BN + wm + 16 * j);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int j = 0; j < T::kMT; ++j)
+            s[j] = s_xs[b & 1][wm + 16 * j + l16] * wscale;
+        // the products of 16 outputs while those of the 16 before are scaled and added
+        floatx4 d[2][T::kMT];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const floatx4 d = mfma16x16x128_fp8(a[i], v[j], floatx4{0.f, 0.f, 0.f, 0.f});
+        for (int i = 0; i <= T::kNT; ++i) {
+            if (i + 1 < T::kNT)
+                a[(i + 1) & 1] = operand(wn + 16 * (i + 1));
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    acc[i][j][e] = __builtin_fmaf(d[e], s[j], acc[i][j][e]);
+            for (int j = 0; j < T::kMT; ++j) {
+                if (i < T::kNT)
+                    d[i & 1][j] = mfma16x16x128_fp8(a[i & 1], v[j], floatx4{0.f, 0.f, 0.f, 0.f});
+                if (i > 0)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        acc[i > 0 ? i - 1 : 0][j][e] =
+                            __builtin_fmaf(d[(i - 1) & 1][j][e], s[j], acc[i > 0 ? i - 1 : 0][j][e]);
+                // the sums stay where they are written: moved behind the products, every product's result would be live
+                if (i > 0)
+                    asm volatile("" : "+v"(acc[i > 0 ? i - 1 : 0][j][0]), "+v"(acc[i > 0 ? i - 1 : 0][j][1]),
+                                 "+v"(acc[i > 0 ? i - 1 : 0][j][2]), "+v"(acc[i > 0 ? i - 1 : 0][j][3]));
+                __builtin_amdgcn_sched_barrier(0);
             }
+        }
+        if (b + 1 < p.blocks)
+            landed(b + 1);
+        lds_barrier();
     }
     E *out = static_cast<E *>(p.out);
+    const bool whole = p.outputs % 4 == 0;  // four outputs of a row are one aligned store
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < T::kMT; ++j) {
         const int m = m0 + wm + 16 * j + l16;
         if (m >= p.rows)
             continue;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < T::kNT; ++i) {
+            const int n = n0 + wn + 16 * i + 4 * g;
+            E *to = out + (size_t)m * p.outputs + n;
+            const E4 y = {(E)acc[i][j][0], (E)acc[i][j][1], (E)acc[i][j][2], (E)acc[i][j][3]};
+            if (whole && n < p.outputs)
+                *(E4 *)to = y;
+            else
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int n = n0 + wn + 16 * i + 4 * g + e;
-                if (n < p.outputs)
-                    out[(size_t)m * p.outputs + n] = (E)acc[i][j][e];
-            }
+                for (int e = 0; e < 4; ++e)
+                    if (n + e < p.outputs)
+                        to[e] = y[e];
+        }
     }
 }
 
@@ -209,12 +295,22 @@ int launch_quantize(const void *x, void *q, float *scales, int rows, int inputs,
     return launched();
 }
 
+template <typename E, int BN, int BM, int kWN, int kWM>
+int launch_tiles(const Linear &p, hipStream_t s)
+{
+    const int64_t tiles = (int64_t)ceil_div(p.rows, BM) * ceil_div(p.outputs, BN);
+    hipLaunchKernelGGL((linear_kernel<E, BN, BM, kWN, kWM>), dim3((unsigned)tiles),
+                       dim3(Tile<BN, BM, kWN, kWM>::kThreads), 0, s, p);
+    return launched();
+}
+
 template <typename E>
 int launch_linear(const Linear &p, hipStream_t s)
 {
-    const int64_t tiles = (int64_t)ceil_div(p.rows, kTile) * ceil_div(p.outputs, kTile);
-    hipLaunchKernelGGL(linear_kernel<E>, dim3((unsigned)tiles), dim3(256), 0, s, p);
-    return launched();
+    const int64_t large = (int64_t)ceil_div(p.rows, 256) * ceil_div(p.outputs, 256);
+    if (large >= current_cu_count())
+        return launch_tiles<E, 256, 256, 2, 4>(p, s);
+    return launch_tiles<E, 128, 64, 4, 2>(p, s);
 }
 
 int quantize(bool bf16, const void *x, void *xq, float *scales, int rows, int inputs, long long x_stride, void *stream)

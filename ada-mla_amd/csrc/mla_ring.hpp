@@ -81,6 +81,15 @@ __device__ __forceinline__ void global_to_lds16_at(const void *base, int off, un
                  : : "v"(off), "s"(base), "s"(lds_addr) : "memory");
 }
 
+// 4 bytes per lane (global_load_lds_dword), to lds_addr + 4 * lane; as above.
+__device__ __forceinline__ void global_to_lds4_at(const void *base, int off, unsigned lds_addr)
+{
+    asm volatile("s_mov_b32 m0, %2\n\t"
+                 "s_nop 0\n\t"
+                 "global_load_lds_dword %0, %1"
+                 : : "v"(off), "s"(base), "s"(lds_addr) : "memory");
+}
+
 // The same load with the LDS destination given as a pointer. The steady-state
 // feeding takes the address instead: its lane offsets are formed once and
 // kept in registers of their own. Offsets recomputed into one shared register
