@@ -32,7 +32,7 @@ constexpr float kMost = 448.0f;  // largest e4m3 value
 // fp32 quotient: with 11 significant bits or less in x and top it is a tie of e4m3's
 // only where the exact quotient is one. It is formed from one reciprocal a block: x and top times the power of
 // two that brings top to [1, 2) (so that nothing overflows), q0 = a r, and the remainder
-// a - q0 t, exact, times r added.
+// a - q0 t, exact, times r added. It is 448 at most: top itself gives that exactly.
 struct BlockScale {
     float scale, up, t, r;  // up: 448 times the power of two
     __device__ __forceinline__ explicit BlockScale(float top)
@@ -50,9 +50,7 @@ struct BlockScale {
     __device__ __forceinline__ float operator()(float x) const
     {
         const float a = x * up, q = a * r;
-        const float y = __builtin_fmaf(__builtin_fmaf(-q, t, a), r, q);
-        // (fminf and fmaxf would drop a NaN)
-        return y > kMost ? kMost : y < -kMost ? -kMost : y;
+        return __builtin_fmaf(__builtin_fmaf(-q, t, a), r, q);
     }
 };
 
@@ -66,8 +64,29 @@ __device__ __forceinline__ uint2 e4m3x8(const float *y)
     return uint2{(unsigned)lo, (unsigned)hi};
 }
 
-// 16 lanes a block of 128 values, 8 values a lane: one 16-byte load, a maximum over the 16 lanes, one
-// 8-byte store. scales: of row m and block b at m row_step + b block_step.
+// A block of 128 values by 16 lanes, 8 values a lane: its scale and the lane's 8 bytes.
+template <typename E8>
+__device__ __forceinline__ uint2 quantized8(E8 v, float &scale)
+{
+    float y[8], top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        y[i] = (float)v[i];
+        top = fmaxf(top, fabsf(y[i]));
+    }
+#pragma unroll
+    for (int d = 8; d > 0; d /= 2)
+        top = fmaxf(top, __shfl_xor(top, d));
+    const BlockScale s(top);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        y[i] = s(y[i]);
+    scale = s.scale;
+    return e4m3x8(y);
+}
+
+// 16 lanes a block: one 16-byte load, a maximum over the 16 lanes, one 8-byte store.
+// scales: of row m and block b at m row_step + b block_step.
 template <typename E>
 __global__ __launch_bounds__(256) void quantize_kernel(const E *__restrict__ x, unsigned char *__restrict__ q,
                                                        float *__restrict__ scales, int rows, int inputs, int blocks,
@@ -84,23 +103,12 @@ __global__ __launch_bounds__(256) void quantize_kernel(const E *__restrict__ x, 
     E8 v = {};
     if (k < inputs)
         v = *(const E8 *)(x + m * x_stride + k);
-    float y[8], top = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        y[i] = (float)v[i];
-        top = fmaxf(top, fabsf(y[i]));
-    }
-#pragma unroll
-    for (int d = 8; d > 0; d /= 2)
-        top = fmaxf(top, __shfl_xor(top, d));
-    const BlockScale s(top);
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-        y[i] = s(y[i]);
+    float scale;
+    const uint2 y = quantized8(v, scale);
     if (k < inputs)
-        *(uint2 *)(q + m * q_stride + k) = e4m3x8(y);
+        *(uint2 *)(q + m * q_stride + k) = y;
     if (j == 0)
-        scales[m * row_step + b * block_step] = s.scale;
+        scales[m * row_step + b * block_step] = scale;
 }
 
 // ---- products ---------------------------------------------------------------
@@ -267,6 +275,309 @@ __global__ __launch_bounds__((Tile<BN, BM, kWN, kWM>::kThreads)) void linear_ker
     }
 }
 
+// Few rows: the weights' bytes are what the call costs, so each wave streams them from memory into the
+// operand registers, kAhead blocks ahead, with nothing between. A workgroup has 16 NT outputs of up to 16 MT
+// rows; its 8 waves take its blocks in turn (so that a row's next kilobyte is read at a time) and add
+// their sums through LDS at the end, wave after wave. kQuantize: the rows are 16-bit (E) and each workgroup
+// quantises them into LDS first, which for few values is cheaper than a launch.
+constexpr int kRowWaves = 8;
+constexpr int kMostOwn = 32768;  // values that a workgroup quantises itself
+
+template <int NT, int MT, bool kQuantize>
+struct RowTile {
+    static constexpr int kAhead = kQuantize ? 5 : MT >= 4 ? 3 : 4;
+    static constexpr int kSums = kRowWaves * NT * MT * 64 * 4;  // floats
+    static constexpr int kRows = kQuantize ? kMostOwn + 16 * (kBlock + 16) + 4 * (kMostOwn / kBlock + 16) : 16;
+};
+
+template <typename E, int NT, int MT, bool kQuantize>
+__global__ __launch_bounds__(64 * kRowWaves, 2) void linear_rows_kernel(Linear p)
+{
+    using T = RowTile<NT, MT, kQuantize>;
+    using E8 = typename Vec<E>::v8;
+    __shared__ __attribute__((aligned(16))) float s_sums[T::kSums];
+    __shared__ __attribute__((aligned(16))) unsigned char s_rows[T::kRows];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int l16 = lane & 15, g = lane >> 4;
+    const int n_tiles = (p.outputs + 16 * NT - 1) / (16 * NT);
+    const int n0 = (int)(blockIdx.x % n_tiles) * 16 * NT, m0 = (int)(blockIdx.x / n_tiles) * 16 * MT;
+    const int mine = p.blocks > wave ? (p.blocks - wave + kRowWaves - 1) / kRowWaves : 0;  // blocks wave, wave + 8, ..
+    // byte offsets of the lane's rows from the tile's first
+    const unsigned char *const w_tile = p.w + n0 * p.w_stride, *const x_tile = p.x + m0 * p.x_stride;
+    const float *const xs_tile = p.xs + m0 * p.xs_row;
+    int w_row[NT], x_row[MT], xs_row[MT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+        w_row[i] = min(16 * i + l16, p.outputs - 1 - n0) * (int)p.w_stride;
+#pragma unroll
+    for (int j = 0; j < MT; ++j) {
+        x_row[j] = min(16 * j + l16, p.rows - 1 - m0) * (int)p.x_stride;
+        xs_row[j] = min(16 * j + l16, p.rows - 1 - m0) * (int)p.xs_row;
+    }
+    // The lane's two 16-byte chunks of a block, bytes 32 g .. 32 g + 31. Behind the inputs' end they re-read the
+    // last 16 bytes there are and are cleared before the product: no load stands under a condition, so that the
+    // compiler's waits count the loads of the blocks ahead.
+    const int last = p.blocks - 1, end = p.inputs - last * kBlock;  // bytes of the last block
+    const bool lost_lo = 32 * g >= end, lost_hi = 32 * g + 16 >= end;
+    constexpr int kA = T::kAhead;
+    uint4 a[kA][NT][2], v[kA][kQuantize ? 1 : MT][2];
+    float s[kA][kQuantize ? 1 : MT];
+    auto load = [&](int d, int it) {  // the wave's block `it` (past its last: that one again)
+        const int b = wave + kRowWaves * min(it, mine - 1);
+        const int lo = min(b * kBlock + 32 * g, p.inputs - 16), hi = min(b * kBlock + 32 * g + 16, p.inputs - 16);
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            a[d][i][0] = *(const uint4 *)(w_tile + (w_row[i] + lo));
+            a[d][i][1] = *(const uint4 *)(w_tile + (w_row[i] + hi));
+        }
+        if constexpr (!kQuantize) {
+            const float *xs = xs_tile + b * p.xs_block;
+#pragma unroll
+            for (int j = 0; j < MT; ++j) {
+                v[d][j][0] = *(const uint4 *)(x_tile + (x_row[j] + lo));
+                v[d][j][1] = *(const uint4 *)(x_tile + (x_row[j] + hi));
+                s[d][j] = xs[xs_row[j]];
+            }
+        }
+    };
+    auto operand = [](const uint4 &lo, const uint4 &hi) {
+        return intx8{(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w, (int)hi.x, (int)hi.y, (int)hi.z, (int)hi.w};
+    };
+    const float *ws = p.ws + (size_t)(n0 / kBlock) * p.blocks;
+    float scales = 0.f;  // of the wave's next 64 blocks, one a lane
+    if (mine > 0) {
+        scales = ws[wave + kRowWaves * min(lane, mine - 1)];
+#pragma unroll
+        for (int d = 0; d < kA; ++d)
+            load(d, d);
+    }
+    const int row_bytes = p.blocks * kBlock + 16;  // in LDS
+    float *const s_xs = reinterpret_cast<float *>(s_rows + p.rows * row_bytes);
+    if constexpr (kQuantize) {
+        const E *x = reinterpret_cast<const E *>(p.x);
+        for (int u = tid >> 4; u < p.rows * p.blocks; u += 4 * kRowWaves) {
+            const int m = u / p.blocks, b = u - m * p.blocks, k = b * kBlock + 8 * (tid & 15);
+            E8 e = {};
+            if (k < p.inputs)
+                e = *(const E8 *)(x + m * p.x_stride + k);
+            float scale;
+            *(uint2 *)(s_rows + m * row_bytes + k) = quantized8(e, scale);
+            if ((tid & 15) == 0)
+                s_xs[u] = scale;
+        }
+        __syncthreads();
+    }
+    float acc[NT][MT][4] = {};
+    auto multiply = [&](int d, int it) {
+        const int b = wave + kRowWaves * it;
+        if ((it & 63) == 0 && it > 0)
+            scales = ws[wave + kRowWaves * min(it + lane, mine - 1)];
+        const float wscale = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(scales), it & 63));
+        if (b == last) {
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                a[d][i][0] = lost_lo ? uint4{0, 0, 0, 0} : a[d][i][0];
+                a[d][i][1] = lost_hi ? uint4{0, 0, 0, 0} : a[d][i][1];
+            }
+            if constexpr (!kQuantize)
+#pragma unroll
+                for (int j = 0; j < MT; ++j) {
+                    v[d][j][0] = lost_lo ? uint4{0, 0, 0, 0} : v[d][j][0];
+                    v[d][j][1] = lost_hi ? uint4{0, 0, 0, 0} : v[d][j][1];
+                }
+        }
+#pragma unroll
+        for (int j = 0; j < MT; ++j) {
+            intx8 x;
+            float f;
+            if constexpr (kQuantize) {
+                const int m = min(l16, p.rows - 1);
+                const unsigned char *at = s_rows + m * row_bytes + b * kBlock + 32 * g;
+                x = operand(*(const uint4 *)at, *(const uint4 *)(at + 16));
+                f = s_xs[m * p.blocks + b] * wscale;
+            } else {
+                x = operand(v[d][j][0], v[d][j][1]);
+                f = s[d][j] * wscale;
+            }
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                const floatx4 y = mfma16x16x128_fp8(operand(a[d][i][0], a[d][i][1]), x, floatx4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    acc[i][j][e] = __builtin_fmaf(y[e], f, acc[i][j][e]);
+            }
+        }
+    };
+    int it0 = 0;
+    for (; it0 + kA <= mine; it0 += kA) {
+#pragma unroll
+        for (int d = 0; d < kA; ++d) {
+            multiply(d, it0 + d);
+            load(d, it0 + d + kA);
+        }
+    }
+#pragma unroll
+    for (int d = 0; d < kA - 1; ++d)
+        if (it0 + d < mine)
+            multiply(d, it0 + d);
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int j = 0; j < MT; ++j)
+            *(floatx4 *)(s_sums + (((wave * NT + i) * MT + j) * 64 + lane) * 4) =
+                floatx4{acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+    __syncthreads();
+    // a thread an output tile's lane: wave after wave, outputs 4 g .. 4 g + 3 of row l16
+    E *out = static_cast<E *>(p.out);
+    for (int t = tid; t < NT * MT * 64; t += 64 * kRowWaves) {
+        floatx4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < kRowWaves; ++w)
+            y += *(const floatx4 *)(s_sums + (w * NT * MT * 64 + t) * 4);
+        const int i = t / (MT * 64), j = t / 64 % MT, l = t & 63;
+        const int m = m0 + 16 * j + (l & 15), n = n0 + 16 * i + 4 * (l >> 4);
+        if (m < p.rows)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (n + e < p.outputs)
+                    out[(size_t)m * p.outputs + n + e] = (E)y[e];
+    }
+}
+
+// Up to 64 rows: as above, but the operands of 16 to 64 rows would fill the registers before enough weight
+// blocks were on their way. Each wave therefore has an LDS ring of its own, fed by direct loads two blocks
+// ahead and read behind counter waits: no workgroup barrier in the loop. Four waves take the blocks in turn.
+constexpr int kFewWaves = 4;
+
+template <int NT, int MT>
+struct FewTile {
+    static constexpr int kSlots = 3;
+    static constexpr int kUnits = 2 * NT + 2 * MT;  // of 8 rows
+    static constexpr int kLoads = kUnits + 1;       // and the rows' scales
+    static constexpr int kSlot = kUnits * 1024 + 256;
+    static constexpr int kRing = kSlots * kSlot;    // a wave's
+    static_assert(kFewWaves * kRing <= 160 * 1024 && kRing >= NT * MT * 1024 && 2 * kLoads <= 63, "ring");
+};
+
+template <typename E, int NT, int MT>
+__global__ __launch_bounds__(64 * kFewWaves) void linear_few_kernel(Linear p)
+{
+    using T = FewTile<NT, MT>;
+    __shared__ __attribute__((aligned(1024))) unsigned char s_ring[kFewWaves * T::kRing];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int l16 = lane & 15, g = lane >> 4;
+    const int n_tiles = (p.outputs + 16 * NT - 1) / (16 * NT);
+    const int n0 = (int)(blockIdx.x % n_tiles) * 16 * NT, m0 = (int)(blockIdx.x / n_tiles) * 16 * MT;
+    const int mine = p.blocks > wave ? (p.blocks - wave + kFewWaves - 1) / kFewWaves : 0;  // blocks wave, wave + 4, ..
+    const unsigned char *const w_tile = p.w + n0 * p.w_stride, *const x_tile = p.x + m0 * p.x_stride;
+    unsigned char *const ring = s_ring + wave * T::kRing;
+    const unsigned ring_lds = (unsigned)(uintptr_t)(const MLA_LDS unsigned char *)ring;
+    // Unit u: rows 8 u .. 8 u + 7 of the slot (16 NT of W, then 16 MT of x), placed as in linear_kernel; then the rows' scales.
+    auto chunk_of = [&](int u) { return (lane & 7) ^ (((8 * u + (lane >> 3)) >> 1) & 7); };
+    int off[T::kUnits];
+#pragma unroll
+    for (int u = 0; u < T::kUnits; ++u) {
+        const int r = 8 * u + (lane >> 3);
+        off[u] = (u < 2 * NT ? min(r, p.outputs - 1 - n0) * (int)p.w_stride
+                             : min(r - 16 * NT, p.rows - 1 - m0) * (int)p.x_stride) + 16 * chunk_of(u);
+    }
+    const int scale_off = 4 * min(lane, p.rows - 1 - m0) * (int)p.xs_row;
+    const int last = p.blocks - 1, tail = p.inputs % kBlock / 16;
+    auto issue = [&](int it) {
+        const int b = wave + kFewWaves * it;
+        const unsigned lds = ring_lds + it % T::kSlots * T::kSlot;
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // what was read of the slot's last block has arrived
+#pragma unroll
+        for (int u = 0; u < T::kUnits; ++u) {
+            int o = off[u];
+            if (tail != 0 && b == last) {  // as in linear_kernel
+                const int c = chunk_of(u);
+                o -= c >= tail ? 16 * c : 0;
+            }
+            global_to_lds16_at((u < 2 * NT ? w_tile : x_tile) + (size_t)b * kBlock, o, lds + 1024 * u);
+        }
+        global_to_lds4_at(p.xs + m0 * p.xs_row + b * p.xs_block, scale_off, lds + 1024 * T::kUnits);
+    };
+    const float *ws = p.ws + (size_t)(n0 / kBlock) * p.blocks;
+    float scales = mine > 0 ? ws[wave + kFewWaves * min(lane, mine - 1)] : 0.f;  // of the wave's next 64 blocks, one a lane
+    asm volatile("" : "+v"(scales));  // (waited for before the loop's loads, which the compiler does not count)
+    if (mine > 0)
+        issue(0);
+    if (mine > 1)
+        issue(1);
+    const int lo_off = l16 * kBlock + 16 * ((2 * g) ^ (l16 >> 1)), hi_off = l16 * kBlock + 16 * ((2 * g + 1) ^ (l16 >> 1));
+    float acc[NT][MT][4] = {};
+    for (int it = 0; it < mine; ++it) {
+        if (it + 2 < mine) {
+            issue(it + 2);
+            MLA_WAIT_VMCNT(2 * T::kLoads);
+        } else if (it + 1 < mine) {
+            MLA_WAIT_VMCNT(T::kLoads);
+        } else {
+            MLA_WAIT_VMCNT(0);
+        }
+        asm volatile("" ::: "memory");
+        unsigned char *const slot = ring + it % T::kSlots * T::kSlot;
+        if (tail != 0 && wave + kFewWaves * it == last) {
+#pragma unroll
+            for (int u = 0; u < T::kUnits; ++u)
+                if (chunk_of(u) >= tail)
+                    *(uint4 *)(slot + 1024 * u + 16 * lane) = uint4{0, 0, 0, 0};
+        }
+        if ((it & 63) == 0 && it > 0) {
+            scales = ws[wave + kFewWaves * min(it + lane, mine - 1)];
+            asm volatile("" : "+v"(scales));
+        }
+        const float wscale = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(scales), it & 63));
+        auto operand = [&](int row0) {
+            const uint4 lo = *(const uint4 *)(slot + row0 * kBlock + lo_off);
+            const uint4 hi = *(const uint4 *)(slot + row0 * kBlock + hi_off);
+            return intx8{(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w, (int)hi.x, (int)hi.y, (int)hi.z, (int)hi.w};
+        };
+        intx8 a[NT], v[MT];
+        float s[MT];
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+            a[i] = operand(16 * i);
+#pragma unroll
+        for (int j = 0; j < MT; ++j) {
+            v[j] = operand(16 * NT + 16 * j);
+            s[j] = *(const float *)(slot + 1024 * T::kUnits + 4 * (16 * j + l16)) * wscale;
+        }
+#pragma unroll
+        for (int j = 0; j < MT; ++j)
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                const floatx4 y = mfma16x16x128_fp8(a[i], v[j], floatx4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    acc[i][j][e] = __builtin_fmaf(y[e], s[j], acc[i][j][e]);
+            }
+    }
+    // the waves' sums, each in its own ring
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int j = 0; j < MT; ++j)
+            *(floatx4 *)(ring + ((i * MT + j) * 64 + lane) * 16) =
+                floatx4{acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+    __syncthreads();
+    E *out = static_cast<E *>(p.out);
+    for (int t = tid; t < NT * MT * 64; t += 64 * kFewWaves) {
+        floatx4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < kFewWaves; ++w)
+            y += *(const floatx4 *)(s_ring + w * T::kRing + t * 16);
+        const int i = t / (MT * 64), j = t / 64 % MT, l = t & 63;
+        const int m = m0 + 16 * j + (l & 15), n = n0 + 16 * i + 4 * (l >> 4);
+        if (m < p.rows)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (n + e < p.outputs)
+                    out[(size_t)m * p.outputs + n + e] = (E)y[e];
+    }
+}
+
 constexpr long long kMostStride = 1 << 22;  // a tile's rows stay within 2^31 bytes
 
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -304,13 +615,49 @@ int launch_tiles(const Linear &p, hipStream_t s)
     return launched();
 }
 
+template <typename E, int NT, int MT, bool kQuantize>
+int launch_rows(const Linear &p, hipStream_t s)
+{
+    const int64_t tiles = (int64_t)ceil_div(p.rows, 16 * MT) * ceil_div(p.outputs, 16 * NT);
+    hipLaunchKernelGGL((linear_rows_kernel<E, NT, MT, kQuantize>), dim3((unsigned)tiles), dim3(64 * kRowWaves), 0, s, p);
+    return launched();
+}
+
+template <typename E, int NT, int MT>
+int launch_few(const Linear &p, hipStream_t s)
+{
+    const int64_t tiles = (int64_t)ceil_div(p.rows, 16 * MT) * ceil_div(p.outputs, 16 * NT);
+    hipLaunchKernelGGL((linear_few_kernel<E, NT, MT>), dim3((unsigned)tiles), dim3(64 * kFewWaves), 0, s, p);
+    return launched();
+}
+
 template <typename E>
 int launch_linear(const Linear &p, hipStream_t s)
 {
+    if (p.rows <= 64) {
+        const bool narrow = ceil_div(p.outputs, 16) <= current_cu_count();
+        if (p.rows <= 16)
+            return narrow ? launch_rows<E, 1, 1, false>(p, s) : launch_rows<E, 2, 1, false>(p, s);
+        if (p.rows <= 32)
+            return narrow ? launch_few<E, 1, 2>(p, s) : launch_few<E, 2, 2>(p, s);
+        return narrow ? launch_few<E, 1, 4>(p, s) : launch_few<E, 2, 4>(p, s);
+    }
     const int64_t large = (int64_t)ceil_div(p.rows, 256) * ceil_div(p.outputs, 256);
     if (large >= current_cu_count())
         return launch_tiles<E, 256, 256, 2, 4>(p, s);
     return launch_tiles<E, 128, 64, 4, 2>(p, s);
+}
+
+// 16-bit rows few enough for every workgroup to quantise them
+bool quantizes_itself(int rows, int inputs)
+{
+    return rows <= 16 && (int64_t)rows * ceil_div(inputs, kBlock) * kBlock <= kMostOwn;
+}
+
+template <typename E>
+int launch_own(const Linear &p, hipStream_t s)
+{
+    return ceil_div(p.outputs, 16) <= current_cu_count() ? launch_rows<E, 1, 1, true>(p, s) : launch_rows<E, 2, 1, true>(p, s);
 }
 
 int quantize(bool bf16, const void *x, void *xq, float *scales, int rows, int inputs, long long x_stride, void *stream)
@@ -337,6 +684,11 @@ int linear(bool bf16, const void *x, const void *w, const float *ws, void *out, 
         return MLA_STATUS_MISALIGNED;
     if (workspace_bytes < mla_linear_fp8_workspace_size(rows, inputs, outputs))
         return MLA_STATUS_WORKSPACE_TOO_SMALL;
+    if (quantizes_itself(rows, inputs)) {
+        const Linear p{static_cast<const unsigned char *>(x), static_cast<const unsigned char *>(w), nullptr, ws, out, rows,
+                       inputs, outputs, ceil_div(inputs, kBlock), x_stride, w_stride, 0, 0};
+        return (bf16 ? launch_own<__bf16> : launch_own<_Float16>)(p, static_cast<hipStream_t>(stream));
+    }
     auto *xq = static_cast<unsigned char *>(workspace);
     auto *xs = reinterpret_cast<float *>(xq + rows_bytes(rows, inputs));
     hipStream_t s = static_cast<hipStream_t>(stream);
