@@ -72,8 +72,8 @@ _SIGNATURES = {
     "mla_linear_fp8_workspace_size": (_sz, [_i] * 3),
     "mla_linear_fp8_fp16": (_i, [_vp] * 5 + [_sz] + [_i] * 3 + [_ll, _ll, _vp]),
     "mla_linear_fp8_bf16": (_i, [_vp] * 5 + [_sz] + [_i] * 3 + [_ll, _ll, _vp]),
-    "mla_linear_fp8_quantized_fp16": (_i, [_vp] * 5 + [_i] * 3 + [_ll, _ll, _vp]),
-    "mla_linear_fp8_quantized_bf16": (_i, [_vp] * 5 + [_i] * 3 + [_ll, _ll, _vp]),
+    "mla_linear_fp8_quantized_fp16": (_i, [_vp] * 6 + [_sz] + [_i] * 3 + [_ll, _ll, _vp]),
+    "mla_linear_fp8_quantized_bf16": (_i, [_vp] * 6 + [_sz] + [_i] * 3 + [_ll, _ll, _vp]),
     "mla_page_tables_workspace_size": (_sz, [_i]),
     "mla_fork_tables": (_i, [_vp] * 12 + [_sz] + [_i] * 6 + [_vp]),
     "mla_compact_tables": (_i, [_vp] * 9 + [_sz] + [_i] * 5 + [_vp]),
@@ -434,23 +434,19 @@ def linear_fp8(x, w, w_scale, x_scale=None, dtype=None, out=None, workspace=None
     (m, k), n = x.shape, w.shape[0]
     assert w.shape == (n, k) and x.stride(1) == 1 and w.stride(1) == 1 and w_scale.is_contiguous()
     assert w_scale.shape == (-(-n // 128), -(-k // 128)) and w_scale.dtype == torch.float32
-    if x_scale is None:
-        if out is None:
-            out = torch.empty((m, n), dtype=x.dtype, device=x.device)
-        ws_bytes = lib.mla_linear_fp8_workspace_size(m, k, n)
-        if ws_bytes == 0:
-            raise MlaError("mla_linear_fp8_workspace_size", STATUS_INVALID_VALUE)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device) if workspace is None else workspace
-        fn = "mla_linear_fp8_" + _suffix(x)
-        _check(fn, getattr(lib, fn)(_ptr(x), _ptr(w), _ptr(w_scale), _ptr(out), _ptr(ws), ws.numel(), m, k, n, x.stride(0),
-                                    w.stride(0), _stream(x)))
-        return out
-    assert x_scale.is_contiguous() and x_scale.shape == (m, -(-k // 128)) and x_scale.dtype == torch.float32
     if out is None:
-        out = torch.empty((m, n), dtype=dtype or torch.bfloat16, device=x.device)
-    fn = "mla_linear_fp8_quantized_" + _suffix(out)
-    _check(fn, getattr(lib, fn)(_ptr(x), _ptr(x_scale), _ptr(w), _ptr(w_scale), _ptr(out), m, k, n, x.stride(0), w.stride(0),
-                                _stream(x)))
+        out = torch.empty((m, n), dtype=x.dtype if x_scale is None else dtype or torch.bfloat16, device=x.device)
+    ws_bytes = lib.mla_linear_fp8_workspace_size(m, k, n)
+    if ws_bytes == 0:
+        raise MlaError("mla_linear_fp8_workspace_size", STATUS_INVALID_VALUE)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device) if workspace is None else workspace
+    if x_scale is None:
+        fn, scale = "mla_linear_fp8_" + _suffix(x), ()
+    else:
+        assert x_scale.is_contiguous() and x_scale.shape == (m, -(-k // 128)) and x_scale.dtype == torch.float32
+        fn, scale = "mla_linear_fp8_quantized_" + _suffix(out), (_ptr(x_scale),)
+    _check(fn, getattr(lib, fn)(_ptr(x), *scale, _ptr(w), _ptr(w_scale), _ptr(out), _ptr(ws), ws.numel(), m, k, n,
+                                x.stride(0), w.stride(0), _stream(x)))
     return out
 
 

@@ -821,17 +821,17 @@ at::Tensor linear_fp8(const at::Tensor &x_in, const at::Tensor &w_in, const at::
     const at::Tensor x = as_rows(x_in, quantised ? 16 : 8), w = as_rows(w_in, 16), ws = ws_in.contiguous();
     const int m = static_cast<int>(rows), k = static_cast<int>(inputs), n = static_cast<int>(outputs);
     const int64_t x_stride = used_stride(x, 0, inputs), w_stride = used_stride(w, 0, inputs);
-    if (quantised) {
-        const at::Tensor xs = xs_in->contiguous();
-        auto f = dt == at::kHalf ? mla_linear_fp8_quantized_fp16 : mla_linear_fp8_quantized_bf16;
-        check_status(f(x.data_ptr(), xs.data_ptr<float>(), w.data_ptr(), ws.data_ptr<float>(), out.data_ptr(), m, k, n,
-                       x_stride, w_stride, stream_of(x)),
-                     fn);
-        return out;
-    }
     const size_t ws_bytes = mla_linear_fp8_workspace_size(m, k, n);
     TORCH_CHECK(ws_bytes > 0, fn, ": unsupported sizes");
     const at::Tensor space = workspace(ws_bytes, x);
+    if (quantised) {
+        const at::Tensor xs = xs_in->contiguous();
+        auto f = dt == at::kHalf ? mla_linear_fp8_quantized_fp16 : mla_linear_fp8_quantized_bf16;
+        check_status(f(x.data_ptr(), xs.data_ptr<float>(), w.data_ptr(), ws.data_ptr<float>(), out.data_ptr(), space.data_ptr(),
+                       ws_bytes, m, k, n, x_stride, w_stride, stream_of(x)),
+                     fn);
+        return out;
+    }
     auto f = dt == at::kHalf ? mla_linear_fp8_fp16 : mla_linear_fp8_bf16;
     check_status(f(x.data_ptr(), w.data_ptr(), ws.data_ptr<float>(), out.data_ptr(), space.data_ptr(), ws_bytes, m, k, n,
                    x_stride, w_stride, stream_of(x)),

@@ -12,6 +12,7 @@
 // cut off (towards 0), in all 1.5e-5 of a sum of N(0, 1) products, 2^-16, where the result's rounding is
 // 2^-9 (bf16) or 2^-12 (fp16). The 16 x 16 x 32 form does the same at half the rate.
 #include <algorithm>
+#include <cmath>
 #include <cstdint>
 
 #include "mla_device.hpp"
@@ -119,37 +120,42 @@ struct Linear {
     void *out;
     int rows, inputs, outputs, blocks;
     long long x_stride, w_stride, xs_row, xs_block;
+    float *parts;      // split calls: [splits][rows][outputs to a multiple of 4]
+    int split_blocks;  // blocks of a split
 };
 
-// A BN x BM tile of y (BN outputs, BM rows): 8 waves, kWN x kWM of them, each with its outputs as the A
+// A BN x BM tile of y (BN outputs, BM rows) by kWN x kWM waves, each with its outputs as the A
 // operand and its rows as B, so that a lane holds four outputs of one row and one scale serves them
-// all. Blocks of 128 inputs go through two LDS slots by direct loads: block b + 1 is on its way
-// while b is multiplied. 16-byte chunk c of row r sits at c ^ (r / 2 mod 8): rows are 128 bytes, two of them an
-// LDS bank period, so 16 rows' chunks are in 16 different places.
-template <int BN, int BM, int kWN, int kWM>
+// all. Blocks of 128 inputs go through kSlots LDS slots by direct loads, kSlots - 1 of them on
+// their way or in use; one barrier a block. 16-byte chunk c of row r sits at c ^ (r / 2 mod 8): rows are 128
+// bytes, two of them an LDS bank period, so 16 rows' chunks are in 16 different places.
+// A split call's workgroup takes `split_blocks` of the blocks and leaves its sums in fp32 (sum_kernel adds them).
+template <int BN, int BM, int kWN, int kWM, int kS>
 struct Tile {
-    static constexpr int kThreads = 64 * kWN * kWM;
+    static constexpr int kWaves = kWN * kWM, kThreads = 64 * kWaves, kSlots = kS;
     static constexpr int kN = BN / kWN, kM = BM / kWM;          // a wave's outputs and rows
     static constexpr int kNT = kN / 16, kMT = kM / 16;
-    static constexpr int kWUnits = BN / 8 / (kWN * kWM);        // loads of 8 rows, a wave and block: of W
-    static constexpr int kUnits = kWUnits + BM / 8 / (kWN * kWM);  // and of x
+    static constexpr int kWUnits = BN / 8 / kWaves;             // loads of 8 rows, a wave and block: of W
+    static constexpr int kUnits = kWUnits + BM / 8 / kWaves;    // and of x
+    static constexpr int kLoads = kUnits + 1;                   // and of 64 rows' scales
     static constexpr int kSlot = (BN + BM) * kBlock;
-    static constexpr int kScales = BM * 4;
-    static_assert(BN / 8 % (kWN * kWM) == 0 && BM / 8 % (kWN * kWM) == 0 && kBlock % kN == 0 && BM % 64 == 0, "tile split");
+    static_assert(BN / 8 % kWaves == 0 && BM / 8 % kWaves == 0 && kBlock % kN == 0 && BM % 64 == 0 &&
+                      kWaves % (BM / 64) == 0 && (kSlots - 2) * kLoads <= 63 && kSlots <= 4, "tile split");
 };
 
-template <typename E, int BN, int BM, int kWN, int kWM>
-__global__ __launch_bounds__((Tile<BN, BM, kWN, kWM>::kThreads)) void linear_kernel(Linear p)
+template <typename E, int BN, int BM, int kWN, int kWM, int kS>
+__global__ __launch_bounds__((Tile<BN, BM, kWN, kWM, kS>::kThreads)) void linear_kernel(Linear p)
 {
-    using T = Tile<BN, BM, kWN, kWM>;
+    using T = Tile<BN, BM, kWN, kWM, kS>;
     using E4 = typename Vec<E>::v4;
-    __shared__ __attribute__((aligned(1024))) unsigned char s_slot[2][T::kSlot];
-    __shared__ __attribute__((aligned(16))) float s_xs[2][BM];
+    __shared__ __attribute__((aligned(1024))) unsigned char s_slot[T::kSlots][T::kSlot];
+    __shared__ __attribute__((aligned(16))) float s_xs[T::kSlots][BM];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l16 = lane & 15, g = lane >> 4;
     const int n_tiles = (p.outputs + BN - 1) / BN;
     const int n0 = (int)(blockIdx.x % n_tiles) * BN, m0 = (int)(blockIdx.x / n_tiles) * BM;
     const int wn = wave % kWN * T::kN, wm = wave / kWN * T::kM;
+    const int b0 = (int)blockIdx.y * p.split_blocks, b1 = min(b0 + p.split_blocks, p.blocks);
 
     // Unit u of a block: rows 8 u .. 8 u + 7 of the slot (its BN weight rows, then its BM x rows); lane -> row
     // lane / 8, stored chunk lane % 8. Rows past the last re-read it.
@@ -165,12 +171,12 @@ __global__ __launch_bounds__((Tile<BN, BM, kWN, kWM>::kThreads)) void linear_ker
         off[i] = (i < T::kWUnits ? min(r, p.outputs - 1 - n0) * (int)p.w_stride : min(r - BN, p.rows - 1 - m0) * (int)p.x_stride) +
                  16 * chunk_of(u);
     }
-    int scale_off = 0;
-    if (wave < BM / 64)
-        scale_off = 4 * min(64 * wave + lane, p.rows - 1 - m0) * (int)p.xs_row;
+    // 64 rows' scales a wave (where there are more waves, several load the same), so that all have as many loads
+    const int scale_rows = 64 * (wave % (BM / 64));
+    const int scale_off = 4 * min(scale_rows + lane, p.rows - 1 - m0) * (int)p.xs_row;
     const int tail = p.inputs % kBlock / 16;  // whole chunks of the last block (0: all 8)
     auto issue = [&](int b) {
-        const unsigned lds = slot_lds + (b & 1) * T::kSlot;
+        const int at = (b - b0) % T::kSlots;
         const bool ragged = tail != 0 && b == p.blocks - 1;
 #pragma unroll
         for (int i = 0; i < T::kUnits; ++i) {
@@ -180,20 +186,24 @@ __global__ __launch_bounds__((Tile<BN, BM, kWN, kWM>::kThreads)) void linear_ker
                 const int c = chunk_of(u);
                 o -= c >= tail ? 16 * c : 0;
             }
-            global_to_lds16_at((i < T::kWUnits ? w_tile : x_tile) + (size_t)b * kBlock, o, lds + 1024 * u);
+            global_to_lds16_at((i < T::kWUnits ? w_tile : x_tile) + (size_t)b * kBlock, o, slot_lds + at * T::kSlot + 1024 * u);
         }
-        if (wave < BM / 64)
-            global_to_lds4_at(p.xs + m0 * p.xs_row + b * p.xs_block, scale_off, scale_lds + (b & 1) * T::kScales + 256 * wave);
+        global_to_lds4_at(p.xs + m0 * p.xs_row + b * p.xs_block, scale_off, scale_lds + (at * BM + scale_rows) * 4);
     };
-    // the wave's loads of block b have landed
+    // the wave's loads of block b have landed; those of the kSlots - 2 blocks behind it may be on their way
     auto landed = [&](int b) {
-        MLA_WAIT_VMCNT(0);
+        if (T::kSlots > 3 && b + 2 < b1)
+            MLA_WAIT_VMCNT(T::kSlots > 3 ? 2 * T::kLoads : 0);
+        else if (T::kSlots > 2 && b + 1 < b1)
+            MLA_WAIT_VMCNT(T::kSlots > 2 ? T::kLoads : 0);
+        else
+            MLA_WAIT_VMCNT(0);
         if (tail != 0 && b == p.blocks - 1) {
 #pragma unroll
             for (int i = 0; i < T::kUnits; ++i) {
                 const int u = unit(i);
                 if (chunk_of(u) >= tail)
-                    *(uint4 *)(&s_slot[b & 1][0] + 1024 * u + 16 * lane) = uint4{0, 0, 0, 0};
+                    *(uint4 *)(&s_slot[(b - b0) % T::kSlots][0] + 1024 * u + 16 * lane) = uint4{0, 0, 0, 0};
             }
         }
     };
@@ -203,13 +213,17 @@ __global__ __launch_bounds__((Tile<BN, BM, kWN, kWM>::kThreads)) void linear_ker
     // a lane's 32 bytes of a row: chunks 2 g and 2 g + 1
     const int lo_off = l16 * kBlock + 16 * ((2 * g) ^ (l16 >> 1)), hi_off = l16 * kBlock + 16 * ((2 * g + 1) ^ (l16 >> 1));
     float acc[T::kNT][T::kMT][4] = {};
-    issue(0);
-    landed(0);
-    lds_barrier();
-    for (int b = 0; b < p.blocks; ++b) {
-        if (b + 1 < p.blocks)
-            issue(b + 1);
-        const unsigned char *slot = &s_slot[b & 1][0];
+#pragma unroll
+    for (int k = 0; k < T::kSlots - 1; ++k)
+        if (b0 + k < b1)
+            issue(b0 + k);
+    for (int b = b0; b < b1; ++b) {
+        landed(b);
+        lds_barrier();  // block b is there for all waves, and none reads block b - 1 any more
+        if (b + T::kSlots - 1 < b1)
+            issue(b + T::kSlots - 1);
+        const int at = (b - b0) % T::kSlots;
+        const unsigned char *slot = &s_slot[at][0];
         // row l16 of the 16 rows from row0 (a multiple of 16) on
         auto operand = [&](int row0) {
             const uint4 lo = *(const uint4 *)(slot + row0 * kBlock + lo_off);
@@ -225,7 +239,7 @@ __global__ __launch_bounds__((Tile<BN, BM, kWN, kWM>::kThreads)) void linear_ker
             v[j] = operand(BN + wm + 16 * j);
 #pragma unroll
         for (int j = 0; j < T::kMT; ++j)
-            s[j] = s_xs[b & 1][wm + 16 * j + l16] * wscale;
+            s[j] = s_xs[at][wm + 16 * j + l16] * wscale;
         // the products of 16 outputs while those of the 16 before are scaled and added
         floatx4 d[2][T::kMT];
 #pragma unroll
@@ -248,12 +262,12 @@ __global__ __launch_bounds__((Tile<BN, BM, kWN, kWM>::kThreads)) void linear_ker
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
-        if (b + 1 < p.blocks)
-            landed(b + 1);
-        lds_barrier();
     }
+    // four outputs of a row are one aligned store where rows start at a multiple of four (partial sums always do)
+    const bool split = p.parts != nullptr;
+    const int stride = split ? (p.outputs + 3) / 4 * 4 : p.outputs;
+    float *parts = p.parts + (size_t)blockIdx.y * p.rows * stride;
     E *out = static_cast<E *>(p.out);
-    const bool whole = p.outputs % 4 == 0;  // four outputs of a row are one aligned store
 #pragma unroll
     for (int j = 0; j < T::kMT; ++j) {
         const int m = m0 + wm + 16 * j + l16;
@@ -262,16 +276,44 @@ __global__ __launch_bounds__((Tile<BN, BM, kWN, kWM>::kThreads)) void linear_ker
 #pragma unroll
         for (int i = 0; i < T::kNT; ++i) {
             const int n = n0 + wn + 16 * i + 4 * g;
-            E *to = out + (size_t)m * p.outputs + n;
-            const E4 y = {(E)acc[i][j][0], (E)acc[i][j][1], (E)acc[i][j][2], (E)acc[i][j][3]};
-            if (whole && n < p.outputs)
-                *(E4 *)to = y;
+            const size_t to = (size_t)m * stride + n;
+            const float *y = acc[i][j];
+            if (n >= p.outputs)
+                continue;
+            if (split)
+                *(floatx4 *)(parts + to) = floatx4{y[0], y[1], y[2], y[3]};
+            else if (stride % 4 == 0)
+                *(E4 *)(out + to) = E4{(E)y[0], (E)y[1], (E)y[2], (E)y[3]};
             else
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                     if (n + e < p.outputs)
-                        to[e] = y[e];
+                        out[to + e] = (E)y[e];
         }
+    }
+}
+
+// The splits' sums added, split after split, and rounded: four outputs a thread.
+template <typename E>
+__global__ __launch_bounds__(256) void sum_kernel(const float *__restrict__ parts, E *__restrict__ out, int splits, int rows,
+                                                  int outputs)
+{
+    const int quads = (outputs + 3) / 4;
+    const long long i = blockIdx.x * 256ll + threadIdx.x, all = (long long)rows * quads;
+    if (i >= all)
+        return;
+    const int m = (int)(i / quads), n = (int)(i % quads) * 4;
+    floatx4 y = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < splits; ++s)
+        y += *(const floatx4 *)(parts + (s * all + i) * 4);
+    E *to = out + (size_t)m * outputs + n;
+    if (outputs % 4 == 0) {
+        *(typename Vec<E>::v4 *)to = typename Vec<E>::v4{(E)y[0], (E)y[1], (E)y[2], (E)y[3]};
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (n + e < outputs)
+                to[e] = (E)y[e];
     }
 }
 
@@ -606,12 +648,21 @@ int launch_quantize(const void *x, void *q, float *scales, int rows, int inputs,
     return launched();
 }
 
-template <typename E, int BN, int BM, int kWN, int kWM>
-int launch_tiles(const Linear &p, hipStream_t s)
+template <typename E, int BN, int BM, int kWN, int kWM, int kS>
+int launch_tiles(Linear p, int splits, hipStream_t s)
 {
     const int64_t tiles = (int64_t)ceil_div(p.rows, BM) * ceil_div(p.outputs, BN);
-    hipLaunchKernelGGL((linear_kernel<E, BN, BM, kWN, kWM>), dim3((unsigned)tiles),
-                       dim3(Tile<BN, BM, kWN, kWM>::kThreads), 0, s, p);
+    p.split_blocks = ceil_div(p.blocks, splits);
+    splits = ceil_div(p.blocks, p.split_blocks);
+    if (splits == 1)
+        p.parts = nullptr;
+    hipLaunchKernelGGL((linear_kernel<E, BN, BM, kWN, kWM, kS>), dim3((unsigned)tiles, splits),
+                       dim3(Tile<BN, BM, kWN, kWM, kS>::kThreads), 0, s, p);
+    if (const int st = launched(); st || splits == 1)
+        return st;
+    const int64_t quads = (int64_t)p.rows * ceil_div(p.outputs, 4);
+    hipLaunchKernelGGL(sum_kernel<E>, dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, s, p.parts, static_cast<E *>(p.out),
+                       splits, p.rows, p.outputs);
     return launched();
 }
 
@@ -631,21 +682,61 @@ int launch_few(const Linear &p, hipStream_t s)
     return launched();
 }
 
-template <typename E>
-int launch_linear(const Linear &p, hipStream_t s)
+// ---- which kernel -----------------------------------------------------------
+
+enum class Form { kOwn, kFew, kTile64, kTile128, kTile256 };
+
+struct LinearPlan {
+    Form form;
+    int splits;
+};
+
+LinearPlan plan_linear(int rows, int inputs, int outputs)
 {
-    if (p.rows <= 64) {
-        const bool narrow = ceil_div(p.outputs, 16) <= current_cu_count();
-        if (p.rows <= 16)
-            return narrow ? launch_rows<E, 1, 1, false>(p, s) : launch_rows<E, 2, 1, false>(p, s);
-        if (p.rows <= 32)
-            return narrow ? launch_few<E, 1, 2>(p, s) : launch_few<E, 2, 2>(p, s);
-        return narrow ? launch_few<E, 1, 4>(p, s) : launch_few<E, 2, 4>(p, s);
+    const int blocks = ceil_div(inputs, kBlock), cus = current_cu_count();
+    if (rows <= 128)
+        return {Form::kFew, 1};
+    LinearPlan best{Form::kTile256, 1};
+    double best_us = 0.0;
+    struct Kind {
+        Form form;
+        int bn, bm;
+        double step_us;
+    };
+    for (const Kind &k : {Kind{Form::kTile256, 256, 256, 1.1}, Kind{Form::kTile128, 128, 128, 0.45}, Kind{Form::kTile64, 128, 64, 0.3}}) {
+        const int64_t tiles = (int64_t)ceil_div(rows, k.bm) * ceil_div(outputs, k.bn);
+        for (int splits = 1; splits <= std::min(blocks, 16); ++splits) {
+            const int per = ceil_div(blocks, splits);
+            if (ceil_div(blocks, per) != splits)
+                continue;
+            const double rounds = std::ceil((double)tiles * splits / cus);
+            double us = rounds * (per + 2) * k.step_us;
+            if (splits > 1)
+                us += 3.0 + 8.0e-6 * splits * rows * (double)outputs / 5.0;
+            if (best_us == 0.0 || us < best_us) {
+                best = {k.form, splits};
+                best_us = us;
+            }
+        }
     }
-    const int64_t large = (int64_t)ceil_div(p.rows, 256) * ceil_div(p.outputs, 256);
-    if (large >= current_cu_count())
-        return launch_tiles<E, 256, 256, 2, 4>(p, s);
-    return launch_tiles<E, 128, 64, 4, 2>(p, s);
+    return best;
+}
+
+template <typename E>
+int launch_linear(const Linear &p, const LinearPlan &plan, hipStream_t s)
+{
+    switch (plan.form) {
+    case Form::kTile256: return launch_tiles<E, 256, 256, 2, 4, 2>(p, plan.splits, s);
+    case Form::kTile128: return launch_tiles<E, 128, 128, 2, 2, 4>(p, plan.splits, s);
+    case Form::kTile64: return launch_tiles<E, 128, 64, 2, 2, 4>(p, plan.splits, s);
+    default: break;
+    }
+    const bool narrow = ceil_div(p.outputs, 16) <= current_cu_count();
+    if (p.rows <= 16)
+        return narrow ? launch_rows<E, 1, 1, false>(p, s) : launch_rows<E, 2, 1, false>(p, s);
+    if (p.rows <= 32)
+        return narrow ? launch_few<E, 1, 2>(p, s) : launch_few<E, 2, 2>(p, s);
+    return narrow ? launch_few<E, 1, 4>(p, s) : launch_few<E, 2, 4>(p, s);
 }
 
 // 16-bit rows few enough for every workgroup to quantise them
@@ -671,47 +762,44 @@ int quantize(bool bf16, const void *x, void *xq, float *scales, int rows, int in
                                                                        1, static_cast<hipStream_t>(stream));
 }
 
-// The quantised rows, then their scales, block by block: [blocks][rows].
-size_t rows_bytes(int rows, int inputs) { return ((size_t)rows * inputs + 255) / 256 * 256; }
+// The workspace: the quantised rows, their scales, block by block ([blocks][rows]), the splits' sums.
+size_t up256(size_t bytes) { return (bytes + 255) / 256 * 256; }
+size_t rows_bytes(int rows, int inputs) { return up256((size_t)rows * inputs); }
+size_t scales_bytes(int rows, int inputs) { return up256(4 * (size_t)rows * ceil_div(inputs, kBlock)); }
+size_t parts_bytes(int rows, int outputs, const LinearPlan &plan)
+{
+    return plan.splits > 1 ? 16 * (size_t)plan.splits * rows * ceil_div(outputs, 4) : 0;
+}
 
-int linear(bool bf16, const void *x, const void *w, const float *ws, void *out, void *workspace, size_t workspace_bytes,
-           int rows, int inputs, int outputs, long long x_stride, long long w_stride, void *stream)
+// xs null: x holds 16-bit rows, of type bf16 or fp16, else e4m3 ones
+int linear(bool bf16, const void *x, const float *xs, const void *w, const float *ws, void *out, void *workspace,
+           size_t workspace_bytes, int rows, int inputs, int outputs, long long x_stride, long long w_stride, void *stream)
 {
     if (!x || !w || !ws || !out || !workspace || !sizes_ok(rows, inputs, outputs) || x_stride < 0 || x_stride > kMostStride ||
         w_stride < 0 || w_stride > kMostStride)
         return MLA_STATUS_INVALID_VALUE;
-    if (!aligned16(x) || !aligned16(w) || !aligned16(out) || !aligned16(workspace) || x_stride % 8 != 0 || w_stride % 16 != 0)
+    if (!aligned16(x) || !aligned16(w) || !aligned16(out) || !aligned16(workspace) || x_stride % (xs ? 16 : 8) != 0 ||
+        w_stride % 16 != 0)
         return MLA_STATUS_MISALIGNED;
     if (workspace_bytes < mla_linear_fp8_workspace_size(rows, inputs, outputs))
         return MLA_STATUS_WORKSPACE_TOO_SMALL;
-    if (quantizes_itself(rows, inputs)) {
-        const Linear p{static_cast<const unsigned char *>(x), static_cast<const unsigned char *>(w), nullptr, ws, out, rows,
-                       inputs, outputs, ceil_div(inputs, kBlock), x_stride, w_stride, 0, 0};
-        return (bf16 ? launch_own<__bf16> : launch_own<_Float16>)(p, static_cast<hipStream_t>(stream));
-    }
-    auto *xq = static_cast<unsigned char *>(workspace);
-    auto *xs = reinterpret_cast<float *>(xq + rows_bytes(rows, inputs));
-    hipStream_t s = static_cast<hipStream_t>(stream);
-    if (const int st = (bf16 ? launch_quantize<__bf16> : launch_quantize<_Float16>)(x, xq, xs, rows, inputs, x_stride, inputs, 1,
-                                                                                   rows, s))
-        return st;
-    const Linear p{xq, static_cast<const unsigned char *>(w), xs, ws, out, rows, inputs, outputs, ceil_div(inputs, kBlock),
-                   inputs, w_stride, 1, rows};
-    return (bf16 ? launch_linear<__bf16> : launch_linear<_Float16>)(p, s);
-}
-
-int linear_quantized(bool bf16, const void *xq, const float *xs, const void *w, const float *ws, void *out, int rows,
-                     int inputs, int outputs, long long x_stride, long long w_stride, void *stream)
-{
-    if (!xq || !xs || !w || !ws || !out || !sizes_ok(rows, inputs, outputs) || x_stride < 0 || x_stride > kMostStride ||
-        w_stride < 0 || w_stride > kMostStride)
-        return MLA_STATUS_INVALID_VALUE;
-    if (!aligned16(xq) || !aligned16(w) || !aligned16(out) || x_stride % 16 != 0 || w_stride % 16 != 0)
-        return MLA_STATUS_MISALIGNED;
     const int blocks = ceil_div(inputs, kBlock);
-    const Linear p{static_cast<const unsigned char *>(xq), static_cast<const unsigned char *>(w), xs, ws, out, rows, inputs,
-                   outputs, blocks, x_stride, w_stride, blocks, 1};
-    return (bf16 ? launch_linear<__bf16> : launch_linear<_Float16>)(p, static_cast<hipStream_t>(stream));
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    Linear p{static_cast<const unsigned char *>(x), static_cast<const unsigned char *>(w), xs, ws, out, rows, inputs, outputs,
+             blocks, x_stride, w_stride, blocks, 1, nullptr, blocks};
+    if (!xs && quantizes_itself(rows, inputs))
+        return (bf16 ? launch_own<__bf16> : launch_own<_Float16>)(p, s);
+    auto *space = static_cast<unsigned char *>(workspace);
+    if (!xs) {
+        auto *scales = reinterpret_cast<float *>(space + rows_bytes(rows, inputs));
+        if (const int st = (bf16 ? launch_quantize<__bf16> : launch_quantize<_Float16>)(x, space, scales, rows, inputs, x_stride,
+                                                                                       inputs, 1, rows, s))
+            return st;
+        p.x = space, p.xs = scales, p.x_stride = inputs, p.xs_row = 1, p.xs_block = rows;
+    }
+    p.parts = reinterpret_cast<float *>(space + rows_bytes(rows, inputs) + scales_bytes(rows, inputs));
+    const LinearPlan plan = plan_linear(rows, inputs, outputs);
+    return (bf16 ? launch_linear<__bf16> : launch_linear<_Float16>)(p, plan, s);
 }
 
 }  // namespace
@@ -733,33 +821,44 @@ size_t mla_linear_fp8_workspace_size(int rows, int inputs, int outputs)
 {
     if (!mla::sizes_ok(rows, inputs, outputs))
         return 0;
-    return mla::rows_bytes(rows, inputs) + (4 * (size_t)rows * mla::ceil_div(inputs, mla::kBlock) + 255) / 256 * 256;
+    return mla::rows_bytes(rows, inputs) + mla::scales_bytes(rows, inputs) +
+           mla::parts_bytes(rows, outputs, mla::plan_linear(rows, inputs, outputs));
 }
 
 int mla_linear_fp8_fp16(const void *x, const void *w, const float *w_scale, void *out, void *workspace,
                         size_t workspace_bytes, int rows, int inputs, int outputs, long long x_stride, long long w_stride,
                         void *stream)
 {
-    return mla::linear(false, x, w, w_scale, out, workspace, workspace_bytes, rows, inputs, outputs, x_stride, w_stride, stream);
+    return mla::linear(false, x, nullptr, w, w_scale, out, workspace, workspace_bytes, rows, inputs, outputs, x_stride, w_stride,
+                       stream);
 }
 
 int mla_linear_fp8_bf16(const void *x, const void *w, const float *w_scale, void *out, void *workspace,
                         size_t workspace_bytes, int rows, int inputs, int outputs, long long x_stride, long long w_stride,
                         void *stream)
 {
-    return mla::linear(true, x, w, w_scale, out, workspace, workspace_bytes, rows, inputs, outputs, x_stride, w_stride, stream);
+    return mla::linear(true, x, nullptr, w, w_scale, out, workspace, workspace_bytes, rows, inputs, outputs, x_stride, w_stride,
+                       stream);
 }
 
 int mla_linear_fp8_quantized_fp16(const void *xq, const float *x_scale, const void *w, const float *w_scale, void *out,
-                                  int rows, int inputs, int outputs, long long x_stride, long long w_stride, void *stream)
+                                  void *workspace, size_t workspace_bytes, int rows, int inputs, int outputs,
+                                  long long x_stride, long long w_stride, void *stream)
 {
-    return mla::linear_quantized(false, xq, x_scale, w, w_scale, out, rows, inputs, outputs, x_stride, w_stride, stream);
+    if (!x_scale)
+        return MLA_STATUS_INVALID_VALUE;
+    return mla::linear(false, xq, x_scale, w, w_scale, out, workspace, workspace_bytes, rows, inputs, outputs, x_stride, w_stride,
+                       stream);
 }
 
 int mla_linear_fp8_quantized_bf16(const void *xq, const float *x_scale, const void *w, const float *w_scale, void *out,
-                                  int rows, int inputs, int outputs, long long x_stride, long long w_stride, void *stream)
+                                  void *workspace, size_t workspace_bytes, int rows, int inputs, int outputs,
+                                  long long x_stride, long long w_stride, void *stream)
 {
-    return mla::linear_quantized(true, xq, x_scale, w, w_scale, out, rows, inputs, outputs, x_stride, w_stride, stream);
+    if (!x_scale)
+        return MLA_STATUS_INVALID_VALUE;
+    return mla::linear(true, xq, x_scale, w, w_scale, out, workspace, workspace_bytes, rows, inputs, outputs, x_stride, w_stride,
+                       stream);
 }
 
 }  // extern "C"

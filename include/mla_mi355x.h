@@ -376,7 +376,8 @@ int mla_project_output_bf16(const void *o_star, const void *w_uv,
  *   out[m][n] = sum_b xs[m][b] w_scale[n / 128][b] sum_{k in b} xq[m][k] w[n][k]
  *   with x quantised so, w [outputs][inputs] E4M3FN (w_stride bytes apart) and
  *   w_scale [ceil(outputs / 128)][ceil(inputs / 128)]; sums in fp32, rounded
- *   once. The workspace holds the quantised rows.
+ *   once. The workspace holds the quantised rows, and fp32 sums where
+ *   the inputs are split over workgroups (the same bits whatever is in it).
  * mla_linear_fp8_quantized_*: the same of rows that are quantised already, xq
  *   (x_stride bytes apart) with x_scale [rows][ceil(inputs / 128)], and out in fp16 or bf16.
  * A NaN or infinity in a row of x makes its row of out NaN, a NaN in a row of w its
@@ -397,14 +398,16 @@ int mla_linear_fp8_bf16(const void *x, const void *w, const float *w_scale,
                         long long w_stride, void *stream);
 int mla_linear_fp8_quantized_fp16(const void *xq, const float *x_scale,
                                   const void *w, const float *w_scale,
-                                  void *out, int rows, int inputs, int outputs,
-                                  long long x_stride, long long w_stride,
-                                  void *stream);
+                                  void *out, void *workspace,
+                                  size_t workspace_bytes, int rows, int inputs,
+                                  int outputs, long long x_stride,
+                                  long long w_stride, void *stream);
 int mla_linear_fp8_quantized_bf16(const void *xq, const float *x_scale,
                                   const void *w, const float *w_scale,
-                                  void *out, int rows, int inputs, int outputs,
-                                  long long x_stride, long long w_stride,
-                                  void *stream);
+                                  void *out, void *workspace,
+                                  size_t workspace_bytes, int rows, int inputs,
+                                  int outputs, long long x_stride,
+                                  long long w_stride, void *stream);
 
 /* Block table, slots and positions of one step's tokens, from the requests'
  * lengths (no reference counterpart). All pointers are on the device and
