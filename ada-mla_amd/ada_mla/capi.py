@@ -72,8 +72,8 @@ _SIGNATURES = {
     "mla_linear_fp8_workspace_size": (_sz, [_i] * 3),
     "mla_linear_fp8_fp16": (_i, [_vp] * 5 + [_sz] + [_i] * 3 + [_ll, _ll, _vp]),
     "mla_linear_fp8_bf16": (_i, [_vp] * 5 + [_sz] + [_i] * 3 + [_ll, _ll, _vp]),
-    "mla_linear_fp8_quantized_fp16": (_i, [_vp] * 6 + [_sz] + [_i] * 3 + [_ll, _ll, _vp]),
-    "mla_linear_fp8_quantized_bf16": (_i, [_vp] * 6 + [_sz] + [_i] * 3 + [_ll, _ll, _vp]),
+    "mla_linear_fp8_quantized_fp16": (_i, [_vp] * 6 + [_sz] + [_i] * 3 + [_ll] * 4 + [_vp]),
+    "mla_linear_fp8_quantized_bf16": (_i, [_vp] * 6 + [_sz] + [_i] * 3 + [_ll] * 4 + [_vp]),
     "mla_page_tables_workspace_size": (_sz, [_i]),
     "mla_fork_tables": (_i, [_vp] * 12 + [_sz] + [_i] * 6 + [_vp]),
     "mla_compact_tables": (_i, [_vp] * 9 + [_sz] + [_i] * 5 + [_vp]),
@@ -414,16 +414,17 @@ def copy_pages(kv_cache, copies):
 
 
 def quantize_fp8(x):
-    """mla_quantize_fp8_*: x [M, K] (last dimension contiguous) -> (float8_e4m3fn [M, K], scales [M, ceil(K / 128)])."""
+    """mla_quantize_fp8_*: x [M, K] (last dimension contiguous) -> (float8_e4m3fn [M, K], scales [M, ceil(K / 128)],
+    a view of what the call writes block by block)."""
     import torch
     lib = load()
     m, k = x.shape
     assert x.stride(1) == 1
     q = torch.empty((m, k), dtype=torch.float8_e4m3fn, device=x.device)
-    scales = torch.empty((m, -(-k // 128)), dtype=torch.float32, device=x.device)
+    scales = torch.empty((-(-k // 128), m), dtype=torch.float32, device=x.device)
     fn = "mla_quantize_fp8_" + _suffix(x)
     _check(fn, getattr(lib, fn)(_ptr(x), _ptr(q), _ptr(scales), m, k, x.stride(0), _stream(x)))
-    return q, scales
+    return q, scales.t()
 
 
 def linear_fp8(x, w, w_scale, x_scale=None, dtype=None, out=None, workspace=None):
@@ -441,12 +442,12 @@ def linear_fp8(x, w, w_scale, x_scale=None, dtype=None, out=None, workspace=None
         raise MlaError("mla_linear_fp8_workspace_size", STATUS_INVALID_VALUE)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device) if workspace is None else workspace
     if x_scale is None:
-        fn, scale = "mla_linear_fp8_" + _suffix(x), ()
+        fn, scale, strides = "mla_linear_fp8_" + _suffix(x), (), ()
     else:
-        assert x_scale.is_contiguous() and x_scale.shape == (m, -(-k // 128)) and x_scale.dtype == torch.float32
-        fn, scale = "mla_linear_fp8_quantized_" + _suffix(out), (_ptr(x_scale),)
+        assert x_scale.shape == (m, -(-k // 128)) and x_scale.dtype == torch.float32
+        fn, scale, strides = "mla_linear_fp8_quantized_" + _suffix(out), (_ptr(x_scale),), x_scale.stride()
     _check(fn, getattr(lib, fn)(_ptr(x), *scale, _ptr(w), _ptr(w_scale), _ptr(out), _ptr(ws), ws.numel(), m, k, n,
-                                x.stride(0), w.stride(0), _stream(x)))
+                                x.stride(0), w.stride(0), *strides, _stream(x)))
     return out
 
 

@@ -777,15 +777,19 @@ std::vector<at::Tensor> quantize_fp8(const at::Tensor &x_in)
     const at::OptionalDeviceGuard guard(x_in.device());
     const auto options = x_in.options().memory_format(at::MemoryFormat::Contiguous);
     at::Tensor q = at::empty(x_in.sizes(), options.dtype(at::kFloat8_e4m3fn));
-    at::Tensor scales = at::empty(with_last(x_in, blocks), options.dtype(at::kFloat));
+    // block by block in memory: [..., blocks] is a view of [blocks, ...]
+    std::vector<int64_t> sizes = x_in.sizes().vec();
+    sizes.pop_back();
+    sizes.insert(sizes.begin(), blocks);
+    at::Tensor scales = at::empty(sizes, options.dtype(at::kFloat));
     if (rows == 0)
-        return {q, scales};
+        return {q, scales.movedim(0, -1)};
     const at::Tensor x = as_rows(x_in, 8);
     auto f = dt == at::kHalf ? mla_quantize_fp8_fp16 : mla_quantize_fp8_bf16;
     check_status(f(x.data_ptr(), q.data_ptr(), scales.data_ptr<float>(), static_cast<int>(rows), static_cast<int>(inputs),
                    used_stride(x, 0, inputs), stream_of(x)),
                  fn);
-    return {q, scales};
+    return {q, scales.movedim(0, -1)};
 }
 
 // No reference code: y = x W^T with W in e4m3 and a scale for each 128 x 128 values.
@@ -825,10 +829,13 @@ at::Tensor linear_fp8(const at::Tensor &x_in, const at::Tensor &w_in, const at::
     TORCH_CHECK(ws_bytes > 0, fn, ": unsupported sizes");
     const at::Tensor space = workspace(ws_bytes, x);
     if (quantised) {
-        const at::Tensor xs = xs_in->contiguous();
+        // rows and blocks any distance apart; leading dimensions that do not make one are copied
+        at::Tensor xs = xs_in->dim() == 2 ? *xs_in : xs_in->reshape({-1, blocks});
+        if (xs.size(0) > 1 && xs.stride(0) > (1 << 22))
+            xs = xs.contiguous();
         auto f = dt == at::kHalf ? mla_linear_fp8_quantized_fp16 : mla_linear_fp8_quantized_bf16;
         check_status(f(x.data_ptr(), xs.data_ptr<float>(), w.data_ptr(), ws.data_ptr<float>(), out.data_ptr(), space.data_ptr(),
-                       ws_bytes, m, k, n, x_stride, w_stride, stream_of(x)),
+                       ws_bytes, m, k, n, x_stride, w_stride, used_stride(xs, 0, 0), used_stride(xs, 1, 0), stream_of(x)),
                      fn);
         return out;
     }
@@ -872,8 +879,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
           "w_o [d_model,n_h*128])",
           pybind11::arg("o_star"), pybind11::arg("w_uv"), pybind11::arg("w_o"));
     m.def("mla_quantize_fp8", &quantize_fp8,
-          "(x in float8_e4m3fn, scales float32 [..., ceil(inputs/128)]) of float16 or bfloat16 x [..., inputs]: each 128 "
-          "values' largest at 448",
+          "(x in float8_e4m3fn, scales float32 [..., ceil(inputs/128)], block by block in memory) of float16 or bfloat16 x "
+          "[..., inputs]: each 128 values' largest at 448",
           pybind11::arg("x"));
     m.def("mla_linear_fp8", &linear_fp8,
           "x W^T [..., outputs] of x [..., inputs] (float16 or bfloat16, quantised as mla_quantize_fp8 does; or "

@@ -128,7 +128,8 @@ struct Linear {
 // operand and its rows as B, so that a lane holds four outputs of one row and one scale serves them
 // all. Blocks of 128 inputs go through kSlots LDS slots by direct loads, kSlots - 1 of them on
 // their way or in use; one barrier a block. 16-byte chunk c of row r sits at c ^ (r / 2 mod 8): rows are 128
-// bytes, two of them an LDS bank period, so 16 rows' chunks are in 16 different places.
+// bytes, two of them an LDS bank period, so chunk g of 16 rows is in 16 different places, and so are those of
+// the 8 rows and 8 others of the next g that the LDS reads at once (chunks 2 g, 2 g + 1: half of its cycles were conflicts).
 // A split call's workgroup takes `split_blocks` of the blocks and leaves its sums in fp32 (sum_kernel adds them).
 template <int BN, int BM, int kWN, int kWM, int kS>
 struct Tile {
@@ -207,11 +208,10 @@ __global__ __launch_bounds__((Tile<BN, BM, kWN, kWM, kS>::kThreads)) void linear
             }
         }
     };
-    const auto *ws = (const __attribute__((address_space(4))) float *)p.ws +
-                     (size_t)min((n0 + wn) / kBlock, (p.outputs - 1) / kBlock) * p.blocks;
-
-    // a lane's 32 bytes of a row: chunks 2 g and 2 g + 1
-    const int lo_off = l16 * kBlock + 16 * ((2 * g) ^ (l16 >> 1)), hi_off = l16 * kBlock + 16 * ((2 * g + 1) ^ (l16 >> 1));
+    const float *ws = p.ws + (size_t)min((n0 + wn) / kBlock, (p.outputs - 1) / kBlock) * p.blocks;
+    float wscales = 0.f;  // of the next 64 blocks, one a lane (a scalar load would be waited for with every LDS read)
+    // a lane's 32 bytes of a row: chunks g and g + 4 (which inputs stand in which lane is free, W and x alike)
+    const int lo_off = l16 * kBlock + 16 * (g ^ (l16 >> 1)), hi_off = l16 * kBlock + 16 * ((g + 4) ^ (l16 >> 1));
     float acc[T::kNT][T::kMT][4] = {};
 #pragma unroll
     for (int k = 0; k < T::kSlots - 1; ++k)
@@ -230,7 +230,11 @@ __global__ __launch_bounds__((Tile<BN, BM, kWN, kWM, kS>::kThreads)) void linear
             const uint4 hi = *(const uint4 *)(slot + row0 * kBlock + hi_off);
             return intx8{(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w, (int)hi.x, (int)hi.y, (int)hi.z, (int)hi.w};
         };
-        const float wscale = ws[b];
+        if (((b - b0) & 63) == 0) {
+            wscales = ws[min(b + lane, p.blocks - 1)];
+            asm volatile("" : "+v"(wscales));
+        }
+        const float wscale = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(wscales), (b - b0) & 63));
         intx8 v[T::kMT], a[2];
         float s[T::kMT];
         a[0] = operand(wn);
@@ -547,7 +551,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_few_kernel(Linear p)
         issue(0);
     if (mine > 1)
         issue(1);
-    const int lo_off = l16 * kBlock + 16 * ((2 * g) ^ (l16 >> 1)), hi_off = l16 * kBlock + 16 * ((2 * g + 1) ^ (l16 >> 1));
+    const int lo_off = l16 * kBlock + 16 * (g ^ (l16 >> 1)), hi_off = l16 * kBlock + 16 * ((g + 4) ^ (l16 >> 1));
     float acc[NT][MT][4] = {};
     for (int it = 0; it < mine; ++it) {
         if (it + 2 < mine) {
@@ -757,9 +761,8 @@ int quantize(bool bf16, const void *x, void *xq, float *scales, int rows, int in
         return MLA_STATUS_INVALID_VALUE;
     if (!aligned16(x) || !aligned16(xq) || x_stride % 8 != 0)
         return MLA_STATUS_MISALIGNED;
-    const int blocks = ceil_div(inputs, kBlock);
-    return (bf16 ? launch_quantize<__bf16> : launch_quantize<_Float16>)(x, xq, scales, rows, inputs, x_stride, inputs, blocks,
-                                                                       1, static_cast<hipStream_t>(stream));
+    return (bf16 ? launch_quantize<__bf16> : launch_quantize<_Float16>)(x, xq, scales, rows, inputs, x_stride, inputs, 1, rows,
+                                                                       static_cast<hipStream_t>(stream));
 }
 
 // The workspace: the quantised rows, their scales, block by block ([blocks][rows]), the splits' sums.
@@ -773,10 +776,11 @@ size_t parts_bytes(int rows, int outputs, const LinearPlan &plan)
 
 // xs null: x holds 16-bit rows, of type bf16 or fp16, else e4m3 ones
 int linear(bool bf16, const void *x, const float *xs, const void *w, const float *ws, void *out, void *workspace,
-           size_t workspace_bytes, int rows, int inputs, int outputs, long long x_stride, long long w_stride, void *stream)
+           size_t workspace_bytes, int rows, int inputs, int outputs, long long x_stride, long long w_stride,
+           long long xs_row, long long xs_block, void *stream)
 {
     if (!x || !w || !ws || !out || !workspace || !sizes_ok(rows, inputs, outputs) || x_stride < 0 || x_stride > kMostStride ||
-        w_stride < 0 || w_stride > kMostStride)
+        w_stride < 0 || w_stride > kMostStride || xs_row < 0 || xs_row > kMostStride || xs_block < 0)
         return MLA_STATUS_INVALID_VALUE;
     if (!aligned16(x) || !aligned16(w) || !aligned16(out) || !aligned16(workspace) || x_stride % (xs ? 16 : 8) != 0 ||
         w_stride % 16 != 0)
@@ -786,7 +790,7 @@ int linear(bool bf16, const void *x, const float *xs, const void *w, const float
     const int blocks = ceil_div(inputs, kBlock);
     hipStream_t s = static_cast<hipStream_t>(stream);
     Linear p{static_cast<const unsigned char *>(x), static_cast<const unsigned char *>(w), xs, ws, out, rows, inputs, outputs,
-             blocks, x_stride, w_stride, blocks, 1, nullptr, blocks};
+             blocks, x_stride, w_stride, xs_row, xs_block, nullptr, blocks};
     if (!xs && quantizes_itself(rows, inputs))
         return (bf16 ? launch_own<__bf16> : launch_own<_Float16>)(p, s);
     auto *space = static_cast<unsigned char *>(workspace);
@@ -830,7 +834,7 @@ int mla_linear_fp8_fp16(const void *x, const void *w, const float *w_scale, void
                         void *stream)
 {
     return mla::linear(false, x, nullptr, w, w_scale, out, workspace, workspace_bytes, rows, inputs, outputs, x_stride, w_stride,
-                       stream);
+                       0, 0, stream);
 }
 
 int mla_linear_fp8_bf16(const void *x, const void *w, const float *w_scale, void *out, void *workspace,
@@ -838,27 +842,29 @@ int mla_linear_fp8_bf16(const void *x, const void *w, const float *w_scale, void
                         void *stream)
 {
     return mla::linear(true, x, nullptr, w, w_scale, out, workspace, workspace_bytes, rows, inputs, outputs, x_stride, w_stride,
-                       stream);
+                       0, 0, stream);
 }
 
 int mla_linear_fp8_quantized_fp16(const void *xq, const float *x_scale, const void *w, const float *w_scale, void *out,
                                   void *workspace, size_t workspace_bytes, int rows, int inputs, int outputs,
-                                  long long x_stride, long long w_stride, void *stream)
+                                  long long x_stride, long long w_stride, long long scale_row_stride,
+                                  long long scale_block_stride, void *stream)
 {
     if (!x_scale)
         return MLA_STATUS_INVALID_VALUE;
     return mla::linear(false, xq, x_scale, w, w_scale, out, workspace, workspace_bytes, rows, inputs, outputs, x_stride, w_stride,
-                       stream);
+                       scale_row_stride, scale_block_stride, stream);
 }
 
 int mla_linear_fp8_quantized_bf16(const void *xq, const float *x_scale, const void *w, const float *w_scale, void *out,
                                   void *workspace, size_t workspace_bytes, int rows, int inputs, int outputs,
-                                  long long x_stride, long long w_stride, void *stream)
+                                  long long x_stride, long long w_stride, long long scale_row_stride,
+                                  long long scale_block_stride, void *stream)
 {
     if (!x_scale)
         return MLA_STATUS_INVALID_VALUE;
     return mla::linear(true, xq, x_scale, w, w_scale, out, workspace, workspace_bytes, rows, inputs, outputs, x_stride, w_stride,
-                       stream);
+                       scale_row_stride, scale_block_stride, stream);
 }
 
 }  // extern "C"

@@ -368,7 +368,7 @@ int mla_project_output_bf16(const void *o_star, const void *w_uv,
  * code).
  *
  * mla_quantize_fp8_*: rows x [rows][inputs] (x_stride values apart) in fp16 or bf16 ->
- *   xq [rows][inputs] and scales [rows][ceil(inputs / 128)]: a block's scale is
+ *   xq [rows][inputs] and scales [ceil(inputs / 128)][rows]: a block's scale is
  *   top / 448 with top = max(max |x|, 2^-100), its values xq = e4m3(448 x / top)
  *   (to nearest even). An infinity makes its block's values NaN and its scale
  *   infinite, a NaN stays one.
@@ -379,7 +379,9 @@ int mla_project_output_bf16(const void *o_star, const void *w_uv,
  *   once. The workspace holds the quantised rows, and fp32 sums where
  *   the inputs are split over workgroups (the same bits whatever is in it).
  * mla_linear_fp8_quantized_*: the same of rows that are quantised already, xq
- *   (x_stride bytes apart) with x_scale [rows][ceil(inputs / 128)], and out in fp16 or bf16.
+ *   (x_stride bytes apart), and out in fp16 or bf16; the scale of row m and block b is
+ *   x_scale[m scale_row_stride + b scale_block_stride] (1 and rows as mla_quantize_fp8_*
+ *   leaves them, which is read fastest).
  * A NaN or infinity in a row of x makes its row of out NaN, a NaN in a row of w its
  * column. inputs must be a multiple of 16, strides of 8 values (16-bit rows) or 16 bytes, and
  * inputs and strides at most 2^22; rows and outputs at most 2^26. */
@@ -401,13 +403,17 @@ int mla_linear_fp8_quantized_fp16(const void *xq, const float *x_scale,
                                   void *out, void *workspace,
                                   size_t workspace_bytes, int rows, int inputs,
                                   int outputs, long long x_stride,
-                                  long long w_stride, void *stream);
+                                  long long w_stride,
+                                  long long scale_row_stride,
+                                  long long scale_block_stride, void *stream);
 int mla_linear_fp8_quantized_bf16(const void *xq, const float *x_scale,
                                   const void *w, const float *w_scale,
                                   void *out, void *workspace,
                                   size_t workspace_bytes, int rows, int inputs,
                                   int outputs, long long x_stride,
-                                  long long w_stride, void *stream);
+                                  long long w_stride,
+                                  long long scale_row_stride,
+                                  long long scale_block_stride, void *stream);
 
 /* Block table, slots and positions of one step's tokens, from the requests'
  * lengths (no reference counterpart). All pointers are on the device and

@@ -142,6 +142,11 @@ def test_sizes(dtype, m, k, n):
     z = ada_mla.mla_linear_fp8(q, w.cuda(), ws.cuda(), x_scale=s, dtype=dtype)
     _check(z, xq, xs, w, ws, dtype, "quantised rows")
     assert torch.equal(z, capi.linear_fp8(q, w.cuda(), ws.cuda(), x_scale=s, dtype=dtype))
+    # scales in any order of memory
+    assert torch.equal(z, ada_mla.mla_linear_fp8(q, w.cuda(), ws.cuda(), x_scale=s.contiguous(), dtype=dtype))
+    apart = torch.full((m, 2, -(-k // 128), 3), float("nan"), device="cuda")
+    apart[:, 1, :, 1] = s
+    assert torch.equal(z, ada_mla.mla_linear_fp8(q, w.cuda(), ws.cuda(), x_scale=apart[:, 1, :, 1], dtype=dtype))
 
 
 @pytest.mark.parametrize("m,k,n", [(3, 272, 200), (40, 640, 130), (150, 1000 // 16 * 16, 300)])
