@@ -831,7 +831,7 @@ at::Tensor linear_fp8(const at::Tensor &x_in, const at::Tensor &w_in, const at::
     if (quantised) {
         // rows and blocks any distance apart; leading dimensions that do not make one are copied
         at::Tensor xs = xs_in->dim() == 2 ? *xs_in : xs_in->reshape({-1, blocks});
-        if (xs.size(0) > 1 && xs.stride(0) > (1 << 22))
+        if (xs.size(0) > 1 && xs.stride(0) > (1 << 20))
             xs = xs.contiguous();
         auto f = dt == at::kHalf ? mla_linear_fp8_quantized_fp16 : mla_linear_fp8_quantized_bf16;
         check_status(f(x.data_ptr(), xs.data_ptr<float>(), w.data_ptr(), ws.data_ptr<float>(), out.data_ptr(), space.data_ptr(),

@@ -14,6 +14,8 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <type_traits>
+#include <utility>
 
 #include "mla_device.hpp"
 #include "mla_internal.hpp"
@@ -124,24 +126,43 @@ struct Linear {
     int split_blocks;  // blocks of a split
 };
 
+// body(0), body(1), .. body(N - 1), each with its number as a constant
+template <int N, typename F, int... I>
+__device__ __forceinline__ void each_of(F &&body, std::integer_sequence<int, I...>)
+{
+    (body(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void each_of(F &&body)
+{
+    each_of<N>(body, std::make_integer_sequence<int, N>{});
+}
+
 // A BN x BM tile of y (BN outputs, BM rows) by kWN x kWM waves, each with its outputs as the A
 // operand and its rows as B, so that a lane holds four outputs of one row and one scale serves them
-// all. Blocks of 128 inputs go through kSlots LDS slots by direct loads, kSlots - 1 of them on
-// their way or in use; one barrier a block. 16-byte chunk c of row r sits at c ^ (r / 2 mod 8): rows are 128
+// all. Blocks of 128 inputs go through kSlots LDS slots by direct loads. A wave's rows of block b + 1 are read
+// into registers, and the loads of block b + kSlots - 1 issued, between the products of block b: behind the one barrier of a
+// block only the first outputs' operand has to be read before products run (with the rows read there, 256 x
+// 256 tiles took 3190 cycles a block, 730 of them for those reads, where the products take 2110).
+// 16-byte chunk c of row r sits at c ^ (r / 2 mod 8): rows are 128
 // bytes, two of them an LDS bank period, so chunk g of 16 rows is in 16 different places, and so are those of
 // the 8 rows and 8 others of the next g that the LDS reads at once (chunks 2 g, 2 g + 1: half of its cycles were conflicts).
 // A split call's workgroup takes `split_blocks` of the blocks and leaves its sums in fp32 (sum_kernel adds them).
 template <int BN, int BM, int kWN, int kWM, int kS>
 struct Tile {
     static constexpr int kWaves = kWN * kWM, kThreads = 64 * kWaves, kSlots = kS;
-    static constexpr int kN = BN / kWN, kM = BM / kWM;          // a wave's outputs and rows
+    static constexpr int kN = BN / kWN, kM = BM / kWM;  // a wave's outputs and rows
     static constexpr int kNT = kN / 16, kMT = kM / 16;
-    static constexpr int kWUnits = BN / 8 / kWaves;             // loads of 8 rows, a wave and block: of W
-    static constexpr int kUnits = kWUnits + BM / 8 / kWaves;    // and of x
-    static constexpr int kLoads = kUnits + 1;                   // and of 64 rows' scales
-    static constexpr int kSlot = (BN + BM) * kBlock;
+    static constexpr int kWUnits = BN / 8 / kWaves;     // loads of 8 rows, a wave and block: of W
+    static constexpr int kXUnits = BM / 8 / kWaves;     // and of x
+    static constexpr int kLoads = kWUnits + kXUnits + 1;  // and of 64 rows' scales
+    static constexpr int kProducts = kNT * kMT;
+    // a second set of registers for the next block's rows; a wave with 32 products has none to spare and reads each
+    // where its last product has been issued
+    static constexpr bool kTwo = kProducts <= 16;
     static_assert(BN / 8 % kWaves == 0 && BM / 8 % kWaves == 0 && kBlock % kN == 0 && BM % 64 == 0 &&
-                      kWaves % (BM / 64) == 0 && (kSlots - 2) * kLoads <= 63 && kSlots <= 4, "tile split");
+                      (kSlots - 1) * kLoads <= 63 && kSlots >= 2 && kSlots <= 4 &&
+                      kProducts + 2 >= kLoads && kProducts >= 8, "tile split");
 };
 
 template <typename E, int BN, int BM, int kWN, int kWM, int kS>
@@ -149,7 +170,7 @@ __global__ __launch_bounds__((Tile<BN, BM, kWN, kWM, kS>::kThreads)) void linear
 {
     using T = Tile<BN, BM, kWN, kWM, kS>;
     using E4 = typename Vec<E>::v4;
-    __shared__ __attribute__((aligned(1024))) unsigned char s_slot[T::kSlots][T::kSlot];
+    __shared__ __attribute__((aligned(1024))) unsigned char s_w[T::kSlots][BN * kBlock], s_x[T::kSlots][BM * kBlock];
     __shared__ __attribute__((aligned(16))) float s_xs[T::kSlots][BM];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l16 = lane & 15, g = lane >> 4;
@@ -158,115 +179,171 @@ __global__ __launch_bounds__((Tile<BN, BM, kWN, kWM, kS>::kThreads)) void linear
     const int wn = wave % kWN * T::kN, wm = wave / kWN * T::kM;
     const int b0 = (int)blockIdx.y * p.split_blocks, b1 = min(b0 + p.split_blocks, p.blocks);
 
-    // Unit u of a block: rows 8 u .. 8 u + 7 of the slot (its BN weight rows, then its BM x rows); lane -> row
-    // lane / 8, stored chunk lane % 8. Rows past the last re-read it.
-    const unsigned slot_lds = (unsigned)(uintptr_t)(const MLA_LDS unsigned char *)&s_slot[0][0];
-    const unsigned scale_lds = (unsigned)(uintptr_t)(const MLA_LDS float *)&s_xs[0][0];
-    const unsigned char *w_tile = p.w + n0 * p.w_stride, *x_tile = p.x + m0 * p.x_stride;
-    auto unit = [&](int i) { return i < T::kWUnits ? wave * T::kWUnits + i : BN / 8 + wave * (T::kUnits - T::kWUnits) + i - T::kWUnits; };
-    auto chunk_of = [&](int u) { return (lane & 7) ^ (((8 * u + (lane >> 3)) >> 1) & 7); };
-    int off[T::kUnits];
+    // Unit u of a block's W (or x): rows 8 u .. 8 u + 7; lane -> row lane / 8, stored chunk lane % 8. Rows past the last
+    // re-read it. A load costs its issue: its offset is kept in a register, its addresses are formed once a block.
+    const int n_last = p.outputs - 1 - n0, m_last = p.rows - 1 - m0;
+    auto chunk_of = [&](int u) { return (lane & 7) ^ ((4 * u + (lane >> 4)) & 7); };
+    int w_off[T::kWUnits], x_off[T::kXUnits];
 #pragma unroll
-    for (int i = 0; i < T::kUnits; ++i) {
-        const int u = unit(i), r = 8 * u + (lane >> 3);
-        off[i] = (i < T::kWUnits ? min(r, p.outputs - 1 - n0) * (int)p.w_stride : min(r - BN, p.rows - 1 - m0) * (int)p.x_stride) +
-                 16 * chunk_of(u);
+    for (int i = 0; i < T::kWUnits; ++i) {
+        const int u = wave * T::kWUnits + i;
+        w_off[i] = min(8 * u + (lane >> 3), n_last) * (int)p.w_stride + 16 * chunk_of(u);
+    }
+#pragma unroll
+    for (int i = 0; i < T::kXUnits; ++i) {
+        const int u = wave * T::kXUnits + i;
+        x_off[i] = min(8 * u + (lane >> 3), m_last) * (int)p.x_stride + 16 * chunk_of(u);
     }
     // 64 rows' scales a wave (where there are more waves, several load the same), so that all have as many loads
     const int scale_rows = 64 * (wave % (BM / 64));
-    const int scale_off = 4 * min(scale_rows + lane, p.rows - 1 - m0) * (int)p.xs_row;
-    const int tail = p.inputs % kBlock / 16;  // whole chunks of the last block (0: all 8)
-    auto issue = [&](int b) {
-        const int at = (b - b0) % T::kSlots;
-        const bool ragged = tail != 0 && b == p.blocks - 1;
-#pragma unroll
-        for (int i = 0; i < T::kUnits; ++i) {
-            const int u = unit(i);
-            int o = off[i];
-            if (ragged) {  // chunks behind the inputs' end read the block's first, and are cleared afterwards
-                const int c = chunk_of(u);
-                o -= c >= tail ? 16 * c : 0;
-            }
-            global_to_lds16_at((i < T::kWUnits ? w_tile : x_tile) + (size_t)b * kBlock, o, slot_lds + at * T::kSlot + 1024 * u);
-        }
-        global_to_lds4_at(p.xs + m0 * p.xs_row + b * p.xs_block, scale_off, scale_lds + (at * BM + scale_rows) * 4);
+    const int scale_off = 4 * min(scale_rows + lane, m_last) * (int)p.xs_row;
+    const unsigned w_lds = (unsigned)(uintptr_t)(const MLA_LDS unsigned char *)&s_w[0][0] + 1024 * wave * T::kWUnits;
+    const unsigned x_lds = (unsigned)(uintptr_t)(const MLA_LDS unsigned char *)&s_x[0][0] + 1024 * wave * T::kXUnits;
+    const unsigned scale_lds = (unsigned)(uintptr_t)(const MLA_LDS float *)&s_xs[0][0] + 4 * scale_rows;
+    const unsigned char *const w_tile = p.w + n0 * p.w_stride, *const x_tile = p.x + m0 * p.x_stride;
+    const float *const xs_tile = p.xs + m0 * p.xs_row;
+    // First byte of a block. A last block that the inputs do not fill is their last 128 instead (there are as many:
+    // plan_linear), whose chunks that the block before it holds too, all but the last `tail`, are cleared when they have landed.
+    // Behind the workgroup's last block come that one's bytes again, so that every group has as many loads and none
+    // stands under a condition.
+    const int tail = p.inputs % kBlock / 16;  // 0: the last block is whole
+    auto byte_of = [&](int b) { return (size_t)min(min(b, b1 - 1) * kBlock, p.inputs - kBlock); };
+    auto slot_of = [&](int b) { return (b - b0) % T::kSlots; };
+    // The loads of group b: W and the scales of block b, x of block b + 1.
+    struct Group {
+        const unsigned char *w, *x;
+        const float *xs;
+        unsigned w_lds, x_lds, scale_lds;
     };
-    // the wave's loads of block b have landed; those of the kSlots - 2 blocks behind it may be on their way
-    auto landed = [&](int b) {
-        if (T::kSlots > 3 && b + 2 < b1)
-            MLA_WAIT_VMCNT(T::kSlots > 3 ? 2 * T::kLoads : 0);
-        else if (T::kSlots > 2 && b + 1 < b1)
-            MLA_WAIT_VMCNT(T::kSlots > 2 ? T::kLoads : 0);
+    auto group = [&](int b) {
+        return Group{w_tile + byte_of(b), x_tile + byte_of(b + 1), xs_tile + min(b, b1 - 1) * p.xs_block,
+                     w_lds + slot_of(b) * BN * kBlock, x_lds + slot_of(b + 1) * BM * kBlock, scale_lds + slot_of(b) * BM * 4};
+    };
+    auto issue = [&](const Group &q, auto kIndex) {
+        constexpr int i = decltype(kIndex)::value;
+        if constexpr (i < T::kWUnits)
+            global_to_lds16_plus<1024 * i>(q.w, w_off[i], q.w_lds);
+        else if constexpr (i < T::kWUnits + T::kXUnits)
+            global_to_lds16_plus<1024 * (i - T::kWUnits)>(q.x, x_off[i - T::kWUnits], q.x_lds);
         else
-            MLA_WAIT_VMCNT(0);
-        if (tail != 0 && b == p.blocks - 1) {
+            global_to_lds4_at(q.xs, scale_off, q.scale_lds);
+    };
+    auto clear_unit = [&](unsigned char *slot, int u) {
+        if (chunk_of(u) < 8 - tail)
+            *(uint4 *)(slot + 1024 * u + 16 * lane) = uint4{0, 0, 0, 0};
+    };
+    auto clear_x = [&](int b) {
+        if (tail != 0 && b == p.blocks - 1)
 #pragma unroll
-            for (int i = 0; i < T::kUnits; ++i) {
-                const int u = unit(i);
-                if (chunk_of(u) >= tail)
-                    *(uint4 *)(&s_slot[(b - b0) % T::kSlots][0] + 1024 * u + 16 * lane) = uint4{0, 0, 0, 0};
-            }
+            for (int i = 0; i < T::kXUnits; ++i)
+                clear_unit(&s_x[slot_of(b)][0], wave * T::kXUnits + i);
+    };
+    // the wave's loads of group b have landed; those of the kSlots - 2 groups behind it may be on their way
+    auto landed = [&](int b) {
+        MLA_WAIT_VMCNT((T::kSlots - 2) * T::kLoads);
+        if (tail != 0 && b + 1 >= p.blocks - 1) {
+            if (b == p.blocks - 1)
+#pragma unroll
+                for (int i = 0; i < T::kWUnits; ++i)
+                    clear_unit(&s_w[slot_of(b)][0], wave * T::kWUnits + i);
+            clear_x(b + 1);
         }
+    };
+    // A lane's 32 bytes of row l16 of 16 rows: chunks g and g + 4 (which inputs stand in which lane is free, W and x alike).
+    const int lo_off = l16 * kBlock + 16 * (g ^ (l16 >> 1)), hi_off = l16 * kBlock + 16 * ((g + 4) ^ (l16 >> 1));
+    auto operand = [&](const unsigned char *rows) {
+        const uint4 lo = *(const uint4 *)(rows + lo_off);
+        const uint4 hi = *(const uint4 *)(rows + hi_off);
+        return intx8{(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w, (int)hi.x, (int)hi.y, (int)hi.z, (int)hi.w};
     };
     const float *ws = p.ws + (size_t)min((n0 + wn) / kBlock, (p.outputs - 1) / kBlock) * p.blocks;
     float wscales = 0.f;  // of the next 64 blocks, one a lane (a scalar load would be waited for with every LDS read)
-    // a lane's 32 bytes of a row: chunks g and g + 4 (which inputs stand in which lane is free, W and x alike)
-    const int lo_off = l16 * kBlock + 16 * (g ^ (l16 >> 1)), hi_off = l16 * kBlock + 16 * ((g + 4) ^ (l16 >> 1));
+
     float acc[T::kNT][T::kMT][4] = {};
+    intx8 v[T::kTwo ? 2 : 1][T::kMT];
+    {
+        const Group first = group(b0 - 1);  // (of it, x of block b0)
+        each_of<T::kXUnits>([&](auto i) {
+            global_to_lds16_plus<1024 * decltype(i)::value>(first.x, x_off[decltype(i)::value], first.x_lds);
+        });
+    }
 #pragma unroll
-    for (int k = 0; k < T::kSlots - 1; ++k)
-        if (b0 + k < b1)
-            issue(b0 + k);
-    for (int b = b0; b < b1; ++b) {
+    for (int k = 0; k < T::kSlots - 1; ++k) {
+        const Group q = group(b0 + k);
+        each_of<T::kLoads>([&](auto i) { issue(q, i); });
+    }
+    MLA_WAIT_VMCNT((T::kSlots - 1) * T::kLoads);
+    clear_x(b0);
+    lds_barrier();
+#pragma unroll
+    for (int j = 0; j < T::kMT; ++j)
+        v[0][j] = operand(&s_x[0][0] + (wm + 16 * j) * kBlock);
+
+    // kCur: which of v holds block b
+    auto multiply = [&](int b, auto kCur) __attribute__((always_inline)) {
+        constexpr int cur = decltype(kCur)::value;
         landed(b);
-        lds_barrier();  // block b is there for all waves, and none reads block b - 1 any more
-        if (b + T::kSlots - 1 < b1)
-            issue(b + T::kSlots - 1);
-        const int at = (b - b0) % T::kSlots;
-        const unsigned char *slot = &s_slot[at][0];
-        // row l16 of the 16 rows from row0 (a multiple of 16) on
-        auto operand = [&](int row0) {
-            const uint4 lo = *(const uint4 *)(slot + row0 * kBlock + lo_off);
-            const uint4 hi = *(const uint4 *)(slot + row0 * kBlock + hi_off);
-            return intx8{(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w, (int)hi.x, (int)hi.y, (int)hi.z, (int)hi.w};
-        };
+        lds_barrier();  // W of block b and x of block b + 1 are there, and nobody reads those before any more
+        const int at = slot_of(b);
+        const unsigned char *w_rows = &s_w[at][0] + wn * kBlock;
+        const unsigned char *next_rows = &s_x[slot_of(b + 1)][0] + wm * kBlock;
         if (((b - b0) & 63) == 0) {
             wscales = ws[min(b + lane, p.blocks - 1)];
             asm volatile("" : "+v"(wscales));
         }
         const float wscale = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(wscales), (b - b0) & 63));
-        intx8 v[T::kMT], a[2];
+        intx8 a[2];
+        a[0] = operand(w_rows);
         float s[T::kMT];
-        a[0] = operand(wn);
 #pragma unroll
         for (int j = 0; j < T::kMT; ++j)
-            v[j] = operand(BN + wm + 16 * j);
+            s[j] = s_xs[at][wm + 16 * j + l16];
 #pragma unroll
         for (int j = 0; j < T::kMT; ++j)
-            s[j] = s_xs[at][wm + 16 * j + l16] * wscale;
-        // the products of 16 outputs while those of the 16 before are scaled and added
-        floatx4 d[2][T::kMT];
+            s[j] *= wscale;
+        // product t while that of kLag before is scaled and added
+        constexpr int kLag = 4;
+        floatx4 d[kLag + 1];
+        const Group later = group(b + T::kSlots - 1);
+        each_of<T::kProducts + kLag>([&](auto kt) {
+            constexpr int t = decltype(kt)::value, i = t / T::kMT, j = t % T::kMT;
+            if constexpr (j == 0 && i + 1 < T::kNT)
+                a[(i + 1) & 1] = operand(w_rows + 16 * (i + 1) * kBlock);
+            if constexpr (t < T::kProducts)
+                d[t % (kLag + 1)] = mfma16x16x128_fp8(a[i & 1], v[cur][j], floatx4{0.f, 0.f, 0.f, 0.f});
+            __builtin_amdgcn_sched_barrier(0);  // (before it, the sums would wait for their products, and this one with them)
+            if constexpr (t >= kLag) {
+                constexpr int q = t - kLag, qi = q / T::kMT, qj = q % T::kMT;
 #pragma unroll
-        for (int i = 0; i <= T::kNT; ++i) {
-            if (i + 1 < T::kNT)
-                a[(i + 1) & 1] = operand(wn + 16 * (i + 1));
-#pragma unroll
-            for (int j = 0; j < T::kMT; ++j) {
-                if (i < T::kNT)
-                    d[i & 1][j] = mfma16x16x128_fp8(a[i & 1], v[j], floatx4{0.f, 0.f, 0.f, 0.f});
-                if (i > 0)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        acc[i > 0 ? i - 1 : 0][j][e] =
-                            __builtin_fmaf(d[(i - 1) & 1][j][e], s[j], acc[i > 0 ? i - 1 : 0][j][e]);
+                for (int e = 0; e < 4; ++e)
+                    acc[qi][qj][e] = __builtin_fmaf(d[q % (kLag + 1)][e], s[qj], acc[qi][qj][e]);
                 // the sums stay where they are written: moved behind the products, every product's result would be live
-                if (i > 0)
-                    asm volatile("" : "+v"(acc[i > 0 ? i - 1 : 0][j][0]), "+v"(acc[i > 0 ? i - 1 : 0][j][1]),
-                                 "+v"(acc[i > 0 ? i - 1 : 0][j][2]), "+v"(acc[i > 0 ? i - 1 : 0][j][3]));
+                asm volatile("" : "+v"(acc[qi][qj][0]), "+v"(acc[qi][qj][1]), "+v"(acc[qi][qj][2]), "+v"(acc[qi][qj][3]));
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            // a later group's loads, one at a time (together they would wait for each other to be taken, and the
+            // products behind them), in the first half of the products
+            constexpr int kEvery = T::kProducts / 2 / T::kLoads > 0 ? T::kProducts / 2 / T::kLoads : 1;
+            if constexpr (t % kEvery == 0 && t / kEvery < T::kLoads) {
+                issue(later, std::integral_constant<int, t / kEvery>{});
                 __builtin_amdgcn_sched_barrier(0);
             }
-        }
+            // the rows of block b + 1 (behind the last block: whatever is there)
+            if constexpr (T::kTwo && t % T::kNT == T::kNT / 2 && t < T::kProducts) {
+                v[1 - cur][t / T::kNT] = operand(next_rows + 16 * (t / T::kNT) * kBlock);
+                __builtin_amdgcn_sched_barrier(0);
+            } else if constexpr (!T::kTwo && t < T::kProducts && i == T::kNT - 1) {
+                v[0][j] = operand(next_rows + 16 * j * kBlock);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        });
+    };
+    for (int b = b0; b < b1; b += 2) {
+        multiply(b, std::integral_constant<int, 0>{});
+        if (b + 1 < b1)
+            multiply(b + 1, std::integral_constant<int, T::kTwo ? 1 : 0>{});
     }
+    MLA_WAIT_VMCNT(0);  // the loads behind the last block, before the LDS is given back
     // four outputs of a row are one aligned store where rows start at a multiple of four (partial sums always do)
     const bool split = p.parts != nullptr;
     const int stride = split ? (p.outputs + 3) / 4 * 4 : p.outputs;
@@ -698,7 +775,7 @@ struct LinearPlan {
 LinearPlan plan_linear(int rows, int inputs, int outputs)
 {
     const int blocks = ceil_div(inputs, kBlock), cus = current_cu_count();
-    if (rows <= 128)
+    if (rows <= 128 || inputs < kBlock)  // (the tiles want a whole block)
         return {Form::kFew, 1};
     LinearPlan best{Form::kTile256, 1};
     double best_us = 0.0;
@@ -780,7 +857,7 @@ int linear(bool bf16, const void *x, const float *xs, const void *w, const float
            long long xs_row, long long xs_block, void *stream)
 {
     if (!x || !w || !ws || !out || !workspace || !sizes_ok(rows, inputs, outputs) || x_stride < 0 || x_stride > kMostStride ||
-        w_stride < 0 || w_stride > kMostStride || xs_row < 0 || xs_row > kMostStride || xs_block < 0)
+        w_stride < 0 || w_stride > kMostStride || xs_row < 0 || xs_row > (1 << 20) || xs_block < 0)
         return MLA_STATUS_INVALID_VALUE;
     if (!aligned16(x) || !aligned16(w) || !aligned16(out) || !aligned16(workspace) || x_stride % (xs ? 16 : 8) != 0 ||
         w_stride % 16 != 0)

@@ -81,6 +81,17 @@ __device__ __forceinline__ void global_to_lds16_at(const void *base, int off, un
                  : : "v"(off), "s"(base), "s"(lds_addr) : "memory");
 }
 
+// The same load to lds_addr + kPlus + 16 * lane, of a wave-uniform lds_addr in a scalar register: the sum is
+// formed in m0 itself.
+template <int kPlus>
+__device__ __forceinline__ void global_to_lds16_plus(const void *base, int off, unsigned lds_addr)
+{
+    asm volatile("s_add_u32 m0, %2, %3\n\t"
+                 "s_nop 0\n\t"
+                 "global_load_lds_dwordx4 %0, %1"
+                 : : "v"(off), "s"(base), "s"(lds_addr), "i"(kPlus) : "memory", "scc");
+}
+
 // 4 bytes per lane (global_load_lds_dword), to lds_addr + 4 * lane; as above.
 __device__ __forceinline__ void global_to_lds4_at(const void *base, int off, unsigned lds_addr)
 {

@@ -151,7 +151,7 @@ def test_linear_argument_errors(t):
     assert size(3, 256, 100) >= 3 * 256 + 3 * 2 * 4 and size(0, 256, 100) == size(3, 24, 100) == size(3, 256, 0) == 0
     names = "x xs w ws out space bytes rows k n xstride wstride srow sblock stream"
     call = _caller("mla_linear_fp8_quantized_" + t, names, {n: ok.get(n, FAKE) for n in names.split()} | dict(srow=2, sblock=1))
-    for bad in (*common, dict(xs=None), dict(space=None), dict(srow=-1), dict(srow=2 ** 22 + 1), dict(sblock=-1)):
+    for bad in (*common, dict(xs=None), dict(space=None), dict(srow=-1), dict(srow=2 ** 20 + 1), dict(sblock=-1)):
         assert call(**bad) == capi.STATUS_INVALID_VALUE, bad
     for bad in (dict(x=FAKE + 8), dict(w=FAKE + 8), dict(out=FAKE + 2), dict(space=FAKE + 4), dict(xstride=264), dict(wstride=264)):
         assert call(**bad) == capi.STATUS_MISALIGNED, bad
