@@ -398,200 +398,37 @@ __global__ __launch_bounds__(256) void sum_kernel(const float *__restrict__ part
     }
 }
 
-// Few rows: the weights' bytes are what the call costs, so each wave streams them from memory into the
-// operand registers, kAhead blocks ahead, with nothing between. A workgroup has 16 NT outputs of up to 16 MT
-// rows; its 8 waves take its blocks in turn (so that a row's next kilobyte is read at a time) and add
-// their sums through LDS at the end, wave after wave. kQuantize: the rows are 16-bit (E) and each workgroup
-// quantises them into LDS first, which for few values is cheaper than a launch.
-constexpr int kRowWaves = 8;
+// Few rows: the weights' bytes are what the call costs. A workgroup has 16 NT outputs of up to 16 MT rows; its
+// waves take its blocks in turn (so that a row's next bytes are read at a time), each through an LDS ring of its own, fed by
+// direct loads kSlots - 1 blocks ahead and read behind counter waits: no barrier in the loop, and as many
+// bytes on their way as LDS holds (in registers, operands of 16 rows and 4 blocks ahead, 64 x 16384 x 5120 took 55 us
+// against 24). The waves' sums are added through LDS at the end, wave after wave.
+// kQuantize: the rows are 16-bit (E), and each workgroup quantises them into LDS itself, which for few values is
+// cheaper than a launch.
 constexpr int kMostOwn = 32768;  // values that a workgroup quantises itself
 
-template <int NT, int MT, bool kQuantize>
-struct RowTile {
-    static constexpr int kAhead = kQuantize ? 5 : MT >= 4 ? 3 : 4;
-    static constexpr int kSums = kRowWaves * NT * MT * 64 * 4;  // floats
-    static constexpr int kRows = kQuantize ? kMostOwn + 16 * (kBlock + 16) + 4 * (kMostOwn / kBlock + 16) : 16;
-};
-
-template <typename E, int NT, int MT, bool kQuantize>
-__global__ __launch_bounds__(64 * kRowWaves, 2) void linear_rows_kernel(Linear p)
-{
-    using T = RowTile<NT, MT, kQuantize>;
-    using E8 = typename Vec<E>::v8;
-    __shared__ __attribute__((aligned(16))) float s_sums[T::kSums];
-    __shared__ __attribute__((aligned(16))) unsigned char s_rows[T::kRows];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int l16 = lane & 15, g = lane >> 4;
-    const int n_tiles = (p.outputs + 16 * NT - 1) / (16 * NT);
-    const int n0 = (int)(blockIdx.x % n_tiles) * 16 * NT, m0 = (int)(blockIdx.x / n_tiles) * 16 * MT;
-    const int mine = p.blocks > wave ? (p.blocks - wave + kRowWaves - 1) / kRowWaves : 0;  // blocks wave, wave + 8, ..
-    // byte offsets of the lane's rows from the tile's first
-    const unsigned char *const w_tile = p.w + n0 * p.w_stride, *const x_tile = p.x + m0 * p.x_stride;
-    const float *const xs_tile = p.xs + m0 * p.xs_row;
-    int w_row[NT], x_row[MT], xs_row[MT];
-#pragma unroll
-    for (int i = 0; i < NT; ++i)
-        w_row[i] = min(16 * i + l16, p.outputs - 1 - n0) * (int)p.w_stride;
-#pragma unroll
-    for (int j = 0; j < MT; ++j) {
-        x_row[j] = min(16 * j + l16, p.rows - 1 - m0) * (int)p.x_stride;
-        xs_row[j] = min(16 * j + l16, p.rows - 1 - m0) * (int)p.xs_row;
-    }
-    // The lane's two 16-byte chunks of a block, bytes 32 g .. 32 g + 31. Behind the inputs' end they re-read the
-    // last 16 bytes there are and are cleared before the product: no load stands under a condition, so that the
-    // compiler's waits count the loads of the blocks ahead.
-    const int last = p.blocks - 1, end = p.inputs - last * kBlock;  // bytes of the last block
-    const bool lost_lo = 32 * g >= end, lost_hi = 32 * g + 16 >= end;
-    constexpr int kA = T::kAhead;
-    uint4 a[kA][NT][2], v[kA][kQuantize ? 1 : MT][2];
-    float s[kA][kQuantize ? 1 : MT];
-    auto load = [&](int d, int it) {  // the wave's block `it` (past its last: that one again)
-        const int b = wave + kRowWaves * min(it, mine - 1);
-        const int lo = min(b * kBlock + 32 * g, p.inputs - 16), hi = min(b * kBlock + 32 * g + 16, p.inputs - 16);
-#pragma unroll
-        for (int i = 0; i < NT; ++i) {
-            a[d][i][0] = *(const uint4 *)(w_tile + (w_row[i] + lo));
-            a[d][i][1] = *(const uint4 *)(w_tile + (w_row[i] + hi));
-        }
-        if constexpr (!kQuantize) {
-            const float *xs = xs_tile + b * p.xs_block;
-#pragma unroll
-            for (int j = 0; j < MT; ++j) {
-                v[d][j][0] = *(const uint4 *)(x_tile + (x_row[j] + lo));
-                v[d][j][1] = *(const uint4 *)(x_tile + (x_row[j] + hi));
-                s[d][j] = xs[xs_row[j]];
-            }
-        }
-    };
-    auto operand = [](const uint4 &lo, const uint4 &hi) {
-        return intx8{(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w, (int)hi.x, (int)hi.y, (int)hi.z, (int)hi.w};
-    };
-    const float *ws = p.ws + (size_t)(n0 / kBlock) * p.blocks;
-    float scales = 0.f;  // of the wave's next 64 blocks, one a lane
-    if (mine > 0) {
-        scales = ws[wave + kRowWaves * min(lane, mine - 1)];
-#pragma unroll
-        for (int d = 0; d < kA; ++d)
-            load(d, d);
-    }
-    const int row_bytes = p.blocks * kBlock + 16;  // in LDS
-    float *const s_xs = reinterpret_cast<float *>(s_rows + p.rows * row_bytes);
-    if constexpr (kQuantize) {
-        const E *x = reinterpret_cast<const E *>(p.x);
-        for (int u = tid >> 4; u < p.rows * p.blocks; u += 4 * kRowWaves) {
-            const int m = u / p.blocks, b = u - m * p.blocks, k = b * kBlock + 8 * (tid & 15);
-            E8 e = {};
-            if (k < p.inputs)
-                e = *(const E8 *)(x + m * p.x_stride + k);
-            float scale;
-            *(uint2 *)(s_rows + m * row_bytes + k) = quantized8(e, scale);
-            if ((tid & 15) == 0)
-                s_xs[u] = scale;
-        }
-        __syncthreads();
-    }
-    float acc[NT][MT][4] = {};
-    auto multiply = [&](int d, int it) {
-        const int b = wave + kRowWaves * it;
-        if ((it & 63) == 0 && it > 0)
-            scales = ws[wave + kRowWaves * min(it + lane, mine - 1)];
-        const float wscale = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(scales), it & 63));
-        if (b == last) {
-#pragma unroll
-            for (int i = 0; i < NT; ++i) {
-                a[d][i][0] = lost_lo ? uint4{0, 0, 0, 0} : a[d][i][0];
-                a[d][i][1] = lost_hi ? uint4{0, 0, 0, 0} : a[d][i][1];
-            }
-            if constexpr (!kQuantize)
-#pragma unroll
-                for (int j = 0; j < MT; ++j) {
-                    v[d][j][0] = lost_lo ? uint4{0, 0, 0, 0} : v[d][j][0];
-                    v[d][j][1] = lost_hi ? uint4{0, 0, 0, 0} : v[d][j][1];
-                }
-        }
-#pragma unroll
-        for (int j = 0; j < MT; ++j) {
-            intx8 x;
-            float f;
-            if constexpr (kQuantize) {
-                const int m = min(l16, p.rows - 1);
-                const unsigned char *at = s_rows + m * row_bytes + b * kBlock + 32 * g;
-                x = operand(*(const uint4 *)at, *(const uint4 *)(at + 16));
-                f = s_xs[m * p.blocks + b] * wscale;
-            } else {
-                x = operand(v[d][j][0], v[d][j][1]);
-                f = s[d][j] * wscale;
-            }
-#pragma unroll
-            for (int i = 0; i < NT; ++i) {
-                const floatx4 y = mfma16x16x128_fp8(operand(a[d][i][0], a[d][i][1]), x, floatx4{0.f, 0.f, 0.f, 0.f});
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    acc[i][j][e] = __builtin_fmaf(y[e], f, acc[i][j][e]);
-            }
-        }
-    };
-    int it0 = 0;
-    for (; it0 + kA <= mine; it0 += kA) {
-#pragma unroll
-        for (int d = 0; d < kA; ++d) {
-            multiply(d, it0 + d);
-            load(d, it0 + d + kA);
-        }
-    }
-#pragma unroll
-    for (int d = 0; d < kA - 1; ++d)
-        if (it0 + d < mine)
-            multiply(d, it0 + d);
-#pragma unroll
-    for (int i = 0; i < NT; ++i)
-#pragma unroll
-        for (int j = 0; j < MT; ++j)
-            *(floatx4 *)(s_sums + (((wave * NT + i) * MT + j) * 64 + lane) * 4) =
-                floatx4{acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
-    __syncthreads();
-    // a thread an output tile's lane: wave after wave, outputs 4 g .. 4 g + 3 of row l16
-    E *out = static_cast<E *>(p.out);
-    for (int t = tid; t < NT * MT * 64; t += 64 * kRowWaves) {
-        floatx4 y = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int w = 0; w < kRowWaves; ++w)
-            y += *(const floatx4 *)(s_sums + (w * NT * MT * 64 + t) * 4);
-        const int i = t / (MT * 64), j = t / 64 % MT, l = t & 63;
-        const int m = m0 + 16 * j + (l & 15), n = n0 + 16 * i + 4 * (l >> 4);
-        if (m < p.rows)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (n + e < p.outputs)
-                    out[(size_t)m * p.outputs + n + e] = (E)y[e];
-    }
-}
-
-// Up to 64 rows: as above, but the operands of 16 to 64 rows would fill the registers before enough weight
-// blocks were on their way. Each wave therefore has an LDS ring of its own, fed by direct loads two blocks
-// ahead and read behind counter waits: no workgroup barrier in the loop. Four waves take the blocks in turn.
-constexpr int kFewWaves = 4;
-
-template <int NT, int MT>
+template <int NT, int MT, int kW, int kS, bool kQuantize>
 struct FewTile {
-    static constexpr int kSlots = 3;
-    static constexpr int kUnits = 2 * NT + 2 * MT;  // of 8 rows
-    static constexpr int kLoads = kUnits + 1;       // and the rows' scales
-    static constexpr int kSlot = kUnits * 1024 + 256;
-    static constexpr int kRing = kSlots * kSlot;    // a wave's
-    static_assert(kFewWaves * kRing <= 160 * 1024 && kRing >= NT * MT * 1024 && 2 * kLoads <= 63, "ring");
+    static constexpr int kUnits = 2 * NT + (kQuantize ? 0 : 2 * MT);  // loads of 8 rows, a wave and block
+    static constexpr int kLoads = kUnits + (kQuantize ? 0 : 1);       // and of the rows' scales
+    static constexpr int kSlot = kUnits * 1024 + (kQuantize ? 0 : 256);
+    static constexpr int kRing = kS * kSlot;  // a wave's
+    // quantised rows, 16 bytes apart more than their blocks, and their scales
+    static constexpr int kRows = kQuantize ? kMostOwn + 16 * 16 + 4 * kMostOwn / kBlock : 0;
+    static_assert(kW * kRing + kRows <= 160 * 1024 && kRing >= NT * MT * 1024 && (kS - 1) * kLoads <= 63, "ring");
 };
 
-template <typename E, int NT, int MT>
-__global__ __launch_bounds__(64 * kFewWaves) void linear_few_kernel(Linear p)
+template <typename E, int NT, int MT, int kW, int kS, bool kQuantize>
+__global__ __launch_bounds__(64 * kW) void linear_few_kernel(Linear p)
 {
-    using T = FewTile<NT, MT>;
-    __shared__ __attribute__((aligned(1024))) unsigned char s_ring[kFewWaves * T::kRing];
+    using T = FewTile<NT, MT, kW, kS, kQuantize>;
+    using E8 = typename Vec<E>::v8;
+    __shared__ __attribute__((aligned(1024))) unsigned char s_ring[kW * T::kRing + T::kRows];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l16 = lane & 15, g = lane >> 4;
     const int n_tiles = (p.outputs + 16 * NT - 1) / (16 * NT);
     const int n0 = (int)(blockIdx.x % n_tiles) * 16 * NT, m0 = (int)(blockIdx.x / n_tiles) * 16 * MT;
-    const int mine = p.blocks > wave ? (p.blocks - wave + kFewWaves - 1) / kFewWaves : 0;  // blocks wave, wave + 4, ..
+    const int mine = p.blocks > wave ? (p.blocks - wave + kW - 1) / kW : 0;  // blocks wave, wave + kW, ..
     const unsigned char *const w_tile = p.w + n0 * p.w_stride, *const x_tile = p.x + m0 * p.x_stride;
     unsigned char *const ring = s_ring + wave * T::kRing;
     const unsigned ring_lds = (unsigned)(uintptr_t)(const MLA_LDS unsigned char *)ring;
@@ -605,67 +442,97 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_few_kernel(Linear p)
                              : min(r - 16 * NT, p.rows - 1 - m0) * (int)p.x_stride) + 16 * chunk_of(u);
     }
     const int scale_off = 4 * min(lane, p.rows - 1 - m0) * (int)p.xs_row;
-    const int last = p.blocks - 1, tail = p.inputs % kBlock / 16;
+    const int last = p.blocks - 1, tail = p.inputs % kBlock / 16;  // whole chunks of the last block (0: all 8)
     auto issue = [&](int it) {
-        const int b = wave + kFewWaves * it;
-        const unsigned lds = ring_lds + it % T::kSlots * T::kSlot;
+        const int b = wave + kW * it;
+        const unsigned lds = ring_lds + it % kS * T::kSlot;
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // what was read of the slot's last block has arrived
 #pragma unroll
         for (int u = 0; u < T::kUnits; ++u) {
             int o = off[u];
-            if (tail != 0 && b == last) {  // as in linear_kernel
+            if (tail != 0 && b == last) {  // chunks behind the inputs' end read the block's first, and are cleared afterwards
                 const int c = chunk_of(u);
                 o -= c >= tail ? 16 * c : 0;
             }
             global_to_lds16_at((u < 2 * NT ? w_tile : x_tile) + (size_t)b * kBlock, o, lds + 1024 * u);
         }
-        global_to_lds4_at(p.xs + m0 * p.xs_row + b * p.xs_block, scale_off, lds + 1024 * T::kUnits);
+        if constexpr (!kQuantize)
+            global_to_lds4_at(p.xs + m0 * p.xs_row + b * p.xs_block, scale_off, lds + 1024 * T::kUnits);
     };
     const float *ws = p.ws + (size_t)(n0 / kBlock) * p.blocks;
-    float scales = mine > 0 ? ws[wave + kFewWaves * min(lane, mine - 1)] : 0.f;  // of the wave's next 64 blocks, one a lane
-    asm volatile("" : "+v"(scales));  // (waited for before the loop's loads, which the compiler does not count)
-    if (mine > 0)
-        issue(0);
-    if (mine > 1)
-        issue(1);
+    float scales = mine > 0 ? ws[wave + kW * min(lane, mine - 1)] : 0.f;  // of the wave's next 64 blocks, one a lane
+    const int row_bytes = p.blocks * kBlock + 16;  // of a quantised row
+    unsigned char *const s_rows = s_ring + kW * T::kRing;
+    float *const s_xs = reinterpret_cast<float *>(s_rows + p.rows * row_bytes);
+    E8 early = {};  // the thread's first 8 values, on their way before the weights
+    auto fetch = [&](int u) {
+        const int m = u / p.blocks, k = (u - m * p.blocks) * kBlock + 8 * (tid & 15);
+        E8 e = {};
+        if (u < p.rows * p.blocks && k < p.inputs)
+            e = *(const E8 *)(reinterpret_cast<const E *>(p.x) + m * p.x_stride + k);
+        return e;
+    };
+    if constexpr (kQuantize)
+        early = fetch(tid >> 4);
+    asm volatile("" : "+v"(scales), "+v"(early));  // (waited for before the ring's loads, which the compiler does not count)
+#pragma unroll
+    for (int k = 0; k < kS - 1; ++k)
+        if (k < mine)
+            issue(k);
+    if constexpr (kQuantize) {
+        for (int u = tid >> 4; u < p.rows * p.blocks; u += 4 * kW) {
+            const int m = u / p.blocks, b = u - m * p.blocks;
+            const E8 e = u == tid >> 4 ? early : fetch(u);
+            float scale;
+            *(uint2 *)(s_rows + m * row_bytes + b * kBlock + 8 * (tid & 15)) = quantized8(e, scale);
+            if ((tid & 15) == 0)
+                s_xs[u] = scale;
+        }
+        __syncthreads();
+    }
     const int lo_off = l16 * kBlock + 16 * (g ^ (l16 >> 1)), hi_off = l16 * kBlock + 16 * ((g + 4) ^ (l16 >> 1));
     float acc[NT][MT][4] = {};
     for (int it = 0; it < mine; ++it) {
-        if (it + 2 < mine) {
-            issue(it + 2);
-            MLA_WAIT_VMCNT(2 * T::kLoads);
-        } else if (it + 1 < mine) {
-            MLA_WAIT_VMCNT(T::kLoads);
+        if (it + kS - 1 < mine) {
+            issue(it + kS - 1);
+            MLA_WAIT_VMCNT((kS - 1) * T::kLoads);
         } else {
             MLA_WAIT_VMCNT(0);
         }
         asm volatile("" ::: "memory");
-        unsigned char *const slot = ring + it % T::kSlots * T::kSlot;
-        if (tail != 0 && wave + kFewWaves * it == last) {
+        const int b = wave + kW * it;
+        unsigned char *const slot = ring + it % kS * T::kSlot;
+        if (tail != 0 && b == last) {
 #pragma unroll
             for (int u = 0; u < T::kUnits; ++u)
                 if (chunk_of(u) >= tail)
                     *(uint4 *)(slot + 1024 * u + 16 * lane) = uint4{0, 0, 0, 0};
         }
         if ((it & 63) == 0 && it > 0) {
-            scales = ws[wave + kFewWaves * min(it + lane, mine - 1)];
+            scales = ws[wave + kW * min(it + lane, mine - 1)];
             asm volatile("" : "+v"(scales));
         }
         const float wscale = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(scales), it & 63));
-        auto operand = [&](int row0) {
-            const uint4 lo = *(const uint4 *)(slot + row0 * kBlock + lo_off);
-            const uint4 hi = *(const uint4 *)(slot + row0 * kBlock + hi_off);
-            return intx8{(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w, (int)hi.x, (int)hi.y, (int)hi.z, (int)hi.w};
+        auto operand = [&](const unsigned char *lo, const unsigned char *hi) {
+            const uint4 a = *(const uint4 *)lo, c = *(const uint4 *)hi;
+            return intx8{(int)a.x, (int)a.y, (int)a.z, (int)a.w, (int)c.x, (int)c.y, (int)c.z, (int)c.w};
         };
         intx8 a[NT], v[MT];
         float s[MT];
 #pragma unroll
         for (int i = 0; i < NT; ++i)
-            a[i] = operand(16 * i);
+            a[i] = operand(slot + 16 * i * kBlock + lo_off, slot + 16 * i * kBlock + hi_off);
 #pragma unroll
         for (int j = 0; j < MT; ++j) {
-            v[j] = operand(16 * NT + 16 * j);
-            s[j] = *(const float *)(slot + 1024 * T::kUnits + 4 * (16 * j + l16)) * wscale;
+            if constexpr (kQuantize) {
+                const int m = min(l16, p.rows - 1);
+                const unsigned char *at = s_rows + m * row_bytes + b * kBlock + 16 * g;
+                v[j] = operand(at, at + 64);
+                s[j] = s_xs[m * p.blocks + b] * wscale;
+            } else {
+                v[j] = operand(slot + 16 * (NT + j) * kBlock + lo_off, slot + 16 * (NT + j) * kBlock + hi_off);
+                s[j] = *(const float *)(slot + 1024 * T::kUnits + 4 * (16 * j + l16)) * wscale;
+            }
         }
 #pragma unroll
         for (int j = 0; j < MT; ++j)
@@ -685,11 +552,12 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_few_kernel(Linear p)
             *(floatx4 *)(ring + ((i * MT + j) * 64 + lane) * 16) =
                 floatx4{acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
     __syncthreads();
+    // a lane of a 16 x 16 tile a thread: outputs 4 g .. 4 g + 3 of row l16
     E *out = static_cast<E *>(p.out);
-    for (int t = tid; t < NT * MT * 64; t += 64 * kFewWaves) {
+    for (int t = tid; t < NT * MT * 64; t += 64 * kW) {
         floatx4 y = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int w = 0; w < kFewWaves; ++w)
+        for (int w = 0; w < kW; ++w)
             y += *(const floatx4 *)(s_ring + w * T::kRing + t * 16);
         const int i = t / (MT * 64), j = t / 64 % MT, l = t & 63;
         const int m = m0 + 16 * j + (l & 15), n = n0 + 16 * i + 4 * (l >> 4);
@@ -747,54 +615,63 @@ int launch_tiles(Linear p, int splits, hipStream_t s)
     return launched();
 }
 
-template <typename E, int NT, int MT, bool kQuantize>
-int launch_rows(const Linear &p, hipStream_t s)
-{
-    const int64_t tiles = (int64_t)ceil_div(p.rows, 16 * MT) * ceil_div(p.outputs, 16 * NT);
-    hipLaunchKernelGGL((linear_rows_kernel<E, NT, MT, kQuantize>), dim3((unsigned)tiles), dim3(64 * kRowWaves), 0, s, p);
-    return launched();
-}
-
-template <typename E, int NT, int MT>
+template <typename E, int NT, int MT, int kW, int kS, bool kQuantize = false>
 int launch_few(const Linear &p, hipStream_t s)
 {
     const int64_t tiles = (int64_t)ceil_div(p.rows, 16 * MT) * ceil_div(p.outputs, 16 * NT);
-    hipLaunchKernelGGL((linear_few_kernel<E, NT, MT>), dim3((unsigned)tiles), dim3(64 * kFewWaves), 0, s, p);
+    hipLaunchKernelGGL((linear_few_kernel<E, NT, MT, kW, kS, kQuantize>), dim3((unsigned)tiles), dim3(64 * kW), 0, s, p);
     return launched();
 }
 
 // ---- which kernel -----------------------------------------------------------
 
-enum class Form { kOwn, kFew, kTile64, kTile128, kTile256 };
+enum class Form { kFew, kTile64, kTile128, kTile256 };
 
 struct LinearPlan {
     Form form;
     int splits;
 };
 
+// Few-row kernel: 16 outputs a workgroup where the CUs hold them all at once, else 32; and how many of its rows' tiles
+// of 16 a workgroup takes.
+bool few_narrow(int outputs) { return ceil_div(outputs, 16) <= current_cu_count(); }
+int few_row_tiles(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
+
+// The form with the smallest modelled time, and how many parts its inputs are split into. Measured on 17 sizes of 32 to
+// 8192 rows with every form and split forced (us, e.g. 256 x 16384 x 5120: 256 tiles 197, 128 tiles 85, in
+// three splits 40; 64 tiles 61, in three 50; the model picks within 6% of the best of all, on 13 the best):
+//   tiles     3.5 + rounds (blocks + 2.5) step; a step (one block) is 0.45, 0.66, 1.55 us with few
+//             workgroups and 0.48, 0.70, 1.80 with every CU busy (the clock falls);
+//   splits    4 for the second launch, and 0.28 a MB of fp32 sums, written and read;
+//   few rows  4 + rounds (blocks / waves) times what a block costs a wave.
 LinearPlan plan_linear(int rows, int inputs, int outputs)
 {
     const int blocks = ceil_div(inputs, kBlock), cus = current_cu_count();
-    if (rows <= 128 || inputs < kBlock)  // (the tiles want a whole block)
-        return {Form::kFew, 1};
-    LinearPlan best{Form::kTile256, 1};
-    double best_us = 0.0;
+    const int few = few_row_tiles(rows);
+    const bool narrow = few_narrow(outputs);
+    const double few_step = few == 1 ? (narrow ? 0.5 : 0.8) : few == 2 ? (narrow ? 0.4 : 0.55) : narrow ? 0.5 : 0.72;
+    const double few_rounds = std::ceil((double)ceil_div(rows, 16 * few) * ceil_div(outputs, narrow ? 16 : 32) / cus);
+    LinearPlan best{Form::kFew, 1};
+    double best_us = 4.0 + few_rounds * ceil_div(blocks, few == 1 ? 8 : 4) * few_step;
+    if (inputs < kBlock)  // (the tiles want a whole block)
+        return best;
     struct Kind {
         Form form;
         int bn, bm;
-        double step_us;
+        double step, busy_step;
     };
-    for (const Kind &k : {Kind{Form::kTile256, 256, 256, 1.1}, Kind{Form::kTile128, 128, 128, 0.45}, Kind{Form::kTile64, 128, 64, 0.3}}) {
+    for (const Kind &k : {Kind{Form::kTile256, 256, 256, 1.55, 1.80}, Kind{Form::kTile128, 128, 128, 0.66, 0.70},
+                          Kind{Form::kTile64, 128, 64, 0.45, 0.48}}) {
         const int64_t tiles = (int64_t)ceil_div(rows, k.bm) * ceil_div(outputs, k.bn);
         for (int splits = 1; splits <= std::min(blocks, 16); ++splits) {
             const int per = ceil_div(blocks, splits);
             if (ceil_div(blocks, per) != splits)
                 continue;
-            const double rounds = std::ceil((double)tiles * splits / cus);
-            double us = rounds * (per + 2) * k.step_us;
+            const double full = (double)tiles * splits / cus;
+            double us = 3.5 + std::ceil(full) * (per + 2.5) * (k.step + (k.busy_step - k.step) * std::min(1.0, full));
             if (splits > 1)
-                us += 3.0 + 8.0e-6 * splits * rows * (double)outputs / 5.0;
-            if (best_us == 0.0 || us < best_us) {
+                us += 4.0 + 0.28e-6 * 4.0 * splits * rows * outputs;
+            if (us < best_us) {
                 best = {k.form, splits};
                 best_us = us;
             }
@@ -812,12 +689,12 @@ int launch_linear(const Linear &p, const LinearPlan &plan, hipStream_t s)
     case Form::kTile64: return launch_tiles<E, 128, 64, 2, 2, 4>(p, plan.splits, s);
     default: break;
     }
-    const bool narrow = ceil_div(p.outputs, 16) <= current_cu_count();
-    if (p.rows <= 16)
-        return narrow ? launch_rows<E, 1, 1, false>(p, s) : launch_rows<E, 2, 1, false>(p, s);
-    if (p.rows <= 32)
-        return narrow ? launch_few<E, 1, 2>(p, s) : launch_few<E, 2, 2>(p, s);
-    return narrow ? launch_few<E, 1, 4>(p, s) : launch_few<E, 2, 4>(p, s);
+    const bool narrow = few_narrow(p.outputs);
+    switch (few_row_tiles(p.rows)) {
+    case 1: return narrow ? launch_few<E, 1, 1, 8, 4>(p, s) : launch_few<E, 2, 1, 8, 3>(p, s);
+    case 2: return narrow ? launch_few<E, 1, 2, 4, 4>(p, s) : launch_few<E, 2, 2, 4, 4>(p, s);
+    default: return narrow ? launch_few<E, 1, 4, 4, 3>(p, s) : launch_few<E, 2, 4, 4, 3>(p, s);
+    }
 }
 
 // 16-bit rows few enough for every workgroup to quantise them
@@ -829,7 +706,7 @@ bool quantizes_itself(int rows, int inputs)
 template <typename E>
 int launch_own(const Linear &p, hipStream_t s)
 {
-    return ceil_div(p.outputs, 16) <= current_cu_count() ? launch_rows<E, 1, 1, true>(p, s) : launch_rows<E, 2, 1, true>(p, s);
+    return few_narrow(p.outputs) ? launch_few<E, 1, 1, 8, 4, true>(p, s) : launch_few<E, 2, 1, 8, 3, true>(p, s);
 }
 
 int quantize(bool bf16, const void *x, void *xq, float *scales, int rows, int inputs, long long x_stride, void *stream)
