@@ -51,6 +51,16 @@ __device__ __forceinline__ int block_before(int v, int *s, int &total)
     return before + sum - v;
 }
 
+// The largest v of the workgroup's threads, added to *s by each wave.
+__device__ __forceinline__ void block_most(int v, int *s)
+{
+#pragma unroll
+    for (int d = 32; d > 0; d /= 2)
+        v = max(v, __shfl_xor(v, d));
+    if ((threadIdx.x & 63) == 0)
+        atomicMax(s, v);
+}
+
 struct Table {
     const int *ids;  // [rows][stride]
     const int *lens;
@@ -69,40 +79,50 @@ struct Table {
 __device__ __forceinline__ bool has(const unsigned *bits, int page) { return (bits[page >> 5] >> (page & 31)) & 1; }
 
 // One bit a page: held by a row of the table, and (kFull) by one of the first full[row]
-// columns of a row. A wave takes 64 rows x 16 columns at once, each lane a column of 16 rows in a row:
-// 16 loads in flight, and the page that a row shares with the row above (a prompt's) is marked once.
-// held, full: columns of each row, in LDS; most: the largest of held.
+// columns of a row. A wave takes pieces of 64 rows x 16 columns, each lane a column of 16 rows in a row, kPieces of them
+// at once (64 loads in flight: a round of one piece was a round trip, 5 of them 16 us of a call with 1024 rows of 77 pages), and
+// the page that a row shares with the row above (a prompt's) is marked once.
+// tokens, full: of each row, in LDS; most: the largest row's pages.
 template <bool kFull>
-__device__ __forceinline__ void mark_pages(const Table &t, const int *held, const int *full, int most, int num_pages,
+__device__ __forceinline__ void mark_pages(const Table &t, const int *tokens, const int *full, int most, int num_pages,
                                            unsigned *held_bits, unsigned *full_bits)
 {
+    constexpr int kPieces = 4;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int chunks = (most + 15) / 16, tasks = (t.rows + 63) / 64 * chunks;
-    for (int task = wave; task < tasks; task += kWaves) {
-        const int row0 = task / chunks * 64 + (lane >> 4) * 16, col = task % chunks * 16 + (lane & 15);
-        int id[16];
+    const int chunks = (most + 15) / 16, pieces = (t.rows + 63) / 64 * chunks;
+    for (int first = wave; first < pieces; first += kPieces * kWaves) {
+        int id[kPieces][16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int row = row0 + i;
-            id[i] = row < t.rows && col < held[row] ? t.ids[(size_t)row * t.stride + col] : -1;
+        for (int k = 0; k < kPieces; ++k) {
+            const int piece = first + k * kWaves;
+            const int row0 = piece / chunks * 64 + (lane >> 4) * 16, col = piece % chunks * 16 + (lane & 15);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int row = row0 + i;
+                id[k][i] = piece < pieces && row < t.rows && col < t.pages(tokens[row]) ? t.ids[(size_t)row * t.stride + col] : -1;
+            }
         }
-        bool above_full = false;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int row = row0 + i;
-            if ((unsigned)id[i] < (unsigned)num_pages) {
-                const bool again = i > 0 && id[i] == id[i > 0 ? i - 1 : 0];
-                const unsigned bit = 1u << (id[i] & 31);
-                if (!again)
-                    atomicOr(held_bits + (id[i] >> 5), bit);
-                if constexpr (kFull) {
-                    const bool whole = col < full[row];
-                    if (whole && !(again && above_full))
-                        atomicOr(full_bits + (id[i] >> 5), bit);
-                    above_full = whole;
+        for (int k = 0; k < kPieces; ++k) {
+            const int piece = first + k * kWaves;
+            const int row0 = piece / chunks * 64 + (lane >> 4) * 16, col = piece % chunks * 16 + (lane & 15);
+            bool above_full = false;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int page = id[k][i];
+                bool whole = false;
+                if ((unsigned)page < (unsigned)num_pages) {
+                    const bool again = i > 0 && page == id[k][i > 0 ? i - 1 : 0];
+                    const unsigned bit = 1u << (page & 31);
+                    if (!again)
+                        atomicOr(held_bits + (page >> 5), bit);
+                    if constexpr (kFull) {
+                        whole = col < full[row0 + i];
+                        if (whole && !(again && above_full))
+                            atomicOr(full_bits + (page >> 5), bit);
+                    }
                 }
-            } else {
-                above_full = false;
+                above_full = whole;
             }
         }
     }
@@ -112,17 +132,17 @@ __device__ __forceinline__ void mark_pages(const Table &t, const int *held, cons
 __device__ __forceinline__ void clear_bits(const int *pinned, int num_pages, unsigned *bits, unsigned *others)
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int base = 256 * wave; base < num_pages; base += 256 * kWaves) {
-        int v[4];
+    for (int base = 1024 * wave; base < num_pages; base += 1024 * kWaves) {
+        int v[16];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 16; ++i) {
             const int p = base + 64 * i + lane;
             v[i] = pinned && p < num_pages ? pinned[p] : 0;
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 16; ++i) {
             const unsigned long long m = __builtin_amdgcn_ballot_w64(v[i] > 0);
-            if (lane < 2) {  // at most 7 words past the last page's; kWords is a multiple of 8
+            if (lane < 2) {  // up to 31 words past the last page's: kWords is a multiple of 32
                 bits[base / 32 + 2 * i + lane] = (unsigned)(m >> (32 * lane));
                 others[base / 32 + 2 * i + lane] = 0;
             }
@@ -144,13 +164,15 @@ struct NewRow {
     int last;                        // that page's id
 };
 
-__device__ __forceinline__ NewRow new_row(const Fork &f, int b)
+// old_tokens(row): of the old table
+template <typename F>
+__device__ __forceinline__ NewRow new_row(const Fork &f, int b, F &&old_tokens)
 {
     NewRow r;
     r.parent = f.parents[b];
     const int kept = f.kept ? max(f.kept[b], 0) : INT_MAX;
     const bool real = (unsigned)r.parent < (unsigned)f.old.rows;
-    r.tokens = real ? min(kept, f.old.tokens(r.parent)) : 0;
+    r.tokens = real ? min(kept, old_tokens(r.parent)) : 0;
     r.full = r.tokens >> f.old.page_shift;
     r.rest = r.tokens & ((1 << f.old.page_shift) - 1);
     r.last = r.rest ? f.old.ids[(size_t)r.parent * f.old.stride + r.full] : -1;
@@ -170,7 +192,7 @@ __device__ __forceinline__ NewRow new_row(const Fork &f, int b)
 __global__ __launch_bounds__(kThreads) void fork_kernel(Fork f)
 {
     __shared__ unsigned s_held[kWords], s_kept[kWords];
-    __shared__ int s_pages[kMostRows], s_full[kMostRows];
+    __shared__ int s_tokens[kMostRows], s_full[kMostRows];
     __shared__ int s_scan[kWaves], s_most;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const Table &t = f.old;
@@ -180,7 +202,7 @@ __global__ __launch_bounds__(kThreads) void fork_kernel(Fork f)
         const long long items = (long long)f.batch * chunks;
         for (long long i = (long long)(blockIdx.x - 1) * kWaves + wave; i < items; i += (long long)(gridDim.x - 1) * kWaves) {
             const int b = (int)(i / chunks), col0 = (int)(i % chunks) * 256;
-            const NewRow r = new_row(f, b);
+            const NewRow r = new_row(f, b, [&](int row) { return t.tokens(row); });
             const int *src = t.ids + (size_t)max(r.parent, 0) * t.stride;
             int *dst = f.table + (size_t)b * t.stride;
             int id[4];
@@ -198,22 +220,22 @@ __global__ __launch_bounds__(kThreads) void fork_kernel(Fork f)
         }
         return;
     }
-    clear_bits(f.pinned, f.num_pages, s_kept, s_held);
+    const int free_start = *f.free_start;
     if (tid == 0)
         s_most = 0;
-    __syncthreads();
     int most = 0;
     for (int row = tid; row < t.rows; row += kThreads) {
-        const int pages = t.pages(t.tokens(row));
-        s_pages[row] = pages;
+        s_tokens[row] = t.tokens(row);
         s_full[row] = 0;
-        most = max(most, pages);
+        most = max(most, t.pages(s_tokens[row]));
     }
-    atomicMax(&s_most, most);
+    clear_bits(f.pinned, f.num_pages, s_kept, s_held);
     __syncthreads();
+    block_most(most, &s_most);
+    auto row_of = [&](int b) { return new_row(f, b, [&](int row) { return s_tokens[row]; }); };
     NewRow mine = {};  // the thread's first row; the others are read again
     for (int b = tid; b < f.batch; b += kThreads) {
-        const NewRow r = new_row(f, b);
+        const NewRow r = row_of(b);
         if (b == tid)
             mine = r;
         f.lens[b] = r.tokens;
@@ -223,12 +245,12 @@ __global__ __launch_bounds__(kThreads) void fork_kernel(Fork f)
             __hip_atomic_store(f.first + r.last, INT_MAX, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     __syncthreads();
-    mark_pages<true>(t, s_pages, s_full, s_most, f.num_pages, s_held, s_kept);
+    mark_pages<true>(t, s_tokens, s_full, s_most, f.num_pages, s_held, s_kept);
     __syncthreads();
     // s_kept: pinned, or held whole by a new row
     auto open = [&](const NewRow &r) { return r.rest && (unsigned)r.last < (unsigned)f.num_pages && !has(s_kept, r.last); };
     for (int b = tid; b < f.batch; b += kThreads) {
-        const NewRow r = b == tid ? mine : new_row(f, b);
+        const NewRow r = b == tid ? mine : row_of(b);
         if (open(r))
             __hip_atomic_fetch_min(f.first + r.last, b, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
@@ -238,7 +260,7 @@ __global__ __launch_bounds__(kThreads) void fork_kernel(Fork f)
     };
     bool mine_goes_on = false;
     for (int b = tid; b < f.batch; b += kThreads) {
-        const NewRow r = b == tid ? mine : new_row(f, b);
+        const NewRow r = b == tid ? mine : row_of(b);
         const bool on = goes_on(r, b);
         if (b == tid)
             mine_goes_on = on;
@@ -254,7 +276,7 @@ __global__ __launch_bounds__(kThreads) void fork_kernel(Fork f)
         count += __builtin_popcount(s_held[w] & ~s_kept[w]);
     int freed;
     const int rank = block_before(count, s_scan, freed);
-    const long long start = (long long)*f.free_start - freed;
+    const long long start = (long long)free_start - freed;
     long long at = start + rank;
     for (int w = w0; w < w1; ++w)
         for (unsigned m = s_held[w] & ~s_kept[w]; m; m &= m - 1, ++at)
@@ -267,7 +289,7 @@ __global__ __launch_bounds__(kThreads) void fork_kernel(Fork f)
         NewRow r = mine;
         bool on = mine_goes_on;
         if (b0 > 0) {
-            r = b < f.batch ? new_row(f, b) : NewRow{};
+            r = b < f.batch ? row_of(b) : NewRow{};
             on = goes_on(r, b);
         }
         const bool takes = b < f.batch && r.rest && (unsigned)r.last < (unsigned)f.num_pages && !on;
@@ -294,60 +316,60 @@ struct Compact {
     Table old;
     const int *pinned, *free_pages, *free_start;
     int *table, *copies, *free_out;
-    int *to;  // [num_pages + 2]: where each page goes; then the moves, and the ids in the list
+    int *move;  // [num_pages + 3]: of a page that moves, which move; then the moves, the ids in the list, the lowest page that moves
     int num_pages, num_free, most_moves;
 };
 
 // Of the movable pages t (held by a row, not pinned) and the free ones f (listed, neither held nor pinned), the k-th
 // highest t moves to the k-th lowest f as long as that is lower. So f is moved to where more t stand above
 // it than f below it, and t moves where more f stand below it than t above it: each page finds its own
-// move from two sums over the bits, and k is the number of t above it (of f below it).
-// One workgroup, as in fork_kernel; remap_kernel then writes what needs no order.
+// move from two sums over the bits, and k is the number of t above it (of f below it). With m moves, the list
+// afterwards is the free pages but the m lowest, and the m highest movable ones, each page's place again a sum.
+// One workgroup, as in fork_kernel, a lane a page; remap_kernel then writes what needs no order.
 __global__ __launch_bounds__(kThreads) void compact_kernel(Compact c)
 {
-    __shared__ unsigned s_held[kWords], s_pinned[kWords], s_free[kWords];
-    __shared__ int s_pages[kMostRows];
-    __shared__ int s_scan[kWaves], s_most;
-    const int tid = threadIdx.x;
+    __shared__ __attribute__((aligned(8))) unsigned s_held[kWords], s_pinned[kWords], s_free[kWords];
+    __shared__ int s_rows[kMostRows];  // tokens of each row, then the pages below each 64: movable, free
+    __shared__ int s_scan[kWaves], s_most, s_moves, s_lowest;
+    static_assert(kMostRows >= 2 * (kMostPages / 64), "the sums take the rows' place");
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const Table &t = c.old;
-    clear_bits(c.pinned, c.num_pages, s_pinned, s_held);
-    const int words = (c.num_pages + 31) / 32;
-    for (int w = tid; w < words; w += kThreads)
-        s_free[w] = 0;
-    for (int p = tid; p < c.num_pages; p += kThreads)
-        c.to[p] = p;
-    if (tid == 0)
-        s_most = 0;
-    __syncthreads();
+    const int start = min(max(*c.free_start, 0), c.num_free);
+    if (tid == 0) {
+        s_most = s_moves = 0;
+        s_lowest = INT_MAX;
+    }
     int most = 0;
     for (int row = tid; row < t.rows; row += kThreads) {
-        const int pages = t.pages(t.tokens(row));
-        s_pages[row] = pages;
-        most = max(most, pages);
+        s_rows[row] = t.tokens(row);
+        most = max(most, t.pages(s_rows[row]));
     }
-    atomicMax(&s_most, most);
-    const int start = min(max(*c.free_start, 0), c.num_free);
-    for (int i0 = start; i0 < c.num_free; i0 += 8 * kThreads) {
-        int id[8];
+    clear_bits(c.pinned, c.num_pages, s_pinned, s_held);
+    const int groups = (c.num_pages + 63) / 64;
+    for (int w = tid; w < 2 * groups; w += kThreads)
+        s_free[w] = 0;
+    __syncthreads();
+    block_most(most, &s_most);
+    for (int i0 = start; i0 < c.num_free; i0 += 16 * kThreads) {
+        int id[16];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
+        for (int k = 0; k < 16; ++k) {
             const long long i = (long long)i0 + k * kThreads + tid;
             id[k] = i < c.num_free ? c.free_pages[i] : -1;
         }
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
+        for (int k = 0; k < 16; ++k)
             if ((unsigned)id[k] < (unsigned)c.num_pages)
                 atomicOr(s_free + (id[k] >> 5), 1u << (id[k] & 31));
-        if (i0 > c.num_free - 8 * kThreads)
+        if (i0 > c.num_free - 16 * kThreads)
             break;  // (i0 would pass 2^31)
     }
     __syncthreads();
-    mark_pages<false>(t, s_pages, nullptr, s_most, c.num_pages, s_held, nullptr);
+    mark_pages<false>(t, s_rows, nullptr, s_most, c.num_pages, s_held, nullptr);
     __syncthreads();
-    const int per = (words + kThreads - 1) / kThreads;
-    const int w0 = min(tid * per, words), w1 = min(w0 + per, words);
+    const int per = (groups + kThreads - 1) / kThreads, g0 = min(tid * per, groups), g1 = min(g0 + per, groups);
     int movable = 0, listed = 0;
-    for (int w = w0; w < w1; ++w) {
+    for (int w = 2 * g0; w < 2 * g1; ++w) {
         const unsigned p = s_pinned[w], h = s_held[w], m = h & ~p, l = s_free[w] & ~h & ~p;
         s_held[w] = m;
         s_free[w] = l;
@@ -355,47 +377,57 @@ __global__ __launch_bounds__(kThreads) void compact_kernel(Compact c)
         listed += __builtin_popcount(l);
     }
     int all_movable, all_free;
-    const int t_first = block_before(movable, s_scan, all_movable), f_first = block_before(listed, s_scan, all_free);
-    // visit(page, is t, moves, k) for the thread's pages, lowest first
+    int t_below = block_before(movable, s_scan, all_movable), f_below = block_before(listed, s_scan, all_free);
+    for (int g = g0; g < g1; ++g) {
+        s_rows[2 * g] = t_below;
+        s_rows[2 * g + 1] = f_below;
+        t_below += __builtin_popcount(s_held[2 * g]) + __builtin_popcount(s_held[2 * g + 1]);
+        f_below += __builtin_popcount(s_free[2 * g]) + __builtin_popcount(s_free[2 * g + 1]);
+    }
+    __syncthreads();
+    // visit(page, is movable, is free, movable ones below it, free ones below it), a lane a page
     auto each = [&](auto &&visit) {
-        int t_below = t_first, f_below = f_first;
-        for (int w = w0; w < w1; ++w) {
-            const unsigned held = s_held[w];
-            for (unsigned m = held | s_free[w]; m; m &= m - 1) {
-                const int bit = __builtin_ctz(m);
-                if ((held >> bit) & 1) {
-                    const int above = all_movable - 1 - t_below++;
-                    visit(32 * w + bit, true, f_below > above, above);
-                } else {
-                    visit(32 * w + bit, false, all_movable - t_below > f_below, f_below);
-                    ++f_below;
-                }
-            }
+        const unsigned long long below = (1ull << lane) - 1;
+        for (int g = wave; g < groups; g += kWaves) {
+            const unsigned long long held = *(const unsigned long long *)(s_held + 2 * g);
+            const unsigned long long free = *(const unsigned long long *)(s_free + 2 * g);
+            visit(64 * g + lane, (held >> lane) & 1, (free >> lane) & 1, s_rows[2 * g] + __builtin_popcountll(held & below),
+                  s_rows[2 * g + 1] + __builtin_popcountll(free & below));
         }
     };
-    int moves = 0, left = 0;
-    each([&](int page, bool is_t, bool moves_it, int k) {
-        if (moves_it) {
-            int *copy = c.copies + 3 * (size_t)k;
-            copy[is_t ? 0 : 1] = page;
-            if (is_t)
-                copy[2] = 1 << t.page_shift;
+    int moves = 0, lowest = INT_MAX;
+    each([&](int page, bool is_t, bool is_f, int tb, int fb) {
+        const int above = all_movable - 1 - tb;
+        if (is_t && fb > above) {
+            c.copies[3 * (size_t)above] = page;
+            c.copies[3 * (size_t)above + 2] = 1 << t.page_shift;
+            c.move[page] = above;
+            lowest = min(lowest, page);
+            ++moves;
+        } else if (is_f && all_movable - tb > fb) {
+            c.copies[3 * (size_t)fb + 1] = page;
         }
-        moves += is_t && moves_it;
-        left += is_t == moves_it;
     });
-    int all_moves, all_left;
-    block_before(moves, s_scan, all_moves);
-    long long at = start + block_before(left, s_scan, all_left);
-    each([&](int page, bool is_t, bool moves_it, int k) {
-        if (is_t && moves_it)
-            c.to[page] = c.copies[3 * (size_t)k + 1];
-        if (is_t == moves_it)
-            c.free_out[at++] = page;
+#pragma unroll
+    for (int d = 32; d > 0; d /= 2) {
+        moves += __shfl_xor(moves, d);
+        lowest = min(lowest, __shfl_xor(lowest, d));
+    }
+    if (lane == 0) {
+        atomicAdd(&s_moves, moves);
+        atomicMin(&s_lowest, lowest);
+    }
+    __syncthreads();
+    const int all_moves = s_moves;
+    each([&](int page, bool is_t, bool is_f, int tb, int fb) {
+        const int moved_below = max(0, tb - (all_movable - all_moves));
+        if (is_t ? tb >= all_movable - all_moves : is_f && fb >= all_moves)
+            c.free_out[(long long)start + fb - all_moves + moved_below] = page;
     });
     if (tid == 0) {
-        c.to[c.num_pages] = all_moves;
-        c.to[c.num_pages + 1] = all_left;
+        c.move[c.num_pages] = all_moves;
+        c.move[c.num_pages + 1] = all_free;
+        c.move[c.num_pages + 2] = s_lowest;
     }
 }
 
@@ -407,6 +439,7 @@ __global__ __launch_bounds__(256) void remap_kernel(Compact c)
     const long long wave = blockIdx.x * 4ll + (threadIdx.x >> 6), waves = gridDim.x * 4ll;
     const int chunks = (t.stride + 255) / 256;
     const long long items = (long long)t.rows * chunks;
+    const int moves = c.move[c.num_pages], lowest = c.move[c.num_pages + 2];
     for (long long i = wave; i < items; i += waves) {
         const int row = (int)(i / chunks), col0 = (int)(i % chunks) * 256;
         const int pages = t.pages(t.tokens(row));
@@ -418,9 +451,9 @@ __global__ __launch_bounds__(256) void remap_kernel(Compact c)
             id[k] = col < pages ? t.ids[base + col] : -1;
         }
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if ((unsigned)id[k] < (unsigned)c.num_pages)
-                id[k] = c.to[id[k]];
+        for (int k = 0; k < 4; ++k)  // every held page from the lowest that moves on does, unless it is pinned
+            if (id[k] >= lowest && id[k] < c.num_pages && !(c.pinned && c.pinned[id[k]] > 0))
+                id[k] = c.copies[3 * (size_t)c.move[id[k]] + 1];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const int col = col0 + 64 * k + lane;
@@ -428,8 +461,7 @@ __global__ __launch_bounds__(256) void remap_kernel(Compact c)
                 c.table[base + col] = id[k];
         }
     }
-    const int start = min(max(*c.free_start, 0), c.num_free);
-    const int moves = c.to[c.num_pages], end = start + c.to[c.num_pages + 1];
+    const int start = min(max(*c.free_start, 0), c.num_free), end = start + c.move[c.num_pages + 1];
     const long long thread = blockIdx.x * 256ll + threadIdx.x, threads = gridDim.x * 256ll;
     for (long long i = 3ll * moves + thread; i < 3ll * c.most_moves; i += threads)
         c.copies[i] = i % 3 == 2 ? 0 : -1;
@@ -440,33 +472,36 @@ __global__ __launch_bounds__(256) void remap_kernel(Compact c)
 
 // ---- copies -----------------------------------------------------------------
 
-// A workgroup takes one page's next chunk of bytes at a time, four 16-byte loads a thread in
-// flight before their stores.
+// A workgroup takes one chunk of a page at a time, four 16-byte loads a thread in flight before their stores.
 __global__ __launch_bounds__(256) void copy_pages_kernel(unsigned char *__restrict__ cache, const int *__restrict__ copies,
-                                                         int count, int layers, int num_pages, int page_size, int row_bytes,
-                                                         int chunk, int chunks)
+                                                         unsigned count, unsigned per_entry, unsigned chunks, int num_pages,
+                                                         int page_size, int row_bytes, int chunk)
 {
-    const long long page_bytes = (long long)page_size * row_bytes, items = (long long)count * chunks * layers;
-    for (long long i = blockIdx.x; i < items; i += gridDim.x) {
-        const long long e = i / chunks;
-        const int layer = (int)(e / count), entry = (int)(e % count);
+    typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+    const size_t page_bytes = (size_t)page_size * row_bytes;
+    // entry blockIdx.x / per_entry first, per_entry = layers x chunks: an entry's chunks are neighbours
+    for (unsigned long long i = blockIdx.x; i < (unsigned long long)count * per_entry; i += gridDim.x) {
+        const unsigned entry = (unsigned)(i / per_entry), part = (unsigned)(i - (unsigned long long)entry * per_entry);
         const int src = copies[3 * (size_t)entry], dst = copies[3 * (size_t)entry + 1];
         const int rows = min(copies[3 * (size_t)entry + 2], page_size);
         if ((unsigned)src >= (unsigned)num_pages || (unsigned)dst >= (unsigned)num_pages || src == dst || rows <= 0)
             continue;
-        const long long first = (i % chunks) * chunk, end = min(first + chunk, (long long)rows * row_bytes);
+        const unsigned layer = part / chunks;
+        const size_t first = (size_t)(part - layer * chunks) * chunk, end = min(first + chunk, (size_t)rows * row_bytes);
         unsigned char *layer_base = cache + (size_t)layer * num_pages * page_bytes;
         const unsigned char *from = layer_base + (size_t)src * page_bytes;
         unsigned char *to = layer_base + (size_t)dst * page_bytes;
-        for (long long o = first + threadIdx.x * 16; o < end; o += 4 * 4096) {
-            uint4 v[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-                v[k] = *(const uint4 *)(from + min(o + 4096 * k, end - 16));
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-                if (o + 4096 * k < end)
-                    *(uint4 *)(to + o + 4096 * k) = v[k];
+        for (size_t o = first + threadIdx.x * 16; o < end; o += 4 * 4096) {
+            const size_t o1 = o + 4096, o2 = o + 2 * 4096, o3 = o + 3 * 4096, last = end - 16;
+            const u32x4 a = *(const u32x4 *)(from + o), b = *(const u32x4 *)(from + min(o1, last));
+            const u32x4 c = *(const u32x4 *)(from + min(o2, last)), d = *(const u32x4 *)(from + min(o3, last));
+            *(u32x4 *)(to + o) = a;
+            if (o1 < end)
+                *(u32x4 *)(to + o1) = b;
+            if (o2 < end)
+                *(u32x4 *)(to + o2) = c;
+            if (o3 < end)
+                *(u32x4 *)(to + o3) = d;
         }
     }
 }
@@ -492,7 +527,7 @@ extern "C" {
 
 size_t mla_page_tables_workspace_size(int num_pages)
 {
-    return num_pages < 1 || num_pages > mla::kMostPages ? 0 : (4 * ((size_t)num_pages + 2) + 255) / 256 * 256;
+    return num_pages < 1 || num_pages > mla::kMostPages ? 0 : (4 * ((size_t)num_pages + 3) + 255) / 256 * 256;
 }
 
 int mla_fork_tables(const int *block_table, const int *lens, const int *parents, const int *kept_lens, const int *pinned,
@@ -560,11 +595,13 @@ int mla_copy_pages(void *kv_cache, const int *copies, int count, int layers, int
     const int64_t page_bytes = (int64_t)page_size * row_bytes;
     const int chunks = (int)((page_bytes + 16383) / 16384);
     const int chunk = (int)(((page_bytes + chunks - 1) / chunks + 4095) / 4096 * 4096);
-    const int64_t items = (int64_t)count * layers * chunks;
-    const int wgs = (int)std::min<int64_t>(items, 16 * (int64_t)mla::current_cu_count());
+    const int64_t per_entry = (int64_t)layers * chunks, items = (int64_t)count * per_entry;
+    if (per_entry > INT32_MAX)
+        return MLA_STATUS_INVALID_VALUE;
+    const int wgs = (int)std::min<int64_t>(items, 64 * (int64_t)mla::current_cu_count());
     hipLaunchKernelGGL(mla::copy_pages_kernel, dim3(wgs), dim3(256), 0, static_cast<hipStream_t>(stream),
-                       static_cast<unsigned char *>(kv_cache), copies, count, layers, num_pages, page_size, row_bytes, chunk,
-                       chunks);
+                       static_cast<unsigned char *>(kv_cache), copies, (unsigned)count, (unsigned)per_entry, (unsigned)chunks,
+                       num_pages, page_size, row_bytes, chunk);
     return mla::launched();
 }
 
