@@ -456,7 +456,7 @@ void check_pool(const at::Tensor &table, const at::Tensor &lens, const at::Tenso
     check_int32(free_start, 1, fn, "free_start");
     TORCH_CHECK(table.size(0) >= 1 && table.size(0) <= 8192 && lens.size(0) == table.size(0), fn,
                 ": lens and block_table must have one entry or row per request, 8192 at most");
-    TORCH_CHECK(table.size(1) >= 1 && table.size(1) <= INT32_MAX, fn, ": block_table needs at least one column");
+    TORCH_CHECK(table.size(1) >= 1 && table.size(1) <= (1 << 20), fn, ": block_table needs at least one column (and 2^20 at most)");
     TORCH_CHECK(free_pages.size(0) <= INT32_MAX, fn, ": too many free pages");
     TORCH_CHECK(free_start.size(0) == 1, fn, ": free_start must have one entry");
     check_page_size(page_size, fn);

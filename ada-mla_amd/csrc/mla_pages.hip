@@ -23,6 +23,7 @@ namespace {
 constexpr int kThreads = 1024, kWaves = kThreads / 64;
 constexpr int kMostPages = 1 << 18;  // 32 KB of bits
 constexpr int kMostRows = 8192;
+constexpr int kMostColumns = 1 << 20;  // 64 rows' offsets stay within 32 bits
 constexpr int kWords = kMostPages / 32;
 
 // Exclusive sums of v over the workgroup's threads; total: over all of them. s: a word of LDS a wave.
@@ -76,78 +77,97 @@ struct Table {
     }
 };
 
-__device__ __forceinline__ bool has(const unsigned *bits, int page) { return (bits[page >> 5] >> (page & 31)) & 1; }
-
-// One bit a page: held by a row of the table, and (kFull) by one of the first full[row]
-// columns of a row. A wave takes pieces of 64 rows x 16 columns, each lane a column of 16 rows in a row, kPieces of them
-// at once (64 loads in flight: a round of one piece was a round trip, 5 of them 16 us of a call with 1024 rows of 77 pages), and
-// the page that a row shares with the row above (a prompt's) is marked once.
-// tokens, full: of each row, in LDS; most: the largest row's pages.
+// One bit a page that a row of the table holds: in bits[w], or (kFull) in bits[2 w], with one in bits[2 w + 1] for a page
+// in the first full[row] columns of a row. A wave takes pieces of 64 rows x 16 columns, each lane a column of 16 rows in a
+// row, kPieces of them at once, and the page that a row shares with the row above (a prompt's) is marked once. One
+// CU does all of it, so it is bound by its instructions (1024 rows of 77 pages: 20 us with a condition around each
+// load and an atomic for each bit, 8 with clamped addresses and one of 64 bits).
+// pages, full: of each row, in LDS, zeros from t.rows to the next multiple of 64; most: the largest row's pages.
 template <bool kFull>
-__device__ __forceinline__ void mark_pages(const Table &t, const int *tokens, const int *full, int most, int num_pages,
-                                           unsigned *held_bits, unsigned *full_bits)
+__device__ __forceinline__ void mark_pages(const Table &t, const int *pages, const int *full, int most, int num_pages,
+                                           unsigned *bits)
 {
+    typedef int i32x4 __attribute__((ext_vector_type(4)));
     constexpr int kPieces = 4;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int chunks = (most + 15) / 16, pieces = (t.rows + 63) / 64 * chunks;
+    const int above = lane >> 4 << 4;  // the lane's first row in a piece
     for (int first = wave; first < pieces; first += kPieces * kWaves) {
         int id[kPieces][16];
 #pragma unroll
         for (int k = 0; k < kPieces; ++k) {
-            const int piece = first + k * kWaves;
-            const int row0 = piece / chunks * 64 + (lane >> 4) * 16, col = piece % chunks * 16 + (lane & 15);
+            const int piece = min(first + k * kWaves, pieces - 1), row0 = piece / chunks * 64;
+            const int *base = t.ids + (size_t)row0 * t.stride;
+            const int col = min(piece % chunks * 16 + (lane & 15), t.stride - 1), last = t.rows - 1 - row0;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int row = row0 + i;
-                id[k][i] = piece < pieces && row < t.rows && col < t.pages(tokens[row]) ? t.ids[(size_t)row * t.stride + col] : -1;
-            }
+            for (int i = 0; i < 16; ++i)
+                id[k][i] = base[min(above + i, last) * t.stride + col];
         }
 #pragma unroll
         for (int k = 0; k < kPieces; ++k) {
             const int piece = first + k * kWaves;
-            const int row0 = piece / chunks * 64 + (lane >> 4) * 16, col = piece % chunks * 16 + (lane & 15);
-            bool above_full = false;
+            if (piece >= pieces)
+                break;
+            const int row0 = piece / chunks * 64 + above, col = piece % chunks * 16 + (lane & 15);
+            int before = -1;
+            bool before_whole = false;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int page = id[k][i];
-                bool whole = false;
-                if ((unsigned)page < (unsigned)num_pages) {
-                    const bool again = i > 0 && page == id[k][i > 0 ? i - 1 : 0];
-                    const unsigned bit = 1u << (page & 31);
-                    if (!again)
-                        atomicOr(held_bits + (page >> 5), bit);
-                    if constexpr (kFull) {
-                        whole = col < full[row0 + i];
-                        if (whole && !(again && above_full))
-                            atomicOr(full_bits + (page >> 5), bit);
+            for (int q = 0; q < 4; ++q) {
+                const i32x4 held = *(const i32x4 *)(pages + row0 + 4 * q);
+                i32x4 most_full = {0, 0, 0, 0};
+                if constexpr (kFull)
+                    most_full = *(const i32x4 *)(full + row0 + 4 * q);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int page = col < held[e] && (unsigned)id[k][4 * q + e] < (unsigned)num_pages ? id[k][4 * q + e] : -1;
+                    const bool whole = kFull && col < most_full[e];
+                    if (page >= 0 && (page != before || (whole && !before_whole))) {
+                        if constexpr (kFull) {
+                            const unsigned long long bit = 1ull << (page & 31);
+                            atomicOr(reinterpret_cast<unsigned long long *>(bits) + (page >> 5), whole ? bit | bit << 32 : bit);
+                        } else {
+                            atomicOr(bits + (page >> 5), 1u << (page & 31));
+                        }
                     }
+                    before = page;
+                    before_whole = whole;
                 }
-                above_full = whole;
             }
         }
     }
 }
 
-// bits <- one bit a page that `pinned` counts as held elsewhere (none if it is null); others <- 0.
+// One bit a page that `pinned` counts as held elsewhere (none if it is null), in bits[step w]; others[step w] <- 0.
+template <int step>
 __device__ __forceinline__ void clear_bits(const int *pinned, int num_pages, unsigned *bits, unsigned *others)
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     for (int base = 1024 * wave; base < num_pages; base += 1024 * kWaves) {
         int v[16];
+        const int last = num_pages - 1;
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            v[i] = pinned ? pinned[min(base + 64 * i + lane, last)] : 0;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            const int p = base + 64 * i + lane;
-            v[i] = pinned && p < num_pages ? pinned[p] : 0;
-        }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const unsigned long long m = __builtin_amdgcn_ballot_w64(v[i] > 0);
+            const unsigned long long m = __builtin_amdgcn_ballot_w64(v[i] > 0 && base + 64 * i + lane <= last);
             if (lane < 2) {  // up to 31 words past the last page's: kWords is a multiple of 32
-                bits[base / 32 + 2 * i + lane] = (unsigned)(m >> (32 * lane));
-                others[base / 32 + 2 * i + lane] = 0;
+                bits[step * (base / 32 + 2 * i + lane)] = (unsigned)(m >> (32 * lane));
+                others[step * (base / 32 + 2 * i + lane)] = 0;
             }
         }
     }
+}
+
+// pages[row] <- the row's pages, in LDS, zeros up to the next multiple of 64 rows; the most of a row into *most.
+__device__ __forceinline__ void row_pages(const Table &t, int *pages, int *most)
+{
+    int largest = 0;
+    for (int row = threadIdx.x; row < (t.rows + 63) / 64 * 64; row += kThreads) {
+        pages[row] = row < t.rows ? t.pages(t.tokens(row)) : 0;
+        largest = max(largest, pages[row]);
+    }
+    block_most(largest, most);
 }
 
 // ---- fork -------------------------------------------------------------------
@@ -164,15 +184,13 @@ struct NewRow {
     int last;                        // that page's id
 };
 
-// old_tokens(row): of the old table
-template <typename F>
-__device__ __forceinline__ NewRow new_row(const Fork &f, int b, F &&old_tokens)
+__device__ __forceinline__ NewRow new_row(const Fork &f, int b)
 {
     NewRow r;
     r.parent = f.parents[b];
     const int kept = f.kept ? max(f.kept[b], 0) : INT_MAX;
     const bool real = (unsigned)r.parent < (unsigned)f.old.rows;
-    r.tokens = real ? min(kept, old_tokens(r.parent)) : 0;
+    r.tokens = real ? min(kept, f.old.tokens(r.parent)) : 0;
     r.full = r.tokens >> f.old.page_shift;
     r.rest = r.tokens & ((1 << f.old.page_shift) - 1);
     r.last = r.rest ? f.old.ids[(size_t)r.parent * f.old.stride + r.full] : -1;
@@ -191,8 +209,8 @@ __device__ __forceinline__ NewRow new_row(const Fork &f, int b, F &&old_tokens)
 // what a call costs.
 __global__ __launch_bounds__(kThreads) void fork_kernel(Fork f)
 {
-    __shared__ unsigned s_held[kWords], s_kept[kWords];
-    __shared__ int s_tokens[kMostRows], s_full[kMostRows];
+    __shared__ __attribute__((aligned(16))) unsigned s_bits[2 * kWords];  // of 32 pages: held before; pinned, or held whole by a new row
+    __shared__ __attribute__((aligned(16))) int s_pages[kMostRows], s_full[kMostRows];
     __shared__ int s_scan[kWaves], s_most;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const Table &t = f.old;
@@ -202,7 +220,7 @@ __global__ __launch_bounds__(kThreads) void fork_kernel(Fork f)
         const long long items = (long long)f.batch * chunks;
         for (long long i = (long long)(blockIdx.x - 1) * kWaves + wave; i < items; i += (long long)(gridDim.x - 1) * kWaves) {
             const int b = (int)(i / chunks), col0 = (int)(i % chunks) * 256;
-            const NewRow r = new_row(f, b, [&](int row) { return t.tokens(row); });
+            const NewRow r = new_row(f, b);
             const int *src = t.ids + (size_t)max(r.parent, 0) * t.stride;
             int *dst = f.table + (size_t)b * t.stride;
             int id[4];
@@ -221,21 +239,19 @@ __global__ __launch_bounds__(kThreads) void fork_kernel(Fork f)
         return;
     }
     const int free_start = *f.free_start;
+    auto held = [&](int w) -> unsigned & { return s_bits[2 * w]; };
+    auto kept = [&](int w) -> unsigned & { return s_bits[2 * w + 1]; };
     if (tid == 0)
         s_most = 0;
-    int most = 0;
-    for (int row = tid; row < t.rows; row += kThreads) {
-        s_tokens[row] = t.tokens(row);
-        s_full[row] = 0;
-        most = max(most, t.pages(s_tokens[row]));
-    }
-    clear_bits(f.pinned, f.num_pages, s_kept, s_held);
     __syncthreads();
-    block_most(most, &s_most);
-    auto row_of = [&](int b) { return new_row(f, b, [&](int row) { return s_tokens[row]; }); };
+    row_pages(t, s_pages, &s_most);
+    for (int row = tid; row < (t.rows + 63) / 64 * 64; row += kThreads)
+        s_full[row] = 0;
+    clear_bits<2>(f.pinned, f.num_pages, s_bits + 1, s_bits);
+    __syncthreads();
     NewRow mine = {};  // the thread's first row; the others are read again
     for (int b = tid; b < f.batch; b += kThreads) {
-        const NewRow r = row_of(b);
+        const NewRow r = new_row(f, b);
         if (b == tid)
             mine = r;
         f.lens[b] = r.tokens;
@@ -245,12 +261,13 @@ __global__ __launch_bounds__(kThreads) void fork_kernel(Fork f)
             __hip_atomic_store(f.first + r.last, INT_MAX, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     __syncthreads();
-    mark_pages<true>(t, s_tokens, s_full, s_most, f.num_pages, s_held, s_kept);
+    mark_pages<true>(t, s_pages, s_full, s_most, f.num_pages, s_bits);
     __syncthreads();
-    // s_kept: pinned, or held whole by a new row
-    auto open = [&](const NewRow &r) { return r.rest && (unsigned)r.last < (unsigned)f.num_pages && !has(s_kept, r.last); };
+    auto open = [&](const NewRow &r) {
+        return r.rest && (unsigned)r.last < (unsigned)f.num_pages && !((kept(r.last >> 5) >> (r.last & 31)) & 1);
+    };
     for (int b = tid; b < f.batch; b += kThreads) {
-        const NewRow r = b == tid ? mine : row_of(b);
+        const NewRow r = b == tid ? mine : new_row(f, b);
         if (open(r))
             __hip_atomic_fetch_min(f.first + r.last, b, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
@@ -260,12 +277,12 @@ __global__ __launch_bounds__(kThreads) void fork_kernel(Fork f)
     };
     bool mine_goes_on = false;
     for (int b = tid; b < f.batch; b += kThreads) {
-        const NewRow r = b == tid ? mine : row_of(b);
+        const NewRow r = b == tid ? mine : new_row(f, b);
         const bool on = goes_on(r, b);
         if (b == tid)
             mine_goes_on = on;
         if (on)
-            atomicAnd(s_held + (r.last >> 5), ~(1u << (r.last & 31)));  // not to be freed
+            atomicAnd(&held(r.last >> 5), ~(1u << (r.last & 31)));  // not to be freed
     }
     __syncthreads();
     // pages to free: each thread a run of words, lowest ids first
@@ -273,13 +290,13 @@ __global__ __launch_bounds__(kThreads) void fork_kernel(Fork f)
     const int w0 = min(tid * per, words), w1 = min(w0 + per, words);
     int count = 0;
     for (int w = w0; w < w1; ++w)
-        count += __builtin_popcount(s_held[w] & ~s_kept[w]);
+        count += __builtin_popcount(held(w) & ~kept(w));
     int freed;
     const int rank = block_before(count, s_scan, freed);
     const long long start = (long long)free_start - freed;
     long long at = start + rank;
     for (int w = w0; w < w1; ++w)
-        for (unsigned m = s_held[w] & ~s_kept[w]; m; m &= m - 1, ++at)
+        for (unsigned m = held(w) & ~kept(w); m; m &= m - 1, ++at)
             if (at >= 0 && at < f.num_free)
                 f.free_pages[at] = 32 * w + __builtin_ctz(m);
     __syncthreads();
@@ -289,7 +306,7 @@ __global__ __launch_bounds__(kThreads) void fork_kernel(Fork f)
         NewRow r = mine;
         bool on = mine_goes_on;
         if (b0 > 0) {
-            r = b < f.batch ? row_of(b) : NewRow{};
+            r = b < f.batch ? new_row(f, b) : NewRow{};
             on = goes_on(r, b);
         }
         const bool takes = b < f.batch && r.rest && (unsigned)r.last < (unsigned)f.num_pages && !on;
@@ -329,7 +346,7 @@ struct Compact {
 __global__ __launch_bounds__(kThreads) void compact_kernel(Compact c)
 {
     __shared__ __attribute__((aligned(8))) unsigned s_held[kWords], s_pinned[kWords], s_free[kWords];
-    __shared__ int s_rows[kMostRows];  // tokens of each row, then the pages below each 64: movable, free
+    __shared__ __attribute__((aligned(16))) int s_rows[kMostRows];  // pages of each row, then the pages below each 64: movable, free
     __shared__ int s_scan[kWaves], s_most, s_moves, s_lowest;
     static_assert(kMostRows >= 2 * (kMostPages / 64), "the sums take the rows' place");
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -339,33 +356,34 @@ __global__ __launch_bounds__(kThreads) void compact_kernel(Compact c)
         s_most = s_moves = 0;
         s_lowest = INT_MAX;
     }
-    int most = 0;
-    for (int row = tid; row < t.rows; row += kThreads) {
-        s_rows[row] = t.tokens(row);
-        most = max(most, t.pages(s_rows[row]));
-    }
-    clear_bits(c.pinned, c.num_pages, s_pinned, s_held);
-    const int groups = (c.num_pages + 63) / 64;
-    for (int w = tid; w < 2 * groups; w += kThreads)
-        s_free[w] = 0;
-    __syncthreads();
-    block_most(most, &s_most);
-    for (int i0 = start; i0 < c.num_free; i0 += 16 * kThreads) {
-        int id[16];
+    // the list's first ids are on their way with the rows' lengths and the pins
+    constexpr int kIds = 16;
+    int id[kIds];
+    auto fetch = [&](int i0) {
 #pragma unroll
-        for (int k = 0; k < 16; ++k) {
+        for (int k = 0; k < kIds; ++k) {
             const long long i = (long long)i0 + k * kThreads + tid;
             id[k] = i < c.num_free ? c.free_pages[i] : -1;
         }
+    };
+    fetch(start);
+    const int groups = (c.num_pages + 63) / 64;
+    for (int w = tid; w < 2 * groups; w += kThreads)
+        s_free[w] = 0;
+    clear_bits<1>(c.pinned, c.num_pages, s_pinned, s_held);
+    __syncthreads();
+    row_pages(t, s_rows, &s_most);
+    for (int i0 = start;;) {
 #pragma unroll
-        for (int k = 0; k < 16; ++k)
+        for (int k = 0; k < kIds; ++k)
             if ((unsigned)id[k] < (unsigned)c.num_pages)
                 atomicOr(s_free + (id[k] >> 5), 1u << (id[k] & 31));
-        if (i0 > c.num_free - 16 * kThreads)
-            break;  // (i0 would pass 2^31)
+        if (i0 >= c.num_free - kIds * kThreads)
+            break;
+        fetch(i0 += kIds * kThreads);
     }
     __syncthreads();
-    mark_pages<false>(t, s_rows, nullptr, s_most, c.num_pages, s_held, nullptr);
+    mark_pages<false>(t, s_rows, nullptr, s_most, c.num_pages, s_held);
     __syncthreads();
     const int per = (groups + kThreads - 1) / kThreads, g0 = min(tid * per, groups), g1 = min(g0 + per, groups);
     int movable = 0, listed = 0;
@@ -511,7 +529,7 @@ bool page_ok(int page_size) { return page_size >= 32 && page_size <= (1 << 20) &
 bool table_ok(const int *block_table, const int *lens, int rows, int num_pages, int page_size, int stride)
 {
     return block_table && lens && rows >= 1 && rows <= kMostRows && num_pages >= 1 && num_pages <= kMostPages &&
-           page_ok(page_size) && stride >= 1;
+           page_ok(page_size) && stride >= 1 && stride <= kMostColumns;
 }
 
 int launched()

@@ -466,7 +466,7 @@ int mla_paged_tables(const int *context_lens, const int *new_lens,
  * written, and a page taken is -1. Ids outside [0, num_pages) are passed on
  * and neither freed nor copied. pinned marks pages that others hold, a prompt
  * cache or another table. rows is at most 8192, num_pages at most 2^18,
- * page_size a power of two from 32 to 2^20. new_table, new_lens and
+ * block_table_stride at most 2^20, page_size a power of two from 32 to 2^20. new_table, new_lens and
  * free_next must not be their inputs. One launch. */
 size_t mla_page_tables_workspace_size(int num_pages);
 int mla_fork_tables(const int *block_table, const int *lens,

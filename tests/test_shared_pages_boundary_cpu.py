@@ -56,7 +56,7 @@ def test_fork_argument_errors():
     for bad in (dict(table=None), dict(lens=None), dict(parents=None), dict(free=None), dict(start=None), dict(new=None),
                 dict(new_lens=None), dict(copies=None), dict(next=None), dict(ws=None), dict(rows=0), dict(rows=8193),
                 dict(batch=0), dict(batch=2 ** 31 - 1), dict(pages=0), dict(pages=2 ** 18 + 1), dict(num_free=-1),
-                dict(page=16), dict(page=48), dict(page=1 << 21), dict(stride=0), dict(new=ok["table"]),
+                dict(page=16), dict(page=48), dict(page=1 << 21), dict(stride=0), dict(stride=2 ** 20 + 1), dict(new=ok["table"]),
                 dict(new_lens=ok["lens"]), dict(next=ok["start"])):
         assert call(**bad) == capi.STATUS_INVALID_VALUE, bad
     assert call(ws=FAKE + 4) == capi.STATUS_MISALIGNED
