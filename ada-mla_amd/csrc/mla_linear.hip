@@ -88,30 +88,42 @@ __device__ __forceinline__ uint2 quantized8(E8 v, float &scale)
     return e4m3x8(y);
 }
 
-// 16 lanes a block: one 16-byte load, a maximum over the 16 lanes, one 8-byte store.
-// scales: of row m and block b at m row_step + b block_step.
+// 16 lanes a block: one 16-byte load, a maximum over the 16 lanes, one 8-byte store; four blocks a thread, so that four
+// loads are on their way (8192 x 7168 bf16, 180 MB: 45 us with one, 3.9 TB/s).
+// scales: of row m and block b at b rows + m.
+constexpr int kQuantizeUnits = 4;
 template <typename E>
 __global__ __launch_bounds__(256) void quantize_kernel(const E *__restrict__ x, unsigned char *__restrict__ q,
                                                        float *__restrict__ scales, int rows, int inputs, int blocks,
-                                                       long long x_stride, long long q_stride, long long row_step,
-                                                       long long block_step)
+                                                       long long x_stride)
 {
     using E8 = typename Vec<E>::v8;
-    const long long units = (long long)rows * blocks;
-    const long long u = blockIdx.x * 16ll + (threadIdx.x >> 4);
+    const unsigned units = (unsigned)rows * blocks, first = blockIdx.x * (16u * kQuantizeUnits) + (threadIdx.x >> 4);
     const int j = threadIdx.x & 15;
-    if (u >= units)
-        return;
-    const int m = (int)(u / blocks), b = (int)(u % blocks), k = b * kBlock + 8 * j;
-    E8 v = {};
-    if (k < inputs)
-        v = *(const E8 *)(x + m * x_stride + k);
-    float scale;
-    const uint2 y = quantized8(v, scale);
-    if (k < inputs)
-        *(uint2 *)(q + m * q_stride + k) = y;
-    if (j == 0)
-        scales[m * row_step + b * block_step] = scale;
+    E8 v[kQuantizeUnits];
+    unsigned m[kQuantizeUnits], b[kQuantizeUnits];
+#pragma unroll
+    for (int i = 0; i < kQuantizeUnits; ++i) {
+        const unsigned u = min(first + 16 * i, units - 1);
+        m[i] = u / (unsigned)blocks;
+        b[i] = u - m[i] * blocks;
+        const int k = (int)b[i] * kBlock + 8 * j;
+        v[i] = *(const E8 *)(x + m[i] * x_stride + min(k, inputs - 8));
+        if (k >= inputs)
+            v[i] = E8{};
+    }
+#pragma unroll
+    for (int i = 0; i < kQuantizeUnits; ++i) {
+        float scale;
+        const uint2 y = quantized8(v[i], scale);
+        const int k = (int)b[i] * kBlock + 8 * j;
+        if (first + 16 * i >= units)
+            return;
+        if (k < inputs)
+            *(uint2 *)(q + (size_t)m[i] * inputs + k) = y;
+        if (j == 0)
+            scales[(size_t)b[i] * rows + m[i]] = scale;
+    }
 }
 
 // ---- products ---------------------------------------------------------------
@@ -577,7 +589,8 @@ int ceil_div(int a, int b) { return (int)(((long long)a + b - 1) / b); }
 bool sizes_ok(int rows, int inputs, int outputs)
 {
     return rows >= 1 && rows <= (1 << 26) && inputs >= 16 && inputs % 16 == 0 && inputs <= kMostStride && outputs >= 1 &&
-           outputs <= (1 << 26) && (int64_t)ceil_div(rows, 16) * ceil_div(outputs, 16) <= INT32_MAX;
+           outputs <= (1 << 26) && (int64_t)ceil_div(rows, 16) * ceil_div(outputs, 16) <= INT32_MAX &&
+           (int64_t)rows * ceil_div(inputs, kBlock) <= INT32_MAX;
 }
 
 int launched()
@@ -587,13 +600,12 @@ int launched()
 }
 
 template <typename E>
-int launch_quantize(const void *x, void *q, float *scales, int rows, int inputs, long long x_stride, long long q_stride,
-                    long long row_step, long long block_step, hipStream_t s)
+int launch_quantize(const void *x, void *q, float *scales, int rows, int inputs, long long x_stride, hipStream_t s)
 {
     const int blocks = ceil_div(inputs, kBlock);
-    const int64_t units = (int64_t)rows * blocks;
-    hipLaunchKernelGGL(quantize_kernel<E>, dim3((unsigned)((units + 15) / 16)), dim3(256), 0, s, static_cast<const E *>(x),
-                       static_cast<unsigned char *>(q), scales, rows, inputs, blocks, x_stride, q_stride, row_step, block_step);
+    const int64_t wgs = ((int64_t)rows * blocks + 16 * kQuantizeUnits - 1) / (16 * kQuantizeUnits);
+    hipLaunchKernelGGL(quantize_kernel<E>, dim3((unsigned)wgs), dim3(256), 0, s, static_cast<const E *>(x),
+                       static_cast<unsigned char *>(q), scales, rows, inputs, blocks, x_stride);
     return launched();
 }
 
@@ -715,7 +727,7 @@ int quantize(bool bf16, const void *x, void *xq, float *scales, int rows, int in
         return MLA_STATUS_INVALID_VALUE;
     if (!aligned16(x) || !aligned16(xq) || x_stride % 8 != 0)
         return MLA_STATUS_MISALIGNED;
-    return (bf16 ? launch_quantize<__bf16> : launch_quantize<_Float16>)(x, xq, scales, rows, inputs, x_stride, inputs, 1, rows,
+    return (bf16 ? launch_quantize<__bf16> : launch_quantize<_Float16>)(x, xq, scales, rows, inputs, x_stride,
                                                                        static_cast<hipStream_t>(stream));
 }
 
@@ -750,8 +762,7 @@ int linear(bool bf16, const void *x, const float *xs, const void *w, const float
     auto *space = static_cast<unsigned char *>(workspace);
     if (!xs) {
         auto *scales = reinterpret_cast<float *>(space + rows_bytes(rows, inputs));
-        if (const int st = (bf16 ? launch_quantize<__bf16> : launch_quantize<_Float16>)(x, space, scales, rows, inputs, x_stride,
-                                                                                       inputs, 1, rows, s))
+        if (const int st = (bf16 ? launch_quantize<__bf16> : launch_quantize<_Float16>)(x, space, scales, rows, inputs, x_stride, s))
             return st;
         p.x = space, p.xs = scales, p.x_stride = inputs, p.xs_row = 1, p.xs_block = rows;
     }
