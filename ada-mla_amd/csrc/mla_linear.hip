@@ -177,11 +177,26 @@ struct Tile {
                       kProducts + 2 >= kLoads && kProducts >= 8, "tile split");
 };
 
+// Four outputs of a row, the first `n` of them if there are fewer: one store, which rows of odd lengths leave at any
+// multiple of two bytes.
+template <typename E>
+__device__ __forceinline__ void store4(E *to, floatx4 y, int n)
+{
+    typedef E E4 __attribute__((ext_vector_type(4), aligned(2)));
+    if (n >= 4) {
+        *(E4 *)to = E4{(E)y[0], (E)y[1], (E)y[2], (E)y[3]};
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 3; ++e)
+        if (e < n)
+            to[e] = (E)y[e];
+}
+
 template <typename E, int BN, int BM, int kWN, int kWM, int kS>
 __global__ __launch_bounds__((Tile<BN, BM, kWN, kWM, kS>::kThreads)) void linear_kernel(Linear p)
 {
     using T = Tile<BN, BM, kWN, kWM, kS>;
-    using E4 = typename Vec<E>::v4;
     __shared__ __attribute__((aligned(1024))) unsigned char s_w[T::kSlots][BN * kBlock], s_x[T::kSlots][BM * kBlock];
     __shared__ __attribute__((aligned(16))) float s_xs[T::kSlots][BM];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -356,7 +371,6 @@ __global__ __launch_bounds__((Tile<BN, BM, kWN, kWM, kS>::kThreads)) void linear
             multiply(b + 1, std::integral_constant<int, T::kTwo ? 1 : 0>{});
     }
     MLA_WAIT_VMCNT(0);  // the loads behind the last block, before the LDS is given back
-    // four outputs of a row are one aligned store where rows start at a multiple of four (partial sums always do)
     const bool split = p.parts != nullptr;
     const int stride = split ? (p.outputs + 3) / 4 * 4 : p.outputs;
     float *parts = p.parts + (size_t)blockIdx.y * p.rows * stride;
@@ -375,13 +389,8 @@ __global__ __launch_bounds__((Tile<BN, BM, kWN, kWM, kS>::kThreads)) void linear
                 continue;
             if (split)
                 *(floatx4 *)(parts + to) = floatx4{y[0], y[1], y[2], y[3]};
-            else if (stride % 4 == 0)
-                *(E4 *)(out + to) = E4{(E)y[0], (E)y[1], (E)y[2], (E)y[3]};
             else
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (n + e < p.outputs)
-                        out[to + e] = (E)y[e];
+                store4(out + to, floatx4{y[0], y[1], y[2], y[3]}, p.outputs - n);
         }
     }
 }
@@ -399,15 +408,7 @@ __global__ __launch_bounds__(256) void sum_kernel(const float *__restrict__ part
     floatx4 y = {0.f, 0.f, 0.f, 0.f};
     for (int s = 0; s < splits; ++s)
         y += *(const floatx4 *)(parts + (s * all + i) * 4);
-    E *to = out + (size_t)m * outputs + n;
-    if (outputs % 4 == 0) {
-        *(typename Vec<E>::v4 *)to = typename Vec<E>::v4{(E)y[0], (E)y[1], (E)y[2], (E)y[3]};
-    } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (n + e < outputs)
-                to[e] = (E)y[e];
-    }
+    store4(out + (size_t)m * outputs + n, y, outputs - n);
 }
 
 // Few rows: the weights' bytes are what the call costs. A workgroup has 16 NT outputs of up to 16 MT rows; its
@@ -573,11 +574,8 @@ __global__ __launch_bounds__(64 * kW) void linear_few_kernel(Linear p)
             y += *(const floatx4 *)(s_ring + w * T::kRing + t * 16);
         const int i = t / (MT * 64), j = t / 64 % MT, l = t & 63;
         const int m = m0 + 16 * j + (l & 15), n = n0 + 16 * i + 4 * (l >> 4);
-        if (m < p.rows)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (n + e < p.outputs)
-                    out[(size_t)m * p.outputs + n + e] = (E)y[e];
+        if (m < p.rows && n < p.outputs)
+            store4(out + (size_t)m * p.outputs + n, y, p.outputs - n);
     }
 }
 
