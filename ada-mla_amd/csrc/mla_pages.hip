@@ -66,11 +66,12 @@ struct Table {
     const int *ids;  // [rows][stride]
     const int *lens;
     int rows, stride, page_shift;
-    __device__ __forceinline__ int tokens(int row) const
+    __device__ __forceinline__ int within(int length) const
     {
         const long long most = (long long)stride << page_shift;
-        return (int)min((long long)max(lens[row], 0), most);
+        return (int)min((long long)max(length, 0), most);
     }
+    __device__ __forceinline__ int tokens(int row) const { return within(lens[row]); }
     __device__ __forceinline__ int pages(int tokens) const
     {
         return (int)(((unsigned)tokens + (1u << page_shift) - 1) >> page_shift);
@@ -78,79 +79,121 @@ struct Table {
 };
 
 // One bit a page that a row of the table holds: in bits[w], or (kFull) in bits[2 w], with one in bits[2 w + 1] for a page
-// in the first full[row] columns of a row. A wave takes pieces of 64 rows x 16 columns, each lane a column of 16 rows in a
-// row, kPieces of them at once, and the page that a row shares with the row above (a prompt's) is marked once. One
-// CU does all of it, so it is bound by its instructions (1024 rows of 77 pages: 20 us with a condition around each
-// load and an atomic for each bit, 8 with clamped addresses and one of 64 bits).
-// pages, full: of each row, in LDS, zeros from t.rows to the next multiple of 64; most: the largest row's pages.
-template <bool kFull>
-__device__ __forceinline__ void mark_pages(const Table &t, const int *pages, const int *full, int most, int num_pages,
-                                           unsigned *bits)
-{
-    typedef int i32x4 __attribute__((ext_vector_type(4)));
-    constexpr int kPieces = 4;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int chunks = (most + 15) / 16, pieces = (t.rows + 63) / 64 * chunks;
-    const int above = lane >> 4 << 4;  // the lane's first row in a piece
-    for (int first = wave; first < pieces; first += kPieces * kWaves) {
-        int id[kPieces][16];
+// in the first full columns of a row. A wave takes pieces of 32 rows x 32 columns, each lane four columns (one load) of 4
+// rows in a row, kPieces of them at once; a page that the four rows share (a prompt's) is marked once. No load
+// stands under a condition: the last pieces' rows and columns overlap the others' (a mark may be made twice). The
+// first pieces' loads (fetch) need no length, so that a caller has them on their way before it knows any.
+// One CU does all of it, bound by its instructions: 1024 rows of 77 columns, of which four share 62 pages, take 8 us (10
+// with each entry compared to the one above it, 14 with one column a load, 20 with a condition around each load).
+// held: of each row its pages, or (kFull) its pages and its full columns; in LDS, zeros from t.rows to the next
+// multiple of 64. most: the largest row's pages. kNarrow: fewer than four columns, loaded one by one.
+template <bool kFull, bool kNarrow>
+struct Marks {
+    typedef int Ids __attribute__((ext_vector_type(4), aligned(4)));
+    static constexpr int kPieces = 4, kStep = kFull ? 2 : 1;
+    const Table &t;
+    const int lane, wave, row_pieces, above;  // above: the lane's first row in a piece
+    Ids id[kPieces][4];
+
+    __device__ __forceinline__ explicit Marks(const Table &table)
+        : t(table), lane(threadIdx.x & 63), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)),
+          row_pieces((t.rows + 31) / 32), above(min(lane >> 3 << 2, max(t.rows - 4, 0)))
+    {
+    }
+    // a piece's first row and the lane's first column
+    __device__ __forceinline__ int row_of(int piece) const { return min(piece % row_pieces * 32, max(t.rows - 32, 0)); }
+    __device__ __forceinline__ int col_of(int piece) const
+    {
+        return min((piece / row_pieces * 8 + (lane & 7)) * 4, max(t.stride - 4, 0));
+    }
+    // pieces first, first + kWaves, ..
+    __device__ __forceinline__ void fetch(int first)
+    {
+        const int last = row_pieces * ((t.stride + 31) / 32) - 1;
 #pragma unroll
         for (int k = 0; k < kPieces; ++k) {
-            const int piece = min(first + k * kWaves, pieces - 1), row0 = piece / chunks * 64;
-            const int *base = t.ids + (size_t)row0 * t.stride;
-            const int col = min(piece % chunks * 16 + (lane & 15), t.stride - 1), last = t.rows - 1 - row0;
+            const int piece = min(first + k * kWaves, last);
+            const int *base = t.ids + (size_t)row_of(piece) * t.stride;
+            const int offset = above * t.stride + col_of(piece);
+            if constexpr (!kNarrow) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                id[k][i] = base[min(above + i, last) * t.stride + col];
-        }
+                for (int i = 0; i < 4; ++i)
+                    id[k][i] = *(const Ids *)(base + (size_t)min(i, t.rows - 1) * t.stride + offset);
+            } else {
 #pragma unroll
-        for (int k = 0; k < kPieces; ++k) {
-            const int piece = first + k * kWaves;
-            if (piece >= pieces)
-                break;
-            const int row0 = piece / chunks * 64 + above, col = piece % chunks * 16 + (lane & 15);
-            int before = -1;
-            bool before_whole = false;
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const i32x4 held = *(const i32x4 *)(pages + row0 + 4 * q);
-                i32x4 most_full = {0, 0, 0, 0};
-                if constexpr (kFull)
-                    most_full = *(const i32x4 *)(full + row0 + 4 * q);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int page = col < held[e] && (unsigned)id[k][4 * q + e] < (unsigned)num_pages ? id[k][4 * q + e] : -1;
-                    const bool whole = kFull && col < most_full[e];
-                    if (page >= 0 && (page != before || (whole && !before_whole))) {
-                        if constexpr (kFull) {
-                            const unsigned long long bit = 1ull << (page & 31);
-                            atomicOr(reinterpret_cast<unsigned long long *>(bits) + (page >> 5), whole ? bit | bit << 32 : bit);
-                        } else {
-                            atomicOr(bits + (page >> 5), 1u << (page & 31));
-                        }
-                    }
-                    before = page;
-                    before_whole = whole;
+                for (int i = 0; i < 4; ++i) {
+                    const int *row = base + (size_t)min(i, t.rows - 1) * t.stride + offset;
+                    id[k][i] = Ids{row[0], row[min(1, t.stride - 1)], row[min(2, t.stride - 1)], -1};
                 }
             }
         }
     }
-}
+    // all pieces, the first kPieces of the wave fetched already
+    __device__ __forceinline__ void mark(const int *held, int most, int num_pages, unsigned *bits)
+    {
+        const int pieces = row_pieces * ((most + 31) / 32);
+        for (int first = wave; first < pieces; first += kPieces * kWaves) {
+            if (first != wave)
+                fetch(first);
+#pragma unroll
+            for (int k = 0; k < kPieces; ++k) {
+                const int piece = first + k * kWaves;
+                if (piece >= pieces)
+                    break;
+                const int first_col = col_of(piece);
+                const int *rows = held + kStep * (row_of(piece) + above);
+                int reached[4], whole[4], reached_most = 0, whole_most = 0;  // columns of the lane's rows
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    reached[i] = rows[kStep * i];
+                    whole[i] = kFull ? rows[kStep * i + kStep - 1] : 0;
+                    reached_most = max(reached_most, reached[i]);
+                    whole_most = max(whole_most, whole[i]);
+                }
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const int col = first_col + c;
+                    auto bit = [&](int page, int reach, int full) {
+                        if (col < reach && (unsigned)page < (unsigned)num_pages) {
+                            const unsigned one = 1u << (page & 31);
+                            if constexpr (kFull)
+                                atomicOr(reinterpret_cast<unsigned long long *>(bits) + (page >> 5),
+                                         one | (unsigned long long)(col < full ? one : 0u) << 32);
+                            else
+                                atomicOr(bits + (page >> 5), one);
+                        }
+                    };
+                    const bool same = id[k][0][c] == id[k][1][c] && id[k][1][c] == id[k][2][c] && id[k][2][c] == id[k][3][c];
+                    bit(id[k][0][c], same ? reached_most : reached[0], same ? whole_most : whole[0]);
+                    if (!same) {
+#pragma unroll
+                        for (int i = 1; i < 4; ++i)
+                            bit(id[k][i][c], reached[i], whole[i]);
+                    }
+                }
+            }
+        }
+    }
+};
 
 // One bit a page that `pinned` counts as held elsewhere (none if it is null), in bits[step w]; others[step w] <- 0.
+// (Without pins the loads read `any` instead: under a condition each would be waited for by itself, which made 17 us
+// of 45 000 pages, now 7 with the list and the first ids.)
 template <int step>
-__device__ __forceinline__ void clear_bits(const int *pinned, int num_pages, unsigned *bits, unsigned *others)
+__device__ __forceinline__ void clear_bits(const int *pinned, const int *any, int num_pages, unsigned *bits, unsigned *others)
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int last = num_pages - 1, last_read = pinned ? last : 0;
+    const int *from = pinned ? pinned : any;
+    const int least = pinned ? 0 : INT_MAX;
     for (int base = 1024 * wave; base < num_pages; base += 1024 * kWaves) {
         int v[16];
-        const int last = num_pages - 1;
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-            v[i] = pinned ? pinned[min(base + 64 * i + lane, last)] : 0;
+            v[i] = from[min(base + 64 * i + lane, last_read)];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            const unsigned long long m = __builtin_amdgcn_ballot_w64(v[i] > 0 && base + 64 * i + lane <= last);
+            const unsigned long long m = __builtin_amdgcn_ballot_w64(v[i] > least && base + 64 * i + lane <= last);
             if (lane < 2) {  // up to 31 words past the last page's: kWords is a multiple of 32
                 bits[step * (base / 32 + 2 * i + lane)] = (unsigned)(m >> (32 * lane));
                 others[step * (base / 32 + 2 * i + lane)] = 0;
@@ -159,13 +202,20 @@ __device__ __forceinline__ void clear_bits(const int *pinned, int num_pages, uns
     }
 }
 
-// pages[row] <- the row's pages, in LDS, zeros up to the next multiple of 64 rows; the most of a row into *most.
-__device__ __forceinline__ void row_pages(const Table &t, int *pages, int *most)
+// held[step row] <- the row's pages, in LDS, the step's others 0; zeros up to the next multiple of 64 rows; the most of
+// a row into *most. length: lens[row] of the thread's first row, or of any if it has none.
+template <int step>
+__device__ __forceinline__ void row_pages(const Table &t, int length, int *held, int *most)
 {
     int largest = 0;
     for (int row = threadIdx.x; row < (t.rows + 63) / 64 * 64; row += kThreads) {
-        pages[row] = row < t.rows ? t.pages(t.tokens(row)) : 0;
-        largest = max(largest, pages[row]);
+        if (row >= kThreads)
+            length = t.lens[min(row, t.rows - 1)];
+        const int pages = row < t.rows ? t.pages(t.within(length)) : 0;
+        held[step * row] = pages;
+        if constexpr (step == 2)
+            held[step * row + 1] = 0;
+        largest = max(largest, pages);
     }
     block_most(largest, most);
 }
@@ -207,10 +257,11 @@ __device__ __forceinline__ NewRow new_row(const Fork &f, int b)
 // the others write the whole columns of the new rows meanwhile, which need none. One launch: its
 // chain of round trips (parents, lengths, ids, marks, first row of each last page, ranks, ids taken) is
 // what a call costs.
+template <bool kNarrow>
 __global__ __launch_bounds__(kThreads) void fork_kernel(Fork f)
 {
     __shared__ __attribute__((aligned(16))) unsigned s_bits[2 * kWords];  // of 32 pages: held before; pinned, or held whole by a new row
-    __shared__ __attribute__((aligned(16))) int s_pages[kMostRows], s_full[kMostRows];
+    __shared__ __attribute__((aligned(16))) int s_rows[2 * kMostRows];  // of a row: its pages, the most of them that a new row holds whole
     __shared__ int s_scan[kWaves], s_most;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const Table &t = f.old;
@@ -241,27 +292,32 @@ __global__ __launch_bounds__(kThreads) void fork_kernel(Fork f)
     const int free_start = *f.free_start;
     auto held = [&](int w) -> unsigned & { return s_bits[2 * w]; };
     auto kept = [&](int w) -> unsigned & { return s_bits[2 * w + 1]; };
+    Marks<true, kNarrow> marks(t);
+    // what needs nothing read before it is on its way at once: lengths, ids, pins
+    const int length = t.lens[min(tid, t.rows - 1)];
+    marks.fetch(marks.wave);
     if (tid == 0)
         s_most = 0;
+    clear_bits<2>(f.pinned, t.lens, f.num_pages, s_bits + 1, s_bits);
+    const long long ahead = (long long)free_start + tid;
+    const int near = f.num_free > 0 ? f.free_pages[min(max(ahead, 0ll), (long long)f.num_free - 1)] : 0;
     __syncthreads();
-    row_pages(t, s_pages, &s_most);
-    for (int row = tid; row < (t.rows + 63) / 64 * 64; row += kThreads)
-        s_full[row] = 0;
-    clear_bits<2>(f.pinned, f.num_pages, s_bits + 1, s_bits);
-    __syncthreads();
+    row_pages<2>(t, length, s_rows, &s_most);
     NewRow mine = {};  // the thread's first row; the others are read again
+    if (tid < f.batch)
+        mine = new_row(f, tid);
+    __syncthreads();
     for (int b = tid; b < f.batch; b += kThreads) {
-        const NewRow r = new_row(f, b);
-        if (b == tid)
-            mine = r;
+        const NewRow r = b == tid ? mine : new_row(f, b);
         f.lens[b] = r.tokens;
         if (r.full)
-            atomicMax(&s_full[r.parent], r.full);
+            atomicMax(&s_rows[2 * r.parent + 1], r.full);
         if (r.rest && (unsigned)r.last < (unsigned)f.num_pages)
             __hip_atomic_store(f.first + r.last, INT_MAX, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     __syncthreads();
-    mark_pages<true>(t, s_pages, s_full, s_most, f.num_pages, s_bits);
+    asm volatile("" : : "v"(near));  // the free list where it will be read, brought to the cache
+    marks.mark(s_rows, s_most, f.num_pages, s_bits);
     __syncthreads();
     auto open = [&](const NewRow &r) {
         return r.rest && (unsigned)r.last < (unsigned)f.num_pages && !((kept(r.last >> 5) >> (r.last & 31)) & 1);
@@ -343,6 +399,7 @@ struct Compact {
 // move from two sums over the bits, and k is the number of t above it (of f below it). With m moves, the list
 // afterwards is the free pages but the m lowest, and the m highest movable ones, each page's place again a sum.
 // One workgroup, as in fork_kernel, a lane a page; remap_kernel then writes what needs no order.
+template <bool kNarrow>
 __global__ __launch_bounds__(kThreads) void compact_kernel(Compact c)
 {
     __shared__ __attribute__((aligned(8))) unsigned s_held[kWords], s_pinned[kWords], s_free[kWords];
@@ -358,32 +415,36 @@ __global__ __launch_bounds__(kThreads) void compact_kernel(Compact c)
     }
     // the list's first ids are on their way with the rows' lengths and the pins
     constexpr int kIds = 16;
+    const int *list = c.num_free > 0 ? c.free_pages : t.lens;  // (one entry is read of an empty list too)
     int id[kIds];
     auto fetch = [&](int i0) {
 #pragma unroll
         for (int k = 0; k < kIds; ++k) {
-            const long long i = (long long)i0 + k * kThreads + tid;
-            id[k] = i < c.num_free ? c.free_pages[i] : -1;
+            const long long i = min((long long)i0 + k * kThreads + tid, (long long)c.num_free - 1);
+            id[k] = list[max(i, 0ll)];
         }
     };
     fetch(start);
+    const int length = t.lens[min(tid, t.rows - 1)];
+    Marks<false, kNarrow> marks(t);
+    marks.fetch(marks.wave);
     const int groups = (c.num_pages + 63) / 64;
     for (int w = tid; w < 2 * groups; w += kThreads)
         s_free[w] = 0;
-    clear_bits<1>(c.pinned, c.num_pages, s_pinned, s_held);
+    clear_bits<1>(c.pinned, t.lens, c.num_pages, s_pinned, s_held);
     __syncthreads();
-    row_pages(t, s_rows, &s_most);
+    row_pages<1>(t, length, s_rows, &s_most);
     for (int i0 = start;;) {
 #pragma unroll
         for (int k = 0; k < kIds; ++k)
-            if ((unsigned)id[k] < (unsigned)c.num_pages)
+            if ((long long)i0 + k * kThreads + tid < c.num_free && (unsigned)id[k] < (unsigned)c.num_pages)
                 atomicOr(s_free + (id[k] >> 5), 1u << (id[k] & 31));
         if (i0 >= c.num_free - kIds * kThreads)
             break;
         fetch(i0 += kIds * kThreads);
     }
     __syncthreads();
-    mark_pages<false>(t, s_rows, nullptr, s_most, c.num_pages, s_held);
+    marks.mark(s_rows, s_most, c.num_pages, s_held);
     __syncthreads();
     const int per = (groups + kThreads - 1) / kThreads, g0 = min(tid * per, groups), g1 = min(g0 + per, groups);
     int movable = 0, listed = 0;
@@ -406,11 +467,24 @@ __global__ __launch_bounds__(kThreads) void compact_kernel(Compact c)
     // visit(page, is movable, is free, movable ones below it, free ones below it), a lane a page
     auto each = [&](auto &&visit) {
         const unsigned long long below = (1ull << lane) - 1;
-        for (int g = wave; g < groups; g += kWaves) {
-            const unsigned long long held = *(const unsigned long long *)(s_held + 2 * g);
-            const unsigned long long free = *(const unsigned long long *)(s_free + 2 * g);
-            visit(64 * g + lane, (held >> lane) & 1, (free >> lane) & 1, s_rows[2 * g] + __builtin_popcountll(held & below),
-                  s_rows[2 * g + 1] + __builtin_popcountll(free & below));
+        constexpr int kAtOnce = 4;  // groups read before they are visited
+        for (int first = wave; first < groups; first += kAtOnce * kWaves) {
+            unsigned long long held[kAtOnce], free[kAtOnce];
+            int2 before[kAtOnce];
+#pragma unroll
+            for (int k = 0; k < kAtOnce; ++k) {
+                const int g = min(first + k * kWaves, groups - 1);
+                held[k] = *(const unsigned long long *)(s_held + 2 * g);
+                free[k] = *(const unsigned long long *)(s_free + 2 * g);
+                before[k] = *(const int2 *)(s_rows + 2 * g);
+            }
+#pragma unroll
+            for (int k = 0; k < kAtOnce; ++k) {
+                const int g = first + k * kWaves;
+                if (g < groups)
+                    visit(64 * g + lane, (held[k] >> lane) & 1, (free[k] >> lane) & 1,
+                          before[k].x + __builtin_popcountll(held[k] & below), before[k].y + __builtin_popcountll(free[k] & below));
+            }
         }
     };
     int moves = 0, lowest = INT_MAX;
@@ -567,7 +641,8 @@ int mla_fork_tables(const int *block_table, const int *lens, const int *parents,
                       static_cast<int *>(workspace), batch, num_pages, num_free};
     const int64_t items = (int64_t)batch * ((block_table_stride + 255) / 256);
     const int writers = (int)std::min<int64_t>((items + mla::kWaves - 1) / mla::kWaves, mla::current_cu_count() - 1);
-    hipLaunchKernelGGL(mla::fork_kernel, dim3(1 + writers), dim3(mla::kThreads), 0, static_cast<hipStream_t>(stream), f);
+    const auto kernel = block_table_stride < 4 ? mla::fork_kernel<true> : mla::fork_kernel<false>;
+    hipLaunchKernelGGL(kernel, dim3(1 + writers), dim3(mla::kThreads), 0, static_cast<hipStream_t>(stream), f);
     return mla::launched();
 }
 
@@ -589,7 +664,8 @@ int mla_compact_tables(const int *block_table, const int *lens, const int *pinne
                          pinned, free_pages, free_start, new_table, copies, new_free_pages,
                          static_cast<int *>(workspace), num_pages, num_free, moves};
     hipStream_t s = static_cast<hipStream_t>(stream);
-    hipLaunchKernelGGL(mla::compact_kernel, dim3(1), dim3(mla::kThreads), 0, s, c);
+    const auto kernel = block_table_stride < 4 ? mla::compact_kernel<true> : mla::compact_kernel<false>;
+    hipLaunchKernelGGL(kernel, dim3(1), dim3(mla::kThreads), 0, s, c);
     if (const int st = mla::launched())
         return st;
     const int64_t waves = std::max((int64_t)rows * ((block_table_stride + 255) / 256), ((int64_t)3 * moves + num_free) / 256);
