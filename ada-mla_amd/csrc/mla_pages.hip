@@ -83,7 +83,7 @@ struct Table {
 // rows in a row, kPieces of them at once; a page that the four rows share (a prompt's) is marked once. No load
 // stands under a condition: the last pieces' rows and columns overlap the others' (a mark may be made twice). The
 // first pieces' loads (fetch) need no length, so that a caller has them on their way before it knows any.
-// One CU does all of it, bound by its instructions: 1024 rows of 77 columns, of which four share 62 pages, take 8 us (10
+// One CU does all of it, bound by its instructions: 1024 rows of 75 columns, of which four share 62 pages, take 8 us (10
 // with each entry compared to the one above it, 14 with one column a load, 20 with a condition around each load).
 // held: of each row its pages, or (kFull) its pages and its full columns; in LDS, zeros from t.rows to the next
 // multiple of 64. most: the largest row's pages. kNarrow: fewer than four columns, loaded one by one.
@@ -178,7 +178,7 @@ struct Marks {
 
 // One bit a page that `pinned` counts as held elsewhere (none if it is null), in bits[step w]; others[step w] <- 0.
 // (Without pins the loads read `any` instead: under a condition each would be waited for by itself, which made 17 us
-// of 45 000 pages, now 7 with the list and the first ids.)
+// of 21 700 pages, now 7 with the list and the first ids.)
 template <int step>
 __device__ __forceinline__ void clear_bits(const int *pinned, const int *any, int num_pages, unsigned *bits, unsigned *others)
 {
@@ -255,8 +255,8 @@ __device__ __forceinline__ NewRow new_row(const Fork &f, int b)
 //
 // Workgroup 0 does what needs an order (who holds what, the ranks in the free list), with a bit a page in LDS;
 // the others write the whole columns of the new rows meanwhile, which need none. One launch: its
-// chain of round trips (parents, lengths, ids, marks, first row of each last page, ranks, ids taken) is
-// what a call costs.
+// chain of round trips (lengths, ids and pins; parents; marks; first row of each last page; ranks; ids taken) is
+// what a call costs: 8.2 us of 64 rows of 11 pages, 20.2 of 1024 of 75, whose marks are 8.
 template <bool kNarrow>
 __global__ __launch_bounds__(kThreads) void fork_kernel(Fork f)
 {
@@ -398,7 +398,8 @@ struct Compact {
 // it than f below it, and t moves where more f stand below it than t above it: each page finds its own
 // move from two sums over the bits, and k is the number of t above it (of f below it). With m moves, the list
 // afterwards is the free pages but the m lowest, and the m highest movable ones, each page's place again a sum.
-// One workgroup, as in fork_kernel, a lane a page; remap_kernel then writes what needs no order.
+// One workgroup, as in fork_kernel, a lane a page; remap_kernel then writes what needs no order. 21 700 pages
+// take 23 us, 9 of them for the two passes over the pages, whose scattered stores one CU makes; 700 pages 9.2.
 template <bool kNarrow>
 __global__ __launch_bounds__(kThreads) void compact_kernel(Compact c)
 {
@@ -466,24 +467,32 @@ __global__ __launch_bounds__(kThreads) void compact_kernel(Compact c)
     __syncthreads();
     // visit(page, is movable, is free, movable ones below it, free ones below it), a lane a page
     auto each = [&](auto &&visit) {
-        const unsigned long long below = (1ull << lane) - 1;
         constexpr int kAtOnce = 4;  // groups read before they are visited
         for (int first = wave; first < groups; first += kAtOnce * kWaves) {
-            unsigned long long held[kAtOnce], free[kAtOnce];
+            uint2 held[kAtOnce], free[kAtOnce];
             int2 before[kAtOnce];
 #pragma unroll
             for (int k = 0; k < kAtOnce; ++k) {
                 const int g = min(first + k * kWaves, groups - 1);
-                held[k] = *(const unsigned long long *)(s_held + 2 * g);
-                free[k] = *(const unsigned long long *)(s_free + 2 * g);
+                held[k] = *(const uint2 *)(s_held + 2 * g);
+                free[k] = *(const uint2 *)(s_free + 2 * g);
                 before[k] = *(const int2 *)(s_rows + 2 * g);
             }
 #pragma unroll
             for (int k = 0; k < kAtOnce; ++k) {
                 const int g = first + k * kWaves;
-                if (g < groups)
-                    visit(64 * g + lane, (held[k] >> lane) & 1, (free[k] >> lane) & 1,
-                          before[k].x + __builtin_popcountll(held[k] & below), before[k].y + __builtin_popcountll(free[k] & below));
+                if (g >= groups)
+                    break;
+                auto word = [](uint2 v) {
+                    return (unsigned long long)(unsigned)__builtin_amdgcn_readfirstlane((int)v.y) << 32 |
+                           (unsigned)__builtin_amdgcn_readfirstlane((int)v.x);
+                };
+                const unsigned long long h = word(held[k]), f = word(free[k]);
+                auto below = [](unsigned long long m, int n) {
+                    return (int)__builtin_amdgcn_mbcnt_hi((unsigned)(m >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)m, (unsigned)n));
+                };
+                visit(64 * g + lane, __builtin_amdgcn_inverse_ballot_w64(h), __builtin_amdgcn_inverse_ballot_w64(f),
+                      below(h, before[k].x), below(f, before[k].y));
             }
         }
     };
@@ -491,13 +500,13 @@ __global__ __launch_bounds__(kThreads) void compact_kernel(Compact c)
     each([&](int page, bool is_t, bool is_f, int tb, int fb) {
         const int above = all_movable - 1 - tb;
         if (is_t && fb > above) {
-            c.copies[3 * (size_t)above] = page;
-            c.copies[3 * (size_t)above + 2] = 1 << t.page_shift;
+            c.copies[3u * above] = page;
+            c.copies[3u * above + 2] = 1 << t.page_shift;
             c.move[page] = above;
             lowest = min(lowest, page);
             ++moves;
         } else if (is_f && all_movable - tb > fb) {
-            c.copies[3 * (size_t)fb + 1] = page;
+            c.copies[3u * fb + 1] = page;
         }
     });
 #pragma unroll
@@ -511,10 +520,11 @@ __global__ __launch_bounds__(kThreads) void compact_kernel(Compact c)
     }
     __syncthreads();
     const int all_moves = s_moves;
+    int *const list_out = c.free_out + start - all_moves;
     each([&](int page, bool is_t, bool is_f, int tb, int fb) {
         const int moved_below = max(0, tb - (all_movable - all_moves));
         if (is_t ? tb >= all_movable - all_moves : is_f && fb >= all_moves)
-            c.free_out[(long long)start + fb - all_moves + moved_below] = page;
+            list_out[fb + moved_below] = page;
     });
     if (tid == 0) {
         c.move[c.num_pages] = all_moves;
@@ -564,7 +574,8 @@ __global__ __launch_bounds__(256) void remap_kernel(Compact c)
 
 // ---- copies -----------------------------------------------------------------
 
-// A workgroup takes one chunk of a page at a time, four 16-byte loads a thread in flight before their stores.
+// A workgroup takes one chunk of a page at a time, four 16-byte loads a thread in flight before their stores (as
+// vectors by themselves: an array of them went to LDS). Bound by HBM: 349 MB in 68 us, 5.1 TB/s.
 __global__ __launch_bounds__(256) void copy_pages_kernel(unsigned char *__restrict__ cache, const int *__restrict__ copies,
                                                          unsigned count, unsigned per_entry, unsigned chunks, int num_pages,
                                                          int page_size, int row_bytes, int chunk)
