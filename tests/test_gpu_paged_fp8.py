@@ -101,6 +101,16 @@ def test_lengths_and_heads(dtype, heads, page, lengths):
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("heads", [16, 64])
+def test_batches_without_a_token(dtype, heads):
+    cache, table, cu, held, gen = _case(1, [0, 0, 0], 32, 1.0)
+    q = torch.randn(3, heads, 576, generator=gen).to(dtype).cuda()
+    for total in (0, 5):  # what the batch has, and an upper bound
+        out = ada_mla.mla_decode_paged(q, cache, table, cu, total_tokens=total)
+        assert (out == 0).all(), total
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("splits", [1, 3, 7, 64, 100000])
 def test_forced_splits(dtype, splits):
     lengths = [300, 0, 1000, 5]
