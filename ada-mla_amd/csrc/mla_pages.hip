@@ -25,6 +25,7 @@ constexpr int kMostPages = 1 << 18;  // 32 KB of bits
 constexpr int kMostRows = 8192;
 constexpr int kMostColumns = 1 << 20;  // 64 rows' offsets stay within 32 bits
 constexpr int kWords = kMostPages / 32;
+constexpr int kRemapHere = 12288;
 
 // Exclusive sums of v over the workgroup's threads; total: over all of them. s: a word of LDS a wave.
 __device__ __forceinline__ int block_before(int v, int *s, int &total)
@@ -391,14 +392,54 @@ struct Compact {
     int *table, *copies, *free_out;
     int *move;  // [num_pages + 3]: of a page that moves, which move; then the moves, the ids in the list, the lowest page that moves
     int num_pages, num_free, most_moves;
+    int remaps;  // the one workgroup that finds the moves writes the table too
 };
+
+// The table with every page where it went, -1 behind a row's last page; the moves that are none; the list's other entries.
+// By `waves` waves, of which this is number `wave`, with so many threads.
+__device__ __forceinline__ void remap(const Compact &c, int moves, int all_free, int lowest, long long wave, long long waves,
+                                      long long thread, long long threads)
+{
+    const Table &t = c.old;
+    const int lane = threadIdx.x & 63;
+    const int chunks = (t.stride + 255) / 256;
+    const long long items = (long long)t.rows * chunks;
+    for (long long i = wave; i < items; i += waves) {
+        const int row = (int)(i / chunks), col0 = (int)(i % chunks) * 256;
+        const int pages = t.pages(t.tokens(row));
+        const size_t base = (size_t)row * t.stride;
+        int id[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int col = col0 + 64 * k + lane;
+            id[k] = col < pages ? t.ids[base + col] : -1;
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)  // every held page from the lowest that moves on does, unless it is pinned
+            if (id[k] >= lowest && id[k] < c.num_pages && !(c.pinned && c.pinned[id[k]] > 0))
+                id[k] = c.copies[3 * (size_t)c.move[id[k]] + 1];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int col = col0 + 64 * k + lane;
+            if (col < t.stride)
+                c.table[base + col] = id[k];
+        }
+    }
+    const int start = min(max(*c.free_start, 0), c.num_free), end = start + all_free;
+    for (long long i = 3ll * moves + thread; i < 3ll * c.most_moves; i += threads)
+        c.copies[i] = i % 3 == 2 ? 0 : -1;
+    for (long long i = thread; i < c.num_free; i += threads)
+        if (i < start || i >= end)
+            c.free_out[i] = -1;
+}
 
 // Of the movable pages t (held by a row, not pinned) and the free ones f (listed, neither held nor pinned), the k-th
 // highest t moves to the k-th lowest f as long as that is lower. So f is moved to where more t stand above
 // it than f below it, and t moves where more f stand below it than t above it: each page finds its own
 // move from two sums over the bits, and k is the number of t above it (of f below it). With m moves, the list
 // afterwards is the free pages but the m lowest, and the m highest movable ones, each page's place again a sum.
-// One workgroup, as in fork_kernel, a lane a page; remap_kernel then writes what needs no order. 21 700 pages
+// One workgroup, as in fork_kernel, a lane a page; remap_kernel then writes what needs no order, where that is enough
+// for a launch. 21 700 pages
 // take 23 us, 9 of them for the two passes over the pages, whose scattered stores one CU makes; 700 pages 9.2.
 template <bool kNarrow>
 __global__ __launch_bounds__(kThreads) void compact_kernel(Compact c)
@@ -526,50 +567,21 @@ __global__ __launch_bounds__(kThreads) void compact_kernel(Compact c)
         if (is_t ? tb >= all_movable - all_moves : is_f && fb >= all_moves)
             list_out[fb + moved_below] = page;
     });
-    if (tid == 0) {
+    if (c.remaps) {
+        __syncthreads();
+        remap(c, all_moves, all_free, s_lowest, wave, kWaves, tid, kThreads);
+    } else if (tid == 0) {
         c.move[c.num_pages] = all_moves;
         c.move[c.num_pages + 1] = all_free;
         c.move[c.num_pages + 2] = s_lowest;
     }
 }
 
-// The table with every page where it went, -1 behind a row's last page; the moves that are none; the list's other entries.
 __global__ __launch_bounds__(256) void remap_kernel(Compact c)
 {
-    const Table &t = c.old;
-    const int lane = threadIdx.x & 63;
-    const long long wave = blockIdx.x * 4ll + (threadIdx.x >> 6), waves = gridDim.x * 4ll;
-    const int chunks = (t.stride + 255) / 256;
-    const long long items = (long long)t.rows * chunks;
-    const int moves = c.move[c.num_pages], lowest = c.move[c.num_pages + 2];
-    for (long long i = wave; i < items; i += waves) {
-        const int row = (int)(i / chunks), col0 = (int)(i % chunks) * 256;
-        const int pages = t.pages(t.tokens(row));
-        const size_t base = (size_t)row * t.stride;
-        int id[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int col = col0 + 64 * k + lane;
-            id[k] = col < pages ? t.ids[base + col] : -1;
-        }
-#pragma unroll
-        for (int k = 0; k < 4; ++k)  // every held page from the lowest that moves on does, unless it is pinned
-            if (id[k] >= lowest && id[k] < c.num_pages && !(c.pinned && c.pinned[id[k]] > 0))
-                id[k] = c.copies[3 * (size_t)c.move[id[k]] + 1];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int col = col0 + 64 * k + lane;
-            if (col < t.stride)
-                c.table[base + col] = id[k];
-        }
-    }
-    const int start = min(max(*c.free_start, 0), c.num_free), end = start + c.move[c.num_pages + 1];
-    const long long thread = blockIdx.x * 256ll + threadIdx.x, threads = gridDim.x * 256ll;
-    for (long long i = 3ll * moves + thread; i < 3ll * c.most_moves; i += threads)
-        c.copies[i] = i % 3 == 2 ? 0 : -1;
-    for (long long i = thread; i < c.num_free; i += threads)
-        if (i < start || i >= end)
-            c.free_out[i] = -1;
+    const int *found = c.move + c.num_pages;
+    remap(c, found[0], found[1], found[2], blockIdx.x * 4ll + (threadIdx.x >> 6), gridDim.x * 4ll,
+          blockIdx.x * 256ll + threadIdx.x, gridDim.x * 256ll);
 }
 
 // ---- copies -----------------------------------------------------------------
@@ -671,13 +683,18 @@ int mla_compact_tables(const int *block_table, const int *lens, const int *pinne
         return MLA_STATUS_MISALIGNED;
     if (workspace_bytes < mla_page_tables_workspace_size(num_pages))
         return MLA_STATUS_WORKSPACE_TOO_SMALL;
+    // Entries of the table, the moves and the list: up to kRemapHere the first workgroup writes them itself (us a call,
+    // in one launch and in two: 1760 entries 10.3, 12.1; 8320 12.6, 13.4; 12 800 14.0, 14.4; 19 200 16.6, 15.5;
+    // 38 400 24.0, 20.6).
+    const int64_t entries = (int64_t)rows * block_table_stride + (int64_t)3 * moves + num_free;
+    const int here = entries <= mla::kRemapHere;
     const mla::Compact c{{block_table, lens, rows, block_table_stride, __builtin_ctz((unsigned)page_size)},
                          pinned, free_pages, free_start, new_table, copies, new_free_pages,
-                         static_cast<int *>(workspace), num_pages, num_free, moves};
+                         static_cast<int *>(workspace), num_pages, num_free, moves, here};
     hipStream_t s = static_cast<hipStream_t>(stream);
     const auto kernel = block_table_stride < 4 ? mla::compact_kernel<true> : mla::compact_kernel<false>;
     hipLaunchKernelGGL(kernel, dim3(1), dim3(mla::kThreads), 0, s, c);
-    if (const int st = mla::launched())
+    if (const int st = mla::launched(); st || here)
         return st;
     const int64_t waves = std::max((int64_t)rows * ((block_table_stride + 255) / 256), ((int64_t)3 * moves + num_free) / 256);
     const int wgs = (int)std::min<int64_t>((waves + 3) / 4 + 1, 4 * mla::current_cu_count());

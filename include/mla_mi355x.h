@@ -486,7 +486,7 @@ int mla_fork_tables(const int *block_table, const int *lens,
  * (-1, -1, 0) behind the last move. new_table gets block_table with every page
  * where it went (columns behind a row's last page: -1), new_free_pages the
  * free ids in ascending order from *free_start on, -1 elsewhere. Workspace,
- * limits and other conditions as for mla_fork_tables. Two launches. */
+ * limits and other conditions as for mla_fork_tables. One or two launches. */
 int mla_compact_tables(const int *block_table, const int *lens,
                        const int *pinned, const int *free_pages,
                        const int *free_start, int *new_table, int *copies,
