@@ -95,7 +95,7 @@ constexpr int kQuantizeUnits = 4;
 template <typename E>
 __global__ __launch_bounds__(256) void quantize_kernel(const E *__restrict__ x, unsigned char *__restrict__ q,
                                                        float *__restrict__ scales, int rows, int inputs, int blocks,
-                                                       long long x_stride)
+                                                       long long x_stride, int q_stride)
 {
     using E8 = typename Vec<E>::v8;
     const unsigned units = (unsigned)rows * blocks, first = blockIdx.x * (16u * kQuantizeUnits) + (threadIdx.x >> 4);
@@ -120,7 +120,7 @@ __global__ __launch_bounds__(256) void quantize_kernel(const E *__restrict__ x, 
         if (first + 16 * i >= units)
             return;
         if (k < inputs)
-            *(uint2 *)(q + (size_t)m[i] * inputs + k) = y;
+            *(uint2 *)(q + (size_t)m[i] * q_stride + k) = y;
         if (j == 0)
             scales[(size_t)b[i] * rows + m[i]] = scale;
     }
@@ -603,12 +603,12 @@ int launched()
 }
 
 template <typename E>
-int launch_quantize(const void *x, void *q, float *scales, int rows, int inputs, long long x_stride, hipStream_t s)
+int launch_quantize(const void *x, void *q, float *scales, int rows, int inputs, long long x_stride, int q_stride, hipStream_t s)
 {
     const int blocks = ceil_div(inputs, kBlock);
     const int64_t wgs = ((int64_t)rows * blocks + 16 * kQuantizeUnits - 1) / (16 * kQuantizeUnits);
     hipLaunchKernelGGL(quantize_kernel<E>, dim3((unsigned)wgs), dim3(256), 0, s, static_cast<const E *>(x),
-                       static_cast<unsigned char *>(q), scales, rows, inputs, blocks, x_stride);
+                       static_cast<unsigned char *>(q), scales, rows, inputs, blocks, x_stride, q_stride);
     return launched();
 }
 
@@ -730,13 +730,14 @@ int quantize(bool bf16, const void *x, void *xq, float *scales, int rows, int in
         return MLA_STATUS_INVALID_VALUE;
     if (!aligned16(x) || !aligned16(xq) || x_stride % 8 != 0)
         return MLA_STATUS_MISALIGNED;
-    return (bf16 ? launch_quantize<__bf16> : launch_quantize<_Float16>)(x, xq, scales, rows, inputs, x_stride,
+    return (bf16 ? launch_quantize<__bf16> : launch_quantize<_Float16>)(x, xq, scales, rows, inputs, x_stride, inputs,
                                                                        static_cast<hipStream_t>(stream));
 }
 
 // The workspace: the quantised rows, their scales, block by block ([blocks][rows]), the splits' sums.
 size_t up256(size_t bytes) { return (bytes + 255) / 256 * 256; }
-size_t rows_bytes(int rows, int inputs) { return up256((size_t)rows * inputs); }
+int pitch(int inputs) { return ceil_div(inputs, kBlock) * kBlock; }  // a row's blocks begin with cache lines
+size_t rows_bytes(int rows, int inputs) { return up256((size_t)rows * pitch(inputs)); }
 size_t scales_bytes(int rows, int inputs) { return up256(4 * (size_t)rows * ceil_div(inputs, kBlock)); }
 size_t parts_bytes(int rows, int outputs, const LinearPlan &plan)
 {
@@ -765,9 +766,10 @@ int linear(bool bf16, const void *x, const float *xs, const void *w, const float
     auto *space = static_cast<unsigned char *>(workspace);
     if (!xs) {
         auto *scales = reinterpret_cast<float *>(space + rows_bytes(rows, inputs));
-        if (const int st = (bf16 ? launch_quantize<__bf16> : launch_quantize<_Float16>)(x, space, scales, rows, inputs, x_stride, s))
+        if (const int st = (bf16 ? launch_quantize<__bf16> : launch_quantize<_Float16>)(x, space, scales, rows, inputs, x_stride,
+                                                                                          pitch(inputs), s))
             return st;
-        p.x = space, p.xs = scales, p.x_stride = inputs, p.xs_row = 1, p.xs_block = rows;
+        p.x = space, p.xs = scales, p.x_stride = pitch(inputs), p.xs_row = 1, p.xs_block = rows;
     }
     p.parts = reinterpret_cast<float *>(space + rows_bytes(rows, inputs) + scales_bytes(rows, inputs));
     const LinearPlan plan = plan_linear(rows, inputs, outputs);
