@@ -159,7 +159,7 @@ __device__ __forceinline__ void each_of(F &&body)
 // Bound by the matrix units, the 256 tiles: 8192 x 7168 x 8192 in 407 us, 2.36 PFLOP/s, 2980 cycles a block; the four sums
 // in fp32 behind each product cost the rest (a product and its sums take 35 to 37 cycles of two waves, 33 the
 // product alone), and the clock, 2.37 GHz with few workgroups, falls to 1.8 with every CU at it. The smaller tiles are for
-// calls that 256 x 256 leave without workgroups: 333 x 2000 x 4999 in 14.8 us; 64 x 16384 x 5120, its inputs split
+// calls that 256 x 256 leave without workgroups: 4096 x 7168 x 2048 in 62.5 us (256 x 128), 333 x 2000 x 4999 in 13.8; 64 x 16384 x 5120, its inputs split
 // in six, in 18.0 (4.7 TB/s of weights).
 // 16-byte chunk c of row r sits at c ^ (r / 2 mod 8): rows are 128
 // bytes, two of them an LDS bank period, so chunk g of 16 rows is in 16 different places, and so are those of
@@ -640,7 +640,7 @@ int launch_few(const Linear &p, hipStream_t s)
 
 // ---- which kernel -----------------------------------------------------------
 
-enum class Form { kFew, kTile64, kTile128, kTile256 };
+enum class Form { kFew, kTile64, kTile128, kTileWide, kTile256 };
 
 struct LinearPlan {
     Form form;
@@ -652,13 +652,15 @@ struct LinearPlan {
 bool few_narrow(int outputs) { return ceil_div(outputs, 16) <= current_cu_count(); }
 int few_row_tiles(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
 
-// The form with the smallest modelled time, and how many parts its inputs are split into. Measured on 17 sizes of 32 to
-// 8192 rows with every form and split forced (us, e.g. 256 x 16384 x 5120: 256 tiles 197, 128 tiles 85, in
-// three splits 40; 64 tiles 61, in three 50; the model picks within 6% of the best of all, on 13 the best):
-//   tiles     3.5 + rounds (blocks + 2.5) step; a step (one block) is 0.45, 0.66, 1.55 us with few
-//             workgroups and 0.48, 0.70, 1.80 with every CU busy (the clock falls);
+// The form with the smallest modelled time, and how many parts its inputs are split into. Measured on 35 sizes of 32 to
+// 8192 rows with forms and splits forced (us, e.g. 256 x 16384 x 5120: 256 tiles 197, 128 tiles 85, in
+// three splits 40; 64 tiles 61, in three 50; the model's choice is within 8% of the best of all):
+//   tiles     3.5 + rounds (blocks + 2.5) step; a step (one block) is 0.45, 0.66, 0.79, 1.55 us with few
+//             workgroups and 0.48, 0.70, 1.00, 1.80 with every CU busy (the clock falls). The 256 x 128 tiles are for
+//             the calls that make about a workgroup a CU of them (4096 x 7168 x 2048: 62.5, 256 tiles in two splits
+//             70.0, 128 tiles 78.6; 1024 x 2048 x 7168: 22.8, 33.3 whole, 29.7);
 //   splits    4 for the second launch, and 0.28 a MB of fp32 sums, written and read;
-//   few rows  4 + rounds (blocks / waves) times what a block costs a wave.
+//   few rows  3 + rounds (1 + blocks / waves times what a block costs a wave).
 LinearPlan plan_linear(int rows, int inputs, int outputs)
 {
     const int blocks = ceil_div(inputs, kBlock), cus = current_cu_count();
@@ -667,7 +669,7 @@ LinearPlan plan_linear(int rows, int inputs, int outputs)
     const double few_step = few == 1 ? (narrow ? 0.5 : 0.8) : few == 2 ? (narrow ? 0.4 : 0.55) : narrow ? 0.5 : 0.72;
     const double few_rounds = std::ceil((double)ceil_div(rows, 16 * few) * ceil_div(outputs, narrow ? 16 : 32) / cus);
     LinearPlan best{Form::kFew, 1};
-    double best_us = 4.0 + few_rounds * ceil_div(blocks, few == 1 ? 8 : 4) * few_step;
+    double best_us = 3.0 + few_rounds * (1.0 + ceil_div(blocks, few == 1 ? 8 : 4) * few_step);
     if (inputs < kBlock)  // (the tiles want a whole block)
         return best;
     struct Kind {
@@ -675,7 +677,8 @@ LinearPlan plan_linear(int rows, int inputs, int outputs)
         int bn, bm;
         double step, busy_step;
     };
-    for (const Kind &k : {Kind{Form::kTile256, 256, 256, 1.55, 1.80}, Kind{Form::kTile128, 128, 128, 0.66, 0.70},
+    for (const Kind &k : {Kind{Form::kTile256, 256, 256, 1.55, 1.80}, Kind{Form::kTileWide, 256, 128, 0.79, 1.00},
+                          Kind{Form::kTile128, 128, 128, 0.66, 0.70},
                           Kind{Form::kTile64, 128, 64, 0.45, 0.48}}) {
         const int64_t tiles = (int64_t)ceil_div(rows, k.bm) * ceil_div(outputs, k.bn);
         for (int splits = 1; splits <= std::min(blocks, 16); ++splits) {
@@ -700,6 +703,7 @@ int launch_linear(const Linear &p, const LinearPlan &plan, hipStream_t s)
 {
     switch (plan.form) {
     case Form::kTile256: return launch_tiles<E, 256, 256, 2, 4, 2>(p, plan.splits, s);
+    case Form::kTileWide: return launch_tiles<E, 256, 128, 4, 2, 3>(p, plan.splits, s);
     case Form::kTile128: return launch_tiles<E, 128, 128, 2, 2, 4>(p, plan.splits, s);
     case Form::kTile64: return launch_tiles<E, 128, 64, 2, 2, 4>(p, plan.splits, s);
     default: break;

@@ -123,7 +123,8 @@ def test_quantised_infinities_and_nans():
 
 
 SIZES = [(1, 16, 1), (1, 128, 128), (2, 144, 3), (7, 1040, 129), (16, 512, 576), (17, 256, 64), (33, 2000, 255), (64, 640, 300),
-         (65, 384, 127), (127, 128, 257), (128, 1152, 128), (129, 272, 640), (200, 1536, 513), (300, 2048, 1024), (513, 400, 385)]
+         (65, 384, 127), (127, 128, 257), (128, 1152, 128), (129, 272, 640), (200, 1536, 513), (300, 2048, 1024), (513, 400, 385),
+         (1000, 528, 4999), (66, 6976, 6698)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
