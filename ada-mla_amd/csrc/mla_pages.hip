@@ -258,7 +258,7 @@ __device__ __forceinline__ NewRow new_row(const Fork &f, int b)
 // Workgroup 0 does what needs an order (who holds what, the ranks in the free list), with a bit a page in LDS;
 // the others write the whole columns of the new rows meanwhile, which need none. One launch: its
 // chain of round trips (lengths, ids and pins; parents; marks; first row of each last page; ranks; ids taken) is
-// what a call costs: 8.2 us of 64 rows of 11 pages, 20.2 of 1024 of 75, whose marks are 8.
+// what a call costs: 8.5 us of 64 rows of 11 pages, 20.2 of 1024 of 75, whose marks are 8.
 template <bool kNarrow>
 __global__ __launch_bounds__(kThreads) void fork_kernel(Fork f)
 {
@@ -441,7 +441,7 @@ __device__ __forceinline__ void remap(const Compact &c, int moves, int all_free,
 // afterwards is the free pages but the m lowest, and the m highest movable ones, each page's place again a sum.
 // One workgroup, as in fork_kernel, a lane a page; remap_kernel then writes what needs no order, where that is enough
 // for a launch. 21 700 pages
-// take 23 us, 9 of them for the two passes over the pages, whose scattered stores one CU makes; 700 pages 9.2.
+// take 23 us, 9 of them for the two passes over the pages, whose scattered stores one CU makes; 700 pages and their table 11.
 template <bool kNarrow>
 __global__ __launch_bounds__(kThreads) void compact_kernel(Compact c)
 {
