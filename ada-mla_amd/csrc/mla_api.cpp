@@ -772,7 +772,7 @@ std::vector<at::Tensor> quantize_fp8(const at::Tensor &x_in)
     TORCH_CHECK(x_in.dim() >= 1, fn, ": x must be [..., inputs]");
     const int64_t inputs = x_in.size(-1), blocks = (inputs + 127) / 128, rows = inputs ? x_in.numel() / inputs : 0;
     check_inputs(inputs, fn);
-    TORCH_CHECK(rows <= (1 << 26), fn, ": too many rows");
+    TORCH_CHECK(rows <= (1 << 26) && rows * blocks <= (1 << 30) - 64, fn, ": too many rows");
     check_devices({&x_in}, fn);
     const at::OptionalDeviceGuard guard(x_in.device());
     const auto options = x_in.options().memory_format(at::MemoryFormat::Contiguous);
@@ -810,7 +810,7 @@ at::Tensor linear_fp8(const at::Tensor &x_in, const at::Tensor &w_in, const at::
     TORCH_CHECK(w_in.scalar_type() == at::kFloat8_e4m3fn && w_in.dim() == 2 && w_in.size(1) == inputs && w_in.size(0) >= 1, fn,
                 ": weight must be a float8_e4m3fn tensor [outputs, ", inputs, "], got ", w_in.sizes());
     const int64_t outputs = w_in.size(0);
-    TORCH_CHECK(rows <= (1 << 26) && outputs <= (1 << 26), fn, ": too many rows or outputs");
+    TORCH_CHECK(rows <= (1 << 26) && outputs <= (1 << 26) && rows * blocks <= (1 << 30) - 64, fn, ": too many rows or outputs");
     TORCH_CHECK(ws_in.scalar_type() == at::kFloat && ws_in.dim() == 2 && ws_in.size(0) == (outputs + 127) / 128 &&
                     ws_in.size(1) == blocks,
                 fn, ": weight_scale must be a float32 tensor [", (outputs + 127) / 128, ", ", blocks, "], got ", ws_in.sizes());

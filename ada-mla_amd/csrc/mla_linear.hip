@@ -589,11 +589,14 @@ constexpr long long kMostStride = 1 << 22;  // a tile's rows stay within 2^31 by
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 int ceil_div(int a, int b) { return (int)(((long long)a + b - 1) / b); }
 
+constexpr int64_t kMostThreads = UINT32_MAX;  // of a grid: a launch counts them in 32 bits
+
+// (2^30 blocks of x: their quantisation takes four threads each)
 bool sizes_ok(int rows, int inputs, int outputs)
 {
     return rows >= 1 && rows <= (1 << 26) && inputs >= 16 && inputs % 16 == 0 && inputs <= kMostStride && outputs >= 1 &&
            outputs <= (1 << 26) && (int64_t)ceil_div(rows, 16) * ceil_div(outputs, 16) <= INT32_MAX &&
-           (int64_t)rows * ceil_div(inputs, kBlock) <= INT32_MAX;
+           (int64_t)rows * ceil_div(inputs, kBlock) <= (1 << 30) - 64;
 }
 
 int launched()
@@ -630,12 +633,30 @@ int launch_tiles(Linear p, int splits, hipStream_t s)
     return launched();
 }
 
+// Rows that one launch of the few-row kernel takes: whole tiles, as many as its grid has threads for (one at least: all
+// outputs are 2^22 tiles, of 512 threads).
+int few_rows_a_launch(int outputs, int tile_outputs, int tile_rows, int threads)
+{
+    return (int)std::min<int64_t>(kMostThreads / threads / ceil_div(outputs, tile_outputs) * tile_rows, 1 << 26);
+}
+
 template <typename E, int NT, int MT, int kW, int kS, bool kQuantize = false>
 int launch_few(const Linear &p, hipStream_t s)
 {
-    const int64_t tiles = (int64_t)ceil_div(p.rows, 16 * MT) * ceil_div(p.outputs, 16 * NT);
-    hipLaunchKernelGGL((linear_few_kernel<E, NT, MT, kW, kS, kQuantize>), dim3((unsigned)tiles), dim3(64 * kW), 0, s, p);
-    return launched();
+    const int most = few_rows_a_launch(p.outputs, 16 * NT, 16 * MT, 64 * kW);
+    for (int first = 0; first < p.rows; first += most) {
+        Linear q = p;
+        q.rows = std::min(most, p.rows - first);
+        q.x += first * p.x_stride;
+        if (p.xs)
+            q.xs += first * p.xs_row;
+        q.out = static_cast<E *>(p.out) + (size_t)first * p.outputs;
+        const int64_t tiles = (int64_t)ceil_div(q.rows, 16 * MT) * ceil_div(p.outputs, 16 * NT);
+        hipLaunchKernelGGL((linear_few_kernel<E, NT, MT, kW, kS, kQuantize>), dim3((unsigned)tiles), dim3(64 * kW), 0, s, q);
+        if (const int st = launched())
+            return st;
+    }
+    return MLA_STATUS_SUCCESS;
 }
 
 // ---- which kernel -----------------------------------------------------------
@@ -674,14 +695,17 @@ LinearPlan plan_linear(int rows, int inputs, int outputs)
         return best;
     struct Kind {
         Form form;
-        int bn, bm;
+        int bn, bm, threads;
         double step, busy_step;
     };
-    for (const Kind &k : {Kind{Form::kTile256, 256, 256, 1.55, 1.80}, Kind{Form::kTileWide, 256, 128, 0.79, 1.00},
-                          Kind{Form::kTile128, 128, 128, 0.66, 0.70},
-                          Kind{Form::kTile64, 128, 64, 0.45, 0.48}}) {
+    const int most_splits = (int64_t)rows * ceil_div(outputs, 4) <= kMostThreads - 255 ? std::min(blocks, 16) : 1;  // (sum_kernel's grid)
+    for (const Kind &k : {Kind{Form::kTile256, 256, 256, 512, 1.55, 1.80}, Kind{Form::kTileWide, 256, 128, 512, 0.79, 1.00},
+                          Kind{Form::kTile128, 128, 128, 256, 0.66, 0.70},
+                          Kind{Form::kTile64, 128, 64, 256, 0.45, 0.48}}) {
         const int64_t tiles = (int64_t)ceil_div(rows, k.bm) * ceil_div(outputs, k.bn);
-        for (int splits = 1; splits <= std::min(blocks, 16); ++splits) {
+        if (tiles * k.threads > kMostThreads)
+            continue;
+        for (int splits = 1; splits <= most_splits; ++splits) {
             const int per = ceil_div(blocks, splits);
             if (ceil_div(blocks, per) != splits)
                 continue;

@@ -384,7 +384,9 @@ int mla_project_output_bf16(const void *o_star, const void *w_uv,
  *   leaves them, which is read fastest).
  * A NaN or infinity in a row of x makes its row of out NaN, a NaN in a row of w its
  * column. inputs must be a multiple of 16, strides of 8 values (16-bit rows) or 16 bytes, and
- * inputs and strides at most 2^22 (scale_row_stride: 2^20); rows and outputs at most 2^26. */
+ * inputs and strides at most 2^22 (scale_row_stride: 2^20); rows and outputs at most 2^26,
+ * their tiles of 16 x 16 less than 2^31, and the blocks of x, rows times
+ * ceil(inputs / 128), at most 2^30 - 64. */
 int mla_quantize_fp8_fp16(const void *x, void *xq, float *scales, int rows,
                           int inputs, long long x_stride, void *stream);
 int mla_quantize_fp8_bf16(const void *x, void *xq, float *scales, int rows,
