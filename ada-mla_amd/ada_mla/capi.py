@@ -70,6 +70,7 @@ _SIGNATURES = {
     "mla_quantize_fp8_fp16": (_i, [_vp] * 3 + [_i, _i, _ll, _vp]),
     "mla_quantize_fp8_bf16": (_i, [_vp] * 3 + [_i, _i, _ll, _vp]),
     "mla_linear_fp8_workspace_size": (_sz, [_i] * 3),
+    "mla_linear_fp8_plan": (_i, [_i] * 4 + [_vp] * 4),
     "mla_linear_fp8_fp16": (_i, [_vp] * 5 + [_sz] + [_i] * 3 + [_ll, _ll, _vp]),
     "mla_linear_fp8_bf16": (_i, [_vp] * 5 + [_sz] + [_i] * 3 + [_ll, _ll, _vp]),
     "mla_linear_fp8_quantized_fp16": (_i, [_vp] * 6 + [_sz] + [_i] * 3 + [_ll] * 4 + [_vp]),
@@ -425,6 +426,13 @@ def quantize_fp8(x):
     fn = "mla_quantize_fp8_" + _suffix(x)
     _check(fn, getattr(lib, fn)(_ptr(x), _ptr(q), _ptr(scales), m, k, x.stride(0), _stream(x)))
     return q, scales.t()
+
+
+def linear_fp8_plan(rows: int, inputs: int, outputs: int, quantized: bool = False):
+    """mla_linear_fp8_plan -> (outputs and rows of a workgroup's tile, splits of the inputs, launches)."""
+    out = [ctypes.c_int() for _ in range(4)]
+    _check("mla_linear_fp8_plan", load().mla_linear_fp8_plan(rows, inputs, outputs, int(quantized), *map(ctypes.byref, out)))
+    return tuple(v.value for v in out)
 
 
 def linear_fp8(x, w, w_scale, x_scale=None, dtype=None, out=None, workspace=None):

@@ -827,6 +827,24 @@ size_t mla_linear_fp8_workspace_size(int rows, int inputs, int outputs)
            mla::parts_bytes(rows, outputs, mla::plan_linear(rows, inputs, outputs));
 }
 
+int mla_linear_fp8_plan(int rows, int inputs, int outputs, int quantized, int *tile_outputs, int *tile_rows, int *splits,
+                        int *launches)
+{
+    using mla::Form;
+    if (!mla::sizes_ok(rows, inputs, outputs) || !tile_outputs || !tile_rows || !splits || !launches)
+        return MLA_STATUS_INVALID_VALUE;
+    const bool own = !quantized && mla::quantizes_itself(rows, inputs);
+    const mla::LinearPlan plan = own ? mla::LinearPlan{Form::kFew, 1} : mla::plan_linear(rows, inputs, outputs);
+    const bool few = plan.form == Form::kFew;
+    const int row_tiles = mla::few_row_tiles(rows);
+    *tile_outputs = few ? mla::few_narrow(outputs) ? 16 : 32 : plan.form == Form::kTile64 || plan.form == Form::kTile128 ? 128 : 256;
+    *tile_rows = few ? 16 * row_tiles : plan.form == Form::kTile64 ? 64 : plan.form == Form::kTile256 ? 256 : 128;
+    *splits = plan.splits;
+    const int most = few ? mla::few_rows_a_launch(outputs, *tile_outputs, *tile_rows, row_tiles == 1 ? 512 : 256) : rows;
+    *launches = (quantized || own ? 0 : 1) + mla::ceil_div(rows, most) + (plan.splits > 1 ? 1 : 0);
+    return MLA_STATUS_SUCCESS;
+}
+
 int mla_linear_fp8_fp16(const void *x, const void *w, const float *w_scale, void *out, void *workspace,
                         size_t workspace_bytes, int rows, int inputs, int outputs, long long x_stride, long long w_stride,
                         void *stream)

@@ -392,6 +392,12 @@ int mla_quantize_fp8_fp16(const void *x, void *xq, float *scales, int rows,
 int mla_quantize_fp8_bf16(const void *x, void *xq, float *scales, int rows,
                           int inputs, long long x_stride, void *stream);
 size_t mla_linear_fp8_workspace_size(int rows, int inputs, int outputs);
+/* What a call of these sizes launches on the current device (quantized: of rows that are quantised already):
+ * workgroups of tile_outputs x tile_rows, the inputs split over `splits` of them, in `launches` launches in all
+ * (quantisation and sum of the splits among them). */
+int mla_linear_fp8_plan(int rows, int inputs, int outputs, int quantized,
+                        int *tile_outputs, int *tile_rows, int *splits,
+                        int *launches);
 int mla_linear_fp8_fp16(const void *x, const void *w, const float *w_scale,
                         void *out, void *workspace, size_t workspace_bytes,
                         int rows, int inputs, int outputs, long long x_stride,

@@ -1,0 +1,62 @@
+"""Which form the plan of the fp8 products takes: that the sizes tested on the GPU reach every form, with a last block
+that the inputs fill and one that they do not, whole and split."""
+import ctypes
+
+import pytest
+
+from ada_mla import capi
+from linear_sizes import OWN, TILES
+
+TAIL = {False, True}
+
+
+@pytest.mark.parametrize("form", TILES)
+def test_sizes_reach_their_form(form):
+    outputs, rows, split = form
+    for size in TILES[form]:
+        got = capi.linear_fp8_plan(*size, quantized=True)
+        assert (got[0], got[1], got[2] > 1) == form, (size, got)
+        assert got[3] == 1 + split, size
+        m, k, n = size
+        assert m % 64 and n % 16, size  # neither fills its tiles
+    assert {k % 128 != 0 for _, k, _ in TILES[form]} == TAIL
+    if split:  # inputs that the splits do not share evenly, for either end
+        uneven = {(k % 128 != 0, -(-k // 128) % capi.linear_fp8_plan(m, k, n, quantized=True)[2] != 0) for m, k, n in TILES[form]}
+        assert (True, True) in uneven and (False, True) in uneven
+
+
+@pytest.mark.parametrize("outputs", OWN)
+def test_sizes_that_quantise_themselves(outputs):
+    for size in OWN[outputs]:
+        assert capi.linear_fp8_plan(*size) == (outputs, 16, 1, 1), size
+    assert {k % 128 != 0 for _, k, _ in OWN[outputs]} == TAIL
+
+
+def test_every_form_is_listed():
+    # forms met over a grid of sizes are those listed
+    met, step = set(), [16 * 2 ** i + 16 * (i % 2) for i in range(3, 11)]
+    for k in step:
+        for n in (16, 100, 576, 2000, 4096, 4999, 8192, 16000):
+            for m in (1, 16, 17, 33, 64, 65, 100, 200, 333, 500, 1000, 2000, 4000, 8192):
+                outputs, rows, splits, launches = capi.linear_fp8_plan(m, k, n, quantized=True)
+                met.add((outputs, rows, splits > 1))
+                assert launches == 1 + (splits > 1)
+                own = capi.linear_fp8_plan(m, k, n)
+                assert own[3] in (1, 2 + (splits > 1)) and (own[3] > 1 or own[1:3] == (16, 1))
+    assert met <= set(TILES)
+
+
+def test_plan_argument_errors():
+    plan = capi.load().mla_linear_fp8_plan
+    out = [ctypes.c_int() for _ in range(4)]
+    at = [ctypes.byref(v) for v in out]
+    assert plan(3, 256, 100, 0, *at) == capi.STATUS_SUCCESS
+    for bad in ((0, 256, 100), (3, 24, 100), (3, 256, 0), (2 ** 26 + 1, 256, 100)):
+        assert plan(*bad, 1, *at) == capi.STATUS_INVALID_VALUE
+    for i in range(4):
+        assert plan(3, 256, 100, 0, *at[:i], None, *at[i + 1:]) == capi.STATUS_INVALID_VALUE
+
+
+def test_rows_in_several_launches():
+    assert capi.linear_fp8_plan(2 ** 26, 64, 256) == (16, 64, 1, 3)  # quantised, then 2^20 row tiles x 16 x 256 threads: two grids
+    assert capi.linear_fp8_plan(2 ** 26 - 64, 64, 256, quantized=True)[3] == 1
