@@ -740,10 +740,20 @@ int launch_linear(const Linear &p, const LinearPlan &plan, hipStream_t s)
     }
 }
 
-// 16-bit rows few enough for every workgroup to quantise them
-bool quantizes_itself(int rows, int inputs)
+// Whether every workgroup quantises the 16-bit rows itself. That costs each round of workgroups about 0.15 us a thousand
+// values, a launch of its own 2 to 3.5 us once (with the few rounds that a small product takes; one row in few
+// workgroups streams its weights meanwhile). Measured, itself and with a launch (us, rows x inputs -> outputs):
+//   one round     16 x 1280 -> 4096 6.9, 7.0; 16 x 1536 7.5, 7.1; 16 x 2048 8.9, 7.4; 1 x 24576 -> 576 12.4, 17.1; -> 8192 41.1, 41.5
+//   two rounds    8 x 1536 -> 16384 11.0, 11.4; 8 x 2048 13.4, 13.2; 16 x 2048 19.0, 13.3
+//   three         8 x 1024 -> 24576 11.4, 12.4; 8 x 1536 15.4, 13.1
+//   four, eight   16 x 256 -> 32768 9.6, 7.2; 1 x 512 -> 65536 15.8, 13.0
+//   one row       1 x 32768 -> 576 15.6, 18.9; -> 2048 21.2, 22.3; -> 4096 36.3, 34.8
+bool quantizes_itself(int rows, int inputs, int outputs)
 {
-    return rows <= 16 && (int64_t)rows * ceil_div(inputs, kBlock) * kBlock <= kMostOwn;
+    const int64_t values = (int64_t)rows * ceil_div(inputs, kBlock) * kBlock;
+    const int workgroups = ceil_div(outputs, few_narrow(outputs) ? 16 : 32), cus = current_cu_count();
+    const int rounds = ceil_div(workgroups, cus);
+    return rows <= 16 && values <= kMostOwn && ((rounds <= 3 && rounds * values <= 24576) || (rows == 1 && workgroups <= cus / 2));
 }
 
 template <typename E>
@@ -789,7 +799,7 @@ int linear(bool bf16, const void *x, const float *xs, const void *w, const float
     hipStream_t s = static_cast<hipStream_t>(stream);
     Linear p{static_cast<const unsigned char *>(x), static_cast<const unsigned char *>(w), xs, ws, out, rows, inputs, outputs,
              blocks, x_stride, w_stride, xs_row, xs_block, nullptr, blocks};
-    if (!xs && quantizes_itself(rows, inputs))
+    if (!xs && quantizes_itself(rows, inputs, outputs))
         return (bf16 ? launch_own<__bf16> : launch_own<_Float16>)(p, s);
     auto *space = static_cast<unsigned char *>(workspace);
     if (!xs) {
@@ -833,7 +843,7 @@ int mla_linear_fp8_plan(int rows, int inputs, int outputs, int quantized, int *t
     using mla::Form;
     if (!mla::sizes_ok(rows, inputs, outputs) || !tile_outputs || !tile_rows || !splits || !launches)
         return MLA_STATUS_INVALID_VALUE;
-    const bool own = !quantized && mla::quantizes_itself(rows, inputs);
+    const bool own = !quantized && mla::quantizes_itself(rows, inputs, outputs);
     const mla::LinearPlan plan = own ? mla::LinearPlan{Form::kFew, 1} : mla::plan_linear(rows, inputs, outputs);
     const bool few = plan.form == Form::kFew;
     const int row_tiles = mla::few_row_tiles(rows);
