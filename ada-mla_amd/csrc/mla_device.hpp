@@ -99,6 +99,12 @@ __device__ __forceinline__ float fast_exp2(float x)
     return __builtin_amdgcn_exp2f(x);
 }
 
+// Where a running maximum of logits starts that others are taken against: finite, so that a logit
+// of -inf has no weight beside it and a NaN stays one, and below every other logit. (A
+// difference of two -inf would make tokens without weight NaN; and a partial whose maximum is
+// -inf is one without tokens.)
+constexpr float kLowestMax = -3.402823466e38f;
+
 // max / sum over the four 16-lane groups of a wave (lanes l, l^16, l^32, l^48)
 // on the VALU lane-swap instructions of gfx950 (v_permlane32_swap,
 // v_permlane16_swap), so the reduction does not queue behind LDS traffic.

@@ -1019,11 +1019,8 @@ void splitkv_fp16_kernel(const E *__restrict__ q,
                     // the partial's max is the O waves' reference (finite, at
                     // most kLazyRescale below the halves' maxima), so that m, l
                     // and O share one scale
-                    float mr = s_mref[h];
+                    const float mr = s_mref[h];
                     const float ls = s_l[0][h] * fast_exp2(s_m[0][m_at(h, 0)] - mr) + s_l[1][h] * fast_exp2(s_m[0][m_at(h, 1)] - mr);
-                    // a query with a NaN leaves its max at -inf, which the combine takes
-                    // for a piece without tokens: its sum, NaN, has to count
-                    mr = ls != ls ? 0.f : mr;
                     float *const mp = m_part + (size_t)slot_out * num_heads + head0 + h;
                     float *const lp = l_part + (size_t)slot_out * num_heads + head0 + h;
                     if (part_plain) {
@@ -1203,7 +1200,7 @@ void splitkv_fp16_kernel(const E *__restrict__ q,
                 float m_ref[T::kNHS];  // per head l16 of sub-tile hs: the accumulator's reference max
 #pragma unroll
                 for (int hs = 0; hs < T::kNHS; ++hs) {
-                    m_ref[hs] = -INFINITY;
+                    m_ref[hs] = kLowestMax;
 #pragma unroll
                     for (int dt = 0; dt < 8; ++dt)
                         o[hs][dt] = floatx4{0.f, 0.f, 0.f, 0.f};
@@ -1272,7 +1269,7 @@ void splitkv_fp16_kernel(const E *__restrict__ q,
                             if (__builtin_amdgcn_ballot_w64(moved) != 0) {
 #pragma unroll
                                 for (int hs = 0; hs < T::kNHS; ++hs) {
-                                    const float mn = fmaxf(m_ref[hs], fmaxf(m0[hs], m1[hs]));  // finite: token p_lo is in half 0
+                                    const float mn = fmaxf(m_ref[hs], fmaxf(m0[hs], m1[hs]));
                                     const float alpha = mn == m_ref[hs] ? 1.0f : fast_exp2(m_ref[hs] - mn);
                                     m_ref[hs] = mn;
                                     const float f = fast_exp2((g < 2 ? m0[hs] : m1[hs]) - mn);
@@ -1290,8 +1287,8 @@ void splitkv_fp16_kernel(const E *__restrict__ q,
                             bool moved = false;
 #pragma unroll
                             for (int hs = 0; hs < T::kNHS; ++hs) {
-                                const float mn = fmaxf(m0[hs], m1[hs]);  // finite: token p_lo is in half 0
-                                const bool up = mn > m_ref[hs] + kLazyRescale;  // always at the first block
+                                const float mn = fmaxf(m0[hs], m1[hs]);  // -inf as long as no logit is more
+                                const bool up = mn > m_ref[hs] + kLazyRescale;  // always at the first block with a weight
                                 alpha[hs] = up ? fast_exp2(m_ref[hs] - mn) : 1.0f;
                                 moved |= up;
                                 if (up)
@@ -1373,7 +1370,8 @@ void splitkv_fp16_kernel(const E *__restrict__ q,
                     const int h = 16 * hs + l16;
                     const float ls = s_l[0][h] * fast_exp2(s_m[0][m_at(h, 0)] - m_ref[hs]) +
                                      s_l[1][h] * fast_exp2(s_m[0][m_at(h, 1)] - m_ref[hs]);
-                    const float inv = out_scale / ls;
+                    // a piece whose tokens have no weight adds nothing to the others (alone it is 0 / 0)
+                    const float inv = !kDirect && ls == 0.f ? 0.f : out_scale / ls;
 #pragma unroll
                     for (int dt = 0; dt < 8; ++dt) {
                         const floatx4 v = o[hs][dt] * inv;

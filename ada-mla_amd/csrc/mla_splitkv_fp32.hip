@@ -403,7 +403,7 @@ void splitkv_fp32_kernel(const float *__restrict__ q,
             MLA_STAMP32(11, nblk);
 
             const int s_row = kSplit ? split_token(l16) : l16;
-            float m_run = -INFINITY, l_run = 0.f;  // sub-tile my_sh; kSplit: the reference m
+            float m_run = kLowestMax, l_run = 0.f;  // sub-tile my_sh; kSplit: the reference m
             for (int t = 0; t <= nblk; ++t) {
 #ifdef MLA_TIMELINE
                 tm = MLA_MT32();
