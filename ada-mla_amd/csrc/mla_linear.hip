@@ -423,7 +423,7 @@ __global__ __launch_bounds__(256) void sum_kernel(const float *__restrict__ part
 // against 24; 16 x 16384 x 5120 take 17.6, 4.8 TB/s, 1 x 5120 x 576 5.0, a launch and two round trips). The waves' sums are added through LDS at the end, wave after wave.
 // kQuantize: the rows are 16-bit (E), and each workgroup quantises them into LDS itself, which for few values is
 // cheaper than a launch.
-constexpr int kMostOwn = 32768;  // values that a workgroup quantises itself
+constexpr int kMostOwn = 24576;  // values that a workgroup quantises itself
 
 template <int NT, int MT, int kW, int kS, bool kQuantize>
 struct FewTile {
@@ -673,24 +673,29 @@ struct LinearPlan {
 bool few_narrow(int outputs) { return ceil_div(outputs, 16) <= current_cu_count(); }
 int few_row_tiles(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
 
-// The form with the smallest modelled time, and how many parts its inputs are split into. Measured on 35 sizes of 32 to
-// 8192 rows with forms and splits forced (us, e.g. 256 x 16384 x 5120: 256 tiles 197, 128 tiles 85, in
-// three splits 40; 64 tiles 61, in three 50; the model's choice is within 8% of the best of all):
+// The form with the smallest modelled time, and how many parts its inputs are split into. Measured on 35 sizes of 20 to
+// 8192 rows with forms and splits forced (us, e.g. 256 x 16384 x 5120: 128 tiles in three splits 41.1, 256 x 128 in five 43.3, in
+// six 43.4, 256 tiles in ten 46.5), the model's choice is within 6% of the best of all; of 174 more sizes of 1 to 64 rows 160 are
+// within 5%, the worst 21% (40 x 16384 x 8192: 64 tiles in four splits 40.4, in three 33.3):
 //   tiles     3.5 + rounds (blocks + 2.5) step; a step (one block) is 0.45, 0.66, 0.79, 1.55 us with few
 //             workgroups and 0.48, 0.70, 1.00, 1.80 with every CU busy (the clock falls). The 256 x 128 tiles are for
-//             the calls that make about a workgroup a CU of them (4096 x 7168 x 2048: 62.5, 256 tiles in two splits
-//             70.0, 128 tiles 78.6; 1024 x 2048 x 7168: 22.8, 33.3 whole, 29.7);
+//             the calls that make about a workgroup a CU of them (4096 x 7168 x 2048: 62.3, 256 tiles in two splits
+//             79.4, 128 tiles 85.0; 1024 x 2048 x 7168: 23.2, 256 tiles 34.1, 128 tiles 31.1);
 //   splits    4 for the second launch, and 0.28 a MB of fp32 sums, written and read;
-//   few rows  3 + rounds (1 + blocks / waves times what a block costs a wave).
+//   few rows  3 + rounds (1 + blocks / waves times what a block costs a wave: 0.5, 0.4 and 0.5 of 16, 32 and 64 rows
+//             with 16 outputs on every CU, down to 0.22, 0.26 and 0.39 on few of them; 0.8, 0.55, 0.72 with 32).
 LinearPlan plan_linear(int rows, int inputs, int outputs)
 {
     const int blocks = ceil_div(inputs, kBlock), cus = current_cu_count();
     const int few = few_row_tiles(rows);
     const bool narrow = few_narrow(outputs);
-    const double few_step = few == 1 ? (narrow ? 0.5 : 0.8) : few == 2 ? (narrow ? 0.4 : 0.55) : narrow ? 0.5 : 0.72;
-    const double few_rounds = std::ceil((double)ceil_div(rows, 16 * few) * ceil_div(outputs, narrow ? 16 : 32) / cus);
+    const double few_full = (double)ceil_div(rows, 16 * few) * ceil_div(outputs, narrow ? 16 : 32) / cus;
+    const double idle = narrow ? 1.0 - std::min(1.0, few_full) : 0.0;
+    const double few_step = few == 1 ? (narrow ? 0.5 - 0.28 * idle : 0.8)
+                            : few == 2 ? (narrow ? 0.4 - 0.14 * idle : 0.55)
+                                       : narrow ? 0.5 - 0.11 * idle : 0.72;
     LinearPlan best{Form::kFew, 1};
-    double best_us = 3.0 + few_rounds * (1.0 + ceil_div(blocks, few == 1 ? 8 : 4) * few_step);
+    double best_us = 3.0 + std::ceil(few_full) * (1.0 + ceil_div(blocks, few == 1 ? 8 : 4) * few_step);
     if (inputs < kBlock)  // (the tiles want a whole block)
         return best;
     struct Kind {
@@ -741,19 +746,16 @@ int launch_linear(const Linear &p, const LinearPlan &plan, hipStream_t s)
 }
 
 // Whether every workgroup quantises the 16-bit rows itself. That costs each round of workgroups about 0.15 us a thousand
-// values, a launch of its own 2 to 3.5 us once (with the few rounds that a small product takes; one row in few
-// workgroups streams its weights meanwhile). Measured, itself and with a launch (us, rows x inputs -> outputs):
-//   one round     16 x 1280 -> 4096 6.9, 7.0; 16 x 1536 7.5, 7.1; 16 x 2048 8.9, 7.4; 1 x 24576 -> 576 12.4, 17.1; -> 8192 41.1, 41.5
+// values, a launch of its own 2 to 3.5 us once. Measured, itself and with a launch (us, rows x inputs -> outputs):
+//   one round     16 x 1280 -> 4096 6.9, 7.0; 16 x 1536 7.5, 7.1; 16 x 2048 8.9, 7.4; 1 x 24576 -> 8192 41.1, 41.5
 //   two rounds    8 x 1536 -> 16384 11.0, 11.4; 8 x 2048 13.4, 13.2; 16 x 2048 19.0, 13.3
 //   three         8 x 1024 -> 24576 11.4, 12.4; 8 x 1536 15.4, 13.1
 //   four, eight   16 x 256 -> 32768 9.6, 7.2; 1 x 512 -> 65536 15.8, 13.0
-//   one row       1 x 32768 -> 576 15.6, 18.9; -> 2048 21.2, 22.3; -> 4096 36.3, 34.8
 bool quantizes_itself(int rows, int inputs, int outputs)
 {
     const int64_t values = (int64_t)rows * ceil_div(inputs, kBlock) * kBlock;
-    const int workgroups = ceil_div(outputs, few_narrow(outputs) ? 16 : 32), cus = current_cu_count();
-    const int rounds = ceil_div(workgroups, cus);
-    return rows <= 16 && values <= kMostOwn && ((rounds <= 3 && rounds * values <= 24576) || (rows == 1 && workgroups <= cus / 2));
+    const int rounds = ceil_div(ceil_div(outputs, few_narrow(outputs) ? 16 : 32), current_cu_count());
+    return rows <= 16 && rounds <= 3 && rounds * values <= kMostOwn;
 }
 
 template <typename E>

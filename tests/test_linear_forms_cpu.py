@@ -33,15 +33,22 @@ def test_sizes_that_quantise_themselves(outputs):
 
 
 @pytest.mark.parametrize("rows,inputs,outputs", [(16, 2048, 576), (16, 2048, 129280), (8, 4096, 4096), (1, 512, 65536), (16, 256, 32768),
-                                                 (8, 1536, 24576), (4, 7168, 16384), (1, 32768, 16384), (1, 16384, 129280)])
+                                                 (8, 1536, 24576), (4, 7168, 16384), (1, 32768, 2048), (1, 32768, 16384), (1, 16384, 129280)])
 def test_rows_quantised_once(rows, inputs, outputs):
     # where the workgroups' own quantisation, round after round, takes longer than a launch for it
     product = capi.linear_fp8_plan(rows, inputs, outputs, quantized=True)
     assert capi.linear_fp8_plan(rows, inputs, outputs) == (*product[:3], product[3] + 1)
 
 
+@pytest.mark.parametrize("rows,inputs,outputs,tiles", [(1, 32768, 70, (16, 16)), (1, 32768, 576, (16, 16)), (16, 32768, 2500, (16, 16)),
+                                                       (20, 10240, 70, (16, 32)), (40, 7168, 576, (16, 64)), (64, 7168, 70, (16, 64))])
+def test_few_workgroups_stream_faster(rows, inputs, outputs, tiles):
+    # a step of the few-row kernel on few CUs is up to half of what it is on all of them: no split tiles for these
+    assert capi.linear_fp8_plan(rows, inputs, outputs, quantized=True) == (*tiles, 1, 1)
+
+
 @pytest.mark.parametrize("rows,inputs,outputs", [(1, 5120, 576), (16, 1280, 4096), (8, 1024, 24576), (1, 7168, 16384), (1, 24576, 576),
-                                                 (1, 32768, 2048), (2, 8192, 4096)])
+                                                 (2, 8192, 4096)])
 def test_rows_quantised_by_every_workgroup(rows, inputs, outputs):
     assert capi.linear_fp8_plan(rows, inputs, outputs) == (16 if outputs <= 4096 else 32, 16, 1, 1)
 
