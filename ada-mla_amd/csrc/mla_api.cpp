@@ -867,7 +867,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
           "paged-KV fp16 / bf16 MLA decode (query [B,n_h,576], kv_cache [pages,page_size,576], "
           "block_table [B,max_pages] int32, cu_seqlens [B+1] int32); total_tokens=-1 reads cu_seqlens[B] "
           "(synchronising); a given total_tokens is not checked: one below cu_seqlens[B] silently "
-          "truncates the trailing sequences. kv_cache of the query's dtype, or float8_e4m3fn holding C / cache_scale",
+          "truncates the trailing sequences. kv_cache of the query's dtype, or float8_e4m3fn holding C / cache_scale (num_heads "
+          "a multiple of 32: the query then to 8 significant bits)",
           pybind11::arg("query"), pybind11::arg("kv_cache"), pybind11::arg("block_table"),
           pybind11::arg("cu_seqlens"), pybind11::arg("total_tokens") = -1, pybind11::arg("num_splits") = 0,
           pybind11::arg("cache_scale") = 1.0);

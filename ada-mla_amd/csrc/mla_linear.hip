@@ -156,11 +156,12 @@ __device__ __forceinline__ void each_of(F &&body)
 // into registers, and the loads of block b + kSlots - 1 issued, between the products of block b: behind the one barrier of a
 // block only the first outputs' operand has to be read before products run (with the rows read there, 256 x
 // 256 tiles took 3190 cycles a block, 730 of them for those reads, where the products take 2110).
-// Bound by the matrix units, the 256 tiles: 8192 x 7168 x 8192 in 407 us, 2.36 PFLOP/s, 2980 cycles a block; the four sums
+// Bound by the matrix units, the 256 tiles: 8192 x 7168 x 8192 in 413 us (404 to 429 of 100 calls behind 1000 others; 421
+// to 557 of the first 20), 2.33 PFLOP/s, 2980 cycles a block; the four sums
 // in fp32 behind each product cost the rest (a product and its sums take 35 to 37 cycles of two waves, 33 the
 // product alone), and the clock, 2.37 GHz with few workgroups, falls to 1.8 with every CU at it. The smaller tiles are for
-// calls that 256 x 256 leave without workgroups: 4096 x 7168 x 2048 in 62.5 us (256 x 128), 333 x 2000 x 4999 in 13.8; 64 x 16384 x 5120, its inputs split
-// in six, in 18.0 (4.7 TB/s of weights).
+// calls that 256 x 256 leave without workgroups: 4096 x 7168 x 2048 in 62.3 us (256 x 128), 333 x 2000 x 4999 in 12.8; 64 x 16384 x 5120, its inputs split
+// in six, in 17.6 (4.8 TB/s of weights).
 // 16-byte chunk c of row r sits at c ^ (r / 2 mod 8): rows are 128
 // bytes, two of them an LDS bank period, so chunk g of 16 rows is in 16 different places, and so are those of
 // the 8 rows and 8 others of the next g that the LDS reads at once (chunks 2 g, 2 g + 1: half of its cycles were conflicts).

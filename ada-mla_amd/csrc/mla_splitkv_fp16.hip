@@ -177,8 +177,8 @@ struct F16Tile {
 // cache; the S and O waves convert their operands to E after each LDS
 // read, exactly (every E4M3 value is an fp16 and a bf16 value). The per-tensor cache
 // scale is folded into scale_log2 and out_scale.
-// Paged (us, with its combine behind it): 4 sequences of 1832 tokens in all at 16 heads, fp16 7.5 + 3.1; 32 of
-// 219 649 at 128 heads, bf16 87.5 + 8.9; 131 000 tokens at 128 heads, fp16 48.5 + 5.8.
+// Paged (us, with its combine behind it; 1000 calls before them): 4 sequences of 1832 tokens in all at 16 heads, fp16
+// 7.2 + 2.9; 32 of 219 649 at 128 heads, bf16 76.4 + 8.7; 131 000 tokens at 128 heads, fp16 42.2 + 5.7.
 // kMode: kModeBatch (cu_seqlens: a chunk may hold pieces of several
 // sequences), kModeSingle (one sequence: the chunk is one piece, whose
 // prologue loads go out at kernel entry) or kModeDirect (kModeSingle with a

@@ -285,7 +285,12 @@ int mla_decode_paged_bf16(const void *query, const void *kv_cache,
  * C / cache_scale (a per-tensor scale > 0), as mla_append_kv_* writes it with
  * MLA_FLAG_FP8_CACHE: query and out in fp16 or bf16, everything else as there.
  * The cache is read at one byte per value; every E4M3FN value is a value of the
- * query's type, so the products see the cache as it stands. */
+ * query's type, so the products see the cache as it stands. A query is held
+ * whole where the plan's head tile is 16, else (num_heads a multiple of 32) as two
+ * fp8 parts a head, 8 significant bits of each value: all that bf16 has, three
+ * less than fp16's. The softmax weights and the split partials are in the query's type. Errors in the 2-norm, of N(0, 1)
+ * queries: fp16 0.00033 with 16 heads and 0.00073 with 128 (rounding the
+ * exact result once: 0.00021), bf16 0.0024 with 128 (0.0017). */
 size_t mla_decode_paged_fp8_workspace_size(int batch, int num_heads,
                                            int total_tokens, int num_splits);
 int mla_decode_paged_fp8_fp16(const void *query, const void *kv_cache_fp8,
@@ -376,7 +381,7 @@ int mla_project_output_bf16(const void *o_star, const void *w_uv,
  *   out[m][n] = sum_b xs[m][b] w_scale[n / 128][b] sum_{k in b} xq[m][k] w[n][k]
  *   with x quantised so, w [outputs][inputs] E4M3FN (w_stride bytes apart) and
  *   w_scale [ceil(outputs / 128)][ceil(inputs / 128)]; sums in fp32, rounded
- *   once. The workspace holds the quantised rows, and fp32 sums where
+ *   once, the product of two scales too, which has to be a finite fp32 value. The workspace holds the quantised rows, and fp32 sums where
  *   the inputs are split over workgroups (the same bits whatever is in it).
  * mla_linear_fp8_quantized_*: the same of rows that are quantised already, xq
  *   (x_stride bytes apart), and out in fp16 or bf16; the scale of row m and block b is
